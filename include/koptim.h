@@ -356,6 +356,48 @@ int ko_argmax_rows(const void* x, long long ld, int M, int N, long long* ids, vo
  * counterpart (the reference's Triton GEMV reads its row-major weights). */
 int ko_gemv_tile(const void* w, void* wt, int rows, int K, void* stream);
 
+/* ---- KV cache held in 4 bits --------------------------------------------------
+ * No counterpart in the reference, whose cache is bf16.
+ * A cache layer is [B, nkv, blocks, bytes]: 32 consecutive keys of a (sequence, KV head)
+ * pair are one block of 32 d + 256 d / group bytes (kernel_optim_amd/csrc/kv4_core.h has its
+ * layout), blocks of a pair contiguous, the sequence and head strides given in BYTES,
+ * multiples of 16; 16-byte aligned. Groups of `group` (32, 64, 128; at most d) values of a head
+ * vector share a bf16 scale s and a bf16 value c: x = c + s (n - 8), n = 0..15, with
+ * c = bf16(7/15 min + 8/15 max), s = bf16(max((max - c) / 7, (c - min) / 8)) (0 below 2^-126)
+ * and n = clamp(rint((x - c) (1 / s) + 8), 0, 15); a group with a NaN or an infinity has
+ * s = c = NaN. d = 64 or 128.
+ *
+ * ko_kv4_write: rows 0 .. lengths[b] - 1 (lengths NULL: S) of k and v [B, nkv, S, d] bf16, inner
+ * stride 1, the other strides in elements, multiples of 8, into the slots from start[b] (NULL: 0)
+ * on. Rows whose slot lies outside [0, cap) are dropped; other slots keep what they hold.
+ * ko_kv4_read: the reverse; rows past lengths[b] or outside [0, cap) are left as they were. */
+int ko_kv4_write(const void* k, long long k_b_stride, long long k_h_stride, long long k_s_stride,
+                 const void* v, long long v_b_stride, long long v_h_stride, long long v_s_stride,
+                 void* cache, long long cache_b_stride, long long cache_h_stride, const int* start,
+                 const int* lengths, int B, int S, int nkv, int cap, int d, int group,
+                 void* stream);
+int ko_kv4_read(const void* cache, long long cache_b_stride, long long cache_h_stride, void* k,
+                long long k_b_stride, long long k_h_stride, long long k_s_stride, void* v,
+                long long v_b_stride, long long v_h_stride, long long v_s_stride, const int* start,
+                const int* lengths, int B, int S, int nkv, int cap, int d, int group,
+                void* stream);
+
+/* ko_qk_norm_rope with the quantised append: qkv [M, (nq+2nkv)*d] bf16, M = B*T, row m is
+ * sequence m/T at position pos[m/T] + m%T; q_out [M, nq*d] bf16, k and v into the cache's slot
+ * at that position. Norm and RoPE run in fp32; q rounds once, k is quantised from fp32.
+ * Positions outside [0, max_pos) (max_pos = min(cap, table rows)) are skipped. */
+int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void* cos,
+                  const void* sin, const int* pos, void* q_out, void* cache, int M, int T,
+                  long long cache_b_stride, long long cache_h_stride, float eps, int nq, int nkv,
+                  int d, int group, int max_pos, void* stream);
+
+/* Decode attention over a 4-bit cache layer: as ko_decode_attn for q [B*T, nq*d] bf16 and out
+ * (another buffer), query t of sequence b at position n - T + t of its n = kv_lens[b] + len_offset
+ * keys (at most cap). A row that sees no key is zero. nq a multiple of nkv. */
+int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
+                long long cache_h_stride, const int* kv_lens, int len_offset, int cap, int B,
+                int T, int nq, int nkv, int d, int group, float scale, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -72,6 +72,15 @@ SIGNATURES = {
     "ko_decode_attn_token_rows": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _int, _ll, _ll,
                                   _int, _int, _int, _int, _int, _int, _int, _f, _c_void_p,
                                   _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "ko_kv4_write": [_c_void_p, _ll, _ll, _ll, _c_void_p, _ll, _ll, _ll, _c_void_p, _ll, _ll,
+                     _c_void_p, _c_void_p, _int, _int, _int, _int, _int, _int, _c_void_p],
+    "ko_kv4_read": [_c_void_p, _ll, _ll, _c_void_p, _ll, _ll, _ll, _c_void_p, _ll, _ll, _ll,
+                    _c_void_p, _c_void_p, _int, _int, _int, _int, _int, _int, _c_void_p],
+    "ko_kv4_append": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                      _c_void_p, _int, _int, _ll, _ll, _f, _int, _int, _int, _int, _int,
+                      _c_void_p],
+    "ko_kv4_attn": [_c_void_p, _c_void_p, _ll, _ll, _c_void_p, _int, _int, _int, _int, _int, _int,
+                    _int, _int, _f, _c_void_p, _c_void_p],
 }
 
 # Entry points whose return value is a size, not a status.

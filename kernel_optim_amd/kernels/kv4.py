@@ -1,0 +1,238 @@
+"""A KV cache held in 4 bits: writing it, reading it back, and decode attention over it.
+
+The ops stand beside ``kernels.fused``'s for the bf16 cache and follow their manner: tensors
+are the caller's, every call launches on the current stream of the current device, allocates
+nothing and never synchronises (so calls can be captured), and a bad argument raises
+ValueError before anything is launched.
+
+- ``kv4_cache`` allocates a cache; ``kv4_write`` quantises bf16 K/V rows into it, ``kv4_read``
+  reads cached keys back as bf16;
+- ``kv4_append``: ``qk_norm_rope`` (engine/kernels/fused.py:99-106) with the quantised append;
+- ``Kv4Attention``: ``DecodeAttention`` (fused.py:204-234) over the 4-bit cache, and its
+  ``decode_qkv`` for the whole of a decode step's attention.
+
+A head vector's values are held in groups of 32, 64 or 128 that share a bf16 scale s and a bf16
+value c: x = c + s (n - 8), n = 0..15, within s / 2 of what was written (up to the rounding of
+s itself, 2^-9 of 7 s); a group of equal bf16 values reads back as it was, a group with a NaN or
+an infinity as NaN throughout. 5, 4.5 or 4.25 bits a value, scales included.
+
+A cache is a uint8 tensor [B, nkv, blocks, bytes]: 32 keys of a (sequence, KV head) pair are one
+block (csrc/kv4_core.h has its layout). Blocks must be contiguous; the two outer strides are
+free, in multiples of 16 bytes. Slots that were never written may hold anything: nothing reads
+past a sequence's length.
+"""
+
+import torch
+
+from .. import _lib
+from .fused import BF16, _is, _need
+
+KV4_KEYS = 32  # keys of a block
+
+
+def kv4_block_bytes(d, group):
+    """Bytes of a block of 32 keys (K and V): 32 d of codes and 256 a group of scales."""
+    _need(d in (64, 128), f"head_dim must be 64 or 128, got {d}")
+    _need(group in (32, 64, 128) and group <= d,
+          f"group must be 32, 64 or 128 and at most head_dim, got {group}")
+    return 32 * d + 256 * (d // group)
+
+
+_FORMATS = {kv4_block_bytes(d, g): (d, g) for d in (64, 128) for g in (32, 64, 128) if g <= d}
+
+
+def kv4_cache(B, nkv, cap, d, device, group=32, layers=None):
+    """An empty cache for cap keys (rounded up to whole blocks) of B sequences and nkv KV heads:
+    uint8 [B, nkv, blocks, bytes], or [layers, ...]."""
+    _need(B >= 1 and nkv >= 1 and cap >= 1, "B, nkv and cap must be positive")
+    shape = (B, nkv, -(-cap // KV4_KEYS), kv4_block_bytes(d, group))
+    return torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8,
+                       device=device)
+
+
+def _here(dev):
+    _need(dev == torch.cuda.current_device(), f"tensors are on cuda:{dev}, the current device is "
+          f"cuda:{torch.cuda.current_device()}")
+
+
+def _tensor(t, name, dtype, shape, dev, contiguous=True):
+    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
+    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
+    _need(tuple(t.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    _need(t.is_cuda and t.get_device() == dev, f"{name} must be on cuda:{dev}")
+    _need(not contiguous or t.is_contiguous(), f"{name} must be contiguous")
+    _need(not t.is_cuda or t.data_ptr() % (4 if dtype == torch.int32 else 16) == 0,
+          f"{name} must be aligned to 16 bytes (int32: 4)")
+
+
+def _no_overlap(t, name):
+    """A tensor that is written holds each element once."""
+    reach = 0
+    for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
+        _need(stride > reach, f"{name}: elements share memory (strides {tuple(t.stride())})")
+        reach += stride * (size - 1)
+
+
+def _check_cache(cache, written):
+    """The cache's (B, nkv, blocks, d, group, device)."""
+    _need(isinstance(cache, torch.Tensor) and cache.dtype == torch.uint8 and cache.dim() == 4,
+          "cache must be a uint8 tensor [B, nkv, blocks, bytes]")
+    B, nkv, nb, size = cache.shape
+    _need(size in _FORMATS, f"cache: {size} bytes are no block's size ({sorted(_FORMATS)})")
+    _need(min(B, nkv, nb) >= 1, "cache must not be empty")
+    _need(cache.is_cuda, "cache must be on the GPU")
+    sb, sh, sk, s1 = cache.stride()
+    _need(s1 == 1 and (sk == size or nb == 1) and (sb % 16 == 0 or B == 1)
+          and (sh % 16 == 0 or nkv == 1) and cache.data_ptr() % 16 == 0,
+          "cache: blocks must be contiguous, outer strides and the address multiples of 16")
+    if written:
+        _no_overlap(cache, "cache")
+    return B, nkv, nb, *_FORMATS[size], cache.get_device()
+
+
+def _outer(t):
+    """The outer strides of a 4-d tensor; those of single rows do not matter."""
+    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(t.dim() - 1)]
+
+
+def _rows(cache, k, v, start, lengths, written, names):
+    """What kv4_write and kv4_read check alike; the C arguments of each."""
+    B, nkv, nb, d, group, dev = _check_cache(cache, written)
+    _here(dev)
+    for t, name in ((k, names[0]), (v, names[1])):
+        _need(isinstance(t, torch.Tensor) and t.dim() == 4, f"{name} must be [B, nkv, S, d]")
+        _tensor(t, name, BF16, (B, nkv, k.shape[2], d), dev, contiguous=False)
+        _need(t.stride(3) == 1, f"{name}: the inner stride must be 1")
+        _need(all(s % 8 == 0 for s in _outer(t)), f"{name}: strides must be multiples of 8")
+        if not written:
+            _no_overlap(t, name)
+    for t, name in ((start, "start"), (lengths, "lengths")):
+        if t is not None:
+            _tensor(t, name, torch.int32, (B,), dev)
+    S = k.shape[2]
+    c = (cache.data_ptr(), *_outer(cache)[:2])
+    kv = (k.data_ptr(), *_outer(k), v.data_ptr(), *_outer(v))
+    rest = (_lib.ptr(start), _lib.ptr(lengths), B, S, nkv, nb * KV4_KEYS, d, group)
+    return S, c, kv, rest
+
+
+def kv4_write(k, v, cache, start=None, lengths=None):
+    """Quantise rows of K and V into the cache: row i of sequence b goes to slot start[b] + i.
+
+    k, v: [B, nkv, S, d] bf16, inner stride 1, other strides multiples of 8 (a projection's
+    [B, S, nkv, d] transposed serves); start: [B] int32 on the GPU (None: 0); lengths: [B] int32,
+    the valid rows of a padded batch (None: S). Rows whose slot lies outside the cache are
+    dropped; other slots keep what they hold."""
+    S, c, kv, rest = _rows(cache, k, v, start, lengths, True, ("k", "v"))
+    if S:
+        _lib.call("ko_kv4_write", *kv, *c, *rest, _lib.stream_ptr())
+
+
+def kv4_read(cache, k_out, v_out, start=None, lengths=None):
+    """Read cached keys back: row i of k_out and v_out [B, nkv, S, d] bf16 receives the values
+    of slot start[b] + i, i < lengths[b] (None: S); other rows are left as they are, as are rows
+    whose slot lies outside the cache. Strides and the other arguments as for kv4_write."""
+    S, c, kv, rest = _rows(cache, k_out, v_out, start, lengths, False, ("k_out", "v_out"))
+    if S:
+        _lib.call("ko_kv4_read", *c, *kv, *rest, _lib.stream_ptr())
+
+
+def _check_qkv(qkv, q_w, k_w, cos, sin, pos, rows, B, nq, nkv, d, dev):
+    _tensor(qkv, "qkv", BF16, (rows, (nq + 2 * nkv) * d), dev)
+    _tensor(q_w, "q_w", BF16, (d,), dev)
+    _tensor(k_w, "k_w", BF16, (d,), dev)
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        _need(isinstance(t, torch.Tensor) and t.dim() == 2 and t.shape[0] >= 1,
+              f"{name} must be [rows, d]")
+        _tensor(t, name, BF16, (t.shape[0], d), dev)
+    _tensor(pos, "pos", torch.int32, (B,), dev)
+
+
+def kv4_append(qkv, q_w, k_w, cos, sin, pos, q_out, cache, T, eps, nq, nkv, d):
+    """qk_norm_rope over the 4-bit cache: qkv [B*T, (nq+2nkv)*d] bf16, row m is sequence m // T at
+    position pos[b] + m % T. Per-head RMSNorm and RoPE of q into q_out [B*T, nq*d], of k into
+    the cache's slot at that position with v, both quantised. Everything is fp32 up to the one
+    rounding of q and the quantisation of k. Positions outside the cache or the RoPE tables
+    [rows, d] are skipped (their q_out rows too)."""
+    B, ck, nb, cd, group, dev = _check_cache(cache, True)
+    _here(dev)
+    _need(T >= 1 and nq >= 1, "T and nq must be positive")
+    _need((ck, cd) == (nkv, d), f"cache has {ck} heads of {cd}, not {nkv} of {d}")
+    _check_qkv(qkv, q_w, k_w, cos, sin, pos, B * T, B, nq, nkv, d, dev)
+    _tensor(q_out, "q_out", BF16, (B * T, nq * d), dev)
+    cb, ch, _ = _outer(cache)
+    _lib.call("ko_kv4_append", qkv.data_ptr(), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
+              sin.data_ptr(), pos.data_ptr(), q_out.data_ptr(), cache.data_ptr(), B * T, T, cb, ch,
+              eps, nq, nkv, d, group, min(nb * KV4_KEYS, cos.shape[0], sin.shape[0]),
+              _lib.stream_ptr())
+
+
+class Kv4Attention:
+    """Decode attention over a 4-bit cache for T query tokens per sequence, fixed (B, T, cap).
+
+    Any number of query heads per KV head and tokens with T * nq / nkv <= 64, T <= 8; head_dim 64
+    or 128. A query row that sees no key is zero. Calls of one object share its workspace:
+    they must not overlap on two streams, nor may graphs captured from them.
+    """
+
+    MAX_T = 8
+
+    def __init__(self, B, T, cap, nq, nkv, d, device, group=32):
+        self.block_bytes = kv4_block_bytes(d, group)
+        _need(B >= 1 and cap >= 1 and nkv >= 1 and nq >= 1 and nq % nkv == 0,
+              "B, cap and nkv must be positive, nq a multiple of nkv")
+        _need(1 <= T <= self.MAX_T, f"T must be in 1..{self.MAX_T}")
+        _need(T * (nq // nkv) <= 64, "at most 64 query rows (T * nq / nkv) a KV head")
+        self.B, self.T, self.cap, self.nq, self.nkv, self.d, self.group = B, T, cap, nq, nkv, d, group
+        dev = torch.device(device)
+        _need(dev.type == "cuda", "device must be a GPU")
+        self.device = torch.cuda.current_device() if dev.index is None else dev.index
+        self.scale = d ** -0.5
+        self.blocks = -(-cap // KV4_KEYS)
+        self._q = torch.empty(B, nq * d, dtype=BF16, device=dev) if T == 1 else None
+        self._q_shape = torch.Size((B * T, nq * d))
+        self._cache_shape = torch.Size((B, nkv, self.blocks, self.block_bytes))
+        self._len_shape = torch.Size((B,))
+
+    def _check_cache(self, cache, written=False):
+        _need(isinstance(cache, torch.Tensor) and cache.shape == self._cache_shape,
+              f"cache must be a uint8 tensor {list(self._cache_shape)}")
+        _need(_check_cache(cache, written)[5] == self.device, f"cache must be on cuda:{self.device}")
+
+    def _run(self, q, cache, lens, len_offset, out):
+        if not (_is(q, BF16, self._q_shape) and _is(out, BF16, self._q_shape)
+                and _is(lens, torch.int32, self._len_shape)
+                and isinstance(cache, torch.Tensor) and cache.dtype is torch.uint8
+                and cache.is_contiguous() and cache.shape == self._cache_shape
+                and cache.get_device() == self.device == q.get_device() == out.get_device()
+                and lens.get_device() == self.device
+                and (q.data_ptr() | cache.data_ptr() | out.data_ptr()) % 16 == 0):
+            _tensor(q, "q", BF16, self._q_shape, self.device)
+            _tensor(out, "out", BF16, self._q_shape, self.device)
+            _tensor(lens, "pos/lengths", torch.int32, self._len_shape, self.device)
+            self._check_cache(cache)
+        _here(self.device)
+        _need(q.data_ptr() != out.data_ptr(), "out must not be q")
+        cb, ch, _, _ = cache.stride()
+        _lib.call("ko_kv4_attn", q.data_ptr(), cache.data_ptr(), cb, ch, lens.data_ptr(), len_offset,
+                  self.cap, self.B, self.T, self.nq, self.nkv, self.d, self.group, self.scale,
+                  out.data_ptr(), _lib.stream_ptr())
+
+    def __call__(self, q, cache, pos, out):
+        """q: [B*T, nq*d] bf16; cache: [B, nkv, blocks, bytes]; pos: [B] int32, the position of a
+        sequence's first query (keys 0 .. pos + T - 1 are cached, query t sees those up to pos +
+        t); out: [B*T, nq*d] bf16."""
+        self._run(q, cache, pos, self.T, out)
+
+    def with_lengths(self, q, cache, lengths, out):
+        """lengths[b] = number of cached keys of sequence b (int32); its T queries sit at the last
+        T positions. Rows in front of the first key (lengths[b] < T) are zero."""
+        self._run(q, cache, lengths, 0, out)
+
+    def decode_qkv(self, qkv, q_w, k_w, cos, sin, pos, cache, out, eps):
+        """A decode step's attention (T = 1) straight from the bf16 QKV projection [B, (nq+2nkv)*d]:
+        kv4_append at pos[b], then attention over keys 0..pos[b] with q kept in bf16."""
+        _need(self.T == 1, "decode_qkv serves one decode token per sequence")
+        self._check_cache(cache, True)
+        kv4_append(qkv, q_w, k_w, cos, sin, pos, self._q, cache, 1, eps, self.nq, self.nkv, self.d)
+        self._run(self._q, cache, pos, 1, out)

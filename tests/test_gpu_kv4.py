@@ -1,0 +1,398 @@
+"""The 4-bit KV cache on the GPU against the oracle: writes bit for bit, values read back, and
+attention over what the cache holds in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from kernel_optim_amd.kernels.kv4 import (KV4_KEYS, Kv4Attention, kv4_append, kv4_block_bytes,
+                                          kv4_cache, kv4_read, kv4_write)
+from oracle import kv4 as O
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+FORMATS = [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def junk(shape, seed):
+    """Bytes of a used cache: any codes, scales that are no numbers."""
+    t = torch.randint(0, 256, shape, generator=gen(seed), dtype=torch.uint8)
+    d = {kv4_block_bytes(d, g): d for d, g in FORMATS}[shape[-1]]
+    t[..., 32 * d:] = 0xff
+    return t
+
+
+def randn(seed, *shape):
+    return torch.randn(*shape, generator=gen(seed))
+
+
+def rows(seed, B, H, S, d):
+    """K or V rows with strong channels and small tokens among them."""
+    x = randn(seed, B, H, S, d)
+    x[..., ::17] *= 9
+    x[:, :, ::5] *= 1e-4
+    return x.to(BF16)
+
+
+def filled(B, H, cap, d, group, lens, seed):
+    """A cache with lens[b] keys of sequence b, and no numbers behind them."""
+    k, v = (rows(seed + i, B, H, cap, d) for i in range(2))
+    (nk, sk, ck), (nv, sv, cv) = O.quantise(k, group), O.quantise(v, group)
+    pad = -cap % 32
+    stack = lambda a, b: torch.nn.functional.pad(torch.stack((a, b)), (0, 0, 0, pad))
+    n, s, c = stack(nk, nv), stack(sk, sv), stack(ck, cv)
+    for b, m in enumerate(lens):
+        s[:, b, :, m:] = c[:, b, :, m:] = math.nan
+    return O.pack(n, s, c)
+
+
+# ---------------------------------------------------------------------------
+# Writing and reading.
+# ---------------------------------------------------------------------------
+CASES = [  # B, nkv, S, blocks, start, lengths
+    (1, 1, 1, 1, [0], None),
+    (2, 3, 32, 2, [0, 32], None),
+    (3, 2, 45, 4, [7, 0, 64], [45, 3, 0]),
+    (2, 1, 100, 3, [-5, 61], [100, 99]),       # rows in front of the cache and behind it
+    (2, 2, 17, 2, [63, 64], None),             # the last slot; none
+    (1, 2, 200, 9, [31], [1000]),
+]
+
+
+@pytest.mark.parametrize("d,group", FORMATS)
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_write_and_read(dev, d, group, case):
+    B, H, S, nb, start, lengths = CASES[case]
+    k, v = rows(1, B, H, S, d), rows(2, B, H, S, d)
+    old = junk((B, H, nb, kv4_block_bytes(d, group)), 3)
+    want = O.write(old, k, v, start, lengths or [S] * B, group)
+    cache = old.to(dev)
+    st = torch.tensor(start, dtype=torch.int32, device=dev)
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=dev)
+    kv4_write(k.to(dev), v.to(dev), cache, start=st, lengths=ln)
+    assert torch.equal(cache.cpu(), want)
+    ko, vo = (torch.full((B, H, S, d), 7.0, dtype=BF16, device=dev) for _ in range(2))
+    kv4_read(cache, ko, vo, start=st, lengths=ln)
+    n, s, c = O.unpack(want, d, group)
+    held = O.values(n, s, c, group).to(torch.float32).to(BF16)
+    for i, got in enumerate((ko.cpu(), vo.cpu())):
+        expect = torch.full_like(got, 7.0)
+        for b in range(B):
+            for r in range(min(S, lengths[b] if lengths else S)):
+                if 0 <= start[b] + r < nb * KV4_KEYS:
+                    expect[b, :, r] = held[i, b, :, start[b] + r]
+        assert torch.equal(got, expect)
+
+
+@pytest.mark.parametrize("d,group", [(128, 32), (64, 64)])
+def test_strided_rows_and_caches(dev, d, group):
+    B, H, S = 2, 3, 50
+    k, v = rows(4, B, S, H, d).transpose(1, 2), rows(5, B, H, S + 6, d)[:, :, 3:-3]
+    size = kv4_block_bytes(d, group)
+    big = junk((B, 2, H, 3, size), 6)
+    want = big.clone()
+    want[:, 1] = O.write(big[:, 1].contiguous(), k, v, [0] * B, [S] * B, group)
+    got = big.to(dev)
+    wide = torch.zeros(B, H, S + 6, d, dtype=BF16, device=dev)
+    wide[:, :, 3:-3] = v.to(dev)
+    kd = k.transpose(1, 2).contiguous().to(dev).transpose(1, 2)
+    kv4_write(kd, wide[:, :, 3:-3], got[:, 1])
+    assert torch.equal(got.cpu(), want)
+    ko = torch.zeros(B, S, H, d, dtype=BF16, device=dev).transpose(1, 2)
+    wide.zero_()
+    kv4_read(got[:, 1], ko, wide[:, :, 3:-3])
+    n, s, c = O.unpack(want[:, 1], d, group)
+    held = O.values(n, s, c, group)[:, :, :, :S].to(torch.float32).to(BF16)
+    assert torch.equal(ko.cpu(), held[0]) and torch.equal(wide[:, :, 3:-3].cpu(), held[1])
+    assert (wide[:, :, :3] == 0).all() and (wide[:, :, -3:] == 0).all()
+
+
+def test_values_at_the_ends(dev):
+    """Groups of one value, zeros, subnormals, NaN and infinities."""
+    d, group = 128, 32
+    k = rows(7, 1, 1, 32, d)
+    k[0, 0, 0] = 0
+    k[0, 0, 1] = -3.0
+    k[0, 0, 2] = 2.0 ** -133
+    k[0, 0, 3] = torch.linspace(-1, 1, d).to(BF16) * 2.0 ** -127
+    k[0, 0, 4, 40] = math.nan
+    k[0, 0, 5, 70] = math.inf
+    k[0, 0, 6, 100] = -math.inf
+    k[0, 0, 7] = torch.linspace(-1, 1, d).to(BF16) * 2.0 ** 120
+    v = k.flip(2).contiguous()
+    cache = kv4_cache(1, 1, 32, d, dev, group)
+    kv4_write(k.to(dev), v.to(dev), cache)
+    got = O.unpack(cache, d, group)
+    want = O.unpack(O.write(torch.zeros_like(cache, device="cpu"), k, v, [0], [32], group), d, group)
+    for a, b in zip(got[1:], want[1:]):
+        assert torch.equal(a.isnan(), b.isnan())
+        assert torch.equal(a.nan_to_num(5.0), b.nan_to_num(5.0))
+    fine = ~want[1].isnan().repeat_interleave(group, -1)
+    assert torch.equal(got[0][fine], want[0][fine])
+    ko, vo = (torch.empty(1, 1, 32, d, dtype=BF16, device=dev) for _ in range(2))
+    kv4_read(cache, ko, vo)
+    assert torch.equal(ko.cpu()[0, 0, :3], k[0, 0, :3])
+    assert ko[0, 0, 4, 32:64].isnan().all() and not ko[0, 0, 4, :32].isnan().any()
+    assert ko[0, 0, 5, 64:96].isnan().all() and ko[0, 0, 6, 96:].isnan().all()
+
+
+# ---------------------------------------------------------------------------
+# The append.
+# ---------------------------------------------------------------------------
+def step_inputs(seed, B, T, nq, nkv, d, n_rows, dev):
+    qkv = (randn(seed, B * T, (nq + 2 * nkv) * d) * 3).to(BF16)
+    q_w, k_w = ((1 + 0.2 * randn(seed + i, d)).to(BF16) for i in (1, 2))
+    ang = torch.arange(n_rows)[:, None] * 10000.0 ** (-torch.arange(0, d, 2) / d)
+    ang = torch.cat((ang, ang), -1)
+    return [t.to(dev) for t in (qkv, q_w, k_w, ang.cos().to(BF16), ang.sin().to(BF16))]
+
+
+def check_appended(cache, old, qkv, k_w, cos, sin, pos, T, eps, nq, nkv, d, group):
+    """The appended slots are the format's of the 64-bit k and of v; every other byte stayed."""
+    B = cache.shape[0]
+    n, s, c = O.unpack(cache, d, group)
+    n0, s0, c0 = (t.clone() for t in O.unpack(old, d, group))
+    cap = min(n.shape[3], cos.shape[0])
+    x = qkv.cpu().view(B, T, nq + 2 * nkv, d)
+    for b in range(B):
+        for t in range(T):
+            p = pos[b] + t
+            if not 0 <= p < cap:
+                continue
+            k = O.norm_rope(x[b, t, nq:nq + nkv], k_w.cpu(), cos[p].cpu(), sin[p].cpu(), eps)
+            _, sk, _ = O.quantise(k, group)
+            got = O.values(n[0, b, :, p], s[0, b, :, p], c[0, b, :, p], group)
+            step = sk.double().repeat_interleave(group, -1)
+            # half a step of an s one bf16 step off (2^-7), 8 s 2^-8 at the ends, and fp32's norm
+            # and rotation (2^-20 of values below 2^4 s)
+            assert ((got - k).abs() <= step * (0.5 + 2.0 ** -7 + 2.0 ** -5 + 2.0 ** -10)).all()
+            assert ((s[0, b, :, p] - sk).abs() <= sk * 2.0 ** -7).all()
+            nv, sv, cv = O.quantise(x[b, t, nq + nkv:], group)
+            assert torch.equal(n[1, b, :, p], nv)
+            assert torch.equal(s[1, b, :, p], sv) and torch.equal(c[1, b, :, p], cv)
+            for a, a0 in ((n, n0), (s, s0), (c, c0)):
+                a0[:, b, :, p] = a[:, b, :, p]
+    assert torch.equal(O.pack(n0, s0, c0), cache.cpu())
+
+
+@pytest.mark.parametrize("d,group", FORMATS)
+@pytest.mark.parametrize("B,T,nq,nkv", [(1, 1, 4, 1), (3, 7, 6, 2), (2, 8, 3, 3)])
+def test_append(dev, d, group, B, T, nq, nkv):
+    nb, eps, n_rows = 3, 1e-6, 90     # the RoPE tables end inside the cache
+    pos = [0, 29, 85][:B] if B > 1 else [63]
+    old = junk((B, nkv, nb, kv4_block_bytes(d, group)), 8)
+    qkv, q_w, k_w, cos, sin = step_inputs(9, B, T, nq, nkv, d, n_rows, dev)
+    cache, q = old.to(dev), torch.full((B * T, nq * d), 7.0, dtype=BF16, device=dev)
+    kv4_append(qkv, q_w, k_w, cos, sin, torch.tensor(pos, dtype=torch.int32, device=dev), q, cache,
+               T, eps, nq, nkv, d)
+    check_appended(cache, old, qkv, k_w, cos, sin, pos, T, eps, nq, nkv, d, group)
+    x, got = qkv.cpu().view(B, T, -1, d)[:, :, :nq], q.cpu().view(B, T, nq, d)
+    for b in range(B):
+        for t in range(T):
+            if pos[b] + t >= n_rows:
+                assert (got[b, t] == 7.0).all()
+                continue
+            want = O.norm_rope(x[b, t], q_w.cpu(), cos[pos[b] + t].cpu(), sin[pos[b] + t].cpu(), eps)
+            # one rounding to bf16, over fp32 sums of terms below 8
+            assert ((got[b, t].double() - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -18).all()
+
+
+# ---------------------------------------------------------------------------
+# Attention.
+# ---------------------------------------------------------------------------
+def check_attention(got, q, cache, lens, T, nq, d, group):
+    want, step, size = O.attention(q, cache, lens, T, nq, d, group)
+    # out's rounding to bf16 (2^-8 of it); p s rounded to bf16 for the matrix product (2^-8 of
+    # the terms p |s (n - 8)|); fp32 scores below 2^6 through exp2 (2^-13 of the terms p |x|)
+    tol = want.abs() * 2.0 ** -8 + step * 2.0 ** -8 + size * 2.0 ** -13 + 1e-30
+    err = (got.cpu().double() - want).abs()
+    assert not got.isnan().any()
+    assert (err <= tol).all(), f"worst {(err / tol).max():.3f} of the bound"
+
+
+def attend(dev, B, T, nq, nkv, d, group, cap, lens, seed=11):
+    cache = filled(B, nkv, cap, d, group, lens, seed).to(dev)
+    q = randn(seed + 5, B * T, nq * d).to(BF16).to(dev)
+    out = torch.full_like(q, math.nan)
+    plan = Kv4Attention(B, T, cap, nq, nkv, d, dev, group=group)
+    ln = torch.tensor(lens, dtype=torch.int32, device=dev)
+    plan.with_lengths(q, cache, ln, out)
+    check_attention(out, q, cache, lens, T, nq, d, group)
+    if min(lens) >= T:   # the same call by position
+        again = torch.full_like(q, math.nan)
+        plan(q, cache, ln - T, again)
+        assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("d,group", FORMATS)
+@pytest.mark.parametrize("n", [0, 1, 2, 7, 31, 32, 33, 64, 100, 257, 1000])
+def test_one_sequence(dev, d, group, n):
+    attend(dev, 1, 1, 8, 2, d, group, max(n, 1), [n])
+
+
+@pytest.mark.parametrize("G", [1, 2, 3, 4, 5, 8, 16, 33, 64])
+@pytest.mark.parametrize("d,group", [(128, 32), (128, 128), (64, 32)])
+def test_head_layouts(dev, G, d, group):
+    attend(dev, 2, 1, 3 * G, 3, d, group, 200, [200, 77])
+
+
+@pytest.mark.parametrize("d,group", FORMATS)
+@pytest.mark.parametrize("T", [2, 3, 4, 5, 7, 8])
+def test_query_tokens(dev, d, group, T):
+    attend(dev, 4, T, 8, 2, d, group, 150, [T, 150, 33, 1])   # a block of rows that see nothing
+
+
+@pytest.mark.parametrize("T,G", [(8, 8), (3, 8), (5, 5), (8, 1), (4, 16), (2, 32)])
+def test_tokens_and_heads(dev, T, G):
+    attend(dev, 2, T, 2 * G, 2, 128, 32, 70, [70, 40])
+    attend(dev, 2, T, 2 * G, 2, 64, 64, 70, [0, 69])
+
+
+@pytest.mark.parametrize("B", [2, 63, 64, 65, 130])
+def test_ragged_batches(dev, B):
+    lens = [(37 * i * i + 11 * i) % 300 for i in range(B)]
+    attend(dev, B, 1, 4, 1, 128, 64, 300, lens)
+
+
+def test_long_sequences(dev):
+    attend(dev, 1, 1, 4, 1, 128, 32, 20000, [19987])
+    attend(dev, 3, 1, 8, 2, 64, 64, 9000, [9000, 1, 4321])
+
+
+def test_lengths_past_the_cache_are_cut(dev):
+    cache = filled(1, 1, 64, 128, 32, [64], 3).to(dev)
+    q = randn(4, 1, 4 * 128).to(BF16).to(dev)
+    plan = Kv4Attention(1, 1, 64, 4, 1, 128, dev)
+    outs = []
+    for n in (64, 1000, 2 ** 31 - 1, -3, -2 ** 31):
+        out = torch.empty_like(q)
+        plan.with_lengths(q, cache, torch.tensor([n], dtype=torch.int32, device=dev), out)
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    assert (outs[3] == 0).all() and (outs[4] == 0).all()
+    out = torch.empty_like(q)   # a position whose sum with T passes 32 bits
+    plan(q, cache, torch.tensor([2 ** 31 - 1], dtype=torch.int32, device=dev), out)
+    assert torch.equal(out, outs[0])
+
+
+def test_a_cache_of_other_strides_and_shared_sequences(dev):
+    B, H, d, group, cap = 3, 2, 128, 32, 100
+    one = filled(1, H, cap, d, group, [cap], 5).to(dev)
+    q = randn(6, B, 8 * d).to(BF16).to(dev)
+    lens = torch.tensor([100, 50, 3], dtype=torch.int32, device=dev)
+    plan = Kv4Attention(B, 1, cap, 8, H, d, dev, group=group)
+    want, got = torch.empty_like(q), torch.empty_like(q)
+    plan.with_lengths(q, one.expand(B, -1, -1, -1).contiguous(), lens, want)
+    plan.with_lengths(q, one.expand(B, -1, -1, -1), lens, got)       # one prefix, three sequences
+    assert torch.equal(want, got)
+    turned = one.expand(B, -1, -1, -1).transpose(0, 1).contiguous().transpose(0, 1)
+    plan.with_lengths(q, turned, lens, got)
+    assert torch.equal(want, got)
+
+
+def test_a_cached_nan_reaches_the_rows_that_see_it(dev):
+    cache = filled(2, 1, 40, 128, 32, [40, 40], 7)
+    n, s, c = O.unpack(cache, 128, 32)
+    s[0, 0, 0, 39, 2] = math.nan       # a key
+    c[1, 1, 0, 38, 1] = math.nan       # a value
+    cache = O.pack(n, s, c).to(dev)
+    q = randn(8, 2 * 2, 4 * 128).to(BF16).to(dev)
+    out = torch.empty_like(q)
+    Kv4Attention(2, 2, 40, 4, 1, 128, dev)(q, cache, torch.tensor([38, 38], dtype=torch.int32,
+                                                                  device=dev), out)
+    assert not out[0].isnan().any() and out[1].isnan().all()
+    bad = out[2:].view(2, 4, 128)
+    assert bad[..., 32:64].isnan().all()
+    assert not bad[..., :32].isnan().any() and not bad[..., 64:].isnan().any()
+
+
+# ---------------------------------------------------------------------------
+# A run of them, as a step uses them.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("d,group", FORMATS)
+@pytest.mark.parametrize("B,T", [(1, 1), (5, 1), (3, 4)])
+def test_prompt_then_steps(dev, d, group, B, T):
+    nq, nkv, cap, eps, S = 8, 2, 96, 1e-6, 30
+    lens = [30, 1, 17, 0, 29][:B]
+    cache = junk((B, nkv, cap // 32, kv4_block_bytes(d, group)), 20).to(dev)
+    k, v = rows(21, B, nkv, S, d).to(dev), rows(22, B, nkv, S, d).to(dev)
+    pos = torch.tensor(lens, dtype=torch.int32, device=dev)
+    kv4_write(k, v, cache, lengths=pos)
+    plan = Kv4Attention(B, T, cap, nq, nkv, d, dev, group=group)
+    for step in range(6):
+        qkv, q_w, k_w, cos, sin = step_inputs(30 + step, B, T, nq, nkv, d, cap, dev)
+        old = cache.cpu()
+        q = torch.empty(B * T, nq * d, dtype=BF16, device=dev)
+        out = torch.empty_like(q)
+        args = (qkv, q_w, k_w, cos, sin, pos)
+        other = cache.clone()
+        kv4_append(*args, q, other, T, eps, nq, nkv, d)
+        if T == 1:
+            plan.decode_qkv(*args, cache, out, eps)
+        else:
+            cache.copy_(other)
+            plan(q, cache, pos, out)
+        at = [n + T * step for n in lens]
+        check_appended(cache, old, qkv, k_w, cos, sin, at, T, eps, nq, nkv, d, group)
+        total = [n + T for n in at]
+        want, mid, size = O.attention(q, cache, total, T, nq, d, group)
+        # check_attention's bound, and for decode_qkv a q that may lie a bf16 step from kv4_append's
+        tol = want.abs() * 2.0 ** -8 + mid * 2.0 ** -8 + size * 2.0 ** -13
+        err = (out.cpu().double() - want).abs()
+        assert (err <= tol + (size * 2.0 ** -7 if T == 1 else 0)).all()
+        pos += T
+
+
+def test_captured_steps_replay(dev):
+    """decode_qkv in a graph: three steps a replay, eager work between the replays, every
+    replay against the same steps made eagerly."""
+    B, nq, nkv, d, group, cap, eps = 2, 8, 2, 128, 32, 128, 1e-6
+    plan, other = (Kv4Attention(B, 1, cap, nq, nkv, d, dev, group=group) for _ in range(2))
+    qkv, q_w, k_w, cos, sin = step_inputs(40, B, 1, nq, nkv, d, cap, dev)
+    start = torch.tensor([5, 40], dtype=torch.int32, device=dev)
+    pos, out, cache = start.clone(), torch.empty(3, B, nq * d, dtype=BF16, device=dev), None
+    cache = filled(B, nkv, cap, d, group, [5, 40], 41).to(dev)
+    first = cache.clone()
+
+    def steps(plan, cache, pos, out):
+        for i in range(3):
+            plan.decode_qkv(qkv, q_w, k_w, cos, sin, pos, cache, out[i], eps)
+            pos.add_(1)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        steps(plan, cache, pos, out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    cache.copy_(first)
+    pos.copy_(start)
+    with torch.cuda.graph(graph):
+        steps(plan, cache, pos, out)
+    cache.copy_(first)
+    pos.copy_(start)
+    e_cache, e_pos, e_out = first.clone(), start.clone(), torch.empty_like(out)
+    for rep in range(4):
+        qkv.copy_(step_inputs(50 + rep, B, 1, nq, nkv, d, cap, dev)[0])
+        steps(other, e_cache, e_pos, e_out)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, e_out) and torch.equal(cache, e_cache) and torch.equal(pos, e_pos)
+
+
+def test_runs_repeat_bit_for_bit(dev):
+    lens = [3000, 17, 801]
+    cache = filled(3, 2, 3000, 128, 32, lens, 60).to(dev)
+    q = randn(61, 3, 8 * 128).to(BF16).to(dev)
+    plan = Kv4Attention(3, 1, 3000, 8, 2, 128, dev)
+    ln = torch.tensor(lens, dtype=torch.int32, device=dev)
+    outs = [torch.empty_like(q) for _ in range(20)]
+    for o in outs:
+        plan.with_lengths(q, cache, ln, o)
+    assert all(torch.equal(o, outs[0]) for o in outs)
