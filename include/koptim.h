@@ -393,10 +393,20 @@ int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void*
 
 /* Decode attention over a 4-bit cache layer: as ko_decode_attn for q [B*T, nq*d] bf16 and out
  * (another buffer), query t of sequence b at position n - T + t of its n = kv_lens[b] + len_offset
- * keys (at most cap). A row that sees no key is zero. nq a multiple of nkv. */
+ * keys (at most cap). A row that sees no key is zero. nq a multiple of nkv, T * nq / nkv <= 64.
+ * The steps of 32 keys of all pairs are cut into equal runs of at least min_run steps, one for
+ * each of the grid workgroups. part: fp32 scratch of part_len >= ko_kv4_attn_scratch(T * nq /
+ * nkv, d, group, grid); counters [grid] int32, zero before the first call, left zero by every
+ * call; calls that share them must not overlap. */
 int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
                 long long cache_h_stride, const int* kv_lens, int len_offset, int cap, int B,
-                int T, int nq, int nkv, int d, int group, float scale, void* out, void* stream);
+                int T, int nq, int nkv, int d, int group, float scale, float* part,
+                long long part_len, int* counters, int grid, int min_run, void* out,
+                void* stream);
+
+/* fp32 elements of ko_kv4_attn's scratch for `rows` query rows a KV head. A size, not a status;
+ * -1 for bad arguments. */
+long long ko_kv4_attn_scratch(int rows, int d, int group, int grid);
 
 #ifdef __cplusplus
 }

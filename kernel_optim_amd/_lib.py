@@ -80,11 +80,13 @@ SIGNATURES = {
                       _c_void_p, _int, _int, _ll, _ll, _f, _int, _int, _int, _int, _int,
                       _c_void_p],
     "ko_kv4_attn": [_c_void_p, _c_void_p, _ll, _ll, _c_void_p, _int, _int, _int, _int, _int, _int,
-                    _int, _int, _f, _c_void_p, _c_void_p],
+                    _int, _int, _f, _c_void_p, _ll, _c_void_p, _int, _int, _c_void_p, _c_void_p],
+    "ko_kv4_attn_scratch": [_int, _int, _int, _int],
 }
 
 # Entry points whose return value is a size, not a status.
-RESTYPES = {"ko_gemv_argmax_scratch": _ll, "ko_decode_attn_qkv_oproj_sync_ints": _ll}
+RESTYPES = {"ko_gemv_argmax_scratch": _ll, "ko_decode_attn_qkv_oproj_sync_ints": _ll,
+            "ko_kv4_attn_scratch": _ll}
 
 _ERRORS = {-22: "invalid argument", -34: "size out of range", -95: "unsupported shape"}
 

@@ -3,126 +3,522 @@
 // Query row (t, h) of sequence b and KV head j, t of T tokens, sees the keys below len - T + t + 1:
 //   score_k = scale sum_g (s_kg sum_{d in g} q_d (n_kd - 8) + c_kg sum_{d in g} q_d)
 //   out_d   = sum_k p_k (c_kg + s_kg (n_kd - 8)) / sum_k p_k,  p_k = exp(score_k - max)
-// A row that sees no key is zero.
+// A row that sees no key is zero. Bound by the bytes of the cache, as long as no more than about
+// three VALU operations fall on a value; so no value is dequantised:
+//
+// - The codes go to the matrix cores as bf16 128 + n: four bits and a constant, one shift and one
+//   bit operation for two values. 16x16x32 products run over d for the scores and over the
+//   keys for the output, 32 keys (one block of the cache) a step.
+// - Scores: A is K (rows = keys), B is q (columns). A group's scale applies to its part of the
+//   sum, so a column is a (query row, group) pair: q with zeros outside the group. GPT groups
+//   share a 16-column tile, 16 / GPT query rows each; one tile holds the 4 heads x 4 groups of
+//   a decode step, and with 16 rows every tile has a group to itself and runs over its d
+//   alone. The tile starts from -136 sum q, so it ends as sum q (n - 8); the lane then adds s
+//   times that and c sum q, and sums over the GPT neighbouring lanes of a row.
+// - The result leaves each lane with 8 consecutive keys of one column, which is the A operand
+//   of the product over keys: p s goes from registers into the matrix cores, no exchange. p s is
+//   rounded to bf16 (2^-9 of each term; the terms add up, their roundings do not); p and sum p c
+//   stay fp32.
+// - Output: B is V, a tile of 16 columns of one group. The offset leaves with the constant -136
+//   in a product of its own, before the codes' product: what accumulates is sum p s (n - 8), as
+//   small as the result, and not 136 sum p s, whose roundings would grow with the length.
+//
+// Work: the steps of all (sequence, KV head) pairs form one list, cut into equal runs, one per
+// workgroup, whatever the lengths; 4 wavefronts take the steps of a run in turn. A pair within
+// one run writes its output; else the workgroup that finishes the pair last merges the
+// partial sums (fp32, in run order: the result does not depend on who is last).
 #include "kv4_core.h"
 
 using namespace ko;
 
 namespace {
 
+constexpr int WAVES = 4;
+constexpr float TAU = 8.0f;            // a running maximum is raised by more than 2^8 only
+constexpr float NEG_BIG = -3.0e38f;
+
 struct Kv4AttnArgs {
   const uint16_t* q;  // [B*T, nq*D]
   const uint8_t* cache;
   long long cb, ch;  // bytes
   const int* lens;
-  int len_off, cap, B, T, nkv, G;
+  int len_off, cap, B, T, nkv, G, min_run;
   float scale_log2;
+  float* part;    // [2 * grid][rows][D], then [2 * grid][rows][2]
+  int* counters;  // [grid], zero; left zero
   uint16_t* out;
 };
 
-// One workgroup per query row; wavefront w takes the blocks w, w + 4, ... Lane (key, half) forms
-// half a score; lane l then owns the columns l and l + 64.
+__device__ __forceinline__ int seq_keys(const Kv4AttnArgs& a, int b) {
+  const long long n = (long long)a.lens[b] + a.len_off;
+  return (int)(n < 0 ? 0 : n < a.cap ? n : a.cap);
+}
+__device__ __forceinline__ int steps_of(int keys) { return keys > 0 ? (keys + 31) >> 5 : 1; }
+
+// Sum over the n neighbouring lanes (1, 2, 4) that hold a row's groups.
+template <int N>
+__device__ __forceinline__ float sum_lanes(float v) {
+  if (N >= 2) v += dpp_f<0xB1>(v);  // quad_perm [1, 0, 3, 2]
+  if (N >= 4) v += dpp_f<0x4E>(v);  // quad_perm [2, 3, 0, 1]
+  return v;
+}
+
+// Two codes from 4 bits of each half of w, shifted to the bottom: bf16 128 + n each.
+__device__ __forceinline__ uint32_t codes2(uint32_t w) { return (w & 0x000f000fu) | 0x43004300u; }
+
+__device__ __forceinline__ f32x4 mfma(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+      __builtin_bit_cast(bf16x8, make_uint4(a[0], a[1], a[2], a[3])),
+      __builtin_bit_cast(bf16x8, make_uint4(b[0], b[1], b[2], b[3])), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ void store2_coherent(float* p, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p),
+                     __builtin_bit_cast(unsigned long long, make_float2(x, y)), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load2_coherent(const float* p) {
+  return __builtin_bit_cast(
+      float2, __hip_atomic_load(reinterpret_cast<unsigned long long*>(const_cast<float*>(p)),
+                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  const u32x2 v = __builtin_nontemporal_load((const __attribute__((address_space(1))) u32x2*)p);
+  return make_uint2(v.x, v.y);
+}
+
+// A block's bytes as one lane holds them.
 template <int D, int NG>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
-  constexpr int HP = D / 64, GS = D / NG;
-  __shared__ float qs[D], ps[4][32], om[4][2], oa[4][D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int row = blockIdx.x;
-  const int h = row % a.G;
-  row /= a.G;
-  const int j = row % a.nkv;
-  row /= a.nkv;
-  const int t = row % a.T, b = row / a.T;
-  const long long qo = ((long long)(b * a.T + t) * a.nkv * a.G + j * a.G + h) * D;
-  if (threadIdx.x < D) qs[threadIdx.x] = bf16_to_f32(a.q[qo + threadIdx.x]);
-  __syncthreads();
-  const long long total = min((long long)a.lens[b] + a.len_off, (long long)a.cap);
-  const int lim = (int)max(total - a.T + t + 1, 0LL);  // keys this row sees
-  const uint8_t* base = a.cache + b * a.cb + j * a.ch;
-  float m = -3.0e38f, l = 0.f, acc[HP] = {};
-  for (int blk = wave; blk * KV4_KEYS < lim; blk += 4) {
-    const uint8_t* p = base + (long long)blk * kv4_block_bytes(D, NG);
-    const uint32_t* ksc = reinterpret_cast<const uint32_t*>(p + 32 * D);
-    const uint32_t* vsc = ksc + 32 * NG;
-    const int key = lane & 31, half = lane >> 5;
-    float s = 0.f;
-    for (int dd = half * (D / 2); dd < (half + 1) * (D / 2); dd += 8) {
-      const int i = dd / 32, kg = dd % 32 / 8;
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(p + key * (D / 2) + kg * (D / 8) + 4 * i);
-      const uint32_t sc = ksc[dd / GS * 32 + key];
-      for (int e = 0; e < 8; ++e) {
-        const int n = (w >> (4 * (e / 2) + 16 * (e & 1))) & 15;
-        s = fmaf(qs[dd + e], fmaf(bf16lo(sc), (float)(n - 8), bf16hi(sc)), s);
+struct Block {
+  uint32_t k[2][D / 32];   // K: keys 8 (r / 4) + r % 4 (+ 4), D / 8 bytes from lane group kg
+  uint32_t v[D / 64][4];   // V: planes, keys 8 kg .. + 7 in pairs
+  uint32_t sc[NG];         // NG of the 64 NG scale dwords
+  __device__ __forceinline__ void load(const uint8_t* p, int r, int kg, int lane) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const uint8_t* kp = p + (8 * (r >> 2) + (r & 3) + 4 * c) * (D / 2) + kg * (D / 8);
+      if constexpr (D == 128) {
+        const uint4 x = ldg16_stream(kp);
+        k[c][0] = x.x, k[c][1] = x.y, k[c][2] = x.z, k[c][3] = x.w;
+      } else {
+        const uint2 x = ldg8(kp);
+        k[c][0] = x.x, k[c][1] = x.y;
       }
     }
-    s = (s + __shfl_xor(s, 32, 64)) * a.scale_log2;
-    if (blk * KV4_KEYS + key >= lim) s = -INFINITY;
-    const float mn = fmaxf(m, wave_max(s));
-    const float al = __builtin_amdgcn_exp2f(m - mn);
-    m = mn;
-    const float pr = __builtin_amdgcn_exp2f(s - m);
-    l = l * al + 0.5f * wave_sum(pr);  // both halves hold every key
-    __builtin_amdgcn_wave_barrier();
-    ps[wave][key] = pr;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int keys = min(lim - blk * KV4_KEYS, KV4_KEYS);
-    for (int c = 0; c < HP; ++c) {
-      const int col = lane + 64 * c;
-      const int jj = 2 * (col / 32) + (col & 1), n = col % 32 / 2;
-      float o = acc[c] * al;
-      for (int k = 0; k < keys; ++k) {
-        const uint8_t* w = p + 16 * D + ((k / 8 * HP + jj / 4) * 16 + n) * 16 + k % 8 * 2;
-        const int code = (*reinterpret_cast<const uint16_t*>(w) >> (4 * (jj & 3))) & 15;
-        const uint32_t sc = vsc[col / GS * 32 + k];
-        o = fmaf(ps[wave][k], fmaf(bf16lo(sc), (float)(code - 8), bf16hi(sc)), o);
-      }
-      acc[c] = o;
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) {
+      const uint4 x = ldg16_stream(p + 16 * D + ((kg * (D / 64) + h) * 16 + r) * 16);
+      v[h][0] = x.x, v[h][1] = x.y, v[h][2] = x.z, v[h][3] = x.w;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    const uint8_t* s = p + 32 * D + 4 * NG * lane;
+    if constexpr (NG == 4) {
+      const uint4 x = ldg16_stream(s);
+      sc[0] = x.x, sc[1] = x.y, sc[2] = x.z, sc[3] = x.w;
+    } else if constexpr (NG == 2) {
+      const uint2 x = ldg8(s);
+      sc[0] = x.x, sc[1] = x.y;
+    } else {
+      sc[0] = *reinterpret_cast<const uint32_t*>(s);
+    }
   }
-  if (lane == 0) om[wave][0] = m, om[wave][1] = l;
-  for (int c = 0; c < HP; ++c) oa[wave][lane + 64 * c] = acc[c];
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float mx = om[0][0], L = 0.f, o = 0.f;
-    for (int w = 1; w < 4; ++w) mx = fmaxf(mx, om[w][0]);
-    for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(om[w][0] - mx);
-      L += f * om[w][1];
-      o += f * oa[w][threadIdx.x];
+  __device__ __forceinline__ void scales_to(uint32_t* lds, int lane) const {
+    if constexpr (NG == 4)
+      reinterpret_cast<uint4*>(lds)[lane] = make_uint4(sc[0], sc[1], sc[2], sc[3]);
+    else if constexpr (NG == 2)
+      reinterpret_cast<uint2*>(lds)[lane] = make_uint2(sc[0], sc[1]);
+    else
+      lds[lane] = sc[0];
+  }
+};
+
+// RB: blocks of 16 query rows (above 1 with GPT = 1): wavefront w serves rows 16 (w % RB) ..,
+// and the steps w / RB, w / RB + 4 / RB, ... of a run.
+template <int D, int NG, int GPT, int RB>
+__global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
+  constexpr int I = D / 32, IPG = I / NG, NT = NG / GPT, RP = 16 / GPT, J = D / 16;
+  constexpr int NWP = WAVES / RB, ROWS = RB * RP;
+  static_assert(GPT == 1 || RB == 1, "more than 16 rows have a tile a group");
+  __shared__ __align__(16) uint32_t lds_sc[WAVES][64 * NG];
+  __shared__ __align__(16) float lds_o[WAVES][RP][D];
+  __shared__ float lds_ml[WAVES][RP][2];
+  __shared__ int lds_prev;
+
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
+  const int rb = wave % RB, wp = wave / RB;
+  const int R = a.T * a.G;
+  const int grid = gridDim.x, wg = blockIdx.x;
+
+  // steps of every sequence: lane b holds sequence b's of the first 64
+  int my_len = 0, my_steps = 0, my_incl = 0, all = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int len = b0 + lane < a.B ? seq_keys(a, b0 + lane) : 0;
+    const int st = b0 + lane < a.B ? steps_of(len) : 0;
+    const int incl = wave_incl_scan(st);
+    all += readlane(incl, 63);
+    if (b0 == 0) my_len = len, my_steps = st, my_incl = incl;
+  }
+  const int total = all * a.nkv;
+  int run = max(a.min_run, (total + grid - 1) / grid);
+  run = (run + NWP - 1) / NWP * NWP;
+  const long long first = (long long)wg * run;
+  if (first >= total) return;
+  const int end = (int)min(first + run, (long long)total);
+
+  const int hh = r / GPT, gg = r % GPT;
+  const int row = min(rb * RP + hh, R - 1);  // rows past R repeat the last; they are not stored
+  const int t = row / a.G, h = row - t * a.G;
+
+  for (int s = (int)first; s < end;) {
+    // the pair of step s: sequence b, KV head, its steps and where they begin in the list
+    int b, len, n, at;
+    if (a.B <= 64) {
+      b = uniform(__popcll(__ballot(my_incl <= s / a.nkv && lane < a.B)));
+      len = readlane(my_len, b);
+      n = readlane(my_steps, b);
+      at = (readlane(my_incl, b) - n) * a.nkv;
+    } else {
+      int below = 0;
+      b = len = n = at = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int l = b0 + lane < a.B ? seq_keys(a, b0 + lane) : 0;
+        const int st = b0 + lane < a.B ? steps_of(l) : 0;
+        const int incl = wave_incl_scan(st) + below;
+        const int k = uniform(__popcll(__ballot(incl <= s / a.nkv && b0 + lane < a.B)));
+        if (k < min(64, a.B - b0)) {
+          b = b0 + k;
+          len = readlane(l, k);
+          n = readlane(st, k);
+          at = (readlane(incl, k) - n) * a.nkv;
+          break;
+        }
+        below = readlane(incl, 63);
+      }
     }
-    a.out[qo + threadIdx.x] = f32_to_bf16(L == 0.f ? 0.f : o / L);
+    const int kvh = (s - at) / n;
+    at += kvh * n;
+    const int st0 = s - at, st1 = min(n, end - at);
+    s = at + st1;
+
+    const uint8_t* base = a.cache + b * a.cb + kvh * a.ch;
+    auto block_at = [&](int st) {
+      return base + (long long)min(st, st1 - 1) * kv4_block_bytes(D, NG);
+    };
+    Block<D, NG> b0, b1;
+    b0.load(block_at(st0 + wp), r, kg, lane);
+    b1.load(block_at(st0 + wp + NWP), r, kg, lane);
+
+    // q: column (row, group): zeros outside the group
+    uint32_t q[I][4];
+    const uint16_t* qp = a.q + (((long long)b * a.T + t) * a.nkv * a.G + kvh * a.G + h) * D;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const uint4 x = ldg16(qp + 32 * i + 8 * kg);
+      const bool mine = i / IPG % GPT == gg;
+      q[i][0] = mine ? x.x : 0u, q[i][1] = mine ? x.y : 0u;
+      q[i][2] = mine ? x.z : 0u, q[i][3] = mine ? x.w : 0u;
+    }
+    float cq[NT];  // sum of q over the group of this lane's column in tile u
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      f32x4 c = {0.f, 0.f, 0.f, 0.f};
+      const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+        if (i / IPG / GPT == u) c = mfma(one, q[i], c);
+      cq[u] = c[0];
+    }
+    const int lim = len - a.T + t + 1;      // keys that this lane's row sees
+    const int full = len - a.T + 1;         // keys that every row sees
+
+    f32x4 acc[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float m = NEG_BIG, l = 0.f, pc[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) pc[u] = 0.f;
+
+    auto step = [&](const Block<D, NG>& x, int st) {
+      uint32_t* lsc = lds_sc[wave];
+      x.scales_to(lsc, lane);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      // ---- scores of keys 8 kg .. + 7 for this lane's row ----
+      float sc[8];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        f32x4 raw[NT];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const float z = -136.f * cq[u];
+          raw[u] = (f32x4){z, z, z, z};
+        }
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+          uint32_t kx[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) kx[e] = codes2(x.k[c][i] >> (4 * e));
+          raw[i / IPG / GPT] = mfma(kx, q[i], raw[i / IPG / GPT]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = 0.f;
+#pragma unroll
+          for (int u = 0; u < NT; ++u) {
+            const uint32_t w = lsc[(u * GPT + gg) * 32 + 8 * kg + 4 * c + e];
+            v += fmaf(bf16lo(w), raw[u][e], bf16hi(w) * cq[u]);
+          }
+          sc[4 * c + e] = sum_lanes<GPT>(v) * a.scale_log2;
+        }
+      }
+      const int k0 = st * KV4_KEYS + 8 * kg;
+      const bool masked = (st + 1) * KV4_KEYS > full;  // uniform
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[e] = k0 + e < lim ? sc[e] : -INFINITY;
+      }
+      float mx = sc[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc[e]);
+      if (__ballot(mx > m + TAU)) {
+        const float mn = fmaxf(m, max_xor32(max_xor16(mx)));
+        const float al = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= al;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) pc[u] *= al;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ar = __shfl(al, 4 * kg + e, 64);  // accumulator row 4 kg + e
+#pragma unroll
+          for (int j = 0; j < J; ++j) acc[j][e] *= ar;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sc[e] = __builtin_amdgcn_exp2f(sc[e] - m);
+        l += sc[e];
+      }
+      // ---- p s, and sum p c ----
+      uint32_t ps[NT][4];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          uint32_t w = lsc[32 * NG + (u * GPT + gg) * 32 + 8 * kg + e];
+          if (masked) w = k0 + e < lim ? w : 0u;  // an unwritten slot's scales may be NaN
+          y[e] = sc[e] * bf16lo(w);
+          pc[u] = fmaf(sc[e], bf16hi(w), pc[u]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ps[u][e] = pack_bf16x2(y[2 * e], y[2 * e + 1]);
+      }
+      // ---- output ----
+      const uint32_t off[4] = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};  // -136
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[j] = mfma(ps[j / 2 / IPG / GPT], off, acc[j]);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        uint32_t vx[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vx[e] = codes2(x.v[j / 4][e] >> (4 * (j % 4)));
+        acc[j] = mfma(ps[j / 2 / IPG / GPT], vx, acc[j]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    };
+
+    for (int st = st0 + wp; st < st1; st += 2 * NWP) {
+      step(b0, st);
+      b0.load(block_at(st + 2 * NWP), r, kg, lane);
+      if (st + NWP >= st1) break;
+      step(b1, st + NWP);
+      b1.load(block_at(st + 3 * NWP), r, kg, lane);
+    }
+
+    // ---- this wavefront's sums to LDS: accumulator row 4 kg + e is column (hh, gg) ----
+    l = sum_xor32(sum_xor16(l));
+    if (kg == 0 && gg == 0) lds_ml[wave][hh][0] = m, lds_ml[wave][hh][1] = l;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const float c = sum_xor32(sum_xor16(pc[u]));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float ce = __shfl(c, 4 * kg + e, 64);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (j / 2 / IPG / GPT == u) acc[j][e] += ce;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < J; j += 2)
+#pragma unroll
+      for (int x = 0; x < 4 / GPT; ++x) {
+        const int e = x * GPT + j / 2 / IPG % GPT;
+        *reinterpret_cast<float2*>(&lds_o[wave][kg * (4 / GPT) + x][16 * j + 2 * r]) =
+            make_float2(acc[j][e], acc[j + 1][e]);
+      }
+    __syncthreads();
+
+    // ---- merge the wavefronts; a whole pair is done, a part goes to the workspace ----
+    const int w0 = at / run, w1 = (at + n - 1) / run;  // the runs that hold the pair
+    const int slot = 2 * wg + (wg == w0 ? 1 : 0);
+    float* po = a.part + (long long)slot * ROWS * D;
+    float* pm = a.part + 2LL * grid * ROWS * D + (long long)slot * ROWS * 2;
+    const long long orow = ((long long)b * a.T * a.nkv + kvh) * a.G;  // + t nkv G + h
+    for (int x = threadIdx.x; x < R * (D / 2); x += 64 * WAVES) {
+      const int rw = x / (D / 2), c2 = x - rw * (D / 2);
+      float M = NEG_BIG, L = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < NWP; ++k) M = fmaxf(M, lds_ml[rw / RP + RB * k][rw % RP][0]);
+#pragma unroll
+      for (int k = 0; k < NWP; ++k) {
+        const int w = rw / RP + RB * k;
+        const float f = __builtin_amdgcn_exp2f(lds_ml[w][rw % RP][0] - M);
+        const float2 o = *reinterpret_cast<const float2*>(&lds_o[w][rw % RP][2 * c2]);
+        L = fmaf(f, lds_ml[w][rw % RP][1], L);
+        o0 = fmaf(f, o.x, o0);
+        o1 = fmaf(f, o.y, o1);
+      }
+      if (w0 == w1) {
+        const int tt = rw / a.G;
+        const long long o = orow + (long long)tt * a.nkv * a.G + (rw - tt * a.G);
+        reinterpret_cast<uint32_t*>(a.out + o * D)[c2] =
+            L == 0.f ? 0u : pack_bf16x2(o0 / L, o1 / L);
+      } else {
+        store2_coherent(po + rw * D + 2 * c2, o0, o1);
+        if (c2 == 0) store2_coherent(pm + rw * 2, M, L);
+      }
+    }
+    if (w0 != w1) {
+      // the stores are performed at the device's coherence point before the run is counted
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      if (threadIdx.x == 0)
+        lds_prev = __hip_atomic_fetch_add(a.counters + w0, 1, __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (lds_prev == w1 - w0) {
+        if (threadIdx.x == 0)
+          __hip_atomic_store(a.counters + w0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // slots of the pair's parts: the first run's second, then every run's first
+        auto slot_of = [&](int k) { return k == 0 ? 2 * w0 + 1 : 2 * (w0 + k); };
+        const int parts = w1 - w0 + 1;
+        const float* ml = a.part + 2LL * grid * ROWS * D;
+        const int c2 = lane & (D / 2 - 1);
+        for (int rw = wave; rw < R; rw += WAVES) {
+          float M = NEG_BIG, L = 0.f, o0 = 0.f, o1 = 0.f;
+          for (int p0 = 0; p0 < parts; p0 += 64) {
+            const int np = min(64, parts - p0);
+            const float2 x = lane < np ? load2_coherent(ml + ((long long)slot_of(p0 + lane) * ROWS + rw) * 2)
+                                       : make_float2(NEG_BIG, 0.f);
+            const float Mn = fmaxf(M, wave_max(x.x));
+            const float old = __builtin_amdgcn_exp2f(M - Mn);
+            const float f = __builtin_amdgcn_exp2f(x.x - Mn);
+            L = fmaf(L, old, wave_sum(f * x.y));
+            o0 *= old;
+            o1 *= old;
+            M = Mn;
+            for (int k0 = 0; k0 < np; k0 += 16) {
+              float2 o[16];
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (k0 + k < np)
+                  o[k] = load2_coherent(a.part + ((long long)slot_of(p0 + k0 + k) * ROWS + rw) * D + 2 * c2);
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (k0 + k < np) {
+                  const float fk = readlane(f, k0 + k);
+                  o0 = fmaf(fk, o[k].x, o0);
+                  o1 = fmaf(fk, o[k].y, o1);
+                }
+            }
+          }
+          const int tt = rw / a.G;
+          const long long o = orow + (long long)tt * a.nkv * a.G + (rw - tt * a.G);
+          if (lane < D / 2)
+            reinterpret_cast<uint32_t*>(a.out + o * D)[c2] =
+                L == 0.f ? 0u : pack_bf16x2(o0 / L, o1 / L);
+        }
+      }
+    }
+    __syncthreads();  // the next pair's sums reuse the LDS
   }
 }
 
+// Query rows a workgroup holds: groups that share a tile (GPT) and blocks of 16 rows (RB).
+int tile_groups(int rows, int ng) {
+  return rows <= 4 && ng == 4 ? 4 : rows <= 8 && ng >= 2 ? 2 : 1;
+}
+int row_blocks(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <int D, int NG>
+int launch(const Kv4AttnArgs& a, int grid, hipStream_t s) {
+  const int rows = a.T * a.G;
+  const dim3 g(grid), blk(64 * WAVES);
+  const int gpt = tile_groups(rows, NG), rb = row_blocks(rows);
+  if constexpr (NG == 4)
+    if (gpt == 4) {
+      hipLaunchKernelGGL((kv4_attn_kernel<D, NG, 4, 1>), g, blk, 0, s, a);
+      return KO_LAUNCH_STATUS();
+    }
+  if constexpr (NG >= 2)
+    if (gpt == 2) {
+      hipLaunchKernelGGL((kv4_attn_kernel<D, NG, 2, 1>), g, blk, 0, s, a);
+      return KO_LAUNCH_STATUS();
+    }
+  if (rb == 1)
+    hipLaunchKernelGGL((kv4_attn_kernel<D, NG, 1, 1>), g, blk, 0, s, a);
+  else if (rb == 2)
+    hipLaunchKernelGGL((kv4_attn_kernel<D, NG, 1, 2>), g, blk, 0, s, a);
+  else
+    hipLaunchKernelGGL((kv4_attn_kernel<D, NG, 1, 4>), g, blk, 0, s, a);
+  return KO_LAUNCH_STATUS();
+}
 
 }  // namespace
 
 extern "C" {
 
+long long ko_kv4_attn_scratch(int rows, int d, int group, int grid) {
+  if (rows < 1 || rows > 64 || !kv4_served(d, group) || grid < 1) return -1;
+  const int held = row_blocks(rows) * 16 / tile_groups(rows, d / group);
+  return 2LL * grid * held * (d + 2);
+}
+
 int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
                 long long cache_h_stride, const int* kv_lens, int len_offset, int cap, int B,
-                int T, int nq, int nkv, int d, int group, float scale, void* out, void* stream) {
-  if (!q || !cache || !kv_lens || !out || B < 1 || T < 1 || nkv < 1 || nq < 1 || cap < 1)
+                int T, int nq, int nkv, int d, int group, float scale, float* part,
+                long long part_len, int* counters, int grid, int min_run, void* out,
+                void* stream) {
+  if (!q || !cache || !kv_lens || !out || !part || !counters || B < 1 || T < 1 || nkv < 1 ||
+      nq < 1 || cap < 1 || grid < 1 || min_run < 1)
     return KO_EINVAL;
-  if (!kv4_served(d, group) || nq % nkv) return KO_ENOTSUP;
+  if (!kv4_served(d, group) || nq % nkv || T > 64 || T * (long long)(nq / nkv) > 64)
+    return KO_ENOTSUP;
   if (!aligned16(q) || !aligned16(cache) || !aligned16(out) || (cache_b_stride & 15) ||
-      (cache_h_stride & 15))
+      (cache_h_stride & 15) || (reinterpret_cast<uintptr_t>(part) & 7))
     return KO_EINVAL;
-  const long long rows = (long long)B * T * nq;
-  if (rows > (1LL << 24) - 1) return KO_ERANGE;
+  const int G = nq / nkv;
+  if (part_len < ko_kv4_attn_scratch(T * G, d, group, grid)) return KO_ERANGE;
+  // the list of steps and the runs are counted in 32 bits
+  const long long blocks = ((long long)cap + 31) / 32;
+  if (grid > (1 << 20) || min_run > (1 << 20) || (long long)B * nkv > (1LL << 30) / blocks)
+    return KO_ERANGE;
   const Kv4AttnArgs a = {static_cast<const uint16_t*>(q), static_cast<const uint8_t*>(cache),
-                         cache_b_stride, cache_h_stride, kv_lens, len_offset, cap, B, T, nkv,
-                         nq / nkv, scale * 1.4426950408889634f, static_cast<uint16_t*>(out)};
-  const dim3 grid((unsigned)rows), block(256);
+                         cache_b_stride, cache_h_stride, kv_lens, len_offset, cap, B, T, nkv, G,
+                         min_run, scale * 1.4426950408889634f, part, counters,
+                         static_cast<uint16_t*>(out)};
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define CALL(D_, NG_) hipLaunchKernelGGL((kv4_attn_kernel<D_, NG_>), grid, block, 0, s, a);
+#define CALL(D_, NG_) return launch<D_, NG_>(a, grid, s);
   KV4_PICK(d, group, CALL)
 #undef CALL
-  return KO_LAUNCH_STATUS();
+  return KO_ENOTSUP;
 }
 
 }  // extern "C"

@@ -176,6 +176,8 @@ class Kv4Attention:
     """
 
     MAX_T = 8
+    GRID = 512     # workgroups: two on each of the 256 CUs
+    MIN_RUN = 8    # least steps of 32 keys in a workgroup's run
 
     def __init__(self, B, T, cap, nq, nkv, d, device, group=32):
         self.block_bytes = kv4_block_bytes(d, group)
@@ -189,6 +191,15 @@ class Kv4Attention:
         self.device = torch.cuda.current_device() if dev.index is None else dev.index
         self.scale = d ** -0.5
         self.blocks = -(-cap // KV4_KEYS)
+        # Workspace: the runs' partial sums, and arrival counters that are zero before the first
+        # call and left zero by every call. Whatever stream that call is on, their fill must be
+        # done: the constructor waits for it, which a capture does not allow.
+        _need(not torch.cuda.is_current_stream_capturing(), "make the object before the capture")
+        self.grid = self.GRID
+        self._part = torch.empty(_lib.lib().ko_kv4_attn_scratch(T * nq // nkv, d, group, self.grid),
+                                 dtype=torch.float32, device=dev)
+        self._counters = torch.zeros(self.grid, dtype=torch.int32, device=dev)
+        torch.cuda.current_stream(dev).synchronize()
         self._q = torch.empty(B, nq * d, dtype=BF16, device=dev) if T == 1 else None
         self._q_shape = torch.Size((B * T, nq * d))
         self._cache_shape = torch.Size((B, nkv, self.blocks, self.block_bytes))
@@ -216,7 +227,8 @@ class Kv4Attention:
         cb, ch, _, _ = cache.stride()
         _lib.call("ko_kv4_attn", q.data_ptr(), cache.data_ptr(), cb, ch, lens.data_ptr(), len_offset,
                   self.cap, self.B, self.T, self.nq, self.nkv, self.d, self.group, self.scale,
-                  out.data_ptr(), _lib.stream_ptr())
+                  self._part.data_ptr(), self._part.numel(), self._counters.data_ptr(), self.grid,
+                  self.MIN_RUN, out.data_ptr(), _lib.stream_ptr())
 
     def __call__(self, q, cache, pos, out):
         """q: [B*T, nq*d] bf16; cache: [B, nkv, blocks, bytes]; pos: [B] int32, the position of a

@@ -84,3 +84,21 @@ def test_c_append_refused(kw, status):
     a = dict(qkv=P, q_w=P, k_w=P, cos=P, sin=P, pos=P, q_out=P, cache=P, M=1, T=1, cb=5120, ch=5120,
              eps=1e-6, nq=4, nkv=1, d=128, group=32, max_pos=32) | kw
     assert _lib.lib().ko_kv4_append(*a.values(), None) == status
+
+
+def test_c_attention_refused():
+    h = _lib.lib()
+    base = dict(q=P, cache=P, cb=5120, ch=5120, lens=P, off=0, cap=32, B=1, T=1, nq=4, nkv=1, d=128,
+                group=32, scale=0.1, part=P, part_len=1 << 30, counters=P, grid=512, min_run=8,
+                out=P)
+    for kw, status in ((dict(q=None), -22), (dict(lens=None), -22), (dict(counters=None), -22),
+                       (dict(T=0), -22), (dict(grid=0), -22), (dict(min_run=0), -22),
+                       (dict(cap=0), -22), (dict(nq=5, nkv=2), -95), (dict(T=8, nq=9), -95),
+                       (dict(d=100), -95), (dict(q=P + 2), -22), (dict(ch=4), -22),
+                       (dict(part_len=100), -34), (dict(grid=1 << 21), -34),
+                       (dict(B=1 << 20, cap=1 << 20), -34)):
+        assert h.ko_kv4_attn(*(base | kw).values(), None) == status, kw
+    assert h.ko_kv4_attn_scratch(4, 128, 32, 512) == 2 * 512 * 4 * 130
+    assert h.ko_kv4_attn_scratch(33, 64, 32, 10) == 2 * 10 * 64 * 66
+    for bad in ((0, 128, 32, 1), (65, 128, 32, 1), (4, 96, 32, 1), (4, 128, 32, 0)):
+        assert h.ko_kv4_attn_scratch(*bad) == -1
