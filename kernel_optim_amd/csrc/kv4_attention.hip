@@ -29,13 +29,15 @@
 // partial sums (fp32, in run order: the result does not depend on who is last).
 #include "kv4_core.h"
 
+#include <type_traits>
+
 using namespace ko;
 
 namespace {
 
 constexpr int WAVES = 4;
 constexpr float TAU = 8.0f;            // a running maximum is raised by more than 2^8 only
-constexpr float NEG_BIG = -3.0e38f;
+constexpr float NEG_BIG = -1.0e30f;
 
 struct Kv4AttnArgs {
   const uint16_t* q;  // [B*T, nq*D]
@@ -55,6 +57,14 @@ __device__ __forceinline__ int seq_keys(const Kv4AttnArgs& a, int b) {
 }
 __device__ __forceinline__ int steps_of(int keys) { return keys > 0 ? (keys + 31) >> 5 : 1; }
 
+// The lane's thread index, opaque: what follows from it is computed where it is used, not
+// ahead of the loop over the pairs, where it would take registers from the steps.
+__device__ __forceinline__ int fresh_tid() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // Sum over the n neighbouring lanes (1, 2, 4) that hold a row's groups.
 template <int N>
 __device__ __forceinline__ float sum_lanes(float v) {
@@ -63,8 +73,16 @@ __device__ __forceinline__ float sum_lanes(float v) {
   return v;
 }
 
-// Two codes from 4 bits of each half of w, shifted to the bottom: bf16 128 + n each.
-__device__ __forceinline__ uint32_t codes2(uint32_t w) { return (w & 0x000f000fu) | 0x43004300u; }
+// Two codes from the 4 bits at k of each half of w: bf16 128 + n each. mask and bias are 0x000f000f
+// and 0x43004300 in registers whose values the compiler does not know: one v_and_or_b32, where
+// two literals would make it two instructions.
+struct Codes {
+  uint32_t mask = 0x000f000fu, bias = 0x43004300u;
+  __device__ __forceinline__ Codes() { asm("" : "+s"(mask), "+v"(bias)); }
+  __device__ __forceinline__ uint32_t operator()(uint32_t w, int k) const {
+    return ((w >> k) & mask) | bias;
+  }
+};
 
 __device__ __forceinline__ f32x4 mfma(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
@@ -95,7 +113,7 @@ struct Block {
   uint32_t k[2][D / 32];   // K: keys 8 (r / 4) + r % 4 (+ 4), D / 8 bytes from lane group kg
   uint32_t v[D / 64][4];   // V: planes, keys 8 kg .. + 7 in pairs
   uint32_t sc[NG];         // NG of the 64 NG scale dwords
-  __device__ __forceinline__ void load(const uint8_t* p, int r, int kg, int lane) {
+  __device__ __forceinline__ void load_k(const uint8_t* p, int r, int kg, int lane) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const uint8_t* kp = p + (8 * (r >> 2) + (r & 3) + 4 * c) * (D / 2) + kg * (D / 8);
@@ -107,11 +125,6 @@ struct Block {
         k[c][0] = x.x, k[c][1] = x.y;
       }
     }
-#pragma unroll
-    for (int h = 0; h < D / 64; ++h) {
-      const uint4 x = ldg16_stream(p + 16 * D + ((kg * (D / 64) + h) * 16 + r) * 16);
-      v[h][0] = x.x, v[h][1] = x.y, v[h][2] = x.z, v[h][3] = x.w;
-    }
     const uint8_t* s = p + 32 * D + 4 * NG * lane;
     if constexpr (NG == 4) {
       const uint4 x = ldg16_stream(s);
@@ -121,6 +134,13 @@ struct Block {
       sc[0] = x.x, sc[1] = x.y;
     } else {
       sc[0] = *reinterpret_cast<const uint32_t*>(s);
+    }
+  }
+  __device__ __forceinline__ void load_v(const uint8_t* p, int r, int kg) {
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) {
+      const uint4 x = ldg16_stream(p + 16 * D + ((kg * (D / 64) + h) * 16 + r) * 16);
+      v[h][0] = x.x, v[h][1] = x.y, v[h][2] = x.z, v[h][3] = x.w;
     }
   }
   __device__ __forceinline__ void scales_to(uint32_t* lds, int lane) const {
@@ -145,16 +165,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   __shared__ float lds_ml[WAVES][RP][2];
   __shared__ int lds_prev;
 
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int rb = wave % RB, wp = wave / RB;
   const int R = a.T * a.G;
+  const Codes codes;
   const int grid = gridDim.x, wg = blockIdx.x;
 
   // steps of every sequence: lane b holds sequence b's of the first 64
   int my_len = 0, my_steps = 0, my_incl = 0, all = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int len = b0 + lane < a.B ? seq_keys(a, b0 + lane) : 0;
-    const int st = b0 + lane < a.B ? steps_of(len) : 0;
+    const int st = b0 + lane < a.B ? max(steps_of(len), a.min_run) : 0;
     const int incl = wave_incl_scan(st);
     all += readlane(incl, 63);
     if (b0 == 0) my_len = len, my_steps = st, my_incl = incl;
@@ -165,10 +186,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   const long long first = (long long)wg * run;
   if (first >= total) return;
   const int end = (int)min(first + run, (long long)total);
-
-  const int hh = r / GPT, gg = r % GPT;
-  const int row = min(rb * RP + hh, R - 1);  // rows past R repeat the last; they are not stored
-  const int t = row / a.G, h = row - t * a.G;
 
   for (int s = (int)first; s < end;) {
     // the pair of step s: sequence b, KV head, its steps and where they begin in the list
@@ -183,7 +200,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       b = len = n = at = 0;
       for (int b0 = 0; b0 < a.B; b0 += 64) {
         const int l = b0 + lane < a.B ? seq_keys(a, b0 + lane) : 0;
-        const int st = b0 + lane < a.B ? steps_of(l) : 0;
+        const int st = b0 + lane < a.B ? max(steps_of(l), a.min_run) : 0;
         const int incl = wave_incl_scan(st) + below;
         const int k = uniform(__popcll(__ballot(incl <= s / a.nkv && b0 + lane < a.B)));
         if (k < min(64, a.B - b0)) {
@@ -198,16 +215,23 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     }
     const int kvh = (s - at) / n;
     at += kvh * n;
-    const int st0 = s - at, st1 = min(n, end - at);
-    s = at + st1;
+    const int st0 = s - at;
+    s = min(at + n, end);
+    n = steps_of(len);  // behind them, a short pair's places in the list are empty
+    const int st1 = min(n, s - at);
+    if (st0 >= st1) continue;
 
+    const int lane = fresh_tid() & 63, r = lane & 15, kg = lane >> 4;
+    const int hh = r / GPT, gg = r % GPT;
+    const int row = min(rb * RP + hh, R - 1);  // rows past R repeat the last; they are not stored
+    const int t = row / a.G, h = row - t * a.G;
     const uint8_t* base = a.cache + b * a.cb + kvh * a.ch;
     auto block_at = [&](int st) {
       return base + (long long)min(st, st1 - 1) * kv4_block_bytes(D, NG);
     };
-    Block<D, NG> b0, b1;
-    b0.load(block_at(st0 + wp), r, kg, lane);
-    b1.load(block_at(st0 + wp + NWP), r, kg, lane);
+    Block<D, NG> x;
+    x.load_k(block_at(st0 + wp), r, kg, lane);
+    x.load_v(block_at(st0 + wp), r, kg);
 
     // q: column (row, group): zeros outside the group
     uint32_t q[I][4];
@@ -229,6 +253,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
         if (i / IPG / GPT == u) c = mfma(one, q[i], c);
       cq[u] = c[0];
     }
+    const float tau = TAU / a.scale_log2;
     const int lim = len - a.T + t + 1;      // keys that this lane's row sees
     const int full = len - a.T + 1;         // keys that every row sees
 
@@ -239,7 +264,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
 #pragma unroll
     for (int u = 0; u < NT; ++u) pc[u] = 0.f;
 
-    auto step = [&](const Block<D, NG>& x, int st) {
+    // The running maximum m is kept in units of the unscaled scores.
+    auto step = [&](int st, auto masked_) {
+      constexpr bool masked = decltype(masked_)::value;
       uint32_t* lsc = lds_sc[wave];
       x.scales_to(lsc, lane);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -259,32 +286,34 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
         for (int i = 0; i < I; ++i) {
           uint32_t kx[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) kx[e] = codes2(x.k[c][i] >> (4 * e));
+          for (int e = 0; e < 4; ++e) kx[e] = codes(x.k[c][i], 4 * e);
           raw[i / IPG / GPT] = mfma(kx, q[i], raw[i / IPG / GPT]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = 0.f;
+          float v;
 #pragma unroll
           for (int u = 0; u < NT; ++u) {
             const uint32_t w = lsc[(u * GPT + gg) * 32 + 8 * kg + 4 * c + e];
-            v += fmaf(bf16lo(w), raw[u][e], bf16hi(w) * cq[u]);
+            const float z = bf16hi(w) * cq[u];
+            v = fmaf(bf16lo(w), raw[u][e], u == 0 ? z : v + z);
           }
-          sc[4 * c + e] = sum_lanes<GPT>(v) * a.scale_log2;
+          sc[4 * c + e] = sum_lanes<GPT>(v);
         }
       }
+      const uint8_t* next = block_at(st + NWP);
+      x.load_k(next, r, kg, lane);
       const int k0 = st * KV4_KEYS + 8 * kg;
-      const bool masked = (st + 1) * KV4_KEYS > full;  // uniform
-      if (masked) {
+      if constexpr (masked) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sc[e] = k0 + e < lim ? sc[e] : -INFINITY;
       }
       float mx = sc[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc[e]);
-      if (__ballot(mx > m + TAU)) {
+      if (__ballot(mx > m + tau)) {
         const float mn = fmaxf(m, max_xor32(max_xor16(mx)));
-        const float al = __builtin_amdgcn_exp2f(m - mn);
+        const float al = __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
         m = mn;
         l *= al;
 #pragma unroll
@@ -296,9 +325,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
           for (int j = 0; j < J; ++j) acc[j][e] *= ar;
         }
       }
+      const float mz = -m * a.scale_log2;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        sc[e] = __builtin_amdgcn_exp2f(sc[e] - m);
+        sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale_log2, mz));
         l += sc[e];
       }
       // ---- p s, and sum p c ----
@@ -309,7 +339,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           uint32_t w = lsc[32 * NG + (u * GPT + gg) * 32 + 8 * kg + e];
-          if (masked) w = k0 + e < lim ? w : 0u;  // an unwritten slot's scales may be NaN
+          if constexpr (masked) w = k0 + e < lim ? w : 0u;  // an unwritten slot's scales may be NaN
           y[e] = sc[e] * bf16lo(w);
           pc[u] = fmaf(sc[e], bf16hi(w), pc[u]);
         }
@@ -324,30 +354,32 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       for (int j = 0; j < J; ++j) {
         uint32_t vx[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) vx[e] = codes2(x.v[j / 4][e] >> (4 * (j % 4)));
+        for (int e = 0; e < 4; ++e) vx[e] = codes(x.v[j / 4][e], 4 * (j % 4));
         acc[j] = mfma(ps[j / 2 / IPG / GPT], vx, acc[j]);
       }
+      x.load_v(next, r, kg);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
     };
 
-    for (int st = st0 + wp; st < st1; st += 2 * NWP) {
-      step(b0, st);
-      b0.load(block_at(st + 2 * NWP), r, kg, lane);
-      if (st + NWP >= st1) break;
-      step(b1, st + NWP);
-      b1.load(block_at(st + 3 * NWP), r, kg, lane);
-    }
+    int st = st0 + wp;
+    for (const int unmasked = min(st1, max(full, 0) >> 5); st < unmasked; st += NWP)
+      step(st, std::false_type{});
+    for (; st < st1; st += NWP) step(st, std::true_type{});
 
     // ---- this wavefront's sums to LDS: accumulator row 4 kg + e is column (hh, gg) ----
+    const int tid = fresh_tid(), el = tid & 63, er = el & 15, ek = el >> 4;
     l = sum_xor32(sum_xor16(l));
-    if (kg == 0 && gg == 0) lds_ml[wave][hh][0] = m, lds_ml[wave][hh][1] = l;
+    if (el < 16 && er % GPT == 0) {
+      lds_ml[wave][er / GPT][0] = m;
+      lds_ml[wave][er / GPT][1] = l;
+    }
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       const float c = sum_xor32(sum_xor16(pc[u]));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float ce = __shfl(c, 4 * kg + e, 64);
+        const float ce = __shfl(c, 4 * ek + e, 64);
 #pragma unroll
         for (int j = 0; j < J; ++j)
           if (j / 2 / IPG / GPT == u) acc[j][e] += ce;
@@ -358,7 +390,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
 #pragma unroll
       for (int x = 0; x < 4 / GPT; ++x) {
         const int e = x * GPT + j / 2 / IPG % GPT;
-        *reinterpret_cast<float2*>(&lds_o[wave][kg * (4 / GPT) + x][16 * j + 2 * r]) =
+        *reinterpret_cast<float2*>(&lds_o[wave][ek * (4 / GPT) + x][16 * j + 2 * er]) =
             make_float2(acc[j][e], acc[j + 1][e]);
       }
     __syncthreads();
@@ -369,7 +401,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     float* po = a.part + (long long)slot * ROWS * D;
     float* pm = a.part + 2LL * grid * ROWS * D + (long long)slot * ROWS * 2;
     const long long orow = ((long long)b * a.T * a.nkv + kvh) * a.G;  // + t nkv G + h
-    for (int x = threadIdx.x; x < R * (D / 2); x += 64 * WAVES) {
+    for (int x = tid; x < R * (D / 2); x += 64 * WAVES) {
       const int rw = x / (D / 2), c2 = x - rw * (D / 2);
       float M = NEG_BIG, L = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll
@@ -377,7 +409,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
 #pragma unroll
       for (int k = 0; k < NWP; ++k) {
         const int w = rw / RP + RB * k;
-        const float f = __builtin_amdgcn_exp2f(lds_ml[w][rw % RP][0] - M);
+        const float f = __builtin_amdgcn_exp2f((lds_ml[w][rw % RP][0] - M) * a.scale_log2);
         const float2 o = *reinterpret_cast<const float2*>(&lds_o[w][rw % RP][2 * c2]);
         L = fmaf(f, lds_ml[w][rw % RP][1], L);
         o0 = fmaf(f, o.x, o0);
@@ -397,51 +429,79 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       // the stores are performed at the device's coherence point before the run is counted
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
-      if (threadIdx.x == 0)
+      if (tid == 0)
         lds_prev = __hip_atomic_fetch_add(a.counters + w0, 1, __ATOMIC_RELAXED,
                                           __HIP_MEMORY_SCOPE_AGENT);
       __syncthreads();
       if (lds_prev == w1 - w0) {
-        if (threadIdx.x == 0)
+        if (tid == 0)
           __hip_atomic_store(a.counters + w0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         // slots of the pair's parts: the first run's second, then every run's first
         auto slot_of = [&](int k) { return k == 0 ? 2 * w0 + 1 : 2 * (w0 + k); };
         const int parts = w1 - w0 + 1;
         const float* ml = a.part + 2LL * grid * ROWS * D;
-        const int c2 = lane & (D / 2 - 1);
-        for (int rw = wave; rw < R; rw += WAVES) {
-          float M = NEG_BIG, L = 0.f, o0 = 0.f, o1 = 0.f;
+        const int c2 = el & (D / 2 - 1);
+        // KR rows a wavefront and PB parts at a time: 32 loads in flight, the first of them
+        // with the loads of (m, l)
+        constexpr int KR = ROWS >= 16 ? 4 : ROWS / 4, PB = 32 / KR;
+        for (int rw0 = wave; rw0 < R; rw0 += WAVES * KR) {
+          float M[KR], L[KR], o0[KR], o1[KR], f[KR];
+          int rw[KR];
+#pragma unroll
+          for (int k = 0; k < KR; ++k) {
+            rw[k] = min(rw0 + WAVES * k, R - 1);
+            M[k] = NEG_BIG, L[k] = o0[k] = o1[k] = 0.f;
+          }
           for (int p0 = 0; p0 < parts; p0 += 64) {
             const int np = min(64, parts - p0);
-            const float2 x = lane < np ? load2_coherent(ml + ((long long)slot_of(p0 + lane) * ROWS + rw) * 2)
-                                       : make_float2(NEG_BIG, 0.f);
-            const float Mn = fmaxf(M, wave_max(x.x));
-            const float old = __builtin_amdgcn_exp2f(M - Mn);
-            const float f = __builtin_amdgcn_exp2f(x.x - Mn);
-            L = fmaf(L, old, wave_sum(f * x.y));
-            o0 *= old;
-            o1 *= old;
-            M = Mn;
-            for (int k0 = 0; k0 < np; k0 += 16) {
-              float2 o[16];
+            float2 x[KR];
 #pragma unroll
-              for (int k = 0; k < 16; ++k)
-                if (k0 + k < np)
-                  o[k] = load2_coherent(a.part + ((long long)slot_of(p0 + k0 + k) * ROWS + rw) * D + 2 * c2);
+            for (int k = 0; k < KR; ++k)
+              x[k] = el < np ? load2_coherent(ml + ((long long)slot_of(p0 + el) * ROWS + rw[k]) * 2)
+                             : make_float2(NEG_BIG, 0.f);
+            for (int q0 = 0; q0 < np; q0 += PB) {
+              float2 o[KR][PB];
 #pragma unroll
-              for (int k = 0; k < 16; ++k)
-                if (k0 + k < np) {
-                  const float fk = readlane(f, k0 + k);
-                  o0 = fmaf(fk, o[k].x, o0);
-                  o1 = fmaf(fk, o[k].y, o1);
+              for (int q = 0; q < PB; ++q) {
+                // past the last part its loads are repeated: no branch between the loads,
+                // which would make each wait for the one before
+                const int part = min(p0 + q0 + q, parts - 1);
+                const float* src = a.part + (long long)slot_of(part) * ROWS * D + 2 * c2;
+#pragma unroll
+                for (int k = 0; k < KR; ++k) o[k][q] = load2_coherent(src + rw[k] * D);
+              }
+              if (q0 == 0) {
+#pragma unroll
+                for (int k = 0; k < KR; ++k) {
+                  const float Mn = fmaxf(M[k], wave_max(x[k].x));
+                  const float old = __builtin_amdgcn_exp2f((M[k] - Mn) * a.scale_log2);
+                  f[k] = __builtin_amdgcn_exp2f((x[k].x - Mn) * a.scale_log2);
+                  L[k] = fmaf(L[k], old, wave_sum(f[k] * x[k].y));
+                  o0[k] *= old;
+                  o1[k] *= old;
+                  M[k] = Mn;
+                }
+              }
+#pragma unroll
+              for (int q = 0; q < PB; ++q)
+                if (q0 + q < np) {
+#pragma unroll
+                  for (int k = 0; k < KR; ++k) {
+                    const float fq = readlane(f[k], q0 + q);
+                    o0[k] = fmaf(fq, o[k][q].x, o0[k]);
+                    o1[k] = fmaf(fq, o[k][q].y, o1[k]);
+                  }
                 }
             }
           }
-          const int tt = rw / a.G;
-          const long long o = orow + (long long)tt * a.nkv * a.G + (rw - tt * a.G);
-          if (lane < D / 2)
-            reinterpret_cast<uint32_t*>(a.out + o * D)[c2] =
-                L == 0.f ? 0u : pack_bf16x2(o0 / L, o1 / L);
+#pragma unroll
+          for (int k = 0; k < KR; ++k) {
+            const int tt = rw[k] / a.G;
+            const long long o = orow + (long long)tt * a.nkv * a.G + (rw[k] - tt * a.G);
+            if (el < D / 2 && rw0 + WAVES * k < R)
+              reinterpret_cast<uint32_t*>(a.out + o * D)[c2] =
+                  L[k] == 0.f ? 0u : pack_bf16x2(o0[k] / L[k], o1[k] / L[k]);
+          }
         }
       }
     }
@@ -499,6 +559,7 @@ int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
   if (!q || !cache || !kv_lens || !out || !part || !counters || B < 1 || T < 1 || nkv < 1 ||
       nq < 1 || cap < 1 || grid < 1 || min_run < 1)
     return KO_EINVAL;
+  if (!(scale > 0.f && scale < 1.0e4f)) return KO_EINVAL;
   if (!kv4_served(d, group) || nq % nkv || T > 64 || T * (long long)(nq / nkv) > 64)
     return KO_ENOTSUP;
   if (!aligned16(q) || !aligned16(cache) || !aligned16(out) || (cache_b_stride & 15) ||
@@ -508,7 +569,8 @@ int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
   if (part_len < ko_kv4_attn_scratch(T * G, d, group, grid)) return KO_ERANGE;
   // the list of steps and the runs are counted in 32 bits
   const long long blocks = ((long long)cap + 31) / 32;
-  if (grid > (1 << 20) || min_run > (1 << 20) || (long long)B * nkv > (1LL << 30) / blocks)
+  if (grid > (1 << 20) || min_run > (1 << 20) ||
+      (long long)B * nkv > (1LL << 30) / (blocks > min_run ? blocks : min_run))
     return KO_ERANGE;
   const Kv4AttnArgs a = {static_cast<const uint16_t*>(q), static_cast<const uint8_t*>(cache),
                          cache_b_stride, cache_h_stride, kv_lens, len_offset, cap, B, T, nkv, G,
