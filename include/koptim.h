@@ -404,6 +404,19 @@ int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
                 long long part_len, int* counters, int grid, int min_run, void* out,
                 void* stream);
 
+/* A decode step's attention straight from the bf16 QKV projection qkv [B, (nq+2nkv)*d] (T = 1):
+ * q/k RMSNorm and RoPE at pos[b] in fp32 (q then rounded to bf16), the quantised append of k and v at
+ * slot pos[b], and attention over keys 0..pos[b], in one launch. A sequence whose position lies
+ * outside [0, min(cap, max_pos)) appends nothing and its out row is zero. rope (optional, [B][2][d]
+ * bf16, 16-byte aligned): the cos and sin rows at pos[b] (ko_rope_rows) in place of the tables'.
+ * Other arguments as for ko_kv4_attn. */
+int ko_kv4_attn_qkv(const void* qkv, const void* q_w, const void* k_w, const void* cos,
+                    const void* sin, int max_pos, const int* pos, void* cache,
+                    long long cache_b_stride, long long cache_h_stride, int cap, int B, int nq,
+                    int nkv, int d, int group, float eps, float scale, float* part,
+                    long long part_len, int* counters, int grid, int min_run, void* out,
+                    const void* rope, void* stream);
+
 /* fp32 elements of ko_kv4_attn's scratch for `rows` query rows a KV head. A size, not a status;
  * -1 for bad arguments. */
 long long ko_kv4_attn_scratch(int rows, int d, int group, int grid);

@@ -95,8 +95,8 @@ def _outer(t):
     return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(t.dim() - 1)]
 
 
-def _rows(cache, k, v, start, lengths, written, names):
-    """What kv4_write and kv4_read check alike; the C arguments of each."""
+def _check_rows(cache, k, v, start, lengths, written, names):
+    """What kv4_write and kv4_read check alike, naming what is wrong."""
     B, nkv, nb, d, group, dev = _check_cache(cache, written)
     _here(dev)
     for t, name in ((k, names[0]), (v, names[1])):
@@ -109,10 +109,42 @@ def _rows(cache, k, v, start, lengths, written, names):
     for t, name in ((start, "start"), (lengths, "lengths")):
         if t is not None:
             _tensor(t, name, torch.int32, (B,), dev)
+
+
+def _ints(t, B, dev):
+    return t is None or (_is(t, torch.int32, (B,)) and t.get_device() == dev)
+
+
+def _rows(cache, k, v, start, lengths, written, names):
+    """The checked C arguments of kv4_write and kv4_read. One test over everything passes the
+    usual call (a prompt of one token costs more in checks that could name each fault, 25 us,
+    than on the GPU); where it does not, _check_rows decides."""
+    if not (isinstance(cache, torch.Tensor) and isinstance(k, torch.Tensor)
+            and isinstance(v, torch.Tensor) and cache.dim() == 4 and k.dim() == 4
+            and cache.shape[3] in _FORMATS):
+        _check_rows(cache, k, v, start, lengths, written, names)
+    B, nkv, nb, size = cache.shape
+    d, group = _FORMATS[size]
     S = k.shape[2]
-    c = (cache.data_ptr(), *_outer(cache)[:2])
-    kv = (k.data_ptr(), *_outer(k), v.data_ptr(), *_outer(v))
-    rest = (_lib.ptr(start), _lib.ptr(lengths), B, S, nkv, nb * KV4_KEYS, d, group)
+    dev = cache.get_device()
+    k0, k1, k2, k3 = k.stride()
+    v0, v1, v2, v3 = v.stride() if v.dim() == 4 else (0, 0, 0, 0)
+    if not (cache.is_cuda and k.is_cuda and v.is_cuda and cache.dtype is torch.uint8
+            and k.dtype is BF16 and v.dtype is BF16 and cache.is_contiguous() and B and nkv and nb
+            and k.shape == v.shape == (B, nkv, S, d) and k3 == 1 and v3 == 1
+            and (k0 | k1 | k2 | v0 | v1 | v2) % 8 == 0
+            and (written or (k.is_contiguous() and v.is_contiguous()))
+            and (cache.data_ptr() | k.data_ptr() | v.data_ptr()) % 16 == 0
+            and dev == k.get_device() == v.get_device() == torch.cuda.current_device()
+            and _ints(start, B, dev) and _ints(lengths, B, dev)):
+        _check_rows(cache, k, v, start, lengths, written, names)
+    c0, c1, _, _ = cache.stride()
+    if c0 % 16 or c1 % 16 or (k0 | k1 | k2 | v0 | v1 | v2) % 8:   # strides of single rows
+        c0, c1, _ = _outer(cache)
+        (k0, k1, k2), (v0, v1, v2) = _outer(k), _outer(v)
+    c = cache.data_ptr(), c0, c1
+    kv = k.data_ptr(), k0, k1, k2, v.data_ptr(), v0, v1, v2
+    rest = _lib.ptr(start), _lib.ptr(lengths), B, S, nkv, nb * KV4_KEYS, d, group
     return S, c, kv, rest
 
 
@@ -138,6 +170,15 @@ def kv4_read(cache, k_out, v_out, start=None, lengths=None):
 
 
 def _check_qkv(qkv, q_w, k_w, cos, sin, pos, rows, B, nq, nkv, d, dev):
+    if (_is(qkv, BF16, (rows, (nq + 2 * nkv) * d)) and _is(q_w, BF16, (d,)) and _is(k_w, BF16, (d,))
+            and _is(pos, torch.int32, (B,)) and isinstance(cos, torch.Tensor) and cos.dim() == 2
+            and cos.shape[0] and _is(cos, BF16, (cos.shape[0], d)) and isinstance(sin, torch.Tensor)
+            and sin.dim() == 2 and sin.shape[0] and _is(sin, BF16, (sin.shape[0], d))
+            and dev == qkv.get_device() == q_w.get_device() == k_w.get_device()
+            == cos.get_device() == sin.get_device() == pos.get_device()
+            and (qkv.data_ptr() | q_w.data_ptr() | k_w.data_ptr() | cos.data_ptr()
+                 | sin.data_ptr()) % 16 == 0):
+        return
     _tensor(qkv, "qkv", BF16, (rows, (nq + 2 * nkv) * d), dev)
     _tensor(q_w, "q_w", BF16, (d,), dev)
     _tensor(k_w, "k_w", BF16, (d,), dev)
@@ -154,13 +195,25 @@ def kv4_append(qkv, q_w, k_w, cos, sin, pos, q_out, cache, T, eps, nq, nkv, d):
     the cache's slot at that position with v, both quantised. Everything is fp32 up to the one
     rounding of q and the quantisation of k. Positions outside the cache or the RoPE tables
     [rows, d] are skipped (their q_out rows too)."""
-    B, ck, nb, cd, group, dev = _check_cache(cache, True)
-    _here(dev)
+    if not (isinstance(cache, torch.Tensor) and cache.is_cuda and cache.dtype is torch.uint8
+            and cache.dim() == 4 and cache.shape[3] in _FORMATS and cache.is_contiguous()
+            and cache.numel() and cache.data_ptr() % 16 == 0):
+        _check_cache(cache, True)
+    B, ck, nb, size = cache.shape
+    cd, group = _FORMATS[size]
+    dev = cache.get_device()
+    if dev != torch.cuda.current_device():
+        _here(dev)
     _need(T >= 1 and nq >= 1, "T and nq must be positive")
-    _need((ck, cd) == (nkv, d), f"cache has {ck} heads of {cd}, not {nkv} of {d}")
+    if (ck, cd) != (nkv, d):
+        raise ValueError(f"cache has {ck} heads of {cd}, not {nkv} of {d}")
     _check_qkv(qkv, q_w, k_w, cos, sin, pos, B * T, B, nq, nkv, d, dev)
-    _tensor(q_out, "q_out", BF16, (B * T, nq * d), dev)
-    cb, ch, _ = _outer(cache)
+    if not (_is(q_out, BF16, (B * T, nq * d)) and q_out.get_device() == dev
+            and q_out.data_ptr() % 16 == 0):
+        _tensor(q_out, "q_out", BF16, (B * T, nq * d), dev)
+    cb, ch, _, _ = cache.stride()
+    if cb % 16 or ch % 16:   # strides of single rows
+        cb, ch, _ = _outer(cache)
     _lib.call("ko_kv4_append", qkv.data_ptr(), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
               sin.data_ptr(), pos.data_ptr(), q_out.data_ptr(), cache.data_ptr(), B * T, T, cb, ch,
               eps, nq, nkv, d, group, min(nb * KV4_KEYS, cos.shape[0], sin.shape[0]),
@@ -200,7 +253,6 @@ class Kv4Attention:
                                  dtype=torch.float32, device=dev)
         self._counters = torch.zeros(self.grid, dtype=torch.int32, device=dev)
         torch.cuda.current_stream(dev).synchronize()
-        self._q = torch.empty(B, nq * d, dtype=BF16, device=dev) if T == 1 else None
         self._q_shape = torch.Size((B * T, nq * d))
         self._cache_shape = torch.Size((B, nkv, self.blocks, self.block_bytes))
         self._len_shape = torch.Size((B,))
@@ -222,9 +274,12 @@ class Kv4Attention:
             _tensor(out, "out", BF16, self._q_shape, self.device)
             _tensor(lens, "pos/lengths", torch.int32, self._len_shape, self.device)
             self._check_cache(cache)
-        _here(self.device)
+        if self.device != torch.cuda.current_device():
+            _here(self.device)
         _need(q.data_ptr() != out.data_ptr(), "out must not be q")
         cb, ch, _, _ = cache.stride()
+        if cb % 16 or ch % 16:   # strides of single rows
+            cb, ch, _ = _outer(cache)
         _lib.call("ko_kv4_attn", q.data_ptr(), cache.data_ptr(), cb, ch, lens.data_ptr(), len_offset,
                   self.cap, self.B, self.T, self.nq, self.nkv, self.d, self.group, self.scale,
                   self._part.data_ptr(), self._part.numel(), self._counters.data_ptr(), self.grid,
@@ -241,10 +296,30 @@ class Kv4Attention:
         T positions. Rows in front of the first key (lengths[b] < T) are zero."""
         self._run(q, cache, lengths, 0, out)
 
-    def decode_qkv(self, qkv, q_w, k_w, cos, sin, pos, cache, out, eps):
+    def decode_qkv(self, qkv, q_w, k_w, cos, sin, pos, cache, out, eps, rope=None):
         """A decode step's attention (T = 1) straight from the bf16 QKV projection [B, (nq+2nkv)*d]:
-        kv4_append at pos[b], then attention over keys 0..pos[b] with q kept in bf16."""
+        kv4_append at pos[b] and attention over keys 0..pos[b] in one launch. A sequence whose
+        position lies outside the cache or the RoPE tables appends nothing and its row of
+        out is zero. rope ([B, 2, d] bf16, optional): the cos and sin rows at pos[b], as
+        fused.rope_rows writes them."""
         _need(self.T == 1, "decode_qkv serves one decode token per sequence")
-        self._check_cache(cache, True)
-        kv4_append(qkv, q_w, k_w, cos, sin, pos, self._q, cache, 1, eps, self.nq, self.nkv, self.d)
-        self._run(self._q, cache, pos, 1, out)
+        B, nq, nkv, d, dev = self.B, self.nq, self.nkv, self.d, self.device
+        if not (isinstance(cache, torch.Tensor) and cache.dtype is torch.uint8
+                and cache.shape == self._cache_shape and cache.get_device() == dev
+                and cache.is_contiguous() and _is(out, BF16, self._q_shape)
+                and out.get_device() == dev == torch.cuda.current_device()
+                and (cache.data_ptr() | out.data_ptr()) % 16 == 0):
+            self._check_cache(cache, True)
+            _tensor(out, "out", BF16, self._q_shape, dev)
+            _here(dev)
+        _check_qkv(qkv, q_w, k_w, cos, sin, pos, B, B, nq, nkv, d, dev)
+        if rope is not None:
+            _tensor(rope, "rope", BF16, (B, 2, d), dev)
+        cb, ch, _, _ = cache.stride()
+        if cb % 16 or ch % 16:   # strides of single rows
+            cb, ch, _ = _outer(cache)
+        _lib.call("ko_kv4_attn_qkv", qkv.data_ptr(), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
+                  sin.data_ptr(), min(cos.shape[0], sin.shape[0]), pos.data_ptr(), cache.data_ptr(),
+                  cb, ch, self.cap, B, nq, nkv, d, self.group, eps, self.scale,
+                  self._part.data_ptr(), self._part.numel(), self._counters.data_ptr(), self.grid,
+                  self.MIN_RUN, out.data_ptr(), _lib.ptr(rope), _lib.stream_ptr())

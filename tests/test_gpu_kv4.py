@@ -8,6 +8,7 @@ import torch
 
 from kernel_optim_amd.kernels.kv4 import (KV4_KEYS, Kv4Attention, kv4_append, kv4_block_bytes,
                                           kv4_cache, kv4_read, kv4_write)
+from kernel_optim_amd.kernels.fused import rope_rows
 from oracle import kv4 as O
 
 pytestmark = pytest.mark.gpu
@@ -346,6 +347,40 @@ def test_prompt_then_steps(dev, d, group, B, T):
         err = (out.cpu().double() - want).abs()
         assert (err <= tol + (size * 2.0 ** -7 if T == 1 else 0)).all()
         pos += T
+
+
+@pytest.mark.parametrize("d,group", FORMATS)
+@pytest.mark.parametrize("nq,nkv", [(3, 3), (8, 1), (40, 2)])
+def test_decode_qkv_head_layouts_and_positions(dev, d, group, nq, nkv):
+    """1, 8 and 20 query heads a KV head; positions at a block's and the cache's ends, and outside
+    the cache and the tables; the RoPE rows from the tables and as rows."""
+    pos = [0, 31, 32, 63, 95, 96, -1, 2 ** 31 - 1, 70, 64]
+    B, cap, n_rows, eps = len(pos), 96, 70, 1e-6
+    plan = Kv4Attention(B, 1, cap, nq, nkv, d, dev, group=group)
+    lens = [min(max(p, 0), cap) for p in pos]
+    old = filled(B, nkv, cap, d, group, lens, 70)
+    qkv, q_w, k_w, cos, sin = step_inputs(71, B, 1, nq, nkv, d, n_rows, dev)
+    at = torch.tensor(pos, dtype=torch.int32, device=dev)
+    cache, out = old.to(dev), torch.full((B, nq * d), math.nan, dtype=BF16, device=dev)
+    plan.decode_qkv(qkv, q_w, k_w, cos, sin, at, cache, out, eps)
+    check_appended(cache, old, qkv, k_w, cos, sin, pos, 1, eps, nq, nkv, d, group)
+    fine = [0 <= p < n_rows for p in pos]
+    x = qkv.cpu().view(B, -1, d)[:, :nq]
+    for b, ok in enumerate(fine):
+        if not ok:
+            assert (out[b] == 0).all()
+            continue
+        q = O.norm_rope(x[b], q_w.cpu(), cos[pos[b]].cpu(), sin[pos[b]].cpu(), eps)
+        want, mid, size = O.attention(q.to(BF16).view(1, -1), cache[b:b + 1], [pos[b] + 1], 1, nq, d,
+                                      group)
+        # check_attention's bound; a few of q's values may lie a bf16 step off
+        tol = want.abs() * 2.0 ** -8 + mid * 2.0 ** -8 + size * (2.0 ** -13 + 2.0 ** -7)
+        assert ((out[b].cpu().double() - want).abs() <= tol).all()
+    rope = torch.zeros(B, 2, d, dtype=BF16, device=dev)
+    rope_rows(at, cos, sin, rope)
+    cache2, out2 = old.to(dev), torch.empty_like(out)
+    plan.decode_qkv(qkv, q_w, k_w, cos, sin, at, cache2, out2, eps, rope=rope)
+    assert torch.equal(out2, out) and torch.equal(cache2, cache)
 
 
 def test_captured_steps_replay(dev):
