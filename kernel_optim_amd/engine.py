@@ -34,6 +34,12 @@ longest agreeing prefix plus the model's own next token is accepted per
 sequence; when the accepted tokens per verify step fall below the measured
 break-even, decoding finishes on the pipelined one-token graph
 (engine.py:403-508).
+
+With ENGINE_KV_CACHE=kv4 (or kv_cache="kv4") K and V are held in 4 bits (kernels.kv4; 5 bits a
+value with the scales of the default groups of 32, ENGINE_KV_GROUP): 3.2 times the keys in
+the same memory and a decode step that reads as much less of them. The prompt attends to
+its own K and V in bf16, layer by layer, before they are quantised; decode and verify
+steps attend to what the cache holds.
 """
 
 import os
@@ -44,6 +50,7 @@ import weakref
 import torch
 
 from .kernels.fused import DecodeAttention, add_rms_norm, qk_norm_rope, rope_rows, silu_mul
+from .kernels.kv4 import Kv4Attention, kv4_append, kv4_block_bytes, kv4_cache, kv4_write
 from .kernels.gemv import (EPI_ARGMAX, EPI_BF16, EPI_RESID, EPI_SWIGLU, ROWS_MAX, Gemv, argmax_rows,
                            embed_ss, tile_weights, uses_tiled)
 from .model import Qwen3Config, load_checkpoint, random_weights
@@ -85,6 +92,9 @@ WINDOW = 8               # verify steps between two acceptance checks
 HOST_MS = 0.2            # host time per verify step (wait, draft, copies)
 MIN_ADVANCE = (float(os.environ["ENGINE_MIN_ADVANCE"]) if "ENGINE_MIN_ADVANCE" in os.environ
                else None)
+# the KV cache: "bf16", or "kv4" (4 bits, in groups of KV_GROUP values)
+KV_CACHE = os.environ.get("ENGINE_KV_CACHE", "bf16")
+KV_GROUP = int(os.environ.get("ENGINE_KV_GROUP", "32"))
 PIN_RESULTS = 64 << 20   # bytes of verify results in pinned memory that callers may hold
 FUSED_VERIFY_ROWS = 16   # verify rows the fused GEMVs take in one weight pass
 
@@ -295,7 +305,8 @@ def decode_layer(gv, W, i, lw, attn, h, qkv, attn_out, act, k_cache, v_cache, co
         attn.decode_qkv_oproj(qkv, lw["q_norm"], lw["k_norm"], cos, sin, pos, k_cache, v_cache,
                               attn_out, eps, lw["o"], h, rope=rope)
     else:
-        attn.decode_qkv(qkv, lw["q_norm"], lw["k_norm"], cos, sin, pos, k_cache, v_cache,
+        attn.decode_qkv(qkv, lw["q_norm"], lw["k_norm"], cos, sin, pos,
+                        *((k_cache,) if v_cache is None else (k_cache, v_cache)),
                         attn_out, eps, rope=rope)
         nxt, xn = _chain(gv, "o", "gu", lw["w_post"])
         gv["o"](attn_out, W["o"][i], h=h, nxt=nxt)
@@ -327,7 +338,7 @@ class HostCopies:
 
 class Engine:
     def __init__(self, model_path: str, keep_logits: bool = False, spec=None,
-                 decode_graph=None) -> None:
+                 decode_graph=None, kv_cache=None) -> None:
         self._t0 = time.monotonic()
         if model_path.startswith("random"):
             seed = int(model_path.split(":", 1)[1]) if ":" in model_path else 0
@@ -347,30 +358,38 @@ class Engine:
             raise FileNotFoundError(
                 f"{model_path}: no *.safetensors weights (pass 'random[:seed]' or set "
                 "ENGINE_RANDOM_INIT=1 for random weights over its config.json)")
-        self._init(cfg, w, keep_logits, spec, decode_graph)
+        self._init(cfg, w, keep_logits, spec, decode_graph, kv_cache)
 
     @classmethod
-    def from_weights(cls, cfg, weights, keep_logits=False, spec=None, decode_graph=None):
+    def from_weights(cls, cfg, weights, keep_logits=False, spec=None, decode_graph=None,
+                     kv_cache=None):
         """Engine over weights already in the decode layout (moved to the GPU)."""
         from .model import weights_to
         self = cls.__new__(cls)
         self._t0 = time.monotonic()
-        self._init(cfg, weights_to(weights, DEVICE), keep_logits, spec, decode_graph)
+        self._init(cfg, weights_to(weights, DEVICE), keep_logits, spec, decode_graph, kv_cache)
         return self
 
-    def _init(self, cfg, w, keep_logits, spec=None, decode_graph=None):
+    def _init(self, cfg, w, keep_logits, spec=None, decode_graph=None, kv_cache=None):
         """spec: prompt-lookup speculation on (True) or off (False); None takes
         ENGINE_SPEC (off unless set to 1). decode_graph: "auto" (the fused-GEMV
         decode graph up to 32 sequences, or 64 where auto_graph says so, the
         hipBLASLt graph above), "timed" (capture both up to FUSED_MAX_TIMED sequences, time them at setup
         and keep the faster), "fused" or "hipblaslt"; None takes
-        ENGINE_DECODE_GRAPH (auto unless set)."""
+        ENGINE_DECODE_GRAPH (auto unless set). kv_cache: "bf16" or "kv4" (K and V in 4
+        bits); None takes ENGINE_KV_CACHE (bf16 unless set)."""
         self.spec = SPEC if spec is None else bool(spec)
         self.min_advance = MIN_ADVANCE   # None: the measured break-even
         kind = DECODE_GRAPH if decode_graph is None else decode_graph
         if kind not in ("auto", "timed", "fused", "hipblaslt"):
             raise ValueError(f"decode_graph must be auto, timed, fused or hipblaslt, not {kind!r}")
         self.decode_graph = kind
+        held = KV_CACHE if kv_cache is None else kv_cache
+        if held not in ("bf16", "kv4"):
+            raise ValueError(f"kv_cache must be bf16 or kv4, not {held!r}")
+        self.kv_cache, self.kv4 = held, None
+        if held == "kv4":
+            kv4_block_bytes(cfg.head_dim, KV_GROUP)   # refuses a group it does not serve
         if cfg.head_dim != 128 or cfg.nq != 4 * cfg.nkv:
             raise ValueError("the decode kernels serve head_dim 128 with 4 query heads per KV head")
         self.cfg, self.w = cfg, w
@@ -396,7 +415,7 @@ class Engine:
             return
         self._shape = None
         self.g1 = self.gk = None
-        self.k_cache = self.v_cache = None
+        self.k_cache = self.v_cache = self.kv4 = None
         torch.cuda.empty_cache()
         cfg = self.cfg
         self.K = draft_len(B) if self.spec and N > 2 else 0
@@ -407,8 +426,12 @@ class Engine:
         self._tables(cap)
         dev = DEVICE
         bf = torch.bfloat16
-        self.k_cache = torch.zeros(cfg.layers, B, cfg.nkv, cap, cfg.head_dim, dtype=bf, device=dev)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        if self.kv_cache == "kv4":
+            self.kv4 = kv4_cache(B, cfg.nkv, cap, cfg.head_dim, dev, KV_GROUP, layers=cfg.layers)
+        else:
+            self.k_cache = torch.zeros(cfg.layers, B, cfg.nkv, cap, cfg.head_dim, dtype=bf,
+                                       device=dev)
+            self.v_cache = torch.zeros_like(self.k_cache)
         self.pos = torch.zeros(B, dtype=torch.int32, device=dev)
         self.ids = torch.zeros(B, dtype=torch.int64, device=dev)
         self.h = torch.zeros(B, cfg.hidden, dtype=bf, device=dev)
@@ -425,11 +448,14 @@ class Engine:
         self._ring_np = self.pin_ids.numpy()
         self.ring_ctr = torch.zeros(B, dtype=torch.int32, device=dev)
         self.events = [torch.cuda.Event() for _ in range(N + 1)]
-        self.attn = DecodeAttention(B, 1, cap, cfg.nq, cfg.nkv, cfg.head_dim, dev,
-                                    unit=ATTN_UNIT or None, fused_combine=True,
-                                    units_per_seq=attn_units_per_seq(B, cfg.nkv))
-        self.attn.oproj_delay_ns = OPROJ_DELAY_NS
-        self.attn.oproj_spin = self.oproj_spin
+        if self.kv4 is not None:
+            self.attn = Kv4Attention(B, 1, cap, cfg.nq, cfg.nkv, cfg.head_dim, dev, KV_GROUP)
+        else:
+            self.attn = DecodeAttention(B, 1, cap, cfg.nq, cfg.nkv, cfg.head_dim, dev,
+                                        unit=ATTN_UNIT or None, fused_combine=True,
+                                        units_per_seq=attn_units_per_seq(B, cfg.nkv))
+            self.attn.oproj_delay_ns = OPROJ_DELAY_NS
+            self.attn.oproj_spin = self.oproj_spin
         L = self.w["layers"]
         raw = dict(qkv=[l["qkv"] for l in L], o=[l["o"] for l in L], gu=[l["gu"] for l in L],
                    down=[l["down"] for l in L], lm=[self.w["lm_head"]])
@@ -494,7 +520,9 @@ class Engine:
         self.qT = torch.zeros(M, cfg.nq * cfg.head_dim, dtype=bf, device=dev)
         self.attT = torch.zeros_like(self.qT)
         self.actT = torch.zeros(M, cfg.inter, dtype=bf, device=dev)
-        if VERIFY_TOKEN_ROWS:
+        if self.kv4 is not None:
+            self.attnk = Kv4Attention(B, T, self.cap, cfg.nq, cfg.nkv, cfg.head_dim, dev, KV_GROUP)
+        elif VERIFY_TOKEN_ROWS:
             # the B*T tokens as rows of the one-token kernel, each row merged by
             # its last unit: one launch
             self.attnk = DecodeAttention(B, T, self.cap, cfg.nq, cfg.nkv, cfg.head_dim, dev,
@@ -557,6 +585,17 @@ class Engine:
             torch.cuda.synchronize()
         return self._tile_cache[name]
 
+    def _caches(self, i):
+        """Layer i's K and V caches, or its 4-bit cache and None."""
+        return ((self.k_cache[i], self.v_cache[i]) if self.kv4 is None else (self.kv4[i], None))
+
+    def _fuse_o(self):
+        return FUSE_OPROJ and self.kv4 is None and self.attn.oproj_fusable()
+
+    def _check_sync(self):
+        if self.kv4 is None:
+            self.attn.check_sync()
+
     def _step1(self):
         """One decode token per sequence at pos[b]; greedy ids; positions advance."""
         cfg = self.cfg
@@ -564,11 +603,11 @@ class Engine:
         # h holds embed[ids] and rope the RoPE rows at pos: both written by the
         # previous step's LM head tail (or by the prefill hand-off)
         h = self.h
-        fuse_o = FUSE_OPROJ and self.attn.oproj_fusable()
+        fuse_o = self._fuse_o()
         L = self.w["layers"]
         for i, lw in enumerate(L):
             decode_layer(g, W, i, lw, self.attn, h, self.qkv, self.attn_out, self.act,
-                         self.k_cache[i], self.v_cache[i], self._cos, self._sin, self.pos,
+                         *self._caches(i), self._cos, self._sin, self.pos,
                          self.rope, cfg.eps, fuse_o,
                          next_norm=L[i + 1]["w_in"] if i + 1 < len(L) else None, normed=i > 0)
         # LM head + greedy ids + pos += 1 + the next step's embedding rows and RoPE
@@ -591,9 +630,9 @@ class Engine:
         for i, lw in enumerate(self.w["layers"]):
             add_rms_norm(h, None, lw["w_in"], self.nrm, eps)
             torch.mm(self.nrm, lw["qkv"].t(), out=self.qkv)
+            caches = (self.kv4[i],) if self.kv4 is not None else self._caches(i)
             self.attn.decode_qkv(self.qkv, lw["q_norm"], lw["k_norm"], self._cos, self._sin,
-                                 self.pos, self.k_cache[i], self.v_cache[i], self.attn_out, eps,
-                                 rope=self.rope)
+                                 self.pos, *caches, self.attn_out, eps, rope=self.rope)
             h.add_(torch.mm(self.attn_out, lw["o"].t()))   # h <- bf16(h + bf16(x @ W^T))
             add_rms_norm(h, None, lw["w_post"], self.nrm, eps)
             torch.mm(self.nrm, lw["gu"].t(), out=self.gu_mm)
@@ -623,10 +662,15 @@ class Engine:
             else:
                 add_rms_norm(h, None, lw["w_in"], self.nT, eps)
                 torch.mm(self.nT, lw["qkv"].t(), out=self.qkvT)
-            qk_norm_rope(self.qkvT, lw["q_norm"], lw["k_norm"], self._cos, self._sin, self.pos,
-                         self.qT, self.k_cache[i], self.v_cache[i], T, eps, cfg.nq, cfg.nkv,
-                         cfg.head_dim)
-            self.attnk(self.qT, self.k_cache[i], self.v_cache[i], self.pos, self.attT)
+            if self.kv4 is not None:
+                kv4_append(self.qkvT, lw["q_norm"], lw["k_norm"], self._cos, self._sin, self.pos,
+                           self.qT, self.kv4[i], T, eps, cfg.nq, cfg.nkv, cfg.head_dim)
+                self.attnk(self.qT, self.kv4[i], self.pos, self.attT)
+            else:
+                qk_norm_rope(self.qkvT, lw["q_norm"], lw["k_norm"], self._cos, self._sin, self.pos,
+                             self.qT, self.k_cache[i], self.v_cache[i], T, eps, cfg.nq, cfg.nkv,
+                             cfg.head_dim)
+                self.attnk(self.qT, self.k_cache[i], self.v_cache[i], self.pos, self.attT)
             if fused:
                 g["o"](self.attT, W["o"][i], h=h)
                 g["gu"](h, W["gu"][i], y=self.actT, nw=lw["w_post"])
@@ -668,8 +712,14 @@ class Engine:
 
     # ---------------------------------------------------------------- forward
     def _prefill(self, prompt):
-        ids, logits = prefill(self.cfg, self.w, prompt, self.k_cache, self.v_cache, self._cos,
-                              self._sin)
+        kc, vc, sink = self.k_cache, self.v_cache, None
+        if self.kv4 is not None:
+            # one layer's K and V in bf16, quantised into the cache as the layers pass
+            B, S = prompt.shape
+            kc, vc = (torch.empty(1, B, self.cfg.nkv, S, self.cfg.head_dim, dtype=torch.bfloat16,
+                                  device=prompt.device) for _ in range(2))
+            sink = lambda i, k, v: kv4_write(k, v, self.kv4[i])
+        ids, logits = prefill(self.cfg, self.w, prompt, kc, vc, self._cos, self._sin, sink)
         self.ids.copy_(ids)
         self._set_pos(prompt.shape[1])
         embed_ss(self.ids, self.w["embed"], self.h, None)   # the first decode step's input
@@ -763,7 +813,7 @@ class Engine:
                 else:
                     ev[j].synchronize()
                 yield ids_h[j].tolist()
-            self.attn.check_sync()
+            self._check_sync()
         finally:
             # a caller that stops early (or an error) leaves no replay in flight
             torch.cuda.synchronize()
@@ -784,7 +834,7 @@ class Engine:
                     raise RuntimeError(f"decode step {j} stored no ids in the host ring")
         if (row < 0).any():
             torch.cuda.synchronize()
-            self.attn.check_sync()
+            self._check_sync()
             raise RuntimeError(f"decode step {j}: the ring holds no ids")
 
     def _generate_spec(self, input_ids, N, stream):
@@ -864,7 +914,7 @@ class Engine:
         row = self.pin_ids[j].tolist()
         if last or min(row) < 0:   # -2: that step's o-projection wait gave up
             torch.cuda.synchronize()
-            self.attn.check_sync()
+            self._check_sync()
             if min(row) < 0:
                 raise RuntimeError(f"decode step {j}: the ring holds no ids")
         for b, t in enumerate(row):
@@ -890,5 +940,5 @@ class Engine:
             self.g1.replay()
             toks.append(self.ids.cpu())
             logits.append(self.logits.cpu())
-            self.attn.check_sync()   # raises at the step whose o-projection wait failed
+            self._check_sync()   # raises at the step whose o-projection wait failed
         return torch.stack(toks, 1), logits

@@ -231,10 +231,12 @@ def _layer_torch(cfg, lw, x, kc, vc, cos, sin, exact_gqa):
 
 
 @torch.no_grad()
-def prefill(cfg, w, prompt, k_cache, v_cache, cos, sin):
+def prefill(cfg, w, prompt, k_cache, v_cache, cos, sin, sink=None):
     """prompt [B, S] int64 on the device; caches [L, B, nkv, cap, d]; cos/sin
     [>= S, d] bf16 (Qwen3RotaryEmbedding's rows for positions 0..S-1). Returns
-    the greedy next ids [B] (int64) and the last-position logits [B, V] (bf16)."""
+    the greedy next ids [B] (int64) and the last-position logits [B, V] (bf16).
+    sink(i, K, V) (optional): called with layer i's K and V [B, nkv, S, d] behind that
+    layer; the caches then hold one layer, which every layer uses in turn."""
     B, S = prompt.shape
     exact_gqa = gqa_exact(prompt.device)
     x = F.embedding(prompt, w["embed"])
@@ -243,12 +245,15 @@ def prefill(cfg, w, prompt, k_cache, v_cache, cos, sin):
     h = torch.empty_like(x) if rows else None
     delta = None   # the last layer's output where it is not yet in x
     for i, lw in enumerate(w["layers"]):
+        kc, vc = (k_cache[i], v_cache[i]) if sink is None else (k_cache[0], v_cache[0])
         if rows and _layer_served(cfg, lw, x):
-            delta = _layer_rows(cfg, lw, x, delta, h, k_cache[i], v_cache[i], cos, sin, exact_gqa)
-            continue
-        if delta is not None:
-            x, delta = x + delta, None
-        x = _layer_torch(cfg, lw, x, k_cache[i], v_cache[i], cos, sin, exact_gqa)
+            delta = _layer_rows(cfg, lw, x, delta, h, kc, vc, cos, sin, exact_gqa)
+        else:
+            if delta is not None:
+                x, delta = x + delta, None
+            x = _layer_torch(cfg, lw, x, kc, vc, cos, sin, exact_gqa)
+        if sink is not None:
+            sink(i, kc[:, :, :S], vc[:, :, :S])
     if delta is not None:
         x = x + delta
     xl = rmsnorm(x[:, -1:], w["final_norm"], cfg.eps)
