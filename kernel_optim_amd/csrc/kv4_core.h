@@ -50,14 +50,20 @@ struct Kv4Group {
     float s = round_bf16(fmaxf((mx - c) * (float)(1.0 / 7.0), (c - mn) * 0.125f));
     if (!(fabsf(mn) < INFINITY && fabsf(mx) < INFINITY)) c = s = __uint_as_float(0x7fc00000u);
     if (s < 1.1754943508222875e-38f) s = 0.f;
-    inv = s == 0.f ? 0.f : 1.0f / s;
+    // 1 / s, rounded correctly: v_rcp_f32 and one Newton step are, for every bf16 from 2^-126 to
+    // 2^126 (all of them compared on the GPU), and s is below 2^126 (no group spans 7 2^126)
+    const float y = __builtin_amdgcn_rcpf(s);
+    inv = s == 0.f ? 0.f : fmaf(fmaf(-s, y, 1.0f), y, y);
     sc = (__float_as_uint(s) >> 16) | (__float_as_uint(c) & 0xffff0000u);
   }
-  __device__ __forceinline__ uint32_t code(float x) const {
+  // The code in the low 4 bits, zeros up to bit 21: 1.5 2^23 + t is rounded to a whole number. What
+  // lies above is shifted out of the way of codes that are put together at bits below 16.
+  __device__ __forceinline__ uint32_t raw(float x) const {
 #pragma clang fp contract(off)
-    const float t = fminf(fmaxf((x - c) * inv + 8.0f, 0.f), 15.f);
-    return (uint32_t)(int)__builtin_rintf(t);
+    const float t = __builtin_amdgcn_fmed3f((x - c) * inv + 8.0f, 0.f, 15.f);
+    return __float_as_uint(t + 12582912.0f);
   }
+  __device__ __forceinline__ uint32_t code(float x) const { return raw(x) & 15u; }
 };
 
 // NaN-propagating minimum and maximum (gfx950's v_minimum3 / v_maximum3).
