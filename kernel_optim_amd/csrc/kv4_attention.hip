@@ -41,6 +41,7 @@ namespace {
 constexpr int WAVES = 4;
 constexpr float TAU = 8.0f;            // a running maximum is raised by more than 2^8 only
 constexpr float NEG_BIG = -1.0e30f;
+constexpr int PAIR_STEPS = 12;         // what a pair costs beside its steps, in steps
 
 struct Kv4AttnArgs {
   const uint16_t* q;  // [B*T, nq*D]
@@ -234,73 +235,158 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   __shared__ int lds_prev;
   __shared__ NewKey<D, NG> lds_new[QKV ? RB : 1];
 
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = uniform(threadIdx.x >> 6), lane0 = threadIdx.x & 63;
   const int rb = wave % RB, wp = wave / RB;
   const int R = a.T * a.G;
   const Codes codes;
   const int grid = gridDim.x, wg = blockIdx.x;
 
-  // steps of every sequence: lane b holds sequence b's of the first 64
-  int my_len = 0, my_steps = 0, my_incl = 0, all = 0;
+  // ---- which steps this workgroup takes ----
+  // Lane b holds the keys, steps and places of sequence b of the first 64.
+  int my_len = 0, all = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int len = b0 + lane < a.B ? seq_keys<QKV>(a, b0 + lane) : 0;
-    const int st = b0 + lane < a.B ? max(steps_of(len), a.min_run) : 0;
-    const int incl = wave_incl_scan(st);
-    all += readlane(incl, 63);
-    if (b0 == 0) my_len = len, my_steps = st, my_incl = incl;
+    const int len = b0 + lane0 < a.B ? seq_keys<QKV>(a, b0 + lane0) : 0;
+    if (b0 == 0) my_len = len;
+    all += readlane(wave_incl_scan(b0 + lane0 < a.B ? steps_of(len) : 0), 63);
   }
-  const int total = all * a.nkv;
-  int run = max(a.min_run, (total + grid - 1) / grid);
-  run = (run + NWP - 1) / NWP * NWP;
-  const long long first = (long long)wg * run;
-  if (first >= total) return;
-  const int end = (int)min(first + run, (long long)total);
-
-  for (int s = (int)first; s < end;) {
-    // the pair of step s: sequence b, KV head, its steps and where they begin in the list
-    int b, len, n, at;
-    if (a.B <= 64) {
-      b = uniform(__popcll(__ballot(my_incl <= s / a.nkv && lane < a.B)));
-      len = readlane(my_len, b);
-      n = readlane(my_steps, b);
-      at = (readlane(my_incl, b) - n) * a.nkv;
-    } else {
-      int below = 0;
-      b = len = n = at = 0;
-      for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int l = b0 + lane < a.B ? seq_keys<QKV>(a, b0 + lane) : 0;
-        const int st = b0 + lane < a.B ? max(steps_of(l), a.min_run) : 0;
-        const int incl = wave_incl_scan(st) + below;
-        const int k = uniform(__popcll(__ballot(incl <= s / a.nkv && b0 + lane < a.B)));
-        if (k < min(64, a.B - b0)) {
-          b = b0 + k;
-          len = readlane(l, k);
-          n = readlane(st, k);
-          at = (readlane(incl, k) - n) * a.nkv;
-          break;
-        }
-        below = readlane(incl, 63);
-      }
+  auto up = [](int n) { return (n + NWP - 1) / NWP * NWP; };
+  const int share = max(a.min_run, (all * a.nkv + grid - 1) / grid);
+  // (1) Every pair cut into parts of `run` steps, a workgroup for each: with the least run for
+  // which the workgroups suffice, if that is at most a half longer than an equal share.
+  int run = up(share), my_places = 0, my_incl = 0, total = 0;
+  auto fits = [&](int r) {
+    my_places = lane0 < a.B ? (steps_of(my_len) + r - 1) / r : 0;
+    my_incl = wave_incl_scan(my_places);
+    return (long long)readlane(my_incl, 63) * a.nkv <= grid;
+  };
+  bool whole = a.B <= 64 && fits(run);
+  if (!whole && a.B <= 64 && fits(run + run / 2 / NWP * NWP)) {
+    int lo = run + NWP, hi = run + run / 2 / NWP * NWP;
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / (2 * NWP) * NWP;
+      if (fits(mid))
+        hi = mid;
+      else
+        lo = mid + NWP;
     }
-    const int kvh = (s - at) / n;
-    at += kvh * n;
-    const int st0 = s - at;
-    s = min(at + n, end);
-    n = steps_of(len);  // behind them, a short pair's places in the list are empty
-    const int st1 = min(n, s - at);
-    if (st0 >= st1) continue;
+    whole = true;
+    run = hi;
+    fits(run);
+  }
+  // (2) Else one list of all pairs' steps, cut into equal runs that cross from pair to pair.
+  // Beginning and ending a pair costs as much as PAIR_STEPS steps: a pair shorter than a
+  // run, which shares it with others, takes so many more places.
+  auto places = [&](int len) {
+    const int n = steps_of(len);
+    return n < share ? n + PAIR_STEPS : n;
+  };
+  if (!whole) {
+    total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const int len = b0 == 0 ? my_len : b0 + lane0 < a.B ? seq_keys<QKV>(a, b0 + lane0) : 0;
+      const int st = b0 + lane0 < a.B ? places(len) : 0;
+      const int in = wave_incl_scan(st);
+      total += readlane(in, 63);
+      if (b0 == 0) my_places = st, my_incl = in;
+    }
+    total *= a.nkv;
+    run = up(max(a.min_run, (total + grid - 1) / grid));
+  }
 
+  // The part of a pair that a workgroup takes: sequence b of len keys and n steps, KV head, the
+  // steps st0 .. st1 - 1; the workgroups w0 .. w1 hold the pair.
+  struct Segment {
+    int b, len, n, kvh, st0, st1, w0, w1;
+  };
+  const long long first = whole ? 0 : (long long)wg * run;
+  int s = (int)min(first, (long long)total);
+  const int end = (int)min(first + run, (long long)total);
+  auto find = [&](Segment& g) {  // the next of this workgroup's segments
+    while (s < end) {
+      const int pair_step = s / a.nkv;
+      g.b = g.len = 0;
+      int n = 0, at = 0;
+      if (a.B <= 64) {
+        g.b = uniform(__popcll(__ballot(my_incl <= pair_step && lane0 < a.B)));
+        g.len = readlane(my_len, g.b);
+        n = readlane(my_places, g.b);
+        at = (readlane(my_incl, g.b) - n) * a.nkv;
+      } else {
+        int below = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64) {
+          const int l = b0 + lane0 < a.B ? seq_keys<QKV>(a, b0 + lane0) : 0;
+          const int st = b0 + lane0 < a.B ? places(l) : 0;
+          const int incl = wave_incl_scan(st) + below;
+          const int k = uniform(__popcll(__ballot(incl <= pair_step && b0 + lane0 < a.B)));
+          if (k < min(64, a.B - b0)) {
+            g.b = b0 + k;
+            g.len = readlane(l, k);
+            n = readlane(st, k);
+            at = (readlane(incl, k) - n) * a.nkv;
+            break;
+          }
+          below = readlane(incl, 63);
+        }
+      }
+      g.kvh = (s - at) / n;
+      at += g.kvh * n;
+      g.st0 = s - at;
+      s = min(at + n, end);
+      g.n = steps_of(g.len);  // behind them, a short pair's places are empty
+      g.st1 = min(g.n, s - at);
+      g.w0 = at / run;
+      g.w1 = (at + g.n - 1) / run;
+      if (g.st0 < g.st1) return true;
+    }
+    return false;
+  };
+  Segment g;
+  if (whole) {
+    const int pair_part = wg / a.nkv;
+    if (pair_part >= readlane(my_incl, 63)) return;
+    g.b = uniform(__popcll(__ballot(my_incl <= pair_part && lane0 < a.B)));
+    g.len = readlane(my_len, g.b);
+    g.n = steps_of(g.len);
+    const int parts = readlane(my_places, g.b);
+    const int at = wg - (readlane(my_incl, g.b) - parts) * a.nkv;
+    g.kvh = at / parts;
+    const int part = at - g.kvh * parts;
+    g.st0 = part * run;
+    g.st1 = min(g.n, g.st0 + run);
+    g.w0 = wg - part;
+    g.w1 = g.w0 + parts - 1;
+  } else if (!find(g)) {
+    return;
+  }
+  auto base_of = [&](const Segment& g) { return a.cache + g.b * a.cb + g.kvh * a.ch; };
+  // steps past the segment's last read it again
+  auto block_of = [&](const Segment& g, int st) {
+    return base_of(g) + (long long)min(st, g.st1 - 1) * kv4_block_bytes(D, NG);
+  };
+  Block<D, NG> x0, x1;  // the wavefront's next two blocks
+  auto load_first = [&](const Segment& g) {
+    const int l = fresh_tid() & 63, r = l & 15, kg = l >> 4;
+    x0.load_k(block_of(g, g.st0 + wp), r, kg, l);
+    x0.load_v(block_of(g, g.st0 + wp), r, kg);
+    x1.load_k(block_of(g, g.st0 + wp + NWP), r, kg, l);
+    x1.load_v(block_of(g, g.st0 + wp + NWP), r, kg);
+  };
+
+  // Output row rw of a pair.
+  auto out_row = [&](int b, int kvh, int rw) {
+    const int t = rw / a.G;
+    const long long row = (((long long)b * a.T + t) * a.nkv + kvh) * a.G + (rw - t * a.G);
+    return reinterpret_cast<uint32_t*>(a.out + row * D);
+  };
+
+  load_first(g);
+  for (;;) {
+    const int b = g.b, len = g.len, n = g.n, kvh = g.kvh, st0 = g.st0, st1 = g.st1;
     const int lane = fresh_tid() & 63, r = lane & 15, kg = lane >> 4;
     const int hh = r / GPT, gg = r % GPT;
     const int row = min(rb * RP + hh, R - 1);  // rows past R repeat the last; they are not stored
     const int t = row / a.G, h = row - t * a.G;
-    const uint8_t* base = a.cache + b * a.cb + kvh * a.ch;
-    auto block_at = [&](int st) {
-      return base + (long long)min(st, st1 - 1) * kv4_block_bytes(D, NG);
-    };
-    Block<D, NG> x;
-    x.load_k(block_at(st0 + wp), r, kg, lane);
-    x.load_v(block_at(st0 + wp), r, kg);
+    [[maybe_unused]] const uint8_t* base = base_of(g);
 
     // q: column (row, group): zeros outside the group
     uint32_t q[I][4];
@@ -418,7 +504,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     for (int u = 0; u < NT; ++u) pc[u] = 0.f;
 
     // The running maximum m is kept in units of the unscaled scores.
-    auto step = [&](int st, auto masked_) {
+    auto step = [&](Block<D, NG>& x, int st, auto masked_) {
       constexpr bool masked = decltype(masked_)::value;
       uint32_t* lsc = lds_sc[wave];
       x.scales_to(lsc, lane);
@@ -478,7 +564,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
           sc[4 * c + e] = sum_lanes<GPT>(v);
         }
       }
-      const uint8_t* next = block_at(st + NWP);
+      const uint8_t* next = block_of(g, st + 2 * NWP);
       x.load_k(next, r, kg, lane);
       const int k0 = st * KV4_KEYS + 8 * kg;
       if constexpr (masked) {
@@ -539,10 +625,31 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       __builtin_amdgcn_wave_barrier();
     };
 
+    auto swap = [&] {
+      const Block<D, NG> y = x0;
+      x0 = x1;
+      x1 = y;
+    };
     int st = st0 + wp;
-    for (const int unmasked = min(st1, max(full, 0) >> 5); st < unmasked; st += NWP)
-      step(st, std::false_type{});
-    for (; st < st1; st += NWP) step(st, std::true_type{});
+    const int unmasked = min(st1, max(full, 0) >> 5);
+    for (; st + NWP < unmasked; st += 2 * NWP) {
+      step(x0, st, std::false_type{});
+      step(x1, st + NWP, std::false_type{});
+    }
+    if (st < unmasked) {
+      step(x0, st, std::false_type{});
+      swap();
+      st += NWP;
+    }
+    for (; st < st1; st += NWP) {
+      step(x0, st, std::true_type{});
+      swap();
+    }
+
+    // the next pair's first blocks come while this one's sums are put together
+    Segment nx;
+    const bool more = find(nx);   // none with (1)
+    if (more) load_first(nx);
 
     // ---- this wavefront's sums to LDS: accumulator row 4 kg + e is column (hh, gg) ----
     const int tid = fresh_tid(), el = tid & 63, er = el & 15, ek = el >> 4;
@@ -573,11 +680,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     __syncthreads();
 
     // ---- merge the wavefronts; a whole pair is done, a part goes to the workspace ----
-    const int w0 = at / run, w1 = (at + n - 1) / run;  // the runs that hold the pair
-    const int slot = 2 * wg + (wg == w0 ? 1 : 0);
-    float* po = a.part + (long long)slot * ROWS * D;
-    float* pm = a.part + 2LL * grid * ROWS * D + (long long)slot * ROWS * 2;
-    const long long orow = ((long long)b * a.T * a.nkv + kvh) * a.G;  // + t nkv G + h
+    const int w0 = g.w0, w1 = g.w1;
+    const int mine = wg == w0 ? 1 : 0;                     // of this run's two slots
+    float* po = a.part + (2LL * wg + mine) * ROWS * D;
+    float* pm = a.part + 2LL * grid * ROWS * D + (2LL * wg + mine) * ROWS * 2;
     for (int x = tid; x < R * (D / 2); x += 64 * WAVES) {
       const int rw = x / (D / 2), c2 = x - rw * (D / 2);
       float M = NEG_BIG, L = 0.f, o0 = 0.f, o1 = 0.f;
@@ -593,10 +699,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
         o1 = fmaf(f, o.y, o1);
       }
       if (w0 == w1) {
-        const int tt = rw / a.G;
-        const long long o = orow + (long long)tt * a.nkv * a.G + (rw - tt * a.G);
-        reinterpret_cast<uint32_t*>(a.out + o * D)[c2] =
-            L == 0.f ? 0u : pack_bf16x2(o0 / L, o1 / L);
+        out_row(b, kvh, rw)[c2] = L == 0.f ? 0u : pack_bf16x2(o0 / L, o1 / L);
       } else {
         store2_coherent(po + rw * D + 2 * c2, o0, o1);
         if (c2 == 0) store2_coherent(pm + rw * 2, M, L);
@@ -610,14 +713,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
         lds_prev = __hip_atomic_fetch_add(a.counters + w0, 1, __ATOMIC_RELAXED,
                                           __HIP_MEMORY_SCOPE_AGENT);
       __syncthreads();
-      if (lds_prev == w1 - w0) {
+      if (lds_prev == w1 - w0) {  // the last of the pair's runs to be counted merges them
         if (tid == 0)
           __hip_atomic_store(a.counters + w0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int parts = w1 - w0 + 1, c2 = el & (D / 2 - 1);
         // slots of the pair's parts: the first run's second, then every run's first
         auto slot_of = [&](int k) { return k == 0 ? 2 * w0 + 1 : 2 * (w0 + k); };
-        const int parts = w1 - w0 + 1;
         const float* ml = a.part + 2LL * grid * ROWS * D;
-        const int c2 = el & (D / 2 - 1);
         // KR rows a wavefront and PB parts at a time: 32 loads in flight, the first of them
         // with the loads of (m, l)
         constexpr int KR = ROWS >= 16 ? 4 : ROWS / 4, PB = 32 / KR;
@@ -672,17 +774,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
             }
           }
 #pragma unroll
-          for (int k = 0; k < KR; ++k) {
-            const int tt = rw[k] / a.G;
-            const long long o = orow + (long long)tt * a.nkv * a.G + (rw[k] - tt * a.G);
+          for (int k = 0; k < KR; ++k)
             if (el < D / 2 && rw0 + WAVES * k < R)
-              reinterpret_cast<uint32_t*>(a.out + o * D)[c2] =
+              out_row(b, kvh, rw[k])[c2] =
                   L[k] == 0.f ? 0u : pack_bf16x2(o0[k] / L[k], o1[k] / L[k]);
-          }
         }
       }
     }
+    if (!more) break;
     __syncthreads();  // the next pair's sums reuse the LDS
+    g = nx;
   }
 }
 
