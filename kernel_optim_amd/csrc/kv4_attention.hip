@@ -41,6 +41,10 @@ namespace {
 constexpr int WAVES = 4;
 constexpr float TAU = 8.0f;            // a running maximum is raised by more than 2^8 only
 constexpr float NEG_BIG = -1.0e30f;
+// Up to SOLO steps a pair is not cut: its 4 steps a wavefront take less than the partial sums'
+// way through memory (one sequence of 512 keys 6.7 against 8.0 us in two parts; 1000 keys 9.8
+// against 8.6 us in four).
+constexpr int SOLO = 16;
 constexpr int PAIR_STEPS = 12;         // what a pair costs beside its steps, in steps
 
 struct Kv4AttnArgs {
@@ -49,6 +53,7 @@ struct Kv4AttnArgs {
   long long cb, ch;  // bytes
   const int* lens;
   int len_off, cap, B, T, nkv, G, min_run;
+  float inv_nkv, inv_grid;
   float scale_log2;
   float* part;    // [2 * grid][rows][D], then [2 * grid][rows][2]
   int* counters;  // [grid], zero; left zero
@@ -83,6 +88,17 @@ __device__ __forceinline__ int fresh_tid() {
   int t = threadIdx.x;
   asm volatile("" : "+v"(t));
   return t;
+}
+
+// a / b for 0 <= a < 2^24, 0 < b, with 1 / b as fp32 has it: two estimates and one correction,
+// a third of the instructions of a 32-bit division; in front of a wavefront's first load.
+__device__ __forceinline__ int quot(int a, int b, float inv) {
+  int q = (int)((float)a * inv);
+  int rem = a - q * b;
+  const int more = (int)((float)rem * inv);
+  q += more;
+  rem -= more * b;
+  return q + (rem >= b ? 1 : 0) - (rem < 0 ? 1 : 0);
 }
 
 // Sum over the n neighbouring lanes (1, 2, 4) that hold a row's groups.
@@ -250,12 +266,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     all += readlane(wave_incl_scan(b0 + lane0 < a.B ? steps_of(len) : 0), 63);
   }
   auto up = [](int n) { return (n + NWP - 1) / NWP * NWP; };
-  const int share = max(a.min_run, (all * a.nkv + grid - 1) / grid);
+  const int share = max(a.min_run, quot(all * a.nkv + grid - 1, grid, a.inv_grid));
   // (1) Every pair cut into parts of `run` steps, a workgroup for each: with the least run for
   // which the workgroups suffice, if that is at most a half longer than an equal share.
   int run = up(share), my_places = 0, my_incl = 0, total = 0;
   auto fits = [&](int r) {
-    my_places = lane0 < a.B ? (steps_of(my_len) + r - 1) / r : 0;
+    const int n = steps_of(my_len);
+    const int parts = n <= SOLO ? 1 : quot(n + r - 1, r, __builtin_amdgcn_rcpf((float)r));
+    my_places = lane0 < a.B ? parts : 0;
     my_incl = wave_incl_scan(my_places);
     return (long long)readlane(my_incl, 63) * a.nkv <= grid;
   };
@@ -303,7 +321,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   const int end = (int)min(first + run, (long long)total);
   auto find = [&](Segment& g) {  // the next of this workgroup's segments
     while (s < end) {
-      const int pair_step = s / a.nkv;
+      const int pair_step = uniform(quot(s, a.nkv, a.inv_nkv));
       g.b = g.len = 0;
       int n = 0, at = 0;
       if (a.B <= 64) {
@@ -342,17 +360,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   };
   Segment g;
   if (whole) {
-    const int pair_part = wg / a.nkv;
+    const int pair_part = quot(wg, a.nkv, a.inv_nkv);
     if (pair_part >= readlane(my_incl, 63)) return;
     g.b = uniform(__popcll(__ballot(my_incl <= pair_part && lane0 < a.B)));
     g.len = readlane(my_len, g.b);
     g.n = steps_of(g.len);
     const int parts = readlane(my_places, g.b);
     const int at = wg - (readlane(my_incl, g.b) - parts) * a.nkv;
-    g.kvh = at / parts;
+    g.kvh = uniform(quot(at, parts, __builtin_amdgcn_rcpf((float)parts)));
     const int part = at - g.kvh * parts;
     g.st0 = part * run;
-    g.st1 = min(g.n, g.st0 + run);
+    g.st1 = parts == 1 ? g.n : min(g.n, g.st0 + run);
     g.w0 = wg - part;
     g.w1 = g.w0 + parts - 1;
   } else if (!find(g)) {
@@ -374,7 +392,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
 
   // Output row rw of a pair.
   auto out_row = [&](int b, int kvh, int rw) {
-    const int t = rw / a.G;
+    const int t = a.T == 1 ? 0 : rw / a.G;
     const long long row = (((long long)b * a.T + t) * a.nkv + kvh) * a.G + (rw - t * a.G);
     return reinterpret_cast<uint32_t*>(a.out + row * D);
   };
@@ -385,7 +403,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     const int lane = fresh_tid() & 63, r = lane & 15, kg = lane >> 4;
     const int hh = r / GPT, gg = r % GPT;
     const int row = min(rb * RP + hh, R - 1);  // rows past R repeat the last; they are not stored
-    const int t = row / a.G, h = row - t * a.G;
+    const int t = a.T == 1 ? 0 : row / a.G, h = row - t * a.G;
     [[maybe_unused]] const uint8_t* base = base_of(g);
 
     // q: column (row, group): zeros outside the group
@@ -835,10 +853,10 @@ int check(const void* cache, long long cb, long long ch, const int* lens, int ca
       (reinterpret_cast<uintptr_t>(part) & 7))
     return KO_EINVAL;
   if (part_len < scratch_floats(T * (nq / nkv), d, group, grid)) return KO_ERANGE;
-  // the list of steps and the runs are counted in 32 bits
+  // the places of the list, and what is divided, stay below 2^24 (quot)
   const long long blocks = ((long long)cap + 31) / 32;
   if (grid > (1 << 20) || min_run > (1 << 20) ||
-      (long long)B * nkv > (1LL << 30) / (blocks > min_run ? blocks : min_run))
+      (long long)B * nkv > ((1LL << 24) - grid - min_run) / (blocks + PAIR_STEPS))
     return KO_ERANGE;
   return KO_OK;
 }
@@ -873,6 +891,8 @@ int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
   a.nkv = nkv;
   a.G = nq / nkv;
   a.min_run = min_run;
+  a.inv_nkv = 1.0f / nkv;
+  a.inv_grid = 1.0f / grid;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = part;
   a.counters = counters;
@@ -908,6 +928,8 @@ int ko_kv4_attn_qkv(const void* qkv, const void* q_w, const void* k_w, const voi
   a.nkv = nkv;
   a.G = nq / nkv;
   a.min_run = min_run;
+  a.inv_nkv = 1.0f / nkv;
+  a.inv_grid = 1.0f / grid;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = part;
   a.counters = counters;
