@@ -394,8 +394,8 @@ int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void*
 /* Decode attention over a 4-bit cache layer: as ko_decode_attn for q [B*T, nq*d] bf16 and out
  * (another buffer), query t of sequence b at position n - T + t of its n = kv_lens[b] + len_offset
  * keys (at most cap). A row that sees no key is zero. nq a multiple of nkv, T * nq / nkv <= 64.
- * The steps of 32 keys of all pairs are cut into equal runs of at least min_run steps, one for
- * each of the grid workgroups. part: fp32 scratch of part_len >= ko_kv4_attn_scratch(T * nq /
+ * The steps of 32 keys of all pairs are dealt out in runs of at least min_run steps to grid
+ * workgroups of 4 wavefronts (or half as many of 8). part: fp32 scratch of part_len >= ko_kv4_attn_scratch(T * nq /
  * nkv, d, group, grid); counters [grid] int32, zero before the first call, left zero by every
  * call; calls that share them must not overlap. */
 int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,

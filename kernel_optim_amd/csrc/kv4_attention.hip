@@ -38,7 +38,6 @@ using namespace ko;
 
 namespace {
 
-constexpr int WAVES = 4;
 constexpr float TAU = 8.0f;            // a running maximum is raised by more than 2^8 only
 constexpr float NEG_BIG = -1.0e30f;
 // Up to SOLO steps a pair is not cut: its 4 steps a wavefront take less than the partial sums'
@@ -53,7 +52,7 @@ struct Kv4AttnArgs {
   long long cb, ch;  // bytes
   const int* lens;
   int len_off, cap, B, T, nkv, G, min_run;
-  float inv_nkv, inv_grid;
+  float inv_nkv;
   float scale_log2;
   float* part;    // [2 * grid][rows][D], then [2 * grid][rows][2]
   int* counters;  // [grid], zero; left zero
@@ -240,7 +239,7 @@ struct NewKey {
 
 // RB: blocks of 16 query rows (above 1 with GPT = 1): wavefront w serves rows 16 (w % RB) ..,
 // and the steps w / RB, w / RB + 4 / RB, ... of a run.
-template <int D, int NG, int GPT, int RB, bool QKV>
+template <int D, int NG, int GPT, int RB, int WAVES, bool QKV>
 __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
   constexpr int I = D / 32, IPG = I / NG, NT = NG / GPT, RP = 16 / GPT, J = D / 16;
   constexpr int NWP = WAVES / RB, ROWS = RB * RP;
@@ -266,7 +265,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     all += readlane(wave_incl_scan(b0 + lane0 < a.B ? steps_of(len) : 0), 63);
   }
   auto up = [](int n) { return (n + NWP - 1) / NWP * NWP; };
-  const int share = max(a.min_run, quot(all * a.nkv + grid - 1, grid, a.inv_grid));
+  const int share = max(a.min_run, quot(all * a.nkv + grid - 1, grid, __builtin_amdgcn_rcpf((float)grid)));
   // (1) Every pair cut into parts of `run` steps, a workgroup for each: with the least run for
   // which the workgroups suffice, if that is at most a half longer than an equal share.
   int run = up(share), my_places = 0, my_incl = 0, total = 0;
@@ -813,23 +812,39 @@ int row_blocks(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Wavefronts of a workgroup (two of 4 or one of 8 fill a CU's registers): 8 where blocks of 16
+// query rows share each step (4 x 7 tokens of ragged sequences 24.0 -> 18.7 us), and where there
+// is a workgroup of 8 for each pair, as 129 to 256 pairs have it: pairs of one length then need
+// no merge (32 x 2048 keys 20.9 -> 17.5 us; a ragged 32 23.7 -> 25.0). Fewer pairs are cut either
+// way (16 x 8192 33.3 and 32.4 us, 4 x 2048 9.0 and 9.2), more take a CU's two workgroups
+// (ragged 64 109 and 119 us).
+int waves_for(int rb, long long pairs) { return rb > 1 || (pairs > 128 && pairs <= 256) ? 8 : 4; }
+
 template <int D, int NG, bool QKV>
 int launch(const Kv4AttnArgs& a, int grid, hipStream_t s) {
   const int rows = a.T * a.G;
-  const dim3 g(grid), blk(64 * WAVES);
   const int gpt = tile_groups(rows, NG), rb = row_blocks(rows);
-#define KV4_LAUNCH(GPT_, RB_)                                                       \
-  {                                                                                 \
-    hipLaunchKernelGGL((kv4_attn_kernel<D, NG, GPT_, RB_, QKV>), g, blk, 0, s, a);  \
-    return KO_LAUNCH_STATUS();                                                      \
+  const int waves = waves_for(rb, (long long)a.B * a.nkv);
+  const dim3 g(waves == 8 ? (grid + 1) / 2 : grid), blk(64 * waves);
+#define KV4_LAUNCH(GPT_, RB_, WAVES_)                                                       \
+  {                                                                                         \
+    hipLaunchKernelGGL((kv4_attn_kernel<D, NG, GPT_, RB_, WAVES_, QKV>), g, blk, 0, s, a);  \
+    return KO_LAUNCH_STATUS();                                                              \
   }
   if constexpr (NG == 4)
-    if (gpt == 4) KV4_LAUNCH(4, 1)
+    if (gpt == 4) {
+      if (waves == 8) KV4_LAUNCH(4, 1, 8)
+      KV4_LAUNCH(4, 1, 4)
+    }
   if constexpr (NG >= 2)
-    if (gpt == 2) KV4_LAUNCH(2, 1)
-  if (rb == 1) KV4_LAUNCH(1, 1)
-  if (rb == 2) KV4_LAUNCH(1, 2)
-  KV4_LAUNCH(1, 4)
+    if (gpt == 2) {
+      if (waves == 8) KV4_LAUNCH(2, 1, 8)
+      KV4_LAUNCH(2, 1, 4)
+    }
+  if (rb == 2) KV4_LAUNCH(1, 2, 8)
+  if (rb == 4) KV4_LAUNCH(1, 4, 8)
+  if (waves == 8) KV4_LAUNCH(1, 1, 8)
+  KV4_LAUNCH(1, 1, 4)
 #undef KV4_LAUNCH
 }
 
@@ -892,7 +907,6 @@ int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
   a.G = nq / nkv;
   a.min_run = min_run;
   a.inv_nkv = 1.0f / nkv;
-  a.inv_grid = 1.0f / grid;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = part;
   a.counters = counters;
@@ -929,7 +943,6 @@ int ko_kv4_attn_qkv(const void* qkv, const void* q_w, const void* k_w, const voi
   a.G = nq / nkv;
   a.min_run = min_run;
   a.inv_nkv = 1.0f / nkv;
-  a.inv_grid = 1.0f / grid;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = part;
   a.counters = counters;

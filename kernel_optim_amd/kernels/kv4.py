@@ -229,7 +229,7 @@ class Kv4Attention:
     """
 
     MAX_T = 8
-    GRID = 512     # workgroups: two on each of the 256 CUs
+    GRID = 512     # workgroups of 4 wavefronts: two on each of the 256 CUs
     MIN_RUN = 8    # least steps of 32 keys in a workgroup's run
 
     def __init__(self, B, T, cap, nq, nkv, d, device, group=32):

@@ -431,3 +431,29 @@ def test_runs_repeat_bit_for_bit(dev):
     for o in outs:
         plan.with_lengths(q, cache, ln, o)
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("d,group", FORMATS)
+def test_a_workgroup_of_8_wavefronts_a_pair(dev, d, group):
+    """129 to 256 pairs, and blocks of 16 query rows: lengths that keep to one part, that are cut,
+    and that share a run."""
+    attend(dev, 40, 1, 16, 4, d, group, 200, [200] * 40)
+    attend(dev, 43, 1, 15, 5, d, group, 700, [(97 * i) % 700 for i in range(43)])
+    attend(dev, 3, 5, 8, 2, d, group, 2100, [2100, 1, 300])
+
+
+def test_decode_qkv_of_many_pairs(dev):
+    B, nq, nkv, d, group, cap, eps = 40, 16, 4, 128, 32, 128, 1e-6
+    pos = [(5 * i) % cap for i in range(B)]
+    old = filled(B, nkv, cap, d, group, pos, 80)
+    qkv, q_w, k_w, cos, sin = step_inputs(81, B, 1, nq, nkv, d, cap, dev)
+    at = torch.tensor(pos, dtype=torch.int32, device=dev)
+    cache, out = old.to(dev), torch.empty(B, nq * d, dtype=BF16, device=dev)
+    plan = Kv4Attention(B, 1, cap, nq, nkv, d, dev, group=group)
+    plan.decode_qkv(qkv, q_w, k_w, cos, sin, at, cache, out, eps)
+    check_appended(cache, old, qkv, k_w, cos, sin, pos, 1, eps, nq, nkv, d, group)
+    q = torch.empty_like(out)
+    kv4_append(qkv, q_w, k_w, cos, sin, at, q, old.to(dev), 1, eps, nq, nkv, d)
+    want, mid, size = O.attention(q, cache, [p + 1 for p in pos], 1, nq, d, group)
+    tol = want.abs() * 2.0 ** -8 + mid * 2.0 ** -8 + size * (2.0 ** -13 + 2.0 ** -7)
+    assert ((out.cpu().double() - want).abs() <= tol).all()
