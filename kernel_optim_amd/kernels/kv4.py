@@ -112,40 +112,44 @@ def _check_rows(cache, k, v, start, lengths, written, names):
 
 
 def _ints(t, B, dev):
-    return t is None or (_is(t, torch.int32, (B,)) and t.get_device() == dev)
+    return t is None or (t.dtype is torch.int32 and t.get_device() == dev and t.shape == (B,)
+                         and t.is_contiguous())
+
+
+def _usual(cache, k, v, start, lengths, written):
+    """Whether a call needs no closer look: contiguous outputs, and inputs whose strides suit as they
+    are. Tests that could name each fault take 25 us, more than a prompt of 500 tokens
+    on the GPU; these take 4."""
+    try:
+        B, nkv, nb, size = cache.shape
+        fmt = _FORMATS.get(size)
+        k0, k1, k2, k3 = k.stride()
+        v0, v1, v2, v3 = v.stride()
+        dev = cache.get_device()
+        return (fmt is not None and k.shape == v.shape == (B, nkv, k.shape[2], fmt[0])
+                and cache.dtype is torch.uint8 and k.dtype is BF16 and v.dtype is BF16
+                and k3 == 1 and v3 == 1 and (k0 | k1 | k2 | v0 | v1 | v2) % 8 == 0
+                and cache.is_contiguous()
+                and (written or (k.is_contiguous() and v.is_contiguous()))
+                and (cache.data_ptr() | k.data_ptr() | v.data_ptr()) % 16 == 0
+                and dev == k.get_device() == v.get_device() == torch.cuda.current_device()
+                and B > 0 and nkv > 0 and nb > 0 and _ints(start, B, dev)
+                and _ints(lengths, B, dev))
+    except (AttributeError, ValueError, IndexError, RuntimeError):
+        return False   # no tensors of these dimensions: _check_rows says which
 
 
 def _rows(cache, k, v, start, lengths, written, names):
-    """The checked C arguments of kv4_write and kv4_read. One test over everything passes the
-    usual call (a prompt of one token costs more in checks that could name each fault, 25 us,
-    than on the GPU); where it does not, _check_rows decides."""
-    if not (isinstance(cache, torch.Tensor) and isinstance(k, torch.Tensor)
-            and isinstance(v, torch.Tensor) and cache.dim() == 4 and k.dim() == 4
-            and cache.shape[3] in _FORMATS):
+    """The checked C arguments of kv4_write and kv4_read."""
+    if _usual(cache, k, v, start, lengths, written):
+        c, ks, vs = cache.stride()[:2], k.stride()[:3], v.stride()[:3]
+    else:
         _check_rows(cache, k, v, start, lengths, written, names)
+        c, ks, vs = _outer(cache)[:2], _outer(k), _outer(v)   # single rows' strides may be odd
     B, nkv, nb, size = cache.shape
-    d, group = _FORMATS[size]
     S = k.shape[2]
-    dev = cache.get_device()
-    k0, k1, k2, k3 = k.stride()
-    v0, v1, v2, v3 = v.stride() if v.dim() == 4 else (0, 0, 0, 0)
-    if not (cache.is_cuda and k.is_cuda and v.is_cuda and cache.dtype is torch.uint8
-            and k.dtype is BF16 and v.dtype is BF16 and cache.is_contiguous() and B and nkv and nb
-            and k.shape == v.shape == (B, nkv, S, d) and k3 == 1 and v3 == 1
-            and (k0 | k1 | k2 | v0 | v1 | v2) % 8 == 0
-            and (written or (k.is_contiguous() and v.is_contiguous()))
-            and (cache.data_ptr() | k.data_ptr() | v.data_ptr()) % 16 == 0
-            and dev == k.get_device() == v.get_device() == torch.cuda.current_device()
-            and _ints(start, B, dev) and _ints(lengths, B, dev)):
-        _check_rows(cache, k, v, start, lengths, written, names)
-    c0, c1, _, _ = cache.stride()
-    if c0 % 16 or c1 % 16 or (k0 | k1 | k2 | v0 | v1 | v2) % 8:   # strides of single rows
-        c0, c1, _ = _outer(cache)
-        (k0, k1, k2), (v0, v1, v2) = _outer(k), _outer(v)
-    c = cache.data_ptr(), c0, c1
-    kv = k.data_ptr(), k0, k1, k2, v.data_ptr(), v0, v1, v2
-    rest = _lib.ptr(start), _lib.ptr(lengths), B, S, nkv, nb * KV4_KEYS, d, group
-    return S, c, kv, rest
+    return (S, (cache.data_ptr(), *c), (k.data_ptr(), *ks, v.data_ptr(), *vs),
+            (_lib.ptr(start), _lib.ptr(lengths), B, S, nkv, nb * KV4_KEYS, *_FORMATS[size]))
 
 
 def kv4_write(k, v, cache, start=None, lengths=None):
