@@ -385,11 +385,13 @@ int ko_kv4_read(const void* cache, long long cache_b_stride, long long cache_h_s
 /* ko_qk_norm_rope with the quantised append: qkv [M, (nq+2nkv)*d] bf16, M = B*T, row m is
  * sequence m/T at position pos[m/T] + m%T; q_out [M, nq*d] bf16, k and v into the cache's slot
  * at that position. Norm and RoPE run in fp32; q rounds once, k is quantised from fp32.
- * Positions outside [0, max_pos) (max_pos = min(cap, table rows)) are skipped. */
+ * Positions outside [0, max_pos) (max_pos = min(cap, table rows)) are skipped. rope (optional, T = 1,
+ * [M][2][d] bf16, 16-byte aligned): the cos and sin rows at the positions (ko_rope_rows) in place
+ * of the tables'. */
 int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void* cos,
                   const void* sin, const int* pos, void* q_out, void* cache, int M, int T,
                   long long cache_b_stride, long long cache_h_stride, float eps, int nq, int nkv,
-                  int d, int group, int max_pos, void* stream);
+                  int d, int group, int max_pos, const void* rope, void* stream);
 
 /* Decode attention over a 4-bit cache layer: as ko_decode_attn for q [B*T, nq*d] bf16 and out
  * (another buffer), query t of sequence b at position n - T + t of its n = kv_lens[b] + len_offset
@@ -405,15 +407,13 @@ int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
                 void* stream);
 
 /* A decode step's attention straight from the bf16 QKV projection qkv [B, (nq+2nkv)*d] (T = 1):
- * q/k RMSNorm and RoPE at pos[b] in fp32 (q then rounded to bf16), the quantised append of k and v at
- * slot pos[b], and attention over keys 0..pos[b], in one launch. A sequence whose position lies
- * outside [0, min(cap, max_pos)) appends nothing and its out row is zero. rope (optional, [B][2][d]
- * bf16, 16-byte aligned): the cos and sin rows at pos[b] (ko_rope_rows) in place of the tables'.
- * Other arguments as for ko_kv4_attn. */
+ * ko_kv4_append at pos[b] with its q [B, nq*d] bf16 as scratch, then ko_kv4_attn over keys
+ * 0..pos[b]. A sequence whose position lies outside [0, min(cap, max_pos)) appends nothing and its
+ * out row is zero. Other arguments as for those two. */
 int ko_kv4_attn_qkv(const void* qkv, const void* q_w, const void* k_w, const void* cos,
                     const void* sin, int max_pos, const int* pos, void* cache,
                     long long cache_b_stride, long long cache_h_stride, int cap, int B, int nq,
-                    int nkv, int d, int group, float eps, float scale, float* part,
+                    int nkv, int d, int group, float eps, float scale, void* q, float* part,
                     long long part_len, int* counters, int grid, int min_run, void* out,
                     const void* rope, void* stream);
 

@@ -78,12 +78,12 @@ SIGNATURES = {
                     _c_void_p, _c_void_p, _int, _int, _int, _int, _int, _int, _c_void_p],
     "ko_kv4_append": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                       _c_void_p, _int, _int, _ll, _ll, _f, _int, _int, _int, _int, _int,
-                      _c_void_p],
+                      _c_void_p, _c_void_p],
     "ko_kv4_attn": [_c_void_p, _c_void_p, _ll, _ll, _c_void_p, _int, _int, _int, _int, _int, _int,
                     _int, _int, _f, _c_void_p, _ll, _c_void_p, _int, _int, _c_void_p, _c_void_p],
     "ko_kv4_attn_qkv": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _int, _c_void_p,
                         _c_void_p, _ll, _ll, _int, _int, _int, _int, _int, _int, _f, _f, _c_void_p,
-                        _ll, _c_void_p, _int, _int, _c_void_p, _c_void_p, _c_void_p],
+                        _c_void_p, _ll, _c_void_p, _int, _int, _c_void_p, _c_void_p, _c_void_p],
     "ko_kv4_attn_scratch": [_int, _int, _int, _int],
 }
 

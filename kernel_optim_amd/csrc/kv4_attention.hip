@@ -3,10 +3,7 @@
 // Query row (t, h) of sequence b and KV head j, t of T tokens, sees the keys below len - T + t + 1:
 //   score_k = scale sum_g (s_kg sum_{d in g} q_d (n_kd - 8) + c_kg sum_{d in g} q_d)
 //   out_d   = sum_k p_k (c_kg + s_kg (n_kd - 8)) / sum_k p_k,  p_k = exp(score_k - max)
-// A row that sees no key is zero. QKV (a decode step, T = 1): the workgroups take q from the bf16
-// projection themselves (RMSNorm and RoPE in fp32, 4 heads in the registers that hold q
-// anyway), and the wavefront with a pair's last step quantises the new key and value into
-// the cache, uses them from LDS, and reads nothing back. Bound by the bytes of the cache, as long as no more than about
+// A row that sees no key is zero. Bound by the bytes of the cache, as long as no more than about
 // three VALU operations fall on a value; so no value is dequantised:
 //
 // - The codes go to the matrix cores as bf16 128 + n: four bits and a constant, one shift and one
@@ -32,18 +29,26 @@
 // partial sums (fp32, in run order: the result does not depend on who is last).
 #include "kv4_core.h"
 
+#include <limits.h>
+
 #include <type_traits>
 
 using namespace ko;
+
+extern "C" int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void* cos,
+                             const void* sin, const int* pos, void* q_out, void* cache, int M, int T,
+                             long long cache_b_stride, long long cache_h_stride, float eps, int nq,
+                             int nkv, int d, int group, int max_pos, const void* rope,
+                             void* stream);
 
 namespace {
 
 constexpr float TAU = 8.0f;            // a running maximum is raised by more than 2^8 only
 constexpr float NEG_BIG = -1.0e30f;
-// Up to SOLO steps a pair is not cut: its 4 steps a wavefront take less than the partial sums'
+// Up to SOLO steps a pair is not cut: its 5 steps a wavefront take less than the partial sums'
 // way through memory (one sequence of 512 keys 6.7 against 8.0 us in two parts; 1000 keys 9.8
 // against 8.6 us in four).
-constexpr int SOLO = 16;
+constexpr int SOLO = 20;
 constexpr int PAIR_STEPS = 12;         // what a pair costs beside its steps, in steps
 
 struct Kv4AttnArgs {
@@ -57,27 +62,12 @@ struct Kv4AttnArgs {
   float* part;    // [2 * grid][rows][D], then [2 * grid][rows][2]
   int* counters;  // [grid], zero; left zero
   uint16_t* out;
-  // decode step (QKV): q and the new key from the projection, T = 1
-  const uint16_t* qkv;   // [B, (nq + 2 nkv)*D]
-  const uint16_t* qw;
-  const uint16_t* kw;
-  const uint16_t* cosb;  // [max_pos, D]
-  const uint16_t* sinb;
-  const uint16_t* rope;  // [B][2][D]: the rows of cosb and sinb at the positions, or null
-  int max_pos;
-  float eps;
+  long long most;  // a sequence of more keys has none
 };
 
-// Keys of sequence b. QKV: a position outside the cache or the RoPE tables has none, so nothing
-// is appended and its row is zero.
-template <bool QKV>
 __device__ __forceinline__ int seq_keys(const Kv4AttnArgs& a, int b) {
-  if (QKV) {
-    const int p = a.lens[b];
-    return p >= 0 && p < min(a.cap, a.max_pos) ? p + 1 : 0;
-  }
   const long long n = (long long)a.lens[b] + a.len_off;
-  return (int)(n < 0 ? 0 : n < a.cap ? n : a.cap);
+  return (int)(n < 0 || n > a.most ? 0 : n < a.cap ? n : a.cap);
 }
 __device__ __forceinline__ int steps_of(int keys) { return keys > 0 ? (keys + 31) >> 5 : 1; }
 
@@ -188,58 +178,9 @@ struct Block {
   }
 };
 
-__device__ __forceinline__ void unpack8(const uint16_t* p, float (&y)[8]) {
-  const uint4 x = ldg16(p);
-  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) y[2 * e] = bf16lo(u[e]), y[2 * e + 1] = bf16hi(u[e]);
-}
-
-// RMSNorm with gain w and RoPE of the head at x, in fp32: lane group kg holds the values 32 i + 8 kg
-// .. + 7, the four groups the whole head; rotate_half's partner is I / 2 steps away.
-template <int D>
-__device__ __forceinline__ void norm_rope(const uint16_t* x, const uint16_t* w, const uint16_t* cs,
-                                          const uint16_t* sn, float eps, int kg,
-                                          float (&y)[D / 32][8]) {
-  constexpr int I = D / 32;
-  float v[I][8], ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < I; ++i) {
-    unpack8(x + 32 * i + 8 * kg, v[i]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(v[i][e], v[i][e], ss);
-  }
-  const float rstd = rsqrtf(sum_xor32(sum_xor16(ss)) * (1.0f / D) + eps);
-#pragma unroll
-  for (int i = 0; i < I; ++i) {
-    float g[8];
-    unpack8(w + 32 * i + 8 * kg, g);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * rstd * g[e];
-  }
-#pragma unroll
-  for (int i = 0; i < I; ++i) {
-    float c[8], s[8];
-    unpack8(cs + 32 * i + 8 * kg, c);
-    unpack8(sn + 32 * i + 8 * kg, s);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      y[i][e] = v[i][e] * c[e] + (i < I / 2 ? -v[i + I / 2][e] : v[i - I / 2][e]) * s[e];
-  }
-}
-
-// The new key's codes and scales, between the wavefront that makes them at its start and the same
-// wavefront's last step.
-template <int D, int NG>
-struct NewKey {
-  uint32_t k[4][D / 32];        // lane group, step
-  uint16_t v[D / 64][16];       // plane, n
-  uint32_t sc[2][NG];
-};
-
 // RB: blocks of 16 query rows (above 1 with GPT = 1): wavefront w serves rows 16 (w % RB) ..,
 // and the steps w / RB, w / RB + 4 / RB, ... of a run.
-template <int D, int NG, int GPT, int RB, int WAVES, bool QKV>
+template <int D, int NG, int GPT, int RB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
   constexpr int I = D / 32, IPG = I / NG, NT = NG / GPT, RP = 16 / GPT, J = D / 16;
   constexpr int NWP = WAVES / RB, ROWS = RB * RP;
@@ -248,7 +189,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   __shared__ __align__(16) float lds_o[WAVES][RP][D];
   __shared__ float lds_ml[WAVES][RP][2];
   __shared__ int lds_prev;
-  __shared__ NewKey<D, NG> lds_new[QKV ? RB : 1];
 
   const int wave = uniform(threadIdx.x >> 6), lane0 = threadIdx.x & 63;
   const int rb = wave % RB, wp = wave / RB;
@@ -260,7 +200,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   // Lane b holds the keys, steps and places of sequence b of the first 64.
   int my_len = 0, all = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int len = b0 + lane0 < a.B ? seq_keys<QKV>(a, b0 + lane0) : 0;
+    const int len = b0 + lane0 < a.B ? seq_keys(a, b0 + lane0) : 0;
     if (b0 == 0) my_len = len;
     all += readlane(wave_incl_scan(b0 + lane0 < a.B ? steps_of(len) : 0), 63);
   }
@@ -300,7 +240,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   if (!whole) {
     total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int len = b0 == 0 ? my_len : b0 + lane0 < a.B ? seq_keys<QKV>(a, b0 + lane0) : 0;
+      const int len = b0 == 0 ? my_len : b0 + lane0 < a.B ? seq_keys(a, b0 + lane0) : 0;
       const int st = b0 + lane0 < a.B ? places(len) : 0;
       const int in = wave_incl_scan(st);
       total += readlane(in, 63);
@@ -331,7 +271,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       } else {
         int below = 0;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
-          const int l = b0 + lane0 < a.B ? seq_keys<QKV>(a, b0 + lane0) : 0;
+          const int l = b0 + lane0 < a.B ? seq_keys(a, b0 + lane0) : 0;
           const int st = b0 + lane0 < a.B ? places(l) : 0;
           const int incl = wave_incl_scan(st) + below;
           const int k = uniform(__popcll(__ballot(incl <= pair_step && b0 + lane0 < a.B)));
@@ -403,100 +343,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     const int hh = r / GPT, gg = r % GPT;
     const int row = min(rb * RP + hh, R - 1);  // rows past R repeat the last; they are not stored
     const int t = a.T == 1 ? 0 : row / a.G, h = row - t * a.G;
-    [[maybe_unused]] const uint8_t* base = base_of(g);
-
     // q: column (row, group): zeros outside the group
     uint32_t q[I][4];
-    const bool has_new = QKV && len > 0 && st1 == n && (n - 1 - st0) % NWP == wp;  // uniform
-    if constexpr (QKV) {
-      const int heads = (a.G + 2) * a.nkv;
-      const uint16_t* src = a.qkv + (long long)b * heads * D;
-      const int p = max(len - 1, 0);
-      const uint16_t* cs = a.rope ? a.rope + (long long)b * 2 * D : a.cosb + (long long)p * D;
-      const uint16_t* sn = a.rope ? cs + D : a.sinb + (long long)p * D;
-      float y[I][8];
-      norm_rope<D>(src + (kvh * a.G + h) * D, a.qw, cs, sn, a.eps, kg, y);
+    const uint16_t* qp = a.q + (((long long)b * a.T + t) * a.nkv * a.G + kvh * a.G + h) * D;
 #pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const bool mine = i / IPG % GPT == gg;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[i][e] = mine ? pack_bf16x2(y[i][2 * e], y[i][2 * e + 1]) : 0u;
-      }
-      if (has_new) {  // quantise the new key and value into the LDS, and one of them into the cache
-        NewKey<D, NG>& nk = lds_new[rb];
-        const bool stores = rb == 0;
-        uint8_t* dst = const_cast<uint8_t*>(base) + (long long)(n - 1) * kv4_block_bytes(D, NG);
-        uint32_t* dsc = reinterpret_cast<uint32_t*>(dst + 32 * D);
-        const int key = p & 31;
-        norm_rope<D>(src + (a.G * a.nkv + kvh) * D, a.kw, cs, sn, a.eps, kg, y);
-        uint32_t w[I];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float mn = y[g * IPG][0], mx = mn;
-#pragma unroll
-          for (int i = g * IPG; i < (g + 1) * IPG; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mn = kv4_min(mn, y[i][e]), mx = kv4_max(mx, y[i][e]);
-          kv4_minmax_xor16(mn, mx);
-          kv4_minmax_xor32(mn, mx);
-          Kv4Group gr;
-          gr.from(mn, mx);
-#pragma unroll
-          for (int i = g * IPG; i < (g + 1) * IPG; ++i) {
-            w[i] = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[i] |= gr.code(y[i][e]) << (4 * (e / 2) + 16 * (e & 1));
-          }
-          if (lane == 0) nk.sc[0][g] = gr.sc;
-          if (lane == 0 && stores) dsc[g * 32 + key] = gr.sc;
-        }
-        if (r == 0) {
-#pragma unroll
-          for (int i = 0; i < I; ++i) {
-            nk.k[kg][i] = w[i];
-            if (stores) reinterpret_cast<uint32_t*>(dst + key * (D / 2) + kg * (D / 8))[i] = w[i];
-          }
-        }
-        // v: lane n = r holds the columns 32 i + 2 n, + 1
-        uint32_t x[I], half[D / 64] = {};
-        const uint16_t* vsrc = src + ((a.G + 1) * a.nkv + kvh) * D + 2 * r;
-#pragma unroll
-        for (int i = 0; i < I; ++i) x[i] = *reinterpret_cast<const uint32_t*>(vsrc + 32 * i);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float mn = bf16lo(x[g * IPG]), mx = mn;
-#pragma unroll
-          for (int i = g * IPG; i < (g + 1) * IPG; ++i) {
-            mn = kv4_min(kv4_min(mn, bf16lo(x[i])), bf16hi(x[i]));
-            mx = kv4_max(kv4_max(mx, bf16lo(x[i])), bf16hi(x[i]));
-          }
-          Kv4Group gr;
-          gr.from(kv4_min_row16(mn), kv4_max_row16(mx));
-#pragma unroll
-          for (int i = g * IPG; i < (g + 1) * IPG; ++i)
-            half[i / 2] |= (gr.code(bf16lo(x[i])) | gr.code(bf16hi(x[i])) << 4) << (8 * (i & 1));
-          if (lane == 0) nk.sc[1][g] = gr.sc;
-          if (lane == 0 && stores) dsc[(NG + g) * 32 + key] = gr.sc;
-        }
-        if (kg == 0) {
-#pragma unroll
-          for (int pl = 0; pl < D / 64; ++pl) {
-            nk.v[pl][r] = (uint16_t)half[pl];
-            if (stores)
-              *reinterpret_cast<uint16_t*>(dst + 16 * D + ((key / 8 * (D / 64) + pl) * 16 + r) * 16 +
-                                           key % 8 * 2) = (uint16_t)half[pl];
-          }
-        }
-      }
-    } else {
-      const uint16_t* qp = a.q + (((long long)b * a.T + t) * a.nkv * a.G + kvh * a.G + h) * D;
-#pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const uint4 x = ldg16(qp + 32 * i + 8 * kg);
-        const bool mine = i / IPG % GPT == gg;
-        q[i][0] = mine ? x.x : 0u, q[i][1] = mine ? x.y : 0u;
-        q[i][2] = mine ? x.z : 0u, q[i][3] = mine ? x.w : 0u;
-      }
+    for (int i = 0; i < I; ++i) {
+      const uint4 x = ldg16(qp + 32 * i + 8 * kg);
+      const bool mine = i / IPG % GPT == gg;
+      q[i][0] = mine ? x.x : 0u, q[i][1] = mine ? x.y : 0u;
+      q[i][2] = mine ? x.z : 0u, q[i][3] = mine ? x.w : 0u;
     }
     float cq[NT];  // sum of q over the group of this lane's column in tile u
 #pragma unroll
@@ -510,8 +365,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     }
     const float tau = TAU / a.scale_log2;
     const int lim = len - a.T + t + 1;      // keys that this lane's row sees
-    // keys that every row sees; the step with the new key is one of the masked ones
-    const int full = QKV ? min(len, (n - 1) * KV4_KEYS) : len - a.T + 1;
+    const int full = len - a.T + 1;         // keys that every row sees
 
     f32x4 acc[J];
 #pragma unroll
@@ -525,30 +379,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       constexpr bool masked = decltype(masked_)::value;
       uint32_t* lsc = lds_sc[wave];
       x.scales_to(lsc, lane);
-      if constexpr (QKV && masked)
-        if (has_new && st == n - 1) {  // what was loaded of the new key's slot is older
-          const int key = (len - 1) & 31;
-          const NewKey<D, NG>& nk = lds_new[rb];
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-          if (lane < 2 * NG) lsc[lane * 32 + key] = nk.sc[lane / NG][lane % NG];
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            if (8 * (r >> 2) + (r & 3) + 4 * c == key)
-#pragma unroll
-              for (int i = 0; i < I; ++i) x.k[c][i] = nk.k[kg][i];
-          if (kg == key / 8) {
-#pragma unroll
-            for (int pl = 0; pl < D / 64; ++pl) {
-              const uint32_t w = nk.v[pl][r];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (e == key % 8 / 2)
-                  x.v[pl][e] = key & 1 ? (x.v[pl][e] & 0xffffu) | w << 16
-                                       : (x.v[pl][e] & 0xffff0000u) | w;
-            }
-          }
-        }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -820,7 +650,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // (ragged 64 109 and 119 us).
 int waves_for(int rb, long long pairs) { return rb > 1 || (pairs > 128 && pairs <= 256) ? 8 : 4; }
 
-template <int D, int NG, bool QKV>
+template <int D, int NG>
 int launch(const Kv4AttnArgs& a, int grid, hipStream_t s) {
   const int rows = a.T * a.G;
   const int gpt = tile_groups(rows, NG), rb = row_blocks(rows);
@@ -828,7 +658,7 @@ int launch(const Kv4AttnArgs& a, int grid, hipStream_t s) {
   const dim3 g(waves == 8 ? (grid + 1) / 2 : grid), blk(64 * waves);
 #define KV4_LAUNCH(GPT_, RB_, WAVES_)                                                       \
   {                                                                                         \
-    hipLaunchKernelGGL((kv4_attn_kernel<D, NG, GPT_, RB_, WAVES_, QKV>), g, blk, 0, s, a);  \
+    hipLaunchKernelGGL((kv4_attn_kernel<D, NG, GPT_, RB_, WAVES_>), g, blk, 0, s, a);       \
     return KO_LAUNCH_STATUS();                                                              \
   }
   if constexpr (NG == 4)
@@ -855,16 +685,16 @@ long long scratch_floats(int rows, int d, int group, int grid) {
 }
 
 // What the two entry points check alike.
-int check(const void* cache, long long cb, long long ch, const int* lens, int cap, int B, int T,
+int check(const void* q, const void* cache, long long cb, long long ch, const int* lens, int cap, int B, int T,
           int nq, int nkv, int d, int group, float scale, const float* part, long long part_len,
           const int* counters, int grid, int min_run, const void* out) {
-  if (!cache || !lens || !out || !part || !counters || B < 1 || T < 1 || nkv < 1 || nq < 1 ||
+  if (!q || !cache || !lens || !out || !part || !counters || B < 1 || T < 1 || nkv < 1 || nq < 1 ||
       cap < 1 || grid < 1 || min_run < 1)
     return KO_EINVAL;
   if (!(scale > 0.f && scale < 1.0e4f)) return KO_EINVAL;
   if (!kv4_served(d, group) || nq % nkv || T > 64 || T * (long long)(nq / nkv) > 64)
     return KO_ENOTSUP;
-  if (!aligned16(cache) || !aligned16(out) || (cb & 15) || (ch & 15) ||
+  if (!aligned16(q) || !aligned16(cache) || !aligned16(out) || (cb & 15) || (ch & 15) ||
       (reinterpret_cast<uintptr_t>(part) & 7))
     return KO_EINVAL;
   if (part_len < scratch_floats(T * (nq / nkv), d, group, grid)) return KO_ERANGE;
@@ -874,6 +704,24 @@ int check(const void* cache, long long cb, long long ch, const int* lens, int ca
       (long long)B * nkv > ((1LL << 24) - grid - min_run) / (blocks + PAIR_STEPS))
     return KO_ERANGE;
   return KO_OK;
+}
+
+int attention(const void* q, const void* cache, long long cb, long long ch, const int* lens,
+              int len_off, int cap, long long most, int B, int T, int nq, int nkv, int d, int group,
+              float scale, float* part, long long part_len, int* counters, int grid, int min_run,
+              void* out, void* stream) {
+  const int st = check(q, cache, cb, ch, lens, cap, B, T, nq, nkv, d, group, scale, part, part_len,
+                       counters, grid, min_run, out);
+  if (st) return st;
+  const Kv4AttnArgs a = {static_cast<const uint16_t*>(q), static_cast<const uint8_t*>(cache), cb, ch,
+                         lens, len_off, cap, B, T, nkv, nq / nkv, min_run, 1.0f / nkv,
+                         scale * 1.4426950408889634f, part, counters, static_cast<uint16_t*>(out),
+                         most};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define CALL(D_, NG_) return launch<D_, NG_>(a, grid, s);
+  KV4_PICK(d, group, CALL)
+#undef CALL
+  return KO_ENOTSUP;
 }
 
 }  // namespace
@@ -889,77 +737,25 @@ int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
                 int T, int nq, int nkv, int d, int group, float scale, float* part,
                 long long part_len, int* counters, int grid, int min_run, void* out,
                 void* stream) {
-  const int st = check(cache, cache_b_stride, cache_h_stride, kv_lens, cap, B, T, nq, nkv, d, group,
-                       scale, part, part_len, counters, grid, min_run, out);
-  if (st) return st;
-  if (!q || !aligned16(q)) return KO_EINVAL;
-  Kv4AttnArgs a = {};
-  a.q = static_cast<const uint16_t*>(q);
-  a.cache = static_cast<const uint8_t*>(cache);
-  a.cb = cache_b_stride;
-  a.ch = cache_h_stride;
-  a.lens = kv_lens;
-  a.len_off = len_offset;
-  a.cap = cap;
-  a.B = B;
-  a.T = T;
-  a.nkv = nkv;
-  a.G = nq / nkv;
-  a.min_run = min_run;
-  a.inv_nkv = 1.0f / nkv;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.part = part;
-  a.counters = counters;
-  a.out = static_cast<uint16_t*>(out);
-  hipStream_t s = static_cast<hipStream_t>(stream);
-#define CALL(D_, NG_) return launch<D_, NG_, false>(a, grid, s);
-  KV4_PICK(d, group, CALL)
-#undef CALL
-  return KO_ENOTSUP;
+  return attention(q, cache, cache_b_stride, cache_h_stride, kv_lens, len_offset, cap, LLONG_MAX, B, T,
+                   nq, nkv, d, group, scale, part, part_len, counters, grid, min_run, out, stream);
 }
 
 int ko_kv4_attn_qkv(const void* qkv, const void* q_w, const void* k_w, const void* cos,
                     const void* sin, int max_pos, const int* pos, void* cache,
                     long long cache_b_stride, long long cache_h_stride, int cap, int B, int nq,
-                    int nkv, int d, int group, float eps, float scale, float* part,
+                    int nkv, int d, int group, float eps, float scale, void* q, float* part,
                     long long part_len, int* counters, int grid, int min_run, void* out,
                     const void* rope, void* stream) {
-  const int st = check(cache, cache_b_stride, cache_h_stride, pos, cap, B, 1, nq, nkv, d, group,
+  const int st = check(q, cache, cache_b_stride, cache_h_stride, pos, cap, B, 1, nq, nkv, d, group,
                        scale, part, part_len, counters, grid, min_run, out);
   if (st) return st;
-  if (!qkv || !q_w || !k_w || !cos || !sin || max_pos < 1 || !aligned16(qkv) || !aligned16(q_w) ||
-      !aligned16(k_w) || !aligned16(cos) || !aligned16(sin) || (rope && !aligned16(rope)))
-    return KO_EINVAL;
-  Kv4AttnArgs a = {};
-  a.cache = static_cast<const uint8_t*>(cache);
-  a.cb = cache_b_stride;
-  a.ch = cache_h_stride;
-  a.lens = pos;
-  a.len_off = 1;
-  a.cap = cap;
-  a.B = B;
-  a.T = 1;
-  a.nkv = nkv;
-  a.G = nq / nkv;
-  a.min_run = min_run;
-  a.inv_nkv = 1.0f / nkv;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.part = part;
-  a.counters = counters;
-  a.out = static_cast<uint16_t*>(out);
-  a.qkv = static_cast<const uint16_t*>(qkv);
-  a.qw = static_cast<const uint16_t*>(q_w);
-  a.kw = static_cast<const uint16_t*>(k_w);
-  a.cosb = static_cast<const uint16_t*>(cos);
-  a.sinb = static_cast<const uint16_t*>(sin);
-  a.rope = static_cast<const uint16_t*>(rope);
-  a.max_pos = max_pos;
-  a.eps = eps;
-  hipStream_t s = static_cast<hipStream_t>(stream);
-#define CALL(D_, NG_) return launch<D_, NG_, true>(a, grid, s);
-  KV4_PICK(d, group, CALL)
-#undef CALL
-  return KO_ENOTSUP;
+  const int limit = cap < max_pos ? cap : max_pos;
+  const int ap = ko_kv4_append(qkv, q_w, k_w, cos, sin, pos, q, cache, B, 1, cache_b_stride,
+                               cache_h_stride, eps, nq, nkv, d, group, limit, rope, stream);
+  if (ap) return ap;
+  return attention(q, cache, cache_b_stride, cache_h_stride, pos, 1, cap, limit, B, 1, nq, nkv, d,
+                   group, scale, part, part_len, counters, grid, min_run, out, stream);
 }
 
 }  // extern "C"

@@ -274,7 +274,7 @@ __global__ __launch_bounds__(NT) void kv4_append_kernel(
     const uint16_t* __restrict__ kw, const uint16_t* __restrict__ cosb,
     const uint16_t* __restrict__ sinb, const int* __restrict__ pos, uint16_t* __restrict__ q_out,
     uint8_t* __restrict__ cache, int M, int T, long long cb, long long ch, float eps, int nq,
-    int nkv, int max_pos) {
+    int nkv, int max_pos, const uint16_t* __restrict__ rope) {
   constexpr int HP = D / 64, IPG = D / 32 / NG;
   const int lane = threadIdx.x & 63, l = lane & (D / 2 - 1);
   const int nh = nq + 2 * nkv;
@@ -289,8 +289,9 @@ __global__ __launch_bounds__(NT) void kv4_append_kernel(
   const bool is_v = hd >= nq + nkv;
   if (!is_v) {
     const uint32_t w = reinterpret_cast<const uint32_t*>(hd < nq ? qw : kw)[l];
-    const uint32_t cw = reinterpret_cast<const uint32_t*>(cosb + p * D)[l];
-    const uint32_t sw = reinterpret_cast<const uint32_t*>(sinb + p * D)[l];
+    const uint32_t cw = reinterpret_cast<const uint32_t*>(rope ? rope + 2LL * b * D : cosb + p * D)[l];
+    const uint32_t sw =
+        reinterpret_cast<const uint32_t*>(rope ? rope + (2LL * b + 1) * D : sinb + p * D)[l];
     // 64 lanes add the squares of a head once (d = 128) or twice (d = 64)
     const float rstd = rsqrtf(wave_sum(x0 * x0 + x1 * x1) * (1.0f / 128.0f) + eps);
     const float n0 = x0 * rstd * bf16lo(w), n1 = x1 * rstd * bf16hi(w);
@@ -392,9 +393,10 @@ int ko_kv4_read(const void* cache, long long cache_b_stride, long long cache_h_s
 int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void* cos,
                   const void* sin, const int* pos, void* q_out, void* cache, int M, int T,
                   long long cache_b_stride, long long cache_h_stride, float eps, int nq, int nkv,
-                  int d, int group, int max_pos, void* stream) {
+                  int d, int group, int max_pos, const void* rope, void* stream) {
   if (!qkv || !q_w || !k_w || !cos || !sin || !pos || !q_out || !cache) return KO_EINVAL;
   if (M < 1 || T < 1 || M % T || nq < 1 || nkv < 1 || max_pos < 1) return KO_EINVAL;
+  if (rope && (T != 1 || !aligned(rope, 16))) return KO_EINVAL;
   if (!kv4_served(d, group)) return KO_ENOTSUP;
   if (!aligned(qkv, 16) || !aligned(q_w, 16) || !aligned(k_w, 16) || !aligned(cos, 16) ||
       !aligned(sin, 16) || !aligned(q_out, 16) || !aligned(cache, 16) || (cache_b_stride & 15) ||
@@ -410,7 +412,7 @@ int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void*
                      static_cast<const uint16_t*>(k_w), static_cast<const uint16_t*>(cos),     \
                      static_cast<const uint16_t*>(sin), pos, static_cast<uint16_t*>(q_out),    \
                      static_cast<uint8_t*>(cache), M, T, cache_b_stride, cache_h_stride, eps,  \
-                     nq, nkv, max_pos);
+                     nq, nkv, max_pos, static_cast<const uint16_t*>(rope));
   KV4_PICK(d, group, CALL)
 #undef CALL
   return KO_LAUNCH_STATUS();

@@ -220,7 +220,7 @@ def kv4_append(qkv, q_w, k_w, cos, sin, pos, q_out, cache, T, eps, nq, nkv, d):
         cb, ch, _ = _outer(cache)
     _lib.call("ko_kv4_append", qkv.data_ptr(), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
               sin.data_ptr(), pos.data_ptr(), q_out.data_ptr(), cache.data_ptr(), B * T, T, cb, ch,
-              eps, nq, nkv, d, group, min(nb * KV4_KEYS, cos.shape[0], sin.shape[0]),
+              eps, nq, nkv, d, group, min(nb * KV4_KEYS, cos.shape[0], sin.shape[0]), None,
               _lib.stream_ptr())
 
 
@@ -257,6 +257,7 @@ class Kv4Attention:
                                  dtype=torch.float32, device=dev)
         self._counters = torch.zeros(self.grid, dtype=torch.int32, device=dev)
         torch.cuda.current_stream(dev).synchronize()
+        self._q = torch.empty(B, nq * d, dtype=BF16, device=dev) if T == 1 else None
         self._q_shape = torch.Size((B * T, nq * d))
         self._cache_shape = torch.Size((B, nkv, self.blocks, self.block_bytes))
         self._len_shape = torch.Size((B,))
@@ -302,7 +303,7 @@ class Kv4Attention:
 
     def decode_qkv(self, qkv, q_w, k_w, cos, sin, pos, cache, out, eps, rope=None):
         """A decode step's attention (T = 1) straight from the bf16 QKV projection [B, (nq+2nkv)*d]:
-        kv4_append at pos[b] and attention over keys 0..pos[b] in one launch. A sequence whose
+        kv4_append at pos[b], then attention over keys 0..pos[b]. A sequence whose
         position lies outside the cache or the RoPE tables appends nothing and its row of
         out is zero. rope ([B, 2, d] bf16, optional): the cos and sin rows at pos[b], as
         fused.rope_rows writes them."""
@@ -325,5 +326,5 @@ class Kv4Attention:
         _lib.call("ko_kv4_attn_qkv", qkv.data_ptr(), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
                   sin.data_ptr(), min(cos.shape[0], sin.shape[0]), pos.data_ptr(), cache.data_ptr(),
                   cb, ch, self.cap, B, nq, nkv, d, self.group, eps, self.scale,
-                  self._part.data_ptr(), self._part.numel(), self._counters.data_ptr(), self.grid,
+                  self._q.data_ptr(), self._part.data_ptr(), self._part.numel(), self._counters.data_ptr(), self.grid,
                   self.MIN_RUN, out.data_ptr(), _lib.ptr(rope), _lib.stream_ptr())

@@ -79,10 +79,10 @@ def test_c_rows_refused(kw, status):
 @pytest.mark.parametrize("kw,status", [
     (dict(qkv=None), -22), (dict(cache=None), -22), (dict(M=0), -22), (dict(T=0), -22),
     (dict(M=3, T=2), -22), (dict(nq=0), -22), (dict(nkv=0), -22), (dict(max_pos=0), -22),
-    (dict(d=80), -95), (dict(cache=P + 4), -22), (dict(cb=8), -22), (dict(M=1 << 30), -34)])
+    (dict(M=2, T=2, rope=P), -22), (dict(rope=P + 8), -22), (dict(d=80), -95), (dict(cache=P + 4), -22), (dict(cb=8), -22), (dict(M=1 << 30), -34)])
 def test_c_append_refused(kw, status):
     a = dict(qkv=P, q_w=P, k_w=P, cos=P, sin=P, pos=P, q_out=P, cache=P, M=1, T=1, cb=5120, ch=5120,
-             eps=1e-6, nq=4, nkv=1, d=128, group=32, max_pos=32) | kw
+             eps=1e-6, nq=4, nkv=1, d=128, group=32, max_pos=32, rope=None) | kw
     assert _lib.lib().ko_kv4_append(*a.values(), None) == status
 
 
