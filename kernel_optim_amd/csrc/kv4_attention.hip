@@ -207,28 +207,41 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   auto up = [](int n) { return (n + NWP - 1) / NWP * NWP; };
   const int share = max(a.min_run, quot(all * a.nkv + grid - 1, grid, __builtin_amdgcn_rcpf((float)grid)));
   // (1) Every pair cut into parts of `run` steps, a workgroup for each: with the least run for
-  // which the workgroups suffice, if that is at most a half longer than an equal share.
+  // which the workgroups suffice, if that is at most a half longer than an equal share. One
+  // workgroup on each CU goes before two, which take half as long again as one (4 x 2049 keys, 288
+  // workgroups of 8 steps 11.0 us, 192 of 12 9.4).
   int run = up(share), my_places = 0, my_incl = 0, total = 0;
-  auto fits = [&](int r) {
+  auto parts_of = [&](int r) {
     const int n = steps_of(my_len);
     const int parts = n <= SOLO ? 1 : quot(n + r - 1, r, __builtin_amdgcn_rcpf((float)r));
     my_places = lane0 < a.B ? parts : 0;
     my_incl = wave_incl_scan(my_places);
-    return (long long)readlane(my_incl, 63) * a.nkv <= grid;
+    return (long long)readlane(my_incl, 63) * a.nkv;
   };
-  bool whole = a.B <= 64 && fits(run);
-  if (!whole && a.B <= 64 && fits(run + run / 2 / NWP * NWP)) {
-    int lo = run + NWP, hi = run + run / 2 / NWP * NWP;
+  auto least = [&](int lo, int hi, int most) {  // the least run of lo .. hi that needs at most most
     while (lo < hi) {
       const int mid = lo + (hi - lo) / (2 * NWP) * NWP;
-      if (fits(mid))
+      if (parts_of(mid) <= most)
         hi = mid;
       else
         lo = mid + NWP;
     }
-    whole = true;
-    run = hi;
-    fits(run);
+    return hi;
+  };
+  bool whole = false;
+  if (a.B <= 64) {
+    const int one = WAVES == 4 ? (grid + 1) / 2 : grid;  // workgroups at one on each CU
+    const int longer = run + run / 2 / NWP * NWP;
+    const long long need = parts_of(run);
+    whole = need <= one;
+    if (!whole && parts_of(longer) <= one) {
+      run = least(run + NWP, longer, one);
+      whole = true;
+    } else if (!whole && (need <= grid || parts_of(longer) <= grid)) {
+      run = need <= grid ? run : least(run + NWP, longer, grid);
+      whole = true;
+    }
+    if (whole) parts_of(run);
   }
   // (2) Else one list of all pairs' steps, cut into equal runs that cross from pair to pair.
   // Beginning and ending a pair costs as much as PAIR_STEPS steps: a pair shorter than a
@@ -316,17 +329,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     return;
   }
   auto base_of = [&](const Segment& g) { return a.cache + g.b * a.cb + g.kvh * a.ch; };
-  // steps past the segment's last read it again
   auto block_of = [&](const Segment& g, int st) {
-    return base_of(g) + (long long)min(st, g.st1 - 1) * kv4_block_bytes(D, NG);
+    return base_of(g) + (long long)st * kv4_block_bytes(D, NG);
   };
-  Block<D, NG> x0, x1;  // the wavefront's next two blocks
+  // The wavefront's steps of a segment: st0 + wp, and every NWP-th from there.
+  auto steps_here = [&](const Segment& g) { return (g.st1 - g.st0 - wp + NWP - 1) / NWP; };
+  // Its next two blocks. They change places from step to step; an odd step goes first, in x1, so
+  // that the rest are pairs (x0, x1) and no register moves. Where there are less than two, the
+  // segment's last block is read in their place.
+  Block<D, NG> x0, x1;
   auto load_first = [&](const Segment& g) {
     const int l = fresh_tid() & 63, r = l & 15, kg = l >> 4;
-    x0.load_k(block_of(g, g.st0 + wp), r, kg, l);
-    x0.load_v(block_of(g, g.st0 + wp), r, kg);
-    x1.load_k(block_of(g, g.st0 + wp + NWP), r, kg, l);
-    x1.load_v(block_of(g, g.st0 + wp + NWP), r, kg);
+    const int odd = steps_here(g) & 1, st = g.st0 + wp;
+    const uint8_t* p0 = block_of(g, min(st + odd * NWP, g.st1 - 1));
+    const uint8_t* p1 = block_of(g, min(st + (1 - odd) * NWP, g.st1 - 1));
+    x0.load_k(p0, r, kg, l);
+    x0.load_v(p0, r, kg);
+    x1.load_k(p1, r, kg, l);
+    x1.load_v(p1, r, kg);
   };
 
   // Output row rw of a pair.
@@ -365,7 +385,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     }
     const float tau = TAU / a.scale_log2;
     const int lim = len - a.T + t + 1;      // keys that this lane's row sees
-    const int full = len - a.T + 1;         // keys that every row sees
 
     f32x4 acc[J];
 #pragma unroll
@@ -375,8 +394,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     for (int u = 0; u < NT; ++u) pc[u] = 0.f;
 
     // The running maximum m is kept in units of the unscaled scores.
-    auto step = [&](Block<D, NG>& x, int st, auto masked_) {
-      constexpr bool masked = decltype(masked_)::value;
+    auto step = [&](Block<D, NG>& x, int st, auto masked_, auto ahead_) {
+      constexpr bool masked = decltype(masked_)::value, ahead = decltype(ahead_)::value;
       uint32_t* lsc = lds_sc[wave];
       x.scales_to(lsc, lane);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -411,8 +430,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
           sc[4 * c + e] = sum_lanes<GPT>(v);
         }
       }
-      const uint8_t* next = block_of(g, st + 2 * NWP);
-      x.load_k(next, r, kg, lane);
+      [[maybe_unused]] const uint8_t* next = block_of(g, st + 2 * NWP);
+      if constexpr (ahead) x.load_k(next, r, kg, lane);
       const int k0 = st * KV4_KEYS + 8 * kg;
       if constexpr (masked) {
 #pragma unroll
@@ -443,19 +462,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       }
       // ---- p s, and sum p c ----
       uint32_t ps[NT][4];
+      int seen = lim - k0;
+      if constexpr (masked) asm("" : "+v"(seen));  // compared again, not held from the scores on
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        float y[8];
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          uint32_t w = lsc[32 * NG + (u * GPT + gg) * 32 + 8 * kg + e];
-          if constexpr (masked) w = k0 + e < lim ? w : 0u;  // an unwritten slot's scales may be NaN
-          y[e] = sc[e] * bf16lo(w);
-          pc[u] = fmaf(sc[e], bf16hi(w), pc[u]);
+        for (int u = 0; u < NT; ++u) {
+          const uint32_t* w = lsc + 32 * NG + (u * GPT + gg) * 32 + 8 * kg + 2 * e;
+          uint32_t w0 = w[0], w1 = w[1];
+          if constexpr (masked) {  // an unwritten slot's scales may be NaN
+            w0 = 2 * e < seen ? w0 : 0u;
+            w1 = 2 * e + 1 < seen ? w1 : 0u;
+          }
+          pc[u] = fmaf(sc[2 * e], bf16hi(w0), pc[u]);
+          pc[u] = fmaf(sc[2 * e + 1], bf16hi(w1), pc[u]);
+          ps[u][e] = pack_bf16x2(sc[2 * e] * bf16lo(w0), sc[2 * e + 1] * bf16lo(w1));
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ps[u][e] = pack_bf16x2(y[2 * e], y[2 * e + 1]);
-      }
       // ---- output ----
       const uint32_t off[4] = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};  // -136
 #pragma unroll
@@ -467,30 +489,30 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
         for (int e = 0; e < 4; ++e) vx[e] = codes(x.v[j / 4][e], 4 * (j % 4));
         acc[j] = mfma(ps[j / 2 / IPG / GPT], vx, acc[j]);
       }
-      x.load_v(next, r, kg);
+      if constexpr (ahead) x.load_v(next, r, kg);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
     };
 
-    auto swap = [&] {
-      const Block<D, NG> y = x0;
-      x0 = x1;
-      x1 = y;
-    };
-    int st = st0 + wp;
-    const int unmasked = min(st1, max(full, 0) >> 5);
-    for (; st + NWP < unmasked; st += 2 * NWP) {
-      step(x0, st, std::false_type{});
-      step(x1, st + NWP, std::false_type{});
-    }
-    if (st < unmasked) {
-      step(x0, st, std::false_type{});
-      swap();
-      st += NWP;
-    }
-    for (; st < st1; st += NWP) {
-      step(x0, st, std::true_type{});
-      swap();
+    // A wavefront's last two steps may be masked: rows that see different numbers of keys, at
+    // most 64 apart, and the end of the sequence.
+    using Yes = std::true_type;
+    using No = std::false_type;
+    int st = st0 + wp, left = steps_here(g);
+    if (left == 1) {
+      step(x1, st, Yes{}, No{});
+    } else if (left > 1) {
+      if (left & 1) {
+        step(x1, st, No{}, Yes{});
+        st += NWP;
+        --left;
+      }
+      for (; left > 2; left -= 2, st += 2 * NWP) {
+        step(x0, st, No{}, Yes{});
+        step(x1, st + NWP, No{}, Yes{});
+      }
+      step(x0, st, Yes{}, No{});
+      step(x1, st + NWP, Yes{}, No{});
     }
 
     // the next pair's first blocks come while this one's sums are put together
