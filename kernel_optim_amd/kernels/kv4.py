@@ -174,15 +174,20 @@ def kv4_read(cache, k_out, v_out, start=None, lengths=None):
 
 
 def _check_qkv(qkv, q_w, k_w, cos, sin, pos, rows, B, nq, nkv, d, dev):
-    if (_is(qkv, BF16, (rows, (nq + 2 * nkv) * d)) and _is(q_w, BF16, (d,)) and _is(k_w, BF16, (d,))
-            and _is(pos, torch.int32, (B,)) and isinstance(cos, torch.Tensor) and cos.dim() == 2
-            and cos.shape[0] and _is(cos, BF16, (cos.shape[0], d)) and isinstance(sin, torch.Tensor)
-            and sin.dim() == 2 and sin.shape[0] and _is(sin, BF16, (sin.shape[0], d))
-            and dev == qkv.get_device() == q_w.get_device() == k_w.get_device()
-            == cos.get_device() == sin.get_device() == pos.get_device()
-            and (qkv.data_ptr() | q_w.data_ptr() | k_w.data_ptr() | cos.data_ptr()
-                 | sin.data_ptr()) % 16 == 0):
-        return
+    try:   # the usual call, 1.5 us; the tests below name what is wrong
+        (rc, dc), (rs, ds) = cos.shape, sin.shape
+        if (qkv.shape == (rows, (nq + 2 * nkv) * d) and q_w.shape == k_w.shape == (d,)
+                and pos.shape == (B,) and dc == ds == d and rc > 0 and rs > 0
+                and qkv.dtype is q_w.dtype is k_w.dtype is cos.dtype is sin.dtype is BF16
+                and pos.dtype is torch.int32 and qkv.is_contiguous() and q_w.is_contiguous()
+                and k_w.is_contiguous() and cos.is_contiguous() and sin.is_contiguous()
+                and pos.is_contiguous() and dev == qkv.get_device() == q_w.get_device()
+                == k_w.get_device() == cos.get_device() == sin.get_device() == pos.get_device()
+                and (qkv.data_ptr() | q_w.data_ptr() | k_w.data_ptr() | cos.data_ptr()
+                     | sin.data_ptr()) % 16 == 0):
+            return
+    except (AttributeError, ValueError, TypeError, RuntimeError):
+        pass
     _tensor(qkv, "qkv", BF16, (rows, (nq + 2 * nkv) * d), dev)
     _tensor(q_w, "q_w", BF16, (d,), dev)
     _tensor(k_w, "k_w", BF16, (d,), dev)
