@@ -369,7 +369,8 @@ int ko_gemv_tile(const void* w, void* wt, int rows, int K, void* stream);
  *
  * ko_kv4_write: rows 0 .. lengths[b] - 1 (lengths NULL: S) of k and v [B, nkv, S, d] bf16, inner
  * stride 1, the other strides in elements, multiples of 8, into the slots from start[b] (NULL: 0)
- * on. Rows whose slot lies outside [0, cap) are dropped; other slots keep what they hold.
+ * on; the cache holds ceil(cap / 32) blocks a pair. Rows whose slot lies outside [0, cap) are
+ * dropped; other slots keep what they hold.
  * ko_kv4_read: the reverse; rows past lengths[b] or outside [0, cap) are left as they were. */
 int ko_kv4_write(const void* k, long long k_b_stride, long long k_h_stride, long long k_s_stride,
                  const void* v, long long v_b_stride, long long v_h_stride, long long v_s_stride,
@@ -394,12 +395,14 @@ int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void*
                   int d, int group, int max_pos, const void* rope, void* stream);
 
 /* Decode attention over a 4-bit cache layer: as ko_decode_attn for q [B*T, nq*d] bf16 and out
- * (another buffer), query t of sequence b at position n - T + t of its n = kv_lens[b] + len_offset
- * keys (at most cap). A row that sees no key is zero. nq a multiple of nkv, T * nq / nkv <= 64.
- * The steps of 32 keys of all pairs are dealt out in runs of at least min_run steps to grid
- * workgroups of 4 wavefronts (or half as many of 8). part: fp32 scratch of part_len >= ko_kv4_attn_scratch(T * nq /
- * nkv, d, group, grid); counters [grid] int32, zero before the first call, left zero by every
- * call; calls that share them must not overlap. */
+ * (another buffer), query t of sequence b at position n - T + t, n = kv_lens[b] + len_offset; the
+ * keys are those below min(n, cap), and the cache holds ceil(cap / 32) blocks a pair. A row that
+ * sees no key is zero. nq a multiple of nkv, T * nq / nkv <= 64, 0 < scale < 10^4. The steps of
+ * 32 keys of all pairs are dealt out in runs of at least min_run steps to grid workgroups of 4
+ * wavefronts (or half as many of 8); B * nkv * (blocks + 12) + grid + min_run <= 2^24. part: fp32
+ * scratch of part_len >= ko_kv4_attn_scratch(T * nq / nkv, d, group, grid); counters [grid]
+ * int32, zero before the first call, left zero by every call; calls that share them must not
+ * overlap. */
 int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
                 long long cache_h_stride, const int* kv_lens, int len_offset, int cap, int B,
                 int T, int nq, int nkv, int d, int group, float scale, float* part,

@@ -65,11 +65,15 @@ struct Kv4AttnArgs {
   long long most;  // a sequence of more keys has none
 };
 
-__device__ __forceinline__ int seq_keys(const Kv4AttnArgs& a, int b) {
-  const long long n = (long long)a.lens[b] + a.len_off;
-  return (int)(n < 0 || n > a.most ? 0 : n < a.cap ? n : a.cap);
+// A sequence's length. One that passes the cache's end still says where its query tokens are, as
+// far as cap + T - 1, where all of them see every key.
+__device__ __forceinline__ int seq_len(const Kv4AttnArgs& a, int b) {
+  const long long n = (long long)a.lens[b] + a.len_off, last = a.cap + a.T - 1;
+  return (int)(n < 0 || n > a.most ? 0 : n < last ? n : last);
 }
-__device__ __forceinline__ int steps_of(int keys) { return keys > 0 ? (keys + 31) >> 5 : 1; }
+__device__ __forceinline__ int steps_of(const Kv4AttnArgs& a, int len) {
+  return len > 0 ? (min(len, a.cap) + 31) >> 5 : 1;
+}
 
 // The lane's thread index, opaque: what follows from it is computed where it is used, not
 // ahead of the loop over the pairs, where it would take registers from the steps.
@@ -209,12 +213,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   const int grid = gridDim.x, wg = blockIdx.x;
 
   // ---- which steps this workgroup takes ----
-  // Lane b holds the keys, steps and places of sequence b of the first 64.
+  // Lane b holds the length, steps and places of sequence b of the first 64.
   int my_len = 0, all = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int len = b0 + lane0 < a.B ? seq_keys(a, b0 + lane0) : 0;
+    const int len = b0 + lane0 < a.B ? seq_len(a, b0 + lane0) : 0;
     if (b0 == 0) my_len = len;
-    all += readlane(wave_incl_scan(b0 + lane0 < a.B ? steps_of(len) : 0), 63);
+    all += readlane(wave_incl_scan(b0 + lane0 < a.B ? steps_of(a, len) : 0), 63);
   }
   auto up = [](int n) { return (n + NWP - 1) / NWP * NWP; };
   const int share = max(a.min_run, quot(all * a.nkv + grid - 1, grid, __builtin_amdgcn_rcpf((float)grid)));
@@ -224,7 +228,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   // workgroups of 8 steps 11.0 us, 192 of 12 9.4).
   int run = up(share), my_places = 0, my_incl = 0, total = 0;
   auto parts_of = [&](int r) {
-    const int n = steps_of(my_len);
+    const int n = steps_of(a, my_len);
     const int parts = n <= SOLO ? 1 : quot(n + r - 1, r, __builtin_amdgcn_rcpf((float)r));
     my_places = lane0 < a.B ? parts : 0;
     my_incl = wave_incl_scan(my_places);
@@ -259,13 +263,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
   // Beginning and ending a pair costs as much as PAIR_STEPS steps: a pair shorter than a
   // run, which shares it with others, takes so many more places.
   auto places = [&](int len) {
-    const int n = steps_of(len);
+    const int n = steps_of(a, len);
     return n < share ? n + PAIR_STEPS : n;
   };
   if (!whole) {
     total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int len = b0 == 0 ? my_len : b0 + lane0 < a.B ? seq_keys(a, b0 + lane0) : 0;
+      const int len = b0 == 0 ? my_len : b0 + lane0 < a.B ? seq_len(a, b0 + lane0) : 0;
       const int st = b0 + lane0 < a.B ? places(len) : 0;
       const int in = wave_incl_scan(st);
       total += readlane(in, 63);
@@ -296,7 +300,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       } else {
         int below = 0;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
-          const int l = b0 + lane0 < a.B ? seq_keys(a, b0 + lane0) : 0;
+          const int l = b0 + lane0 < a.B ? seq_len(a, b0 + lane0) : 0;
           const int st = b0 + lane0 < a.B ? places(l) : 0;
           const int incl = wave_incl_scan(st) + below;
           const int k = uniform(__popcll(__ballot(incl <= pair_step && b0 + lane0 < a.B)));
@@ -314,7 +318,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       at += g.kvh * n;
       g.st0 = s - at;
       s = min(at + n, end);
-      g.n = steps_of(g.len);  // behind them, a short pair's places are empty
+      g.n = steps_of(a, g.len);  // behind them, a short pair's places are empty
       g.st1 = min(g.n, s - at);
       g.w0 = at / run;
       g.w1 = (at + g.n - 1) / run;
@@ -328,7 +332,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     if (pair_part >= readlane(my_incl, 63)) return;
     g.b = uniform(__popcll(__ballot(my_incl <= pair_part && lane0 < a.B)));
     g.len = readlane(my_len, g.b);
-    g.n = steps_of(g.len);
+    g.n = steps_of(a, g.len);
     const int parts = readlane(my_places, g.b);
     const int at = wg - (readlane(my_incl, g.b) - parts) * a.nkv;
     g.kvh = uniform(quot(at, parts, __builtin_amdgcn_rcpf((float)parts)));
@@ -396,7 +400,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       cq[u] = c[0];
     }
     const float tau = TAU / a.scale_log2;
-    const int lim = len - a.T + t + 1;      // keys that this lane's row sees
+    const int lim = min(len - a.T + t + 1, a.cap);  // keys that this lane's row sees
 
     f32x4 acc[J];
 #pragma unroll

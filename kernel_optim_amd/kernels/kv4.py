@@ -167,8 +167,10 @@ def kv4_write(k, v, cache, start=None, lengths=None):
 def kv4_read(cache, k_out, v_out, start=None, lengths=None):
     """Read cached keys back: row i of k_out and v_out [B, nkv, S, d] bf16 receives the values
     of slot start[b] + i, i < lengths[b] (None: S); other rows are left as they are, as are rows
-    whose slot lies outside the cache. Strides and the other arguments as for kv4_write."""
+    whose slot lies outside the cache. The two must not overlap. Strides and the other
+    arguments as for kv4_write."""
     S, c, kv, rest = _rows(cache, k_out, v_out, start, lengths, False, ("k_out", "v_out"))
+    _need(kv[0] != kv[4] or not S, "k_out and v_out must be two buffers")
     if S:
         _lib.call("ko_kv4_read", *c, *kv, *rest, _lib.stream_ptr())
 
@@ -230,7 +232,8 @@ def kv4_append(qkv, q_w, k_w, cos, sin, pos, q_out, cache, T, eps, nq, nkv, d):
 
 
 class Kv4Attention:
-    """Decode attention over a 4-bit cache for T query tokens per sequence, fixed (B, T, cap).
+    """Decode attention over a 4-bit cache for T query tokens per sequence, fixed (B, T, cap); cap is
+    rounded up to whole blocks, as kv4_cache does.
 
     Any number of query heads per KV head and tokens with T * nq / nkv <= 64, T <= 8; head_dim 64
     or 128. A query row that sees no key is zero. Calls of one object share its workspace:
@@ -240,6 +243,7 @@ class Kv4Attention:
     MAX_T = 8
     GRID = 512     # workgroups of 4 wavefronts: two on each of the 256 CUs
     MIN_RUN = 8    # least steps of 32 keys in a workgroup's run
+    PAIR_STEPS, MAX_STEPS = 12, (1 << 24) - GRID - MIN_RUN   # the C entry's limit
 
     def __init__(self, B, T, cap, nq, nkv, d, device, group=32):
         self.block_bytes = kv4_block_bytes(d, group)
@@ -247,12 +251,15 @@ class Kv4Attention:
               "B, cap and nkv must be positive, nq a multiple of nkv")
         _need(1 <= T <= self.MAX_T, f"T must be in 1..{self.MAX_T}")
         _need(T * (nq // nkv) <= 64, "at most 64 query rows (T * nq / nkv) a KV head")
-        self.B, self.T, self.cap, self.nq, self.nkv, self.d, self.group = B, T, cap, nq, nkv, d, group
+        self.B, self.T, self.nq, self.nkv, self.d, self.group = B, T, nq, nkv, d, group
         dev = torch.device(device)
         _need(dev.type == "cuda", "device must be a GPU")
+        self.blocks = -(-cap // KV4_KEYS)
+        self.cap = self.blocks * KV4_KEYS
+        _need(B * nkv * (self.blocks + self.PAIR_STEPS) <= self.MAX_STEPS,
+              f"B * nkv * blocks of {KV4_KEYS} keys must stay below 2^24")
         self.device = torch.cuda.current_device() if dev.index is None else dev.index
         self.scale = d ** -0.5
-        self.blocks = -(-cap // KV4_KEYS)
         # Workspace: the runs' partial sums, and arrival counters that are zero before the first
         # call and left zero by every call. Whatever stream that call is on, their fill must be
         # done: the constructor waits for it, which a capture does not allow.
@@ -298,12 +305,13 @@ class Kv4Attention:
     def __call__(self, q, cache, pos, out):
         """q: [B*T, nq*d] bf16; cache: [B, nkv, blocks, bytes]; pos: [B] int32, the position of a
         sequence's first query (keys 0 .. pos + T - 1 are cached, query t sees those up to pos +
-        t); out: [B*T, nq*d] bf16."""
+        t, none behind the cache's end); out: [B*T, nq*d] bf16."""
         self._run(q, cache, pos, self.T, out)
 
     def with_lengths(self, q, cache, lengths, out):
         """lengths[b] = number of cached keys of sequence b (int32); its T queries sit at the last
-        T positions. Rows in front of the first key (lengths[b] < T) are zero."""
+        T positions. Rows in front of the first key (lengths[b] < T) are zero. A length that passes
+        the cache's end places the queries; the keys are those up to the end."""
         self._run(q, cache, lengths, 0, out)
 
     def decode_qkv(self, qkv, q_w, k_w, cos, sin, pos, cache, out, eps, rope=None):

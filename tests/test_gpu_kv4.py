@@ -457,3 +457,56 @@ def test_decode_qkv_of_many_pairs(dev):
     want, mid, size = O.attention(q, cache, [p + 1 for p in pos], 1, nq, d, group)
     tol = want.abs() * 2.0 ** -8 + mid * 2.0 ** -8 + size * (2.0 ** -13 + 2.0 ** -7)
     assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("nq,nkv,d,group", [(4, 1, 128, 32), (16, 2, 64, 64)])
+@pytest.mark.parametrize("T", [2, 7])
+def test_tokens_behind_the_cache_do_not_move_the_others(dev, nq, nkv, d, group, T):
+    """Queries at pos .. pos + T - 1 of which the last lie behind the cache: each sees the keys up to
+    its own position that there are."""
+    cap = 64
+    pos = [60, 63, 64, 100, 2 ** 31 - 1, cap - T]
+    cache = filled(len(pos), nkv, cap, d, group, [cap] * len(pos), 90).to(dev)
+    q = randn(91, len(pos) * T, nq * d).to(BF16).to(dev)
+    out = torch.full_like(q, math.nan)
+    Kv4Attention(len(pos), T, cap, nq, nkv, d, dev, group=group)(
+        q, cache, torch.tensor(pos, dtype=torch.int32, device=dev), out)
+    for b, p in enumerate(pos):
+        for t in range(T):
+            row = slice(b * T + t, b * T + t + 1)
+            check_attention(out[row], q[row], cache[b:b + 1], [min(p + t + 1, cap)], 1, nq, d, group)
+
+
+def test_a_capacity_is_whole_blocks(dev):
+    """kv4_cache, kv4_append and the attention agree on the slots of a cap between two blocks."""
+    nq, nkv, d, cap, eps, pos = 4, 1, 128, 33, 1e-6, [40, 63, 64]
+    B = len(pos)
+    cache = kv4_cache(B, nkv, cap, d, dev)
+    assert cache.shape[2] == 2
+    cache.copy_(filled(B, nkv, 64, d, 32, [40, 63, 64], 92))
+    qkv, q_w, k_w, cos, sin = step_inputs(93, B, 1, nq, nkv, d, 100, dev)
+    at = torch.tensor(pos, dtype=torch.int32, device=dev)
+    out = torch.full((B, nq * d), math.nan, dtype=BF16, device=dev)
+    plan = Kv4Attention(B, 1, cap, nq, nkv, d, dev)
+    plan.decode_qkv(qkv, q_w, k_w, cos, sin, at, cache, out, eps)
+    assert (out[2] == 0).all()
+    want = torch.empty_like(out)
+    Kv4Attention(B, 1, 64, nq, nkv, d, dev).with_lengths(plan._q, cache, at + 1, want)
+    assert torch.equal(out[:2], want[:2])
+
+
+@pytest.mark.parametrize("grid,min_run", [(1, 1), (2, 8), (5, 3), (64, 1), (512, 40)])
+@pytest.mark.parametrize("T,nq,nkv,d,group", [(1, 8, 2, 128, 32), (5, 8, 2, 64, 64)])
+def test_any_number_of_workgroups(dev, grid, min_run, T, nq, nkv, d, group):
+    """Few workgroups, whose runs cross from pair to pair, and short or long runs."""
+    lens = [700, 3, 0, 1500, 33, 64, 901]
+    B, cap = len(lens), 1500
+    cache = filled(B, nkv, cap, d, group, lens, 94).to(dev)
+    q = randn(95, B * T, nq * d).to(BF16).to(dev)
+    plan = Kv4Attention(B, T, cap, nq, nkv, d, dev, group=group)
+    plan.grid, plan.MIN_RUN = grid, min_run
+    for _ in range(2):   # the second finds the counters as the first left them
+        out = torch.full_like(q, math.nan)
+        plan.with_lengths(q, cache, torch.tensor(lens, dtype=torch.int32, device=dev), out)
+        check_attention(out, q, cache, lens, T, nq, d, group)
+    assert not plan._counters.any()

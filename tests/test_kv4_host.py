@@ -102,3 +102,15 @@ def test_c_attention_refused():
     assert h.ko_kv4_attn_scratch(33, 64, 32, 10) == 2 * 10 * 64 * 66
     for bad in ((0, 128, 32, 1), (65, 128, 32, 1), (4, 96, 32, 1), (4, 128, 32, 0)):
         assert h.ko_kv4_attn_scratch(*bad) == -1
+
+
+def test_more_steps_than_the_kernel_counts_are_refused():
+    # 64 x 8 pairs of 32768 blocks: 2^24 steps
+    with pytest.raises(ValueError, match="24"):
+        K.Kv4Attention(64, 1, 1 << 20, 32, 8, 128, "cuda:0")
+    kw = dict(q=P, cache=P, cb=5120, ch=5120, lens=P, off=0, T=1, nq=32, nkv=8, d=128, group=32,
+              scale=0.1, part=P, part_len=1 << 40, counters=P, grid=512, min_run=8, out=P)
+    a = {k: kw.get(k) for k in ("q", "cache", "cb", "ch", "lens", "off", "cap", "B", "T", "nq", "nkv",
+                                "d", "group", "scale", "part", "part_len", "counters", "grid",
+                                "min_run", "out")} | dict(cap=1 << 20, B=64)
+    assert _lib.lib().ko_kv4_attn(*a.values(), None) == -34
