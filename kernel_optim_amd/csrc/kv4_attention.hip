@@ -23,10 +23,18 @@
 //   in a product of its own, before the codes' product: what accumulates is sum p s (n - 8), as
 //   small as the result, and not 136 sum p s, whose roundings would grow with the length.
 //
-// Work: the steps of all (sequence, KV head) pairs form one list, cut into equal runs, one per
-// workgroup, whatever the lengths; 4 wavefronts take the steps of a run in turn. A pair within
-// one run writes its output; else the workgroup that finishes the pair last merges the
-// partial sums (fp32, in run order: the result does not depend on who is last).
+// Work: the steps of all (sequence, KV head) pairs are dealt out from the lengths, on the device, to
+// two workgroups of 4 wavefronts on a CU or one of 8: each pair cut into parts of equal runs where
+// the workgroups suffice, else one list of all steps, cut into equal runs. The wavefronts take the
+// steps of a run in turn, each with two blocks in flight. A pair within one run writes its output;
+// else the workgroup that finishes the pair last merges the partial sums (fp32, in run order:
+// the result does not depend on who is last).
+//
+// Measured, 32 query and 8 KV heads of 128 in groups of 32: 16 x 8192 keys (168 MB) 32.8 us, 16 x
+// 32768 108-111 us (6.0-6.2 TB/s; the bf16 cache's attention reads at 6.6), 512 keys 7.2 us. Per
+// step and wavefront 290 VALU instructions with up to 4 query rows, 375 with 16, of about 4
+// cycles: two wavefronts on a SIMD keep ahead of the HBM with one query token, not with 4 and more
+// (16 x 8192 keys, 5 tokens: 59 us).
 #include "kv4_core.h"
 
 #include <limits.h>
@@ -221,7 +229,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     all += readlane(wave_incl_scan(b0 + lane0 < a.B ? steps_of(a, len) : 0), 63);
   }
   auto up = [](int n) { return (n + NWP - 1) / NWP * NWP; };
-  const int share = max(a.min_run, quot(all * a.nkv + grid - 1, grid, __builtin_amdgcn_rcpf((float)grid)));
+  const int share =
+      max(a.min_run, quot(all * a.nkv + grid - 1, grid, __builtin_amdgcn_rcpf((float)grid)));
   // (1) Every pair cut into parts of `run` steps, a workgroup for each: with the least run for
   // which the workgroups suffice, if that is at most a half longer than an equal share. One
   // workgroup on each CU goes before two, which take half as long again as one (4 x 2049 keys, 288
@@ -723,9 +732,9 @@ long long scratch_floats(int rows, int d, int group, int grid) {
 }
 
 // What the two entry points check alike.
-int check(const void* q, const void* cache, long long cb, long long ch, const int* lens, int cap, int B, int T,
-          int nq, int nkv, int d, int group, float scale, const float* part, long long part_len,
-          const int* counters, int grid, int min_run, const void* out) {
+int check(const void* q, const void* cache, long long cb, long long ch, const int* lens, int cap,
+          int B, int T, int nq, int nkv, int d, int group, float scale, const float* part,
+          long long part_len, const int* counters, int grid, int min_run, const void* out) {
   if (!q || !cache || !lens || !out || !part || !counters || B < 1 || T < 1 || nkv < 1 || nq < 1 ||
       cap < 1 || grid < 1 || min_run < 1)
     return KO_EINVAL;
@@ -775,8 +784,8 @@ int ko_kv4_attn(const void* q, const void* cache, long long cache_b_stride,
                 int T, int nq, int nkv, int d, int group, float scale, float* part,
                 long long part_len, int* counters, int grid, int min_run, void* out,
                 void* stream) {
-  return attention(q, cache, cache_b_stride, cache_h_stride, kv_lens, len_offset, cap, LLONG_MAX, B, T,
-                   nq, nkv, d, group, scale, part, part_len, counters, grid, min_run, out, stream);
+  return attention(q, cache, cache_b_stride, cache_h_stride, kv_lens, len_offset, cap, LLONG_MAX, B,
+                   T, nq, nkv, d, group, scale, part, part_len, counters, grid, min_run, out, stream);
 }
 
 int ko_kv4_attn_qkv(const void* qkv, const void* q_w, const void* k_w, const void* cos,

@@ -53,8 +53,8 @@ __device__ __forceinline__ bool locate(const Kv4Rows& a, long long item, int& b,
 // A writing lane holds 32 consecutive values of a key, so a group's smallest and largest come from
 // its registers (and its 1 or 3 neighbours') and its scale is computed once. (With V in the layout
 // it is stored in, 16 lanes a key, every lane computed the scales of 32 groups: 57 against 36
-// us for 32768 tokens of 8 heads of 128 in groups of 32, 4.9 TB/s, a copy's rate.) K's codes leave as they are, V's through LDS, which holds
-// the block as the cache does.
+// us for 32768 tokens of 8 heads of 128 in groups of 32, 4.9 TB/s, a copy's rate.) K's codes leave
+// as they are, V's through LDS, which holds the block as the cache does.
 template <int D, int NG, bool V>
 __device__ __forceinline__ void write_block(const uint16_t* src, long long stride, uint8_t* dst,
                                             int row0, int rows, int lane, uint8_t* lds) {
@@ -267,7 +267,8 @@ __global__ __launch_bounds__(NT) void kv4_read_kernel(Kv4Rows a) {
 // ---- q/k RMSNorm + RoPE + quantised append: one wavefront per (row, head) ----
 // Lane l holds the pair of elements 2 l, 2 l + 1 (d = 64: both halves of the wavefront hold
 // the head). Norm and RoPE run in fp32 throughout and q rounds once at the end; k is
-// quantised from fp32, so no rounding to bf16 moves a value over a code's border.
+// quantised from fp32, so no rounding to bf16 moves a value over a code's border. 2.8-3.4 us for
+// 1 to 32 rows of 48 heads of 128: a launch's latency.
 template <int D, int NG>
 __global__ __launch_bounds__(NT) void kv4_append_kernel(
     const uint16_t* __restrict__ qkv, const uint16_t* __restrict__ qw,

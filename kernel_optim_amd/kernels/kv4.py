@@ -58,7 +58,8 @@ def _here(dev):
 def _tensor(t, name, dtype, shape, dev, contiguous=True):
     _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
     _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
-    _need(tuple(t.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    _need(tuple(t.shape) == tuple(shape),
+          f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     _need(t.is_cuda and t.get_device() == dev, f"{name} must be on cuda:{dev}")
     _need(not contiguous or t.is_contiguous(), f"{name} must be contiguous")
     _need(not t.is_cuda or t.data_ptr() % (4 if dtype == torch.int32 else 16) == 0,
@@ -339,5 +340,6 @@ class Kv4Attention:
         _lib.call("ko_kv4_attn_qkv", qkv.data_ptr(), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
                   sin.data_ptr(), min(cos.shape[0], sin.shape[0]), pos.data_ptr(), cache.data_ptr(),
                   cb, ch, self.cap, B, nq, nkv, d, self.group, eps, self.scale,
-                  self._q.data_ptr(), self._part.data_ptr(), self._part.numel(), self._counters.data_ptr(), self.grid,
-                  self.MIN_RUN, out.data_ptr(), _lib.ptr(rope), _lib.stream_ptr())
+                  self._q.data_ptr(), self._part.data_ptr(), self._part.numel(),
+                  self._counters.data_ptr(), self.grid, self.MIN_RUN, out.data_ptr(),
+                  _lib.ptr(rope), _lib.stream_ptr())
