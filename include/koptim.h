@@ -399,7 +399,7 @@ int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void*
  * keys are those below min(n, cap), and the cache holds ceil(cap / 32) blocks a pair. A row that
  * sees no key is zero. nq a multiple of nkv, T * nq / nkv <= 64, 0 < scale < 10^4. The steps of
  * 32 keys of all pairs are dealt out in runs of at least min_run steps to grid workgroups of 4
- * wavefronts (or half as many of 8); B * nkv * (blocks + 12) + grid + min_run <= 2^24. part: fp32
+ * wavefronts (or half as many of 8); B * nkv * (blocks + 24) + grid + min_run <= 2^24. part: fp32
  * scratch of part_len >= ko_kv4_attn_scratch(T * nq / nkv, d, group, grid); counters [grid]
  * int32, zero before the first call, left zero by every call; calls that share them must not
  * overlap. */

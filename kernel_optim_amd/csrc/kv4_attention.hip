@@ -57,7 +57,8 @@ constexpr float NEG_BIG = -1.0e30f;
 // way through memory (one sequence of 512 keys 6.7 against 8.0 us in two parts; 1000 keys 9.8
 // against 8.6 us in four).
 constexpr int SOLO = 20;
-constexpr int PAIR_STEPS = 12;         // what a pair costs beside its steps, in steps
+// What a pair costs beside its steps, about 3 us, in steps of a workgroup of 4 or 8 wavefronts.
+__host__ __device__ constexpr int pair_steps(int waves) { return 3 * waves; }
 
 struct Kv4AttnArgs {
   const uint16_t* q;  // [B*T, nq*D]
@@ -269,12 +270,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     if (whole) parts_of(run);
   }
   // (2) Else one list of all pairs' steps, cut into equal runs that cross from pair to pair.
-  // Beginning and ending a pair costs as much as PAIR_STEPS steps: a pair shorter than a
-  // run, which shares it with others, takes so many more places.
-  auto places = [&](int len) {
-    const int n = steps_of(a, len);
-    return n < share ? n + PAIR_STEPS : n;
-  };
+  // Beginning and ending a pair costs as much as pair_steps steps, and takes so many places more
+  // (with none: a ragged 64 of up to 16384 keys 136 us; 12 for the pairs shorter than a run 107, for
+  // all 105.5; two thirds or twice of it 106 both, a ragged 24 of up to 4600 21.6 and 23.3 for 21.8).
+  auto places = [&](int len) { return steps_of(a, len) + pair_steps(WAVES); };
   if (!whole) {
     total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -327,7 +326,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
       at += g.kvh * n;
       g.st0 = s - at;
       s = min(at + n, end);
-      g.n = steps_of(a, g.len);  // behind them, a short pair's places are empty
+      g.n = steps_of(a, g.len);  // the places behind them are empty
       g.st1 = min(g.n, s - at);
       g.w0 = at / run;
       g.w1 = (at + g.n - 1) / run;
@@ -748,7 +747,7 @@ int check(const void* q, const void* cache, long long cb, long long ch, const in
   // the places of the list, and what is divided, stay below 2^24 (quot)
   const long long blocks = ((long long)cap + 31) / 32;
   if (grid > (1 << 20) || min_run > (1 << 20) ||
-      (long long)B * nkv > ((1LL << 24) - grid - min_run) / (blocks + PAIR_STEPS))
+      (long long)B * nkv > ((1LL << 24) - grid - min_run) / (blocks + pair_steps(8)))
     return KO_ERANGE;
   return KO_OK;
 }

@@ -244,7 +244,7 @@ class Kv4Attention:
     MAX_T = 8
     GRID = 512     # workgroups of 4 wavefronts: two on each of the 256 CUs
     MIN_RUN = 8    # least steps of 32 keys in a workgroup's run
-    PAIR_STEPS, MAX_STEPS = 12, (1 << 24) - GRID - MIN_RUN   # the C entry's limit
+    PAIR_STEPS, MAX_STEPS = 24, (1 << 24) - GRID - MIN_RUN   # the C entry's limit
 
     def __init__(self, B, T, cap, nq, nkv, d, device, group=32):
         self.block_bytes = kv4_block_bytes(d, group)
