@@ -613,9 +613,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
         // slots of the pair's parts: the first run's second, then every run's first
         auto slot_of = [&](int k) { return k == 0 ? 2 * w0 + 1 : 2 * (w0 + k); };
         const float* ml = a.part + 2LL * grid * ROWS * D;
-        // KR rows a wavefront and PB parts at a time: 32 loads in flight, the first of them
-        // with the loads of (m, l)
-        constexpr int KR = ROWS >= 16 ? 4 : ROWS / 4, PB = 32 / KR;
+        // A wavefront takes KR rows and a batch of parts at a time, their loads in flight together,
+        // the first with those of (m, l). All of a batch's loads are made, and coherent loads cost, so
+        // it is not much larger than the parts there are: with one row 4 to 32 (32 always: 4 x 2049
+        // keys, 8 parts, 9.9 against 9.2 us, 16 x 8192 33.7 and 32.3); with 2 and 4 rows 8 kB,
+        // of one size (16 kB: 4 x 7 tokens 18.7 against 17.8, 4 x 2048 keys with 2 9.8 and 9.2; in
+        // three sizes 18.5, and a kernel of 20 heads of 64 5 % slower).
+        constexpr int KR = ROWS >= 16 ? 4 : ROWS / 4;
         for (int rw0 = wave; rw0 < R; rw0 += WAVES * KR) {
           float M[KR], L[KR], o0[KR], o1[KR], f[KR];
           int rw[KR];
@@ -631,7 +635,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
             for (int k = 0; k < KR; ++k)
               x[k] = el < np ? load2_coherent(ml + ((long long)slot_of(p0 + el) * ROWS + rw[k]) * 2)
                              : make_float2(NEG_BIG, 0.f);
-            for (int q0 = 0; q0 < np; q0 += PB) {
+            auto batch = [&](int q0, auto size) __attribute__((always_inline)) {
+              constexpr int PB = decltype(size)::value;
               float2 o[KR][PB];
 #pragma unroll
               for (int q = 0; q < PB; ++q) {
@@ -664,6 +669,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
                     o1[k] = fmaf(fq, o[k][q].y, o1[k]);
                   }
                 }
+              return q0 + PB;
+            };
+            for (int q0 = 0; q0 < np;) {
+              [[maybe_unused]] const int left = np - q0;
+              if constexpr (KR == 1)
+                q0 = left > 16  ? batch(q0, std::integral_constant<int, 32>{})
+                     : left > 8 ? batch(q0, std::integral_constant<int, 16>{})
+                     : left > 4 ? batch(q0, std::integral_constant<int, 8>{})
+                                : batch(q0, std::integral_constant<int, 4>{});
+              else
+                q0 = batch(q0, std::integral_constant<int, 2048 / D / KR>{});
             }
           }
 #pragma unroll
