@@ -30,7 +30,7 @@
 // else the workgroup that finishes the pair last merges the partial sums (fp32, in run order:
 // the result does not depend on who is last).
 //
-// Measured, 32 query and 8 KV heads of 128 in groups of 32: 16 x 8192 keys (168 MB) 32.8 us, 16 x
+// Measured, 32 query and 8 KV heads of 128 in groups of 32: 16 x 8192 keys (168 MB) 32.3 us, 16 x
 // 32768 108-111 us (6.0-6.2 TB/s; the bf16 cache's attention reads at 6.6), 512 keys 7.2 us. Per
 // step and wavefront 290 VALU instructions with up to 4 query rows, 375 with 16, of about 4
 // cycles: two wavefronts on a SIMD keep ahead of the HBM with one query token, not with 4 and more
@@ -262,12 +262,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
     whole = need <= one;
     if (!whole && parts_of(longer) <= one) {
       run = least(run + NWP, longer, one);
+      parts_of(run);
       whole = true;
     } else if (!whole && (need <= grid || parts_of(longer) <= grid)) {
       run = need <= grid ? run : least(run + NWP, longer, grid);
+      parts_of(run);
       whole = true;
     }
-    if (whole) parts_of(run);
   }
   // (2) Else one list of all pairs' steps, cut into equal runs that cross from pair to pair.
   // Beginning and ending a pair costs as much as pair_steps steps, and takes so many places more
