@@ -52,7 +52,7 @@ extern "C" int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, 
 namespace {
 
 constexpr float TAU = 8.0f;            // a running maximum is raised by more than 2^8 only
-constexpr float NEG_BIG = -1.0e30f;
+constexpr float NEG_BIG = -1.0e30f;    // a key whose q k lies below counts for nothing
 // Up to SOLO steps a pair is not cut: its 5 steps a wavefront take less than the partial sums'
 // way through memory (one sequence of 512 keys 6.7 against 8.0 us in two parts; 1000 keys 9.8
 // against 8.6 us in four).

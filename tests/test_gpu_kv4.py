@@ -510,3 +510,63 @@ def test_any_number_of_workgroups(dev, grid, min_run, T, nq, nkv, d, group):
         plan.with_lengths(q, cache, torch.tensor(lens, dtype=torch.int32, device=dev), out)
         check_attention(out, q, cache, lens, T, nq, d, group)
     assert not plan._counters.any()
+
+
+@pytest.mark.parametrize("T,d,group", [(17, 128, 32), (33, 128, 128), (64, 64, 32), (64, 128, 64)])
+def test_more_query_tokens_than_the_op_offers(dev, monkeypatch, T, d, group):
+    """The C entry serves T * nq / nkv up to 64, whatever T: the last tokens' limits then lie in three
+    blocks."""
+    monkeypatch.setattr(Kv4Attention, "MAX_T", 64)
+    attend(dev, 3, T, 2, 2, d, group, 400, [385, T, 70])
+    attend(dev, 1, T, 1, 1, d, group, 1500, [1473])
+
+
+def test_offsets_past_32_bits(dev):
+    """Sequences 5 GiB apart in the cache, and 6 GiB in the rows that are written and read."""
+    d, group, nb, S, eps = 128, 32, 3, 70, 1e-6
+    far, row = 5 << 30, 3 << 30
+    size = kv4_block_bytes(d, group)
+    hold = torch.empty(far + nb * size, dtype=torch.uint8, device=dev)
+    cache = hold.as_strided((2, 1, nb, size), (far, nb * size, size, 1))
+    rows_k = torch.empty(row + S * d, dtype=BF16, device=dev).as_strided((2, 1, S, d), (row, S * d, d, 1))
+    k, v = rows(100, 2, 1, S, d).to(dev), rows(101, 2, 1, S, d).to(dev)
+    near = kv4_cache(2, 1, nb * KV4_KEYS, d, dev, group)
+    cache.copy_(near)
+    rows_k.copy_(k)
+    kv4_write(k, v, near)
+    kv4_write(rows_k, v, cache)
+    assert torch.equal(cache, near)
+    rows_k.zero_()
+    k1, v1, v2 = (torch.zeros_like(k) for _ in range(3))
+    kv4_read(near, k1, v1)
+    kv4_read(cache, rows_k, v2)
+    assert torch.equal(rows_k, k1) and torch.equal(v2, v1)
+    pos = torch.tensor([S, S - 3], dtype=torch.int32, device=dev)
+    qkv, q_w, k_w, cos, sin = step_inputs(102, 2, 1, 4, 1, d, 96, dev)
+    plan = Kv4Attention(2, 1, nb * KV4_KEYS, 4, 1, d, dev, group=group)
+    out = torch.empty(2, 2, 4 * d, dtype=BF16, device=dev)
+    plan.decode_qkv(qkv, q_w, k_w, cos, sin, pos, near, out[0], eps)
+    plan.decode_qkv(qkv, q_w, k_w, cos, sin, pos, cache, out[1], eps)
+    assert torch.equal(cache, near) and torch.equal(out[0], out[1])
+
+
+def test_two_objects_on_two_streams(dev):
+    """Calls of two objects at once, each with its own workspace, against the same calls in turn."""
+    lens = [[2500, 31, 900], [1200, 2000, 5]]
+    caches = [filled(3, 2, 2500, 128, 32, n, 110 + i).to(dev) for i, n in enumerate(lens)]
+    q = [randn(112 + i, 3, 8 * 128).to(BF16).to(dev) for i in range(2)]
+    ln = [torch.tensor(n, dtype=torch.int32, device=dev) for n in lens]
+    plans = [Kv4Attention(3, 1, 2500, 8, 2, 128, dev) for _ in range(2)]
+    want = [torch.empty_like(x) for x in q]
+    for i in range(2):
+        plans[i].with_lengths(q[i], caches[i], ln[i], want[i])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[torch.empty_like(x) for _ in range(20)] for x in q]
+    torch.cuda.synchronize()
+    for j in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                plans[i].with_lengths(q[i], caches[i], ln[i], outs[i][j])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
