@@ -25,7 +25,7 @@ past a sequence's length.
 import torch
 
 from .. import _lib
-from .fused import BF16, _is, _need
+from .fused import BF16, _need
 
 KV4_KEYS = 32  # keys of a block
 
@@ -48,6 +48,12 @@ def kv4_cache(B, nkv, cap, d, device, group=32, layers=None):
     shape = (B, nkv, -(-cap // KV4_KEYS), kv4_block_bytes(d, group))
     return torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8,
                        device=device)
+
+
+# The current device and its stream's handle, for devices that are known to be initialised: a third
+# of the time of torch.cuda.current_device() and of _lib.stream_ptr().
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.stream_ptr)
 
 
 def _here(dev):
@@ -118,39 +124,45 @@ def _ints(t, B, dev):
 
 
 def _usual(cache, k, v, start, lengths, written):
-    """Whether a call needs no closer look: contiguous outputs, and inputs whose strides suit as they
-    are. Tests that could name each fault take 25 us, more than a prompt of 500 tokens
-    on the GPU; these take 4."""
+    """The C arguments of a call that needs no closer look: contiguous outputs, and inputs whose
+    strides suit as they are; else None. Tests that could name each fault take 25 us, more
+    than a prompt of 500 tokens on the GPU; these take 2."""
     try:
         B, nkv, nb, size = cache.shape
-        fmt = _FORMATS.get(size)
-        k0, k1, k2, k3 = k.stride()
-        v0, v1, v2, v3 = v.stride()
-        dev = cache.get_device()
-        return (fmt is not None and k.shape == v.shape == (B, nkv, k.shape[2], fmt[0])
-                and cache.dtype is torch.uint8 and k.dtype is BF16 and v.dtype is BF16
-                and k3 == 1 and v3 == 1 and (k0 | k1 | k2 | v0 | v1 | v2) % 8 == 0
-                and cache.is_contiguous()
+        d, group = _FORMATS[size]
+        shape, dev = k.shape, cache.get_device()
+        S = shape[2]
+        kb, kh, ks, k1 = k.stride()
+        vb, vh, vs, v1 = v.stride()
+        cp, kp, vp = cache.data_ptr(), k.data_ptr(), v.data_ptr()
+        if (shape == v.shape == (B, nkv, S, d) and cache.dtype is torch.uint8
+                and k.dtype is v.dtype is BF16 and k1 == v1 == 1
+                and (kb | kh | ks | vb | vh | vs) % 8 == 0 and cache.is_contiguous()
                 and (written or (k.is_contiguous() and v.is_contiguous()))
-                and (cache.data_ptr() | k.data_ptr() | v.data_ptr()) % 16 == 0
-                and dev == k.get_device() == v.get_device() == torch.cuda.current_device()
-                and B > 0 and nkv > 0 and nb > 0 and _ints(start, B, dev)
-                and _ints(lengths, B, dev))
-    except (AttributeError, ValueError, IndexError, RuntimeError):
-        return False   # no tensors of these dimensions: _check_rows says which
+                and (cp | kp | vp) % 16 == 0 and B > 0 and nkv > 0 and nb > 0
+                and dev == k.get_device() == v.get_device() == _current_device()
+                and _ints(start, B, dev) and _ints(lengths, B, dev)):
+            return (S, (cp, nkv * nb * size, nb * size), (kp, kb, kh, ks, vp, vb, vh, vs),
+                    (None if start is None else start.data_ptr(),
+                     None if lengths is None else lengths.data_ptr(),
+                     B, S, nkv, nb * KV4_KEYS, d, group), dev)
+    except (AttributeError, KeyError, ValueError, IndexError, TypeError, RuntimeError):
+        pass   # no tensors of these dimensions: _check_rows says which
+    return None
 
 
 def _rows(cache, k, v, start, lengths, written, names):
     """The checked C arguments of kv4_write and kv4_read."""
-    if _usual(cache, k, v, start, lengths, written):
-        c, ks, vs = cache.stride()[:2], k.stride()[:3], v.stride()[:3]
-    else:
-        _check_rows(cache, k, v, start, lengths, written, names)
-        c, ks, vs = _outer(cache)[:2], _outer(k), _outer(v)   # single rows' strides may be odd
+    usual = _usual(cache, k, v, start, lengths, written)
+    if usual is not None:
+        return usual
+    _check_rows(cache, k, v, start, lengths, written, names)
     B, nkv, nb, size = cache.shape
-    S = k.shape[2]
-    return (S, (cache.data_ptr(), *c), (k.data_ptr(), *ks, v.data_ptr(), *vs),
-            (_lib.ptr(start), _lib.ptr(lengths), B, S, nkv, nb * KV4_KEYS, *_FORMATS[size]))
+    S = k.shape[2]   # single rows' strides may be odd: _outer's are passed
+    return (S, (cache.data_ptr(), *_outer(cache)[:2]),
+            (k.data_ptr(), *_outer(k), v.data_ptr(), *_outer(v)),
+            (_lib.ptr(start), _lib.ptr(lengths), B, S, nkv, nb * KV4_KEYS, *_FORMATS[size]),
+            cache.get_device())
 
 
 def kv4_write(k, v, cache, start=None, lengths=None):
@@ -160,9 +172,9 @@ def kv4_write(k, v, cache, start=None, lengths=None):
     [B, S, nkv, d] transposed serves); start: [B] int32 on the GPU (None: 0); lengths: [B] int32,
     the valid rows of a padded batch (None: S). Rows whose slot lies outside the cache are
     dropped; other slots keep what they hold."""
-    S, c, kv, rest = _rows(cache, k, v, start, lengths, True, ("k", "v"))
+    S, c, kv, rest, dev = _rows(cache, k, v, start, lengths, True, ("k", "v"))
     if S:
-        _lib.call("ko_kv4_write", *kv, *c, *rest, _lib.stream_ptr())
+        _lib.call("ko_kv4_write", *kv, *c, *rest, _stream(dev))
 
 
 def kv4_read(cache, k_out, v_out, start=None, lengths=None):
@@ -170,15 +182,17 @@ def kv4_read(cache, k_out, v_out, start=None, lengths=None):
     of slot start[b] + i, i < lengths[b] (None: S); other rows are left as they are, as are rows
     whose slot lies outside the cache. The two must not overlap. Strides and the other
     arguments as for kv4_write."""
-    S, c, kv, rest = _rows(cache, k_out, v_out, start, lengths, False, ("k_out", "v_out"))
+    S, c, kv, rest, dev = _rows(cache, k_out, v_out, start, lengths, False, ("k_out", "v_out"))
     _need(kv[0] != kv[4] or not S, "k_out and v_out must be two buffers")
     if S:
-        _lib.call("ko_kv4_read", *c, *kv, *rest, _lib.stream_ptr())
+        _lib.call("ko_kv4_read", *c, *kv, *rest, _stream(dev))
 
 
 def _check_qkv(qkv, q_w, k_w, cos, sin, pos, rows, B, nq, nkv, d, dev):
+    """The addresses of the first five, and the rows that both tables have."""
     try:   # the usual call, 1.5 us; the tests below name what is wrong
         (rc, dc), (rs, ds) = cos.shape, sin.shape
+        ptrs = (qkv.data_ptr(), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(), sin.data_ptr())
         if (qkv.shape == (rows, (nq + 2 * nkv) * d) and q_w.shape == k_w.shape == (d,)
                 and pos.shape == (B,) and dc == ds == d and rc > 0 and rs > 0
                 and qkv.dtype is q_w.dtype is k_w.dtype is cos.dtype is sin.dtype is BF16
@@ -186,9 +200,8 @@ def _check_qkv(qkv, q_w, k_w, cos, sin, pos, rows, B, nq, nkv, d, dev):
                 and k_w.is_contiguous() and cos.is_contiguous() and sin.is_contiguous()
                 and pos.is_contiguous() and dev == qkv.get_device() == q_w.get_device()
                 == k_w.get_device() == cos.get_device() == sin.get_device() == pos.get_device()
-                and (qkv.data_ptr() | q_w.data_ptr() | k_w.data_ptr() | cos.data_ptr()
-                     | sin.data_ptr()) % 16 == 0):
-            return
+                and (ptrs[0] | ptrs[1] | ptrs[2] | ptrs[3] | ptrs[4]) % 16 == 0):
+            return ptrs, rc if rc < rs else rs
     except (AttributeError, ValueError, TypeError, RuntimeError):
         pass
     _tensor(qkv, "qkv", BF16, (rows, (nq + 2 * nkv) * d), dev)
@@ -199,6 +212,7 @@ def _check_qkv(qkv, q_w, k_w, cos, sin, pos, rows, B, nq, nkv, d, dev):
               f"{name} must be [rows, d]")
         _tensor(t, name, BF16, (t.shape[0], d), dev)
     _tensor(pos, "pos", torch.int32, (B,), dev)
+    return tuple(t.data_ptr() for t in (qkv, q_w, k_w, cos, sin)), min(cos.shape[0], sin.shape[0])
 
 
 def kv4_append(qkv, q_w, k_w, cos, sin, pos, q_out, cache, T, eps, nq, nkv, d):
@@ -207,29 +221,28 @@ def kv4_append(qkv, q_w, k_w, cos, sin, pos, q_out, cache, T, eps, nq, nkv, d):
     the cache's slot at that position with v, both quantised. Everything is fp32 up to the one
     rounding of q and the quantisation of k. Positions outside the cache or the RoPE tables
     [rows, d] are skipped (their q_out rows too)."""
-    if not (isinstance(cache, torch.Tensor) and cache.is_cuda and cache.dtype is torch.uint8
-            and cache.dim() == 4 and cache.shape[3] in _FORMATS and cache.is_contiguous()
-            and cache.numel() and cache.data_ptr() % 16 == 0):
-        _check_cache(cache, True)
-    B, ck, nb, size = cache.shape
-    cd, group = _FORMATS[size]
-    dev = cache.get_device()
-    if dev != torch.cuda.current_device():
+    try:   # the usual call; the tests below name what is wrong
+        B, ck, nb, size = cache.shape
+        cd, group = _FORMATS[size]
+        dev, qp, cp = cache.get_device(), q_out.data_ptr(), cache.data_ptr()
+        cb, ch = ck * nb * size, nb * size
+        usual = (cache.dtype is torch.uint8 and cache.is_contiguous() and ck == nkv and cd == d
+                 and T >= 1 and nq >= 1 and B > 0 and nkv > 0 and nb > 0
+                 and q_out.shape == (B * T, nq * d) and q_out.dtype is BF16
+                 and q_out.is_contiguous() and (qp | cp) % 16 == 0
+                 and dev == q_out.get_device() == _current_device())
+    except (AttributeError, KeyError, ValueError, TypeError, RuntimeError):
+        usual = False
+    if not usual:
+        B, ck, nb, cd, group, dev = _check_cache(cache, True)
         _here(dev)
-    _need(T >= 1 and nq >= 1, "T and nq must be positive")
-    if (ck, cd) != (nkv, d):
-        raise ValueError(f"cache has {ck} heads of {cd}, not {nkv} of {d}")
-    _check_qkv(qkv, q_w, k_w, cos, sin, pos, B * T, B, nq, nkv, d, dev)
-    if not (_is(q_out, BF16, (B * T, nq * d)) and q_out.get_device() == dev
-            and q_out.data_ptr() % 16 == 0):
+        _need(T >= 1 and nq >= 1, "T and nq must be positive")
+        _need((ck, cd) == (nkv, d), f"cache has {ck} heads of {cd}, not {nkv} of {d}")
         _tensor(q_out, "q_out", BF16, (B * T, nq * d), dev)
-    cb, ch, _, _ = cache.stride()
-    if cb % 16 or ch % 16:   # strides of single rows
-        cb, ch, _ = _outer(cache)
-    _lib.call("ko_kv4_append", qkv.data_ptr(), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
-              sin.data_ptr(), pos.data_ptr(), q_out.data_ptr(), cache.data_ptr(), B * T, T, cb, ch,
-              eps, nq, nkv, d, group, min(nb * KV4_KEYS, cos.shape[0], sin.shape[0]), None,
-              _lib.stream_ptr())
+        qp, cp, (cb, ch, _) = q_out.data_ptr(), cache.data_ptr(), _outer(cache)
+    ptrs, n_rows = _check_qkv(qkv, q_w, k_w, cos, sin, pos, B * T, B, nq, nkv, d, dev)
+    _lib.call("ko_kv4_append", *ptrs, pos.data_ptr(), qp, cp, B * T, T, cb, ch, eps, nq, nkv, d,
+              group, min(nb * KV4_KEYS, n_rows), None, _stream(dev))
 
 
 class Kv4Attention:
@@ -270,6 +283,7 @@ class Kv4Attention:
                                  dtype=torch.float32, device=dev)
         self._counters = torch.zeros(self.grid, dtype=torch.int32, device=dev)
         torch.cuda.current_stream(dev).synchronize()
+        self._work = self._part.data_ptr(), self._part.numel(), self._counters.data_ptr()
         self._q = torch.empty(B, nq * d, dtype=BF16, device=dev) if T == 1 else None
         self._q_shape = torch.Size((B * T, nq * d))
         self._cache_shape = torch.Size((B, nkv, self.blocks, self.block_bytes))
@@ -281,27 +295,31 @@ class Kv4Attention:
         _need(_check_cache(cache, written)[5] == self.device, f"cache must be on cuda:{self.device}")
 
     def _run(self, q, cache, lens, len_offset, out):
-        if not (_is(q, BF16, self._q_shape) and _is(out, BF16, self._q_shape)
-                and _is(lens, torch.int32, self._len_shape)
-                and isinstance(cache, torch.Tensor) and cache.dtype is torch.uint8
-                and cache.is_contiguous() and cache.shape == self._cache_shape
-                and cache.get_device() == self.device == q.get_device() == out.get_device()
-                and lens.get_device() == self.device
-                and (q.data_ptr() | cache.data_ptr() | out.data_ptr()) % 16 == 0):
-            _tensor(q, "q", BF16, self._q_shape, self.device)
-            _tensor(out, "out", BF16, self._q_shape, self.device)
-            _tensor(lens, "pos/lengths", torch.int32, self._len_shape, self.device)
+        dev = self.device
+        try:   # the usual call; the tests below name what is wrong
+            qp, cp, op = q.data_ptr(), cache.data_ptr(), out.data_ptr()
+            usual = (q.shape == out.shape == self._q_shape and q.dtype is out.dtype is BF16
+                     and q.is_contiguous() and out.is_contiguous() and lens.shape == self._len_shape
+                     and lens.dtype is torch.int32 and lens.is_contiguous()
+                     and cache.shape == self._cache_shape and cache.dtype is torch.uint8
+                     and cache.is_contiguous() and dev == q.get_device() == out.get_device()
+                     == lens.get_device() == cache.get_device() and (qp | cp | op) % 16 == 0)
+        except (AttributeError, ValueError, TypeError, RuntimeError):
+            usual = False
+        if not usual:
+            _tensor(q, "q", BF16, self._q_shape, dev)
+            _tensor(out, "out", BF16, self._q_shape, dev)
+            _tensor(lens, "pos/lengths", torch.int32, self._len_shape, dev)
             self._check_cache(cache)
-        if self.device != torch.cuda.current_device():
-            _here(self.device)
-        _need(q.data_ptr() != out.data_ptr(), "out must not be q")
+        if dev != _current_device():
+            _here(dev)
+        _need(qp != op, "out must not be q")
         cb, ch, _, _ = cache.stride()
         if cb % 16 or ch % 16:   # strides of single rows
             cb, ch, _ = _outer(cache)
-        _lib.call("ko_kv4_attn", q.data_ptr(), cache.data_ptr(), cb, ch, lens.data_ptr(), len_offset,
-                  self.cap, self.B, self.T, self.nq, self.nkv, self.d, self.group, self.scale,
-                  self._part.data_ptr(), self._part.numel(), self._counters.data_ptr(), self.grid,
-                  self.MIN_RUN, out.data_ptr(), _lib.stream_ptr())
+        _lib.call("ko_kv4_attn", qp, cp, cb, ch, lens.data_ptr(), len_offset, self.cap, self.B,
+                  self.T, self.nq, self.nkv, self.d, self.group, self.scale, *self._work, self.grid,
+                  self.MIN_RUN, op, _stream(dev))
 
     def __call__(self, q, cache, pos, out):
         """q: [B*T, nq*d] bf16; cache: [B, nkv, blocks, bytes]; pos: [B] int32, the position of a
@@ -323,23 +341,24 @@ class Kv4Attention:
         fused.rope_rows writes them."""
         _need(self.T == 1, "decode_qkv serves one decode token per sequence")
         B, nq, nkv, d, dev = self.B, self.nq, self.nkv, self.d, self.device
-        if not (isinstance(cache, torch.Tensor) and cache.dtype is torch.uint8
-                and cache.shape == self._cache_shape and cache.get_device() == dev
-                and cache.is_contiguous() and _is(out, BF16, self._q_shape)
-                and out.get_device() == dev == torch.cuda.current_device()
-                and (cache.data_ptr() | out.data_ptr()) % 16 == 0):
+        try:   # the usual call; the tests below name what is wrong
+            cp, op = cache.data_ptr(), out.data_ptr()
+            usual = (cache.shape == self._cache_shape and cache.dtype is torch.uint8
+                     and cache.is_contiguous() and out.shape == self._q_shape and out.dtype is BF16
+                     and out.is_contiguous() and (cp | op) % 16 == 0
+                     and dev == cache.get_device() == out.get_device() == _current_device())
+        except (AttributeError, ValueError, TypeError, RuntimeError):
+            usual = False
+        if not usual:
             self._check_cache(cache, True)
             _tensor(out, "out", BF16, self._q_shape, dev)
             _here(dev)
-        _check_qkv(qkv, q_w, k_w, cos, sin, pos, B, B, nq, nkv, d, dev)
+        ptrs, n_rows = _check_qkv(qkv, q_w, k_w, cos, sin, pos, B, B, nq, nkv, d, dev)
         if rope is not None:
             _tensor(rope, "rope", BF16, (B, 2, d), dev)
         cb, ch, _, _ = cache.stride()
         if cb % 16 or ch % 16:   # strides of single rows
             cb, ch, _ = _outer(cache)
-        _lib.call("ko_kv4_attn_qkv", qkv.data_ptr(), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
-                  sin.data_ptr(), min(cos.shape[0], sin.shape[0]), pos.data_ptr(), cache.data_ptr(),
-                  cb, ch, self.cap, B, nq, nkv, d, self.group, eps, self.scale,
-                  self._q.data_ptr(), self._part.data_ptr(), self._part.numel(),
-                  self._counters.data_ptr(), self.grid, self.MIN_RUN, out.data_ptr(),
-                  _lib.ptr(rope), _lib.stream_ptr())
+        _lib.call("ko_kv4_attn_qkv", *ptrs, n_rows, pos.data_ptr(), cp, cb, ch, self.cap, B,
+                  nq, nkv, d, self.group, eps, self.scale, self._q.data_ptr(), *self._work,
+                  self.grid, self.MIN_RUN, op, _lib.ptr(rope), _stream(dev))

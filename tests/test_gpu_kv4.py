@@ -570,3 +570,52 @@ def test_two_objects_on_two_streams(dev):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+def test_refusals(dev):
+    """What each op names, of tensors on the GPU."""
+    B, nq, nkv, d, S = 2, 4, 2, 128, 5
+    cache = kv4_cache(B, nkv, 64, d, dev)
+    k = torch.zeros(B, nkv, S, d, dtype=BF16, device=dev)
+    ints = torch.zeros(B, dtype=torch.int32, device=dev)
+    for args, kw in (((k.float(), k, cache), {}), ((k, k[:, :1], cache), {}),
+                     ((k[..., ::2], k, cache), {}), ((k, k, cache[0]), {}), ((k, k, cache[..., 1:]), {}),
+                     ((k, k, cache.float()), {}), ((k, k, cache), dict(start=ints.long())),
+                     ((k, k, cache), dict(lengths=ints[:1])), ((k, k.cpu(), cache), {}),
+                     ((k, k, cache), dict(lengths=ints.cpu())), ((k, None, cache), {}),
+                     ((k, k, cache[:1].expand(B, -1, -1, -1)), {}),
+                     ((k.flatten()[1:-7].view(-1), k, cache), {})):
+        with pytest.raises(ValueError):
+            kv4_write(*args, **kw)
+    for a, b in ((k, k), (k, k[:1].expand(B, -1, -1, -1)), (k, k.float())):
+        with pytest.raises(ValueError):
+            kv4_read(cache, a, b)
+    qkv, w = torch.zeros(B, (nq + 2 * nkv) * d, dtype=BF16, device=dev), torch.zeros(d, dtype=BF16, device=dev)
+    tab, q = torch.zeros(64, d, dtype=BF16, device=dev), torch.zeros(B, nq * d, dtype=BF16, device=dev)
+    plan, out = Kv4Attention(B, 1, 64, nq, nkv, d, dev), torch.zeros_like(q)
+    good = [qkv, w, w, tab, tab, ints]
+    for i, bad in ((0, qkv[:1]), (0, qkv.float()), (1, w[:64]), (2, w.cpu()), (3, tab[:0]), (4, tab[0]),
+                   (3, tab.t()), (5, ints.long()), (5, None)):
+        args = good[:i] + [bad] + good[i + 1:]
+        with pytest.raises(ValueError):
+            kv4_append(*args, q, cache, 1, 1e-6, nq, nkv, d)
+        with pytest.raises(ValueError):
+            plan.decode_qkv(*args, cache, out, 1e-6)
+    for bad in (dict(T=0), dict(T=2), dict(nkv=1), dict(d=64), dict(q=q[:1]), dict(q=None),
+                dict(cache=cache.cpu()), dict(cache=cache[:1].expand(B, -1, -1, -1))):
+        a = dict(q=q, cache=cache, T=1, nkv=nkv, d=d) | bad
+        with pytest.raises(ValueError):
+            kv4_append(*good, a["q"], a["cache"], a["T"], 1e-6, nq, a["nkv"], a["d"])
+    for a in ((q, cache, ints, q), (q[:1], cache, ints, out), (q, cache[:1], ints, out),
+              (q, cache, ints.long(), out), (q, cache, ints, out.float()), (None, cache, ints, out),
+              (q, cache.cpu(), ints, out), (q, cache, ints, None)):
+        with pytest.raises(ValueError):
+            plan(*a)
+    with pytest.raises(ValueError):
+        Kv4Attention(B, 2, 64, nq, nkv, d, dev).decode_qkv(*good, cache, out, 1e-6)
+    with pytest.raises(ValueError):
+        plan.decode_qkv(*good, cache[:1].expand(B, -1, -1, -1), out, 1e-6)
+    with pytest.raises(ValueError):
+        plan.decode_qkv(*good, cache, out, 1e-6, rope=tab)
+    torch.cuda.synchronize()
+    assert not cache.any() and not out.any() and not q.any()
