@@ -365,7 +365,8 @@ int ko_gemv_tile(const void* w, void* wt, int rows, int K, void* stream);
  * vector share a bf16 scale s and a bf16 value c: x = c + s (n - 8), n = 0..15, with
  * c = bf16(7/15 min + 8/15 max), s = bf16(max((max - c) / 7, (c - min) / 8)) (0 below 2^-126)
  * and n = clamp(rint((x - c) (1 / s) + 8), 0, 15); a group with a NaN or an infinity has
- * s = c = NaN. d = 64 or 128.
+ * s = c = NaN. Where c + s (n - 8) passes bf16's largest value, ko_kv4_read returns that value.
+ * d = 64 or 128.
  *
  * ko_kv4_write: rows 0 .. lengths[b] - 1 (lengths NULL: S) of k and v [B, nkv, S, d] bf16, inner
  * stride 1, the other strides in elements, multiples of 8, into the slots from start[b] (NULL: 0)

@@ -7,7 +7,8 @@
 //   c = bf16(7/15 min + 8/15 max),  s = bf16(max((max - c) / 7, (c - min) / 8)),
 //   n = clamp(rint((x - c) (1 / s) + 8), 0, 15).
 // A step below 2^-126 is taken as 0 (then x = c); a NaN or an infinity anywhere in a group
-// makes s and c NaN, so the group reads NaN. 8 is chosen, rather than the middle 7.5, because
+// makes s and c NaN, so the group reads NaN. Where the roundings of s and c put an end of a group past
+// bf16's largest value, a read returns that value. 8 is chosen, rather than the middle 7.5, because
 // bf16 holds 128 + n and 136 exactly: a matrix instruction takes the codes as 128 + n, one
 // bit operation per pair, and the offset leaves with the constant 136.
 //
@@ -47,11 +48,13 @@ struct Kv4Group {
   __device__ __forceinline__ void from(float mn, float mx) {
 #pragma clang fp contract(off)
     c = round_bf16(mn * (float)(7.0 / 15.0) + mx * (float)(8.0 / 15.0));
-    float s = round_bf16(fmaxf((mx - c) * (float)(1.0 / 7.0), (c - mn) * 0.125f));
+    // eighths before their difference: c - mn is up to 8/15 2^129 and may pass fp32's range, mx - c
+    // at 7/15 2^129 does not; the eighths are exact
+    float s = round_bf16(fmaxf((mx - c) * (float)(1.0 / 7.0), c * 0.125f - mn * 0.125f));
     if (!(fabsf(mn) < INFINITY && fabsf(mx) < INFINITY)) c = s = __uint_as_float(0x7fc00000u);
     if (s < 1.1754943508222875e-38f) s = 0.f;
     // 1 / s, rounded correctly: v_rcp_f32 and one Newton step are, for every bf16 from 2^-126 to
-    // 2^126 (all of them compared on the GPU), and s is below 2^126 (no group spans 7 2^126)
+    // 2^126 (all of them compared on the GPU), and s, about 1/15 of a span below 2^129, is below 2^126
     const float y = __builtin_amdgcn_rcpf(s);
     inv = s == 0.f ? 0.f : fmaf(fmaf(-s, y, 1.0f), y, y);
     sc = (__float_as_uint(s) >> 16) | (__float_as_uint(c) & 0xffff0000u);

@@ -143,9 +143,15 @@ __global__ __launch_bounds__(NT) void kv4_write_kernel(Kv4Rows a) {
                               lds[wave]);
 }
 
-// c + s (n - 8): the product is exact in fp32 (8 by 4 bits), the sum rounds once.
-__device__ __forceinline__ float kv4_value(uint32_t n, uint32_t sc) {
-  return fmaf(bf16lo(sc), (float)(int)(n & 15u) - 8.0f, bf16hi(sc));
+// c + s (n - 8): the product is exact in fp32 (8 by 4 bits), the sum rounds once. Past bf16's largest
+// value it is that value: lim is, and NaN where s or c is (v_med3_f32 of three NaN is one; with
+// two numbers beside a NaN it would be a number).
+__device__ __forceinline__ float kv4_lim(uint32_t sc) {
+  return fmaf(bf16lo(sc), 0.f, fmaf(bf16hi(sc), 0.f, 0x1.fep127f));
+}
+__device__ __forceinline__ float kv4_value(uint32_t n, uint32_t sc, float lim) {
+  const float x = fmaf(bf16lo(sc), (float)(int)(n & 15u) - 8.0f, bf16hi(sc));
+  return __builtin_amdgcn_fmed3f(x, -lim, lim);
 }
 
 template <int D, int NG>
@@ -171,10 +177,11 @@ __device__ __forceinline__ void read_k(const uint8_t* src, uint16_t* kp, long lo
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const uint32_t x = w[half][i], c = sc[half][i / IPG];
+      const float lim = kv4_lim(c);
       uint32_t o[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        o[e] = pack_bf16x2(kv4_value(x >> (4 * e), c), kv4_value(x >> (4 * e + 16), c));
+        o[e] = pack_bf16x2(kv4_value(x >> (4 * e), c, lim), kv4_value(x >> (4 * e + 16), c, lim));
       if (live)
         *reinterpret_cast<uint4*>(kp + row * ks + 32 * i + 8 * q) = make_uint4(o[0], o[1], o[2], o[3]);
     }
@@ -229,7 +236,9 @@ __device__ __forceinline__ void read_v(const uint8_t* src, uint16_t* vp, long lo
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const uint32_t n = w[i / 2][e / 2] >> (16 * (e & 1) + 8 * (i & 1));
-      o[i] = pack_bf16x2(kv4_value(n, sc[i / IPG][e]), kv4_value(n >> 4, sc[i / IPG][e]));
+      const uint32_t c = sc[i / IPG][e];
+      const float lim = kv4_lim(c);
+      o[i] = pack_bf16x2(kv4_value(n, c, lim), kv4_value(n >> 4, c, lim));
     }
     // 4 lanes hold 8 neighbouring columns of each step i. They exchange, so that lane n stores 16
     // bytes of step n % 4 (d = 64: 8 bytes of step n % 2), and a key's row leaves in one

@@ -18,7 +18,8 @@ def quantise(x, group):
     x = x.to(F32).unflatten(-1, (-1, group))
     lo, hi = x.amin(-1), x.amax(-1)
     c = (lo * (7 / 15) + hi * (8 / 15)).to(BF16).to(F32)
-    s = torch.maximum((hi - c) * (1 / 7), (c - lo) * 0.125).to(BF16).to(F32)
+    # (c - lo) / 8 of the parts: the difference itself may pass fp32's range
+    s = torch.maximum((hi - c) * (1 / 7), c * 0.125 - lo * 0.125).to(BF16).to(F32)
     bad = ~(torch.isfinite(lo) & torch.isfinite(hi))
     c, s = (t.masked_fill(bad, math.nan) for t in (c, s))
     s = s.masked_fill(s < 2.0 ** -126, 0.0)
@@ -31,6 +32,13 @@ def values(n, s, c, group, dtype=F64):
     """What codes, s and c stand for."""
     n = n.to(dtype).unflatten(-1, (-1, group)) - 8
     return (c.to(dtype)[..., None] + s.to(dtype)[..., None] * n).flatten(-2)
+
+
+def read_back(n, s, c, group):
+    """The bf16 that a read returns: a value that the step's rounding puts past bf16's largest
+    comes back as that."""
+    top = torch.finfo(BF16).max
+    return values(n, s, c, group).clamp(-top, top).to(F32).to(BF16)
 
 
 def places(d):

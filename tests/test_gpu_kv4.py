@@ -10,6 +10,7 @@ from kernel_optim_amd.kernels.kv4 import (KV4_KEYS, Kv4Attention, kv4_append, kv
                                           kv4_cache, kv4_read, kv4_write)
 from kernel_optim_amd.kernels.fused import rope_rows
 from oracle import kv4 as O
+from tests.test_oracle_kv4 import top_groups
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -619,3 +620,35 @@ def test_refusals(dev):
         plan.decode_qkv(*good, cache, out, 1e-6, rope=tab)
     torch.cuda.synchronize()
     assert not cache.any() and not out.any() and not q.any()
+
+
+@pytest.mark.parametrize("d,group", FORMATS)
+def test_the_top_of_the_range(dev, d, group):
+    """Finite groups whose ends lie further apart than fp32's largest number, or next to bf16's: held
+    as any other group is, by both writers, and read back finite."""
+    g = top_groups()
+    per, reps = d // group, group // 32
+    S = -(-len(g) // per)
+    x = torch.cat((g, g[:S * per - len(g)])).repeat_interleave(reps, 1)
+    x = x.reshape(1, 1, S, d)
+    k, v = torch.cat((x, x.flip(2)), 1), torch.cat((-x, x), 1)
+    nb = -(-S // KV4_KEYS)
+    old = junk((1, 2, nb, kv4_block_bytes(d, group)), 120)
+    want = O.write(old, k, v, [0], [S], group)
+    cache = old.to(dev)
+    kv4_write(k.to(dev), v.to(dev), cache)
+    assert torch.equal(cache.cpu(), want)
+    ko, vo = (torch.empty(1, 2, S, d, dtype=BF16, device=dev) for _ in range(2))
+    kv4_read(cache, ko, vo)
+    held = O.read_back(*O.unpack(want, d, group), group)[:, :, :, :S]
+    assert held.isfinite().all()
+    assert torch.equal(ko.cpu(), held[0]) and torch.equal(vo.cpu(), held[1])
+    # the append: the same rows as V of one sequence's tokens
+    qkv = torch.zeros(S, 1 + 2 * 2, d, dtype=BF16)
+    qkv[:, 3:] = v[0].transpose(0, 1)
+    w, tab = torch.ones(d, dtype=BF16, device=dev), torch.ones(S, d, dtype=BF16, device=dev)
+    q, cache = torch.empty(S, d, dtype=BF16, device=dev), old.to(dev)
+    kv4_append(qkv.flatten(1).to(dev), w, w, tab, tab, torch.zeros(1, dtype=torch.int32, device=dev),
+               q, cache, S, 1e-6, 1, 2, d)
+    for got, ref in zip(O.unpack(cache, d, group), O.unpack(want, d, group)):
+        assert torch.equal(got[1, :, :, :S], ref[1, :, :, :S])

@@ -60,3 +60,39 @@ def test_attention_of_an_empty_row_is_zero():
     cache[..., 32 * 64:] = 0xff   # NaN everywhere: nothing may read it
     out, _, _ = O.attention(torch.ones(2, 64), cache, [0], 2, 1, 64, 64)
     assert (out == 0).all()
+
+
+BF16_MAX = torch.finfo(O.BF16).max
+
+
+def top_groups():
+    """Groups whose span passes fp32's range by up to twice, and groups of one sign near the largest
+    value: [N, 32] bf16, both ends among them."""
+    t = torch.cat((torch.linspace(2.9e38, BF16_MAX, 40), torch.tensor([1e38, 2.0 ** 120])))
+    t = t.to(O.BF16).double()
+    lo = torch.cat((-t, -t, -t, t[:20]))
+    hi = torch.cat((t, t.flip(0), -t.flip(0) / 8, torch.full((20,), BF16_MAX, dtype=torch.float64)))
+    lo, hi = torch.minimum(lo, hi), torch.maximum(lo, hi)
+    # one whose code 0 lies past the largest value, where code 1 is more than half a step off
+    lo = torch.cat((lo, torch.tensor([-3.3895313892515355e38])))
+    hi = torch.cat((hi, torch.tensor([-3.083808950221005e38])))
+    at = torch.linspace(0, 1, 32, dtype=torch.float64)
+    return (lo[:, None] + (hi - lo)[:, None] * at).to(O.BF16)
+
+
+def test_groups_at_the_top_of_the_range():
+    """Any finite group is held within the bound of the others, and reads back finite."""
+    x = top_groups()
+    n, s, c = O.quantise(x, 32)
+    assert s.isfinite().all() and c.isfinite().all()
+    err = (O.values(n, s, c, 32) - x.double()).abs()
+    assert (err <= s.double() * (0.5 + 2.0 ** -5 + 2.0 ** -10)).all()
+    back = O.read_back(n, s, c, 32)
+    assert back.isfinite().all()
+    # clamping brings a value nearer; then bf16's rounding
+    err = (back.double() - x.double()).abs()
+    assert (err <= s.double() * (0.5 + 2.0 ** -5 + 2.0 ** -10) + x.double().abs() * 2.0 ** -8).all()
+    for bad in (math.nan, math.inf, -math.inf):
+        y = x.clone()
+        y[:, 5] = bad
+        assert O.read_back(*O.quantise(y, 32), 32).isnan().all()
