@@ -53,8 +53,11 @@ struct Kv4Group {
     float s = round_bf16(fmaxf((mx - c) * (float)(1.0 / 7.0), c * 0.125f - mn * 0.125f));
     if (!(fabsf(mn) < INFINITY && fabsf(mx) < INFINITY)) c = s = __uint_as_float(0x7fc00000u);
     if (s < 1.1754943508222875e-38f) s = 0.f;
-    // 1 / s, rounded correctly: v_rcp_f32 and one Newton step are, for every bf16 from 2^-126 to
-    // 2^126 (all of them compared on the GPU), and s, about 1/15 of a span below 2^129, is below 2^126
+    // 1 / s, rounded correctly: with y = (1 + e) / s from v_rcp_f32, |e| < 2^-22, the inner fma is exact
+    // and the outer one rounds (1 - e^2) / s, 2^-44 off; but 1 / s of an 8-bit significand m lies
+    // at least 2^-32 of itself from any border between two floats (|2^32 - j m| >= 1 for its
+    // denominator m 2^32), a power of two on a float. s, about 1/15 of a span below 2^129, is below 2^126,
+    // so y is normal.
     const float y = __builtin_amdgcn_rcpf(s);
     inv = s == 0.f ? 0.f : fmaf(fmaf(-s, y, 1.0f), y, y);
     sc = (__float_as_uint(s) >> 16) | (__float_as_uint(c) & 0xffff0000u);

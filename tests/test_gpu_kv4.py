@@ -652,3 +652,32 @@ def test_the_top_of_the_range(dev, d, group):
                q, cache, S, 1e-6, 1, 2, d)
     for got, ref in zip(O.unpack(cache, d, group), O.unpack(want, d, group)):
         assert torch.equal(got[1, :, :, :S], ref[1, :, :, :S])
+
+
+def test_every_scale_and_the_borders_of_its_codes(dev):
+    """Groups whose scale takes every normal bf16 below 2^125 (from there on only the widest
+    spans, test_the_top_of_the_range), with the values on both sides of each border between two
+    codes: a reciprocal of s that is off by its last bit moves codes of 3,800 of them."""
+    s = (torch.arange(0x0080, 0x7e00, dtype=torch.int32) << 16).view(torch.float32).double()
+    lo, hi = -8 * s, (7 * s).to(BF16).double()
+    border = (torch.arange(15, dtype=torch.float64) - 7.5) * s[:, None]
+    near = border.to(BF16)
+    # the neighbour on the border's other side, where the border is no bf16 itself: one bit pattern
+    # further from zero or nearer to it
+    bits = near.view(torch.int16)
+    further = near.double().abs() < border.abs()
+    other = (bits + torch.where(further, 1, -1).to(torch.int16)).view(BF16)
+    x = torch.cat((lo[:, None], hi[:, None], near.double(), other.double()), 1)
+    x = torch.minimum(torch.maximum(x, lo[:, None]), hi[:, None]).to(BF16)
+    d, group = 128, 32
+    S = len(s) // 4
+    k = x.reshape(1, 1, S, d)
+    v = k.flip(2).contiguous()
+    cache = kv4_cache(1, 1, S, d, dev, group)
+    kv4_write(k.to(dev), v.to(dev), cache)
+    n, sc, c = O.unpack(cache, d, group)
+    for i, rows_ in enumerate((k, v)):
+        want = O.quantise(rows_, group)
+        for got, w in zip((n[i], sc[i], c[i]), want):
+            assert torch.equal(got[:, :, :S], w)
+    assert torch.equal(sc[0, 0, 0, :S].flatten().double(), s)   # every scale occurs
