@@ -681,3 +681,27 @@ def test_every_scale_and_the_borders_of_its_codes(dev):
         for got, w in zip((n[i], sc[i], c[i]), want):
             assert torch.equal(got[:, :, :S], w)
     assert torch.equal(sc[0, 0, 0, :S].flatten().double(), s)   # every scale occurs
+
+
+def exact_step(dev, B, nq, nkv, d, group, cap, pos, seed):
+    """decode_qkv against kv4_append and with_lengths, bit for bit, and the result within the
+    attention's own bound of the 64-bit one over the same q."""
+    old = filled(B, nkv, cap, d, group, pos, seed)
+    qkv, q_w, k_w, cos, sin = step_inputs(seed + 1, B, 1, nq, nkv, d, cap, dev)
+    at = torch.tensor(pos, dtype=torch.int32, device=dev)
+    cache, out = old.to(dev), torch.full((B, nq * d), math.nan, dtype=BF16, device=dev)
+    plan = Kv4Attention(B, 1, cap, nq, nkv, d, dev, group=group)
+    plan.decode_qkv(qkv, q_w, k_w, cos, sin, at, cache, out, 1e-6)
+    apart, q, again = old.to(dev), torch.empty_like(out), torch.full_like(out, math.nan)
+    kv4_append(qkv, q_w, k_w, cos, sin, at, q, apart, 1, 1e-6, nq, nkv, d)
+    plan.with_lengths(q, apart, at + 1, again)
+    assert torch.equal(cache, apart) and torch.equal(out, again)
+    check_attention(out, q, cache, [p + 1 for p in pos], 1, nq, d, group)
+
+
+@pytest.mark.parametrize("d,group", FORMATS)
+def test_a_decode_step_is_its_two_ops(dev, d, group):
+    exact_step(dev, 1, 8, 2, d, group, 96, [64], 130)
+    exact_step(dev, 5, 8, 2, d, group, 96, [30, 1, 17, 0, 95], 132)
+    exact_step(dev, 40, 16, 4, d, group, 128, [(5 * i) % 128 for i in range(40)], 134)
+    exact_step(dev, 2, 8, 1, d, group, 3000, [2900, 77], 136)
