@@ -705,3 +705,14 @@ def test_a_decode_step_is_its_two_ops(dev, d, group):
     exact_step(dev, 5, 8, 2, d, group, 96, [30, 1, 17, 0, 95], 132)
     exact_step(dev, 40, 16, 4, d, group, 128, [(5 * i) % 128 for i in range(40)], 134)
     exact_step(dev, 2, 8, 1, d, group, 3000, [2900, 77], 136)
+
+
+@pytest.mark.parametrize("T,nq,nkv,d,group", [
+    (1, 8, 1, 128, 32),    # 8 held rows: 2 a wavefront in the merge
+    (1, 4, 1, 64, 64),     # one group a head: 16 held rows, 4 a wavefront
+    (5, 4, 1, 128, 32),    # 20 query rows in two blocks of 16, 8 wavefronts
+    (8, 8, 1, 128, 32),    # 64 in four
+    (8, 4, 1, 64, 32)])
+def test_more_than_64_parts_of_a_pair(dev, T, nq, nkv, d, group):
+    """The merge takes 64 parts at a time and rescales what it has; 79 parts here."""
+    attend(dev, 1, T, nq, nkv, d, group, 20000, [19987])
