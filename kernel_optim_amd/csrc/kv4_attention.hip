@@ -17,8 +17,9 @@
 //   times that and c sum q, and sums over the GPT neighbouring lanes of a row.
 // - The result leaves each lane with 8 consecutive keys of one column, which is the A operand
 //   of the product over keys: p s goes from registers into the matrix cores, no exchange. p s is
-//   rounded to bf16 (2^-9 of each term; the terms add up, their roundings do not); p and sum p c
-//   stay fp32.
+//   rounded to bf16, the type that the matrix cores take (up to 2^-8 of each term; the terms add
+//   up, their roundings do not: 0.0023 of the output in 2-norm against 0.0017 for its own rounding
+//   alone), as P is over the bf16 cache; p and sum p c stay fp32.
 // - Output: B is V, a tile of 16 columns of one group. The offset leaves with the constant -136
 //   in a product of its own, before the codes' product: what accumulates is sum p s (n - 8), as
 //   small as the result, and not 136 sum p s, whose roundings would grow with the length.

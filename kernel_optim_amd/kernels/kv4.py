@@ -13,7 +13,7 @@ ValueError before anything is launched.
 
 A head vector's values are held in groups of 32, 64 or 128 that share a bf16 scale s and a bf16
 value c: x = c + s (n - 8), n = 0..15, within s / 2 of what was written (up to the rounding of
-s itself, 2^-9 of 7 s); a group of equal bf16 values reads back as it was, a group with a NaN or
+s itself, 2^-8 of up to 8 s); a group of equal bf16 values reads back as it was, a group with a NaN or
 an infinity as NaN throughout, a finite group finite. 5, 4.5 or 4.25 bits a value, scales included.
 
 A cache is a uint8 tensor [B, nkv, blocks, bytes]: 32 keys of a (sequence, KV head) pair are one
