@@ -36,7 +36,7 @@ break-even, decoding finishes on the pipelined one-token graph
 (engine.py:403-508).
 
 With ENGINE_KV_CACHE=kv4 (or kv_cache="kv4") K and V are held in 4 bits (kernels.kv4; 5 bits a
-value with the scales of the default groups of 32, ENGINE_KV_GROUP): 3.2 times the keys in
+value with the scales of the default groups of 32, ENGINE_KV_GROUP or kv_group): 3.2 times the keys in
 the same memory and a decode step that reads as much less of them. The prompt attends to
 its own K and V in bf16, layer by layer, before they are quantised; decode and verify
 steps attend to what the cache holds.
@@ -338,7 +338,7 @@ class HostCopies:
 
 class Engine:
     def __init__(self, model_path: str, keep_logits: bool = False, spec=None,
-                 decode_graph=None, kv_cache=None) -> None:
+                 decode_graph=None, kv_cache=None, kv_group=None) -> None:
         self._t0 = time.monotonic()
         if model_path.startswith("random"):
             seed = int(model_path.split(":", 1)[1]) if ":" in model_path else 0
@@ -358,26 +358,29 @@ class Engine:
             raise FileNotFoundError(
                 f"{model_path}: no *.safetensors weights (pass 'random[:seed]' or set "
                 "ENGINE_RANDOM_INIT=1 for random weights over its config.json)")
-        self._init(cfg, w, keep_logits, spec, decode_graph, kv_cache)
+        self._init(cfg, w, keep_logits, spec, decode_graph, kv_cache, kv_group)
 
     @classmethod
     def from_weights(cls, cfg, weights, keep_logits=False, spec=None, decode_graph=None,
-                     kv_cache=None):
+                     kv_cache=None, kv_group=None):
         """Engine over weights already in the decode layout (moved to the GPU)."""
         from .model import weights_to
         self = cls.__new__(cls)
         self._t0 = time.monotonic()
-        self._init(cfg, weights_to(weights, DEVICE), keep_logits, spec, decode_graph, kv_cache)
+        self._init(cfg, weights_to(weights, DEVICE), keep_logits, spec, decode_graph, kv_cache,
+                   kv_group)
         return self
 
-    def _init(self, cfg, w, keep_logits, spec=None, decode_graph=None, kv_cache=None):
+    def _init(self, cfg, w, keep_logits, spec=None, decode_graph=None, kv_cache=None,
+              kv_group=None):
         """spec: prompt-lookup speculation on (True) or off (False); None takes
         ENGINE_SPEC (off unless set to 1). decode_graph: "auto" (the fused-GEMV
         decode graph up to 32 sequences, or 64 where auto_graph says so, the
         hipBLASLt graph above), "timed" (capture both up to FUSED_MAX_TIMED sequences, time them at setup
         and keep the faster), "fused" or "hipblaslt"; None takes
         ENGINE_DECODE_GRAPH (auto unless set). kv_cache: "bf16" or "kv4" (K and V in 4
-        bits); None takes ENGINE_KV_CACHE (bf16 unless set)."""
+        bits); None takes ENGINE_KV_CACHE (bf16 unless set). kv_group: the 4-bit cache's values
+        that share a scale, 32, 64 or 128; None takes ENGINE_KV_GROUP (32 unless set)."""
         self.spec = SPEC if spec is None else bool(spec)
         self.min_advance = MIN_ADVANCE   # None: the measured break-even
         kind = DECODE_GRAPH if decode_graph is None else decode_graph
@@ -388,8 +391,9 @@ class Engine:
         if held not in ("bf16", "kv4"):
             raise ValueError(f"kv_cache must be bf16 or kv4, not {held!r}")
         self.kv_cache, self.kv4 = held, None
+        self.kv_group = KV_GROUP if kv_group is None else kv_group
         if held == "kv4":
-            kv4_block_bytes(cfg.head_dim, KV_GROUP)   # refuses a group it does not serve
+            kv4_block_bytes(cfg.head_dim, self.kv_group)   # refuses a group it does not serve
         if cfg.head_dim != 128 or cfg.nq != 4 * cfg.nkv:
             raise ValueError("the decode kernels serve head_dim 128 with 4 query heads per KV head")
         self.cfg, self.w = cfg, w
@@ -427,7 +431,8 @@ class Engine:
         dev = DEVICE
         bf = torch.bfloat16
         if self.kv_cache == "kv4":
-            self.kv4 = kv4_cache(B, cfg.nkv, cap, cfg.head_dim, dev, KV_GROUP, layers=cfg.layers)
+            self.kv4 = kv4_cache(B, cfg.nkv, cap, cfg.head_dim, dev, self.kv_group,
+                                 layers=cfg.layers)
         else:
             self.k_cache = torch.zeros(cfg.layers, B, cfg.nkv, cap, cfg.head_dim, dtype=bf,
                                        device=dev)
@@ -449,7 +454,7 @@ class Engine:
         self.ring_ctr = torch.zeros(B, dtype=torch.int32, device=dev)
         self.events = [torch.cuda.Event() for _ in range(N + 1)]
         if self.kv4 is not None:
-            self.attn = Kv4Attention(B, 1, cap, cfg.nq, cfg.nkv, cfg.head_dim, dev, KV_GROUP)
+            self.attn = Kv4Attention(B, 1, cap, cfg.nq, cfg.nkv, cfg.head_dim, dev, self.kv_group)
         else:
             self.attn = DecodeAttention(B, 1, cap, cfg.nq, cfg.nkv, cfg.head_dim, dev,
                                         unit=ATTN_UNIT or None, fused_combine=True,
@@ -521,7 +526,8 @@ class Engine:
         self.attT = torch.zeros_like(self.qT)
         self.actT = torch.zeros(M, cfg.inter, dtype=bf, device=dev)
         if self.kv4 is not None:
-            self.attnk = Kv4Attention(B, T, self.cap, cfg.nq, cfg.nkv, cfg.head_dim, dev, KV_GROUP)
+            self.attnk = Kv4Attention(B, T, self.cap, cfg.nq, cfg.nkv, cfg.head_dim, dev,
+                                      self.kv_group)
         elif VERIFY_TOKEN_ROWS:
             # the B*T tokens as rows of the one-token kernel, each row merged by
             # its last unit: one launch
