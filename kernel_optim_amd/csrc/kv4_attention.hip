@@ -480,10 +480,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_attn_kernel(Kv4AttnArgs a) 
           for (int j = 0; j < J; ++j) acc[j][e] *= ar;
         }
       }
-      const float mz = -m * a.scale_log2;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale_log2, mz));
+        // the difference first: in fma(sc, scale, -m scale) the rounding of m scale stays, and
+        // passes exp2's range for scores of 2^31 (the fma is at most 1 % faster: 512 keys 7.24 for
+        // 7.32 us, 16 x 32768 109.6 for 110.1)
+        sc[e] = __builtin_amdgcn_exp2f((sc[e] - m) * a.scale_log2);
         l += sc[e];
       }
       // ---- p s, and sum p c ----

@@ -716,3 +716,45 @@ def test_a_decode_step_is_its_two_ops(dev, d, group):
 def test_more_than_64_parts_of_a_pair(dev, T, nq, nkv, d, group):
     """The merge takes 64 parts at a time and rescales what it has; 79 parts here."""
     attend(dev, 1, T, nq, nkv, d, group, 20000, [19987])
+
+
+def scaled(cache, d, group, by_k, by_v):
+    """The cache with its K and V values times powers of two."""
+    n, s, c = O.unpack(cache, d, group)
+    by = torch.tensor([by_k, by_v]).view(2, 1, 1, 1, 1)
+    return O.pack(n, s * by, c * by)
+
+
+@pytest.mark.parametrize("T,nq,nkv,d,group", [(1, 8, 2, 128, 32), (1, 8, 1, 64, 64), (5, 8, 2, 128, 64),
+                                              (1, 4, 4, 128, 128)])
+@pytest.mark.parametrize("power", [4, 10, 15, 20, 38])
+def test_large_scores(dev, T, nq, nkv, d, group, power):
+    """q and K of 2^power: the scores' differences decide, whatever the scores are. One wavefront's
+    steps, several wavefronts and several parts."""
+    for lens in ([40, 7], [300, 257], [2900, 1031]):
+        B, cap = 2, max(lens)
+        cache = scaled(filled(B, nkv, cap, d, group, lens, 140 + power), d, group, 2.0 ** power, 1.0)
+        cache = cache.to(dev)
+        q = (randn(141, B * T, nq * d) * 2.0 ** power).to(BF16)
+        # fp32 scores are off by up to 2^-14 of sum |q k| (codes as 128 + n: 136 / 8 of 2^-23 a term
+        # and the sum's roundings); far below the distance of a row's two largest
+        n, s, c = O.unpack(cache, d, group)
+        clear = torch.zeros(B, T, nq, dtype=torch.bool)
+        for b in range(B):
+            for t in range(T):
+                m = lens[b] - T + t + 1
+                k = O.values(n[0, b, :, :m], s[0, b, :, :m], c[0, b, :, :m], group)
+                x = q.double().view(B, T, nkv, -1, d)[b, t] @ k.transpose(1, 2).contiguous()
+                size = q.double().view(B, T, nkv, -1, d)[b, t].abs() @ k.abs().transpose(1, 2).contiguous()
+                top = x.topk(2, -1).values
+                clear[b, t] = (top[..., 0] - top[..., 1] > 2.0 ** -12 * size.amax(-1)).flatten()
+        q, ln = q.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)
+        out = torch.full_like(q, math.nan)
+        Kv4Attention(B, T, cap, nq, nkv, d, dev, group=group).with_lengths(q, cache, ln, out)
+        want, step, size = O.attention(q, cache, lens, T, nq, d, group)
+        assert not out.isnan().any()
+        if power >= 10:   # one key takes all of a row's weight
+            tol = want.abs() * 2.0 ** -8 + step * 2.0 ** -8 + size * 2.0 ** -13 + 1e-30
+            fine = (out.cpu().double() - want).abs() <= tol
+            assert clear.float().mean() > 0.9
+            assert fine.view(B, T, nq, d)[clear].all()
