@@ -398,7 +398,8 @@ int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void*
 /* Decode attention over a 4-bit cache layer: as ko_decode_attn for q [B*T, nq*d] bf16 and out
  * (another buffer), query t of sequence b at position n - T + t, n = kv_lens[b] + len_offset; the
  * keys are those below min(n, cap), and the cache holds ceil(cap / 32) blocks a pair. A row that
- * sees no key is zero. nq a multiple of nkv, T * nq / nkv <= 64, 0 < scale < 10^4. The steps of
+ * sees no key is zero. Sums run unnormalised in fp32: |v| times the number of keys may reach 2^115,
+ * and |q . k| 1e30. nq a multiple of nkv, T * nq / nkv <= 64, 0 < scale < 10^4. The steps of
  * 32 keys of all pairs are dealt out in runs of at least min_run steps to grid workgroups of 4
  * wavefronts (or half as many of 8); B * nkv * (blocks + 24) + grid + min_run <= 2^24. part: fp32
  * scratch of part_len >= ko_kv4_attn_scratch(T * nq / nkv, d, group, grid); counters [grid]

@@ -250,7 +250,8 @@ class Kv4Attention:
     rounded up to whole blocks, as kv4_cache does.
 
     Any number of query heads per KV head and tokens with T * nq / nkv <= 64, T <= 8; head_dim 64
-    or 128. A query row that sees no key is zero. Calls of one object share its workspace:
+    or 128. A query row that sees no key is zero. Sums run unnormalised in fp32, of V's codes 17
+    times the size of its values: |v| times the number of keys may reach 2^115, and |q . k| 1e30. Calls of one object share its workspace:
     they must not overlap on two streams, nor may graphs captured from them.
     """
 

@@ -758,3 +758,19 @@ def test_large_scores(dev, T, nq, nkv, d, group, power):
             fine = (out.cpu().double() - want).abs() <= tol
             assert clear.float().mean() > 0.9
             assert fine.view(B, T, nq, d)[clear].all()
+
+
+@pytest.mark.parametrize("T,nq,nkv,d,group", [(1, 8, 2, 128, 32), (5, 8, 2, 64, 64)])
+def test_large_values(dev, T, nq, nkv, d, group):
+    """V of the largest magnitude that the attention's sums are promised for: 2^115 over the keys."""
+    lens = [1000, 333]
+    cache = filled(2, nkv, 1000, d, group, lens, 150)
+    n, s, c = O.unpack(cache, d, group)
+    top = O.values(n[1], s[1], c[1], group).nan_to_num(0).abs().max().item()
+    by = 2.0 ** math.floor(math.log2(2.0 ** 115 / 1000 / top))
+    cache = scaled(cache, d, group, 1.0, by).to(dev)
+    q = randn(151, 2 * T, nq * d).to(BF16).to(dev)
+    out = torch.full_like(q, math.nan)
+    Kv4Attention(2, T, 1000, nq, nkv, d, dev, group=group).with_lengths(
+        q, cache, torch.tensor(lens, dtype=torch.int32, device=dev), out)
+    check_attention(out, q, cache, lens, T, nq, d, group)
