@@ -80,6 +80,31 @@ def _no_overlap(t, name):
         reach += stride * (size - 1)
 
 
+def _meet(a, b):
+    """Whether two tensors of one shape, each without elements that share memory, have an element
+    in common. Layouts of different strides are taken to, where one lies within the other's reach."""
+    size, strides = a.element_size(), sorted(
+        ((s, n) for s, n in zip(a.stride(), a.shape) if n > 1), reverse=True)
+    span = 1 + sum(s * (n - 1) for s, n in strides)
+    other = 1 + sum(s * (n - 1) for s, n in zip(b.stride(), b.shape) if n > 1)
+    off = abs(b.data_ptr() - a.data_ptr())
+    if off >= size * (span if b.data_ptr() > a.data_ptr() else other):
+        return False
+    if off % size or strides != sorted(
+            ((s, n) for s, n in zip(b.stride(), b.shape) if n > 1), reverse=True):
+        return True
+
+    # off = sum of stride * i with |i| < n: the largest stride first, by at most its two neighbours
+    def reached(off, i):
+        if i == len(strides):
+            return off == 0
+        stride, n = strides[i]
+        return any(abs(k) < n and reached(off - k * stride, i + 1)
+                   for k in (off // stride, off // stride + 1))
+
+    return reached(off // size, 0)
+
+
 def _check_cache(cache, written):
     """The cache's (B, nkv, blocks, d, group, device)."""
     _need(isinstance(cache, torch.Tensor) and cache.dtype == torch.uint8 and cache.dim() == 4,
@@ -183,8 +208,10 @@ def kv4_read(cache, k_out, v_out, start=None, lengths=None):
     whose slot lies outside the cache. The two must not overlap. Strides and the other
     arguments as for kv4_write."""
     S, c, kv, rest, dev = _rows(cache, k_out, v_out, start, lengths, False, ("k_out", "v_out"))
-    _need(kv[0] != kv[4] or not S, "k_out and v_out must be two buffers")
     if S:
+        if abs(kv[0] - kv[4]) < 2 * k_out.numel() or not (k_out.is_contiguous()
+                                                          and v_out.is_contiguous()):
+            _need(not _meet(k_out, v_out), "k_out and v_out must not overlap")
         _lib.call("ko_kv4_read", *c, *kv, *rest, _stream(dev))
 
 
@@ -220,7 +247,8 @@ def kv4_append(qkv, q_w, k_w, cos, sin, pos, q_out, cache, T, eps, nq, nkv, d):
     position pos[b] + m % T. Per-head RMSNorm and RoPE of q into q_out [B*T, nq*d], of k into
     the cache's slot at that position with v, both quantised. Everything is fp32 up to the one
     rounding of q and the quantisation of k. Positions outside the cache or the RoPE tables
-    [rows, d] are skipped (their q_out rows too)."""
+    [rows, d] are skipped (their q_out rows too). q_out must not overlap qkv; of a single row it
+    may be the first nq*d values."""
     try:   # the usual call; the tests below name what is wrong
         B, ck, nb, size = cache.shape
         cd, group = _FORMATS[size]
@@ -241,6 +269,9 @@ def kv4_append(qkv, q_w, k_w, cos, sin, pos, q_out, cache, T, eps, nq, nkv, d):
         _tensor(q_out, "q_out", BF16, (B * T, nq * d), dev)
         qp, cp, (cb, ch, _) = q_out.data_ptr(), cache.data_ptr(), _outer(cache)
     ptrs, n_rows = _check_qkv(qkv, q_w, k_w, cos, sin, pos, B * T, B, nq, nkv, d, dev)
+    off, row = qp - ptrs[0], 2 * B * T * d   # bytes
+    _need(off >= row * (nq + 2 * nkv) or -off >= row * nq or (off == 0 and B * T == 1),
+          "q_out must not overlap qkv")
     _lib.call("ko_kv4_append", *ptrs, pos.data_ptr(), qp, cp, B * T, T, cb, ch, eps, nq, nkv, d,
               group, min(nb * KV4_KEYS, n_rows), None, _stream(dev))
 
@@ -250,8 +281,8 @@ class Kv4Attention:
     rounded up to whole blocks, as kv4_cache does.
 
     Any number of query heads per KV head and tokens with T * nq / nkv <= 64, T <= 8; head_dim 64
-    or 128. A query row that sees no key is zero. Sums run unnormalised in fp32, of V's codes 17
-    times the size of its values: |v| times the number of keys may reach 2^115, and |q . k| 1e30. Calls of one object share its workspace:
+    or 128. A query row that sees no key is zero. Sums run unnormalised in fp32: |v|
+    times the number of keys may reach 2^115, and |q . k| 1e30. Calls of one object share its workspace:
     they must not overlap on two streams, nor may graphs captured from them.
     """
 
@@ -287,6 +318,7 @@ class Kv4Attention:
         self._work = self._part.data_ptr(), self._part.numel(), self._counters.data_ptr()
         self._q = torch.empty(B, nq * d, dtype=BF16, device=dev) if T == 1 else None
         self._q_shape = torch.Size((B * T, nq * d))
+        self._q_bytes = 2 * B * T * nq * d
         self._cache_shape = torch.Size((B, nkv, self.blocks, self.block_bytes))
         self._len_shape = torch.Size((B,))
 
@@ -314,7 +346,7 @@ class Kv4Attention:
             self._check_cache(cache)
         if dev != _current_device():
             _here(dev)
-        _need(qp != op, "out must not be q")
+        _need(abs(qp - op) >= self._q_bytes, "out must not overlap q")
         cb, ch, _, _ = cache.stride()
         if cb % 16 or ch % 16:   # strides of single rows
             cb, ch, _ = _outer(cache)

@@ -774,3 +774,49 @@ def test_large_values(dev, T, nq, nkv, d, group):
     Kv4Attention(2, T, 1000, nq, nkv, d, dev, group=group).with_lengths(
         q, cache, torch.tensor(lens, dtype=torch.int32, device=dev), out)
     check_attention(out, q, cache, lens, T, nq, d, group)
+
+
+def test_outputs_that_overlap_are_refused(dev):
+    """Two outputs of a read, or an output and the rows that other workgroups still read, in one piece
+    of memory: by any distance, in any layout. Neighbours in one buffer are served."""
+    B, nq, nkv, d, S = 2, 4, 2, 128, 8
+    cache = filled(B, nkv, 64, d, 32, [64, 64], 160).to(dev)
+    hold = torch.zeros(1 << 16, dtype=BF16, device=dev)
+    n = B * nkv * S * d
+
+    def at(offset, *strides):
+        return hold.as_strided((B, nkv, S, d), strides or (nkv * S * d, S * d, d, 1), offset)
+
+    both = (2 * nkv * S * d, S * d, d, 1)     # [B, 2, nkv, S, d]
+    turned = (S * 2 * nkv * d, d, 2 * nkv * d, 1)   # [B, S, 2, nkv, d]
+    for a, b in ((at(0), at(8)), (at(n - 8), at(0)), (at(0), at(n - d)),
+                 (at(0, *both), at(S * d, *both)), (at(0, *turned), at(d, *turned)),
+                 (at(2 * nkv * d, *turned), at(0, *turned)), (at(0, *both), at(0, *turned))):
+        for k, v in ((a, b), (b, a)):
+            with pytest.raises(ValueError, match="overlap"):
+                kv4_read(cache, k, v)
+    want = [torch.empty(B, nkv, S, d, dtype=BF16, device=dev) for _ in range(2)]
+    kv4_read(cache, *want)
+    for a, b in ((at(0), at(n)), (at(n + 64), at(0)), (at(0, *both), at(nkv * S * d, *both)),
+                 (at(nkv * d, *turned), at(0, *turned)), (at(0, *turned), at(2 * n))):
+        kv4_read(cache, a, b)
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    plan = Kv4Attention(B, 1, 64, nq, nkv, d, dev)
+    ints = torch.full((B,), 3, dtype=torch.int32, device=dev)
+    row = lambda offset, cols: hold[offset:offset + B * cols].view(B, cols)
+    for offset in (0, 8, B * nq * d - 8):
+        for q, out in ((0, offset), (offset, 0)):
+            with pytest.raises(ValueError, match="overlap"):
+                plan(row(q, nq * d), cache, ints, row(out, nq * d))
+    plan(row(0, nq * d), cache, ints, row(B * nq * d, nq * d))
+    w, tab, wide = torch.ones(d, dtype=BF16, device=dev), torch.ones(64, d, dtype=BF16, device=dev), nq + 2 * nkv
+    for x, q in ((0, 0), (0, 8), (0, B * wide * d - 8), (B * nq * d - 8, 0)):
+        with pytest.raises(ValueError, match="overlap"):
+            kv4_append(row(x, wide * d), w, w, tab, tab, ints, row(q, nq * d), cache, 1, 1e-6, nq, nkv, d)
+    # one row in place: every head reads and writes its own values
+    hold.copy_(randn(161, 1 << 16))
+    x, one = hold[:wide * d].view(1, -1), cache[:1].clone()
+    q, again = torch.empty(1, nq * d, dtype=BF16, device=dev), cache[:1].clone()
+    kv4_append(x, w, w, tab, tab, ints[:1], q, one, 1, 1e-6, nq, nkv, d)
+    kv4_append(x, w, w, tab, tab, ints[:1], x[:, :nq * d], again, 1, 1e-6, nq, nkv, d)
+    assert torch.equal(x[:, :nq * d], q) and torch.equal(again, one)

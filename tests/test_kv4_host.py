@@ -114,3 +114,17 @@ def test_more_steps_than_the_kernel_counts_are_refused():
                                 "d", "group", "scale", "part", "part_len", "counters", "grid",
                                 "min_run", "out")} | dict(cap=1 << 20, B=64)
     assert _lib.lib().ko_kv4_attn(*a.values(), None) == -34
+
+
+def test_tensors_that_meet():
+    """_meet against the elements' addresses, over offsets and layouts."""
+    hold = torch.arange(500)
+    layouts = [((2, 3, 2, 4), s) for s in ((24, 8, 4, 1), (48, 8, 4, 1), (48, 4, 12, 1), (24, 4, 12, 1),
+                                           (12, 24, 4, 1))]
+    layouts += [((1, 3, 1, 4), (7, 12, 5, 1)), ((1, 1, 1, 4), (1, 1, 1, 1))]
+    for shape, strides in layouts:
+        a = hold.as_strided(shape, strides, 100)
+        for offset in range(250):
+            b = hold.as_strided(shape, strides, offset)
+            meet = bool(set(a.flatten().tolist()) & set(b.flatten().tolist()))
+            assert K._meet(a, b) == K._meet(b, a) == meet, (strides, offset)
