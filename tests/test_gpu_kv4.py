@@ -820,3 +820,57 @@ def test_outputs_that_overlap_are_refused(dev):
     kv4_append(x, w, w, tab, tab, ints[:1], q, one, 1, 1e-6, nq, nkv, d)
     kv4_append(x, w, w, tab, tab, ints[:1], x[:, :nq * d], again, 1, 1e-6, nq, nkv, d)
     assert torch.equal(x[:, :nq * d], q) and torch.equal(again, one)
+
+
+def test_captured_prompts_and_verify_steps_replay(dev):
+    """kv4_write, kv4_append, the attention and kv4_read in one graph, with other rows, starts,
+    lengths and positions in every replay, each against the same calls made eagerly between them."""
+    B, T, nq, nkv, d, group, cap, S = 3, 4, 8, 2, 128, 32, 256, 70
+    plans = [Kv4Attention(B, T, cap, nq, nkv, d, dev, group=group) for _ in range(2)]
+    qkv, q_w, k_w, cos, sin = step_inputs(170, B, T, nq, nkv, d, cap, dev)
+    k, v = (torch.empty(B, nkv, S, d, dtype=BF16, device=dev) for _ in range(2))
+    start, lengths, pos = (torch.zeros(B, dtype=torch.int32, device=dev) for _ in range(3))
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32)
+
+    def state():
+        return dict(cache=junk((B, nkv, cap // 32, kv4_block_bytes(d, group)), 171).to(dev),
+                    q=torch.zeros(B * T, nq * d, dtype=BF16, device=dev),
+                    out=torch.zeros(B * T, nq * d, dtype=BF16, device=dev),
+                    back=torch.zeros(2, B, nkv, S + T, d, dtype=BF16, device=dev))
+
+    def calls(plan, st):
+        kv4_write(k, v, st["cache"], start=start, lengths=lengths)
+        kv4_append(qkv, q_w, k_w, cos, sin, pos, st["q"], st["cache"], T, 1e-6, nq, nkv, d)
+        plan(st["q"], st["cache"], pos, st["out"])
+        kv4_read(st["cache"], *st["back"], start=start, lengths=lengths)
+
+    def inputs(rep):
+        k.copy_(rows(172 + rep, B, nkv, S, d))
+        v.copy_(rows(182 + rep, B, nkv, S, d))
+        qkv.copy_(step_inputs(192 + rep, B, T, nq, nkv, d, cap, dev)[0])
+        n = [(S, 1 + 9 * rep, S - rep), (7, S, 33), (S, S, S)][rep % 3]
+        at = [ints(0, 0, 0), ints(5, 31, 32), ints(100, 64, 186)][rep % 3]
+        start.copy_(at)
+        lengths.copy_(ints(*n))
+        pos.copy_(at + ints(*n))
+
+    graphed, eager = state(), state()
+    inputs(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls(plans[0], graphed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(plans[0], graphed)
+    graphed["cache"].copy_(eager["cache"])
+    for rep in range(6):
+        inputs(rep)
+        calls(plans[1], eager)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name in eager:
+            same = torch.equal(eager[name].view(torch.uint8), graphed[name].view(torch.uint8))
+            assert same, (rep, name)
