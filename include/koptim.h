@@ -372,7 +372,8 @@ int ko_gemv_tile(const void* w, void* wt, int rows, int K, void* stream);
  * stride 1, the other strides in elements, multiples of 8, into the slots from start[b] (NULL: 0)
  * on; the cache holds ceil(cap / 32) blocks a pair. Rows whose slot lies outside [0, cap) are
  * dropped; other slots keep what they hold.
- * ko_kv4_read: the reverse; rows past lengths[b] or outside [0, cap) are left as they were. */
+ * ko_kv4_read: the reverse; rows past lengths[b] or outside [0, cap) are left as they were; k and v
+ * must not overlap. */
 int ko_kv4_write(const void* k, long long k_b_stride, long long k_h_stride, long long k_s_stride,
                  const void* v, long long v_b_stride, long long v_h_stride, long long v_s_stride,
                  void* cache, long long cache_b_stride, long long cache_h_stride, const int* start,
@@ -389,14 +390,14 @@ int ko_kv4_read(const void* cache, long long cache_b_stride, long long cache_h_s
  * at that position. Norm and RoPE run in fp32; q rounds once, k is quantised from fp32.
  * Positions outside [0, max_pos) (max_pos = min(cap, table rows)) are skipped. rope (optional, T = 1,
  * [M][2][d] bf16, 16-byte aligned): the cos and sin rows at the positions (ko_rope_rows) in place
- * of the tables'. */
+ * of the tables'. q_out must not overlap qkv (of a single row it may be its first nq*d values). */
 int ko_kv4_append(const void* qkv, const void* q_w, const void* k_w, const void* cos,
                   const void* sin, const int* pos, void* q_out, void* cache, int M, int T,
                   long long cache_b_stride, long long cache_h_stride, float eps, int nq, int nkv,
                   int d, int group, int max_pos, const void* rope, void* stream);
 
 /* Decode attention over a 4-bit cache layer: as ko_decode_attn for q [B*T, nq*d] bf16 and out
- * (another buffer), query t of sequence b at position n - T + t, n = kv_lens[b] + len_offset; the
+ * (which must not overlap q), query t of sequence b at position n - T + t, n = kv_lens[b] + len_offset; the
  * keys are those below min(n, cap), and the cache holds ceil(cap / 32) blocks a pair. A row that
  * sees no key is zero. Sums run unnormalised in fp32: |v| times the number of keys may reach 2^115,
  * and |q . k| 1e30. nq a multiple of nkv, T * nq / nkv <= 64, 0 < scale < 10^4. The steps of

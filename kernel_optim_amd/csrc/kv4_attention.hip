@@ -31,11 +31,12 @@
 // else the workgroup that finishes the pair last merges the partial sums (fp32, in run order:
 // the result does not depend on who is last).
 //
-// Measured, 32 query and 8 KV heads of 128 in groups of 32: 16 x 8192 keys (168 MB) 32.3 us, 16 x
-// 32768 108-111 us (6.0-6.2 TB/s; the bf16 cache's attention reads at 6.6), 512 keys 7.2 us. Per
-// step and wavefront 290 VALU instructions with up to 4 query rows, 375 with 16, of about 4
+// Measured, 32 query and 8 KV heads of 128 in groups of 32: 16 x 8192 keys (168 MB) 31.5-33.2 us, 16 x
+// 32768 108-111 us (6.0-6.2 TB/s; the bf16 cache's attention reads at 6.6), 512 keys 7.1-7.4 us. Per
+// step and wavefront 297 VALU instructions with up to 4 query rows, 381 with 16, of about 4
 // cycles: two wavefronts on a SIMD keep ahead of the HBM with one query token, not with 4 and more
-// (16 x 8192 keys, 5 tokens: 59 us).
+// (16 x 8192 keys, 5 tokens: 59-62 us). With groups of 32 of 128 and more than 8 query rows 8 to 11
+// registers spill, stored ahead of the loop over pairs and read outside that over steps.
 #include "kv4_core.h"
 
 #include <limits.h>

@@ -145,7 +145,9 @@ __global__ __launch_bounds__(NT) void kv4_write_kernel(Kv4Rows a) {
 
 // c + s (n - 8): the product is exact in fp32 (8 by 4 bits), the sum rounds once. Past bf16's largest
 // value it is that value: lim is, and NaN where s or c is (v_med3_f32 of three NaN is one; with
-// two numbers beside a NaN it would be a number).
+// two numbers beside a NaN it would be a number). 32768 tokens of 8 heads of 128: 39.1 us, 38.5 without
+// the clamp (groups of 128: 38.8, 37.1). A smaller s cannot take its place: where (max - c) / 7 is far
+// above (c - min) / 8, codes that are used stay past the end.
 __device__ __forceinline__ float kv4_lim(uint32_t sc) {
   return fmaf(bf16lo(sc), 0.f, fmaf(bf16hi(sc), 0.f, 0x1.fep127f));
 }
@@ -276,9 +278,8 @@ __global__ __launch_bounds__(NT) void kv4_read_kernel(Kv4Rows a) {
 // ---- q/k RMSNorm + RoPE + quantised append: one wavefront per (row, head) ----
 // Lane l holds the pair of elements 2 l, 2 l + 1 (d = 64: both halves of the wavefront hold
 // the head). Norm and RoPE run in fp32 throughout and q rounds once at the end, to the bf16 that the
-// attention's matrix products take; k is
-// quantised from fp32, so no rounding to bf16 moves a value over a code's border. 2.8-3.4 us for
-// 1 to 32 rows of 48 heads of 128: a launch's latency.
+// attention's matrix products take; k is quantised from fp32, so no rounding to bf16 moves a value
+// over a code's border. 2.8-3.4 us for 1 to 32 rows of 48 heads of 128: a launch's latency.
 template <int D, int NG>
 __global__ __launch_bounds__(NT) void kv4_append_kernel(
     const uint16_t* __restrict__ qkv, const uint16_t* __restrict__ qw,

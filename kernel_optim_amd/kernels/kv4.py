@@ -3,7 +3,8 @@
 The ops stand beside ``kernels.fused``'s for the bf16 cache and follow their manner: tensors
 are the caller's, every call launches on the current stream of the current device, allocates
 nothing and never synchronises (so calls can be captured), and a bad argument raises
-ValueError before anything is launched.
+ValueError before anything is launched (RuntimeError where a call is too large for one launch: 2^26
+heads of rows to append, 2^25 blocks to write or read).
 
 - ``kv4_cache`` allocates a cache; ``kv4_write`` quantises bf16 K/V rows into it, ``kv4_read``
   reads cached keys back as bf16;
