@@ -427,6 +427,31 @@ int ko_kv4_attn_qkv(const void* qkv, const void* q_w, const void* k_w, const voi
  * -1 for bad arguments. */
 long long ko_kv4_attn_scratch(int rows, int d, int group, int grid);
 
+/* ---- Matrices held in 8-bit floating point --------------------------------------
+ * No counterpart in the reference, whose weights are bf16.
+ * A matrix [rows, K], K % 8 == 0, is held as e4m3 codes and one power-of-two scale for each row
+ * and block of 128 values: codes uint8 [tiles][ceil(K / 128)][2048], scales uint8
+ * [tiles][ceil(K / 512)][64] (kernel_optim_amd/csrc/fp8_core.h has the layout), tiles =
+ * ceil(rows / 16), or of a pair (gate | up: even rows, the halves' tiles alternating)
+ * 2 ceil(rows / 32). The scale is the least 2^e >= 2^-127 with max |x| <= 448 * 2^e, a code x / 2^e
+ * rounded to nearest (ties to even); a block with a NaN or an infinity holds NaN. All pointers
+ * 16-byte aligned.
+ *
+ * ko_fp8_quantize: x [rows, K] bf16 (x_f32 0) or fp32, row stride in elements (a multiple of 8, or 0),
+ * into codes and scales, which must not overlap x. nw (optional, [K] bf16; bf16 rows, no pair): the
+ * rows go through bf16(nw * bf16(x * rsqrt(mean(x^2) + eps))) first.
+ * ko_fp8_read: the reverse, into out [rows, K] bf16 or fp32. */
+int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K, int pair,
+                    const void* nw, float eps, void* codes, void* scales, void* stream);
+int ko_fp8_read(const void* codes, const void* scales, int rows, int K, int pair, void* out,
+                int out_f32, long long stride, void* stream);
+
+/* y[M, N] = x W^T of x [M, K] (codes xc, scales xs) and W [N, K] (wc, ws), sums in fp32. epi 0: y
+ * fp32; 1: bf16; 2 (RESID): y = bf16(h + bf16(sum)), h [M, N] bf16, which may be y; 3 (SWIGLU): W is
+ * gate | up [2 N, K] held as a pair, y = bf16(bf16(silu(bf16(gate sum))) * bf16(up sum)). */
+int ko_fp8_linear(const void* xc, const void* xs, const void* wc, const void* ws, void* y,
+                  const void* h, int M, int N, int K, int epi, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

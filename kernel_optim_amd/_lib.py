@@ -85,6 +85,11 @@ SIGNATURES = {
                         _c_void_p, _ll, _ll, _int, _int, _int, _int, _int, _int, _f, _f, _c_void_p,
                         _c_void_p, _ll, _c_void_p, _int, _int, _c_void_p, _c_void_p, _c_void_p],
     "ko_kv4_attn_scratch": [_int, _int, _int, _int],
+    "ko_fp8_quantize": [_c_void_p, _int, _ll, _int, _int, _int, _c_void_p, _f, _c_void_p, _c_void_p,
+                        _c_void_p],
+    "ko_fp8_read": [_c_void_p, _c_void_p, _int, _int, _int, _c_void_p, _int, _ll, _c_void_p],
+    "ko_fp8_linear": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _int, _int,
+                      _int, _int, _c_void_p],
 }
 
 # Entry points whose return value is a size, not a status.

@@ -1,0 +1,102 @@
+// The layout of a matrix held in 8-bit floating point, and what its kernels share.
+//
+// A matrix [rows, K] is held as OCP e4m3 codes with one scale 2^(b - 127), b a byte, for each
+// (row, 128 values of K): value = code * scale. b is the least with max |x| <= 448 * scale, so
+// the largest value's code lies in (224, 448] and a code is within 2^-4 of its value (relative;
+// below 2^-6 of the scale within 2^-10 of it). A power of two costs nothing against a scale of
+// more bits: codes are floating point themselves, dividing by it is exact, and the instructions
+// that take codes apply it, so sums stay in the accumulators.
+// A block with a NaN or an infinity holds NaN codes and b = 255: it reads back as NaN.
+//
+// Codes lie in the order in which v_mfma_scale_f32_16x16x128_f8f6f4 takes them: a tile of 16 rows
+// and 128 values is one block of 2 KB, the blocks of a tile follow one another along K. In a block, lane l of a
+// wavefront owns the bytes [16 l, 16 l + 16) of either KB j: row l % 16, values
+// 64 j + 16 (l / 16) + 0..15. Loads are 1 KB a wavefront, to registers or LDS alike, and LDS
+// holds blocks as they are with no bank conflicts. Any order of K inside a block would do, as
+// both factors have the same and all 128 values of a row share a scale.
+//
+// Two ways to multiply blocks, both with fp32 accumulators:
+// - that instruction on the codes (5 PFLOP/s dense at this GPU's peak). Of the 8 products of a
+//   lane's 8 neighbouring bytes it keeps what lies above 2^-13 of the largest one's binade
+//   (measured with one product 2^k beside one of 1 + 2^-2 + 2^-6: bits below 2^(k - 13) are cut off,
+//   across neighbouring eights none): each product loses less than 2^-13 of its eight's largest,
+//   where its codes' own rounding is 2^-4. A typical sum is 2^-14 off.
+// - the codes times their scale as bf16 (exact: 4 significant bits) on
+//   v_mfma_f32_16x16x32_bf16, half the rate, whose sums are fp32 throughout.
+// Few rows wait for memory, not for the matrix cores, and an fp32 result shows its sums' last bits:
+// these take the second; many rows with bf16 results, whose step is 2^-8, the first.
+//
+// Scales: [tile][quad of blocks][16 rows][4 blocks] bytes, so a lane's dword holds its row's
+// scales of 4 blocks and the instruction's op_sel picks one. Rows past the end and values past
+// K are zeros; so is the padding of scales.
+//
+// A pair (gate | up, [2 n, K]) has its tiles alternate: 2 t is rows 16 t.. of the first half,
+// 2 t + 1 of the second, each half padded to whole tiles.
+#pragma once
+
+#include "ko_common.h"
+
+namespace ko {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int FP8_BLOCK = 2048;   // bytes of a block of codes: 16 rows, 128 values
+
+__host__ __device__ __forceinline__ int fp8_blocks(int K) { return (K + 127) >> 7; }
+__host__ __device__ __forceinline__ int fp8_quads(int K) { return (K + 511) >> 9; }
+__host__ __device__ __forceinline__ long long fp8_tiles(int rows, bool pair) {
+  return pair ? 2ll * ((rows / 2 + 15) / 16) : (rows + 15ll) / 16;
+}
+
+// The row of [rows, K] that row r of tile t holds, or -1.
+__device__ __forceinline__ int fp8_row(long long t, int r, int rows, bool pair) {
+  if (!pair) {
+    const long long row = t * 16 + r;
+    return row < rows ? (int)row : -1;
+  }
+  const int n = rows >> 1;
+  const long long row = (t >> 1) * 16 + r;
+  return row < n ? (int)((t & 1) * n + row) : -1;
+}
+
+// The scale's byte for a block whose largest |x| has these bits (NaN and infinity sort above
+// every number): 448 = 1.75 * 2^8.
+__device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax_bits) {
+  const int e = (int)(amax_bits >> 23), b = e - 8 + ((amax_bits & 0x7fffffu) > 0x600000u);
+  return e == 255 ? 255u : (uint32_t)max(b, 0);
+}
+// 2^-(b - 127), b <= 247; the product with a value of the block is exact down to fp32's
+// subnormals, far below what a code can hold.
+__device__ __forceinline__ float fp8_inverse(uint32_t b) { return __uint_as_float((254u - b) << 23); }
+__device__ __forceinline__ float fp8_scale(uint32_t b) {
+  return b == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(b ? b << 23 : 0x400000u);
+}
+
+// Four codes of v * inv (to nearest, ties to even), or of NaN.
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float inv) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true);
+  return (uint32_t)w;
+}
+
+__device__ __forceinline__ uint32_t umax_xor16(uint32_t u) {
+  const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return max((uint32_t)p[0], (uint32_t)p[1]);
+}
+__device__ __forceinline__ uint32_t umax_xor32(uint32_t u) {
+  const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return max((uint32_t)p[0], (uint32_t)p[1]);
+}
+
+// 8 codes (the dwords w0, w1) times 2^(b - 127) as bf16; scale = b << 23.
+__device__ __forceinline__ bf16x8 fp8_to_bf16(uint32_t w0, uint32_t w1, float scale) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
+  return (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+}  // namespace ko

@@ -1,0 +1,249 @@
+// Rows to 8-bit floating point and back (layout: fp8_core.h).
+//
+// A wavefront takes a block of 16 rows and 128 values: lane l holds 2 x 16 values of row l % 16,
+// the maximum over the row's 128 takes two lane swaps, and the codes leave in two stores of 1 KB.
+#include "fp8_core.h"
+
+namespace {
+
+using namespace ko;
+
+// The 16 values [k, k + 16) of a row as fp32; values from K on are zero. K is a multiple of 8
+// and rows are 16-byte aligned.
+template <bool F32IN>
+__device__ __forceinline__ void load16(const void* x, long long at, int k, int K, bool ok,
+                                       float (&v)[16]) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const bool in = ok && k + 8 * p < K;
+    if constexpr (F32IN) {
+      const float* s = static_cast<const float*>(x) + at + k + 8 * p;
+      const uint4 a = in ? ldg16(s) : make_uint4(0, 0, 0, 0);
+      const uint4 b = in ? ldg16(s + 4) : make_uint4(0, 0, 0, 0);
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[8 * p + i] = __uint_as_float(w[i]);
+    } else {
+      const uint4 a = in ? ldg16(static_cast<const uint16_t*>(x) + at + k + 8 * p)
+                         : make_uint4(0, 0, 0, 0);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[8 * p + 2 * i] = bf16lo(w[i]);
+        v[8 * p + 2 * i + 1] = bf16hi(w[i]);
+      }
+    }
+  }
+}
+
+// One block's codes from the lane's 2 x 16 values; returns the row's scale byte.
+__device__ __forceinline__ uint32_t store_block(const float (&v)[2][16], uint8_t* block, int lane) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+  top = umax_xor32(umax_xor16(top));
+  const uint32_t b = fp8_scale_byte(top);
+  const float inv = fp8_inverse(min(b, 247u));
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = b == 255 ? 0x7f7f7f7fu
+                      : fp8_pack4(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
+    *reinterpret_cast<uint4*>(block + 1024 * j + 16 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return b;
+}
+
+// A wavefront for each quad of blocks of a tile.
+template <bool F32IN>
+__global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ x, long long stride,
+                                                       int rows, int K, int pair,
+                                                       uint8_t* __restrict__ codes,
+                                                       uint32_t* __restrict__ scales,
+                                                       long long units) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int Q = fp8_quads(K), KB = fp8_blocks(K);
+  const long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (u >= units) return;
+  const long long t = u / Q;
+  const int q = (int)(u - t * Q);
+  const int row = fp8_row(t, r, rows, pair);
+  const long long at = (long long)max(row, 0) * stride;
+  uint32_t sc = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int kb = 4 * q + i;
+    if (kb < KB) {
+      float v[2][16];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) load16<F32IN>(x, at, kb * 128 + 64 * j + 16 * g, K, row >= 0, v[j]);
+      sc |= store_block(v, codes + (t * KB + kb) * FP8_BLOCK, lane) << (8 * i);
+    }
+  }
+  if (g == 0) scales[(t * Q + q) * 16 + r] = sc;
+}
+
+constexpr int NORM_WAVES = 16;
+
+// RMSNorm in front (bf16 rows): a workgroup takes a tile, sums the squares of its 16 rows in
+// fp32, and its wavefronts quantise bf16(nw * bf16(x * rstd)) quad by quad. The rows are read
+// twice, the second time from the caches (16 rows of 2560 values: 80 KB).
+__global__ __launch_bounds__(64 * NORM_WAVES) void quantize_norm_kernel(
+    const uint16_t* __restrict__ x, long long stride, int rows, int K,
+    const uint16_t* __restrict__ nw, float eps, uint8_t* __restrict__ codes,
+    uint32_t* __restrict__ scales) {
+  __shared__ float s_sq[NORM_WAVES][16];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int Q = fp8_quads(K), KB = fp8_blocks(K);
+  const long long t = blockIdx.x;
+  const int row = fp8_row(t, r, rows, false);
+  const long long at = (long long)max(row, 0) * stride;
+  float sq = 0.f;
+  for (int kb = wv; kb < KB; kb += NORM_WAVES) {
+    float v[2][16];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load16<false>(x, at, kb * 128 + 64 * j + 16 * g, K, row >= 0, v[j]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sq += v[j][i] * v[j][i];
+  }
+  sq = sum_xor32(sum_xor16(sq));
+  if (g == 0) s_sq[wv][r] = sq;
+  __syncthreads();
+  float tot = 0.f;
+#pragma unroll
+  for (int i = 0; i < NORM_WAVES; ++i) tot += s_sq[i][r];
+  const float rstd = row >= 0 ? rsqrtf(tot / (float)K + eps) : 0.f;   // eps may be 0
+  uint8_t* sc = reinterpret_cast<uint8_t*>(scales);
+  for (int kb = wv; kb < 4 * Q; kb += NORM_WAVES) {
+    uint32_t b = 0;
+    if (kb < KB) {
+      float v[2][16], w[16];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        load16<false>(x, at, kb * 128 + 64 * j + 16 * g, K, row >= 0, v[j]);
+        load16<false>(nw, 0, kb * 128 + 64 * j + 16 * g, K, row >= 0, w);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[j][i] = round_bf16(w[i] * round_bf16(v[j][i] * rstd));
+      }
+      b = store_block(v, codes + (t * KB + kb) * FP8_BLOCK, lane);
+    }
+    if (g == 0) sc[((t * Q + (kb >> 2)) * 16 + r) * 4 + (kb & 3)] = (uint8_t)b;
+  }
+}
+
+// The values back: a wavefront for each block, rows written in pieces of 16 values.
+template <bool F32OUT>
+__global__ __launch_bounds__(256) void read_kernel(const uint8_t* __restrict__ codes,
+                                                   const uint32_t* __restrict__ scales, int rows,
+                                                   int K, int pair, void* __restrict__ out,
+                                                   long long stride, long long units) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int Q = fp8_quads(K), KB = fp8_blocks(K);
+  const long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (u >= units) return;
+  const long long t = u / KB;
+  const int kb = (int)(u - t * KB);
+  const int row = fp8_row(t, r, rows, pair);
+  if (row < 0) return;
+  const uint32_t b = (scales[(t * Q + (kb >> 2)) * 16 + r] >> (8 * (kb & 3))) & 255u;
+  const float s = fp8_scale(b);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint4 c = ldg16(codes + u * FP8_BLOCK + 1024 * j + 16 * lane);
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    const int k = kb * 128 + 64 * j + 16 * g;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false);
+      const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+      v[4 * i] = lo[0] * s;
+      v[4 * i + 1] = lo[1] * s;
+      v[4 * i + 2] = hi[0] * s;
+      v[4 * i + 3] = hi[1] * s;
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (k + 8 * p >= K) break;
+      const float* e = v + 8 * p;
+      if constexpr (F32OUT) {
+        float* o = static_cast<float*>(out) + row * stride + k + 8 * p;
+        *reinterpret_cast<float4*>(o) = make_float4(e[0], e[1], e[2], e[3]);
+        *reinterpret_cast<float4*>(o + 4) = make_float4(e[4], e[5], e[6], e[7]);
+      } else {
+        uint16_t* o = static_cast<uint16_t*>(out) + row * stride + k + 8 * p;
+        *reinterpret_cast<uint4*>(o) =
+            make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
+                       pack_bf16x2(e[6], e[7]));
+      }
+    }
+  }
+}
+
+// Sizes whose units fit one launch and whose byte offsets fit 63 bits.
+int check(int rows, int K, int pair, long long stride) {
+  if (rows < 1 || K < 8 || (K & 7) || stride < 0 || (stride & 7) || (pair && (rows & 1)))
+    return KO_EINVAL;
+  if (fp8_tiles(rows, pair) * fp8_blocks(K) > 0x7fffffffll) return KO_ERANGE;
+  return KO_OK;
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K, int pair,
+                    const void* nw, float eps, void* codes, void* scales, void* stream) {
+  if (!x || !codes || !scales) return KO_EINVAL;
+  if (const int st = check(rows, K, pair, stride)) return st;
+  if (!al16(x) || !al16(codes) || !al16(scales) || (nw && !al16(nw))) return KO_EINVAL;
+  if (nw && (x_f32 || pair)) return KO_ENOTSUP;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const long long tiles = fp8_tiles(rows, pair);
+  uint8_t* c = static_cast<uint8_t*>(codes);
+  uint32_t* sc = static_cast<uint32_t*>(scales);
+  if (nw) {
+    hipLaunchKernelGGL(quantize_norm_kernel, dim3((unsigned)tiles), dim3(64 * NORM_WAVES), 0, s,
+                       static_cast<const uint16_t*>(x), stride, rows, K,
+                       static_cast<const uint16_t*>(nw), eps, c, sc);
+    return KO_LAUNCH_STATUS();
+  }
+  const long long units = tiles * fp8_quads(K);
+  const dim3 grid((unsigned)((units + 3) / 4));
+  if (x_f32)
+    hipLaunchKernelGGL(quantize_kernel<true>, grid, dim3(256), 0, s, x, stride, rows, K, pair, c,
+                       sc, units);
+  else
+    hipLaunchKernelGGL(quantize_kernel<false>, grid, dim3(256), 0, s, x, stride, rows, K, pair, c,
+                       sc, units);
+  return KO_LAUNCH_STATUS();
+}
+
+int ko_fp8_read(const void* codes, const void* scales, int rows, int K, int pair, void* out,
+                int out_f32, long long stride, void* stream) {
+  if (!codes || !scales || !out) return KO_EINVAL;
+  if (const int st = check(rows, K, pair, stride)) return st;
+  if (!al16(codes) || !al16(scales) || !al16(out)) return KO_EINVAL;
+  const long long units = fp8_tiles(rows, pair) * fp8_blocks(K);
+  const dim3 grid((unsigned)((units + 3) / 4));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (out_f32)
+    hipLaunchKernelGGL(read_kernel<true>, grid, dim3(256), 0, s,
+                       static_cast<const uint8_t*>(codes), static_cast<const uint32_t*>(scales),
+                       rows, K, pair, out, stride, units);
+  else
+    hipLaunchKernelGGL(read_kernel<false>, grid, dim3(256), 0, s,
+                       static_cast<const uint8_t*>(codes), static_cast<const uint32_t*>(scales),
+                       rows, K, pair, out, stride, units);
+  return KO_LAUNCH_STATUS();
+}
+
+}  // extern "C"

@@ -1,0 +1,197 @@
+"""Matrices held in 8-bit floating point, and the projections of a decode step or a prompt on them.
+
+The ops stand beside ``kernels.gemv``'s for bf16 weights and follow their manner: tensors are the
+caller's, every call launches on the current stream of the current device and never synchronises
+(so calls can be captured), and a bad argument raises ValueError before anything is launched.
+
+- ``fp8_quantize``: rows [rows, K] in bf16 or fp32, behind an RMSNorm if asked, to 8 bits (a
+  weight once at load, a projection's input in every call); ``fp8_read`` gives the values back;
+- ``Fp8Linear``: ``Gemv`` (engine/kernels/gemv.py:109-150) with both factors in 8 bits, for any
+  number of rows: y = x W^T with a norm in front and the F32, BF16, RESID or SWIGLU epilogue.
+
+A value is held as an OCP e4m3 code times its block's scale, a power of two: a block is 128
+neighbouring values of a row, and the scale the least 2^e >= 2^-127 with max |x| <= 448 * 2^e. A code
+is x / 2^e rounded to nearest (ties to even): within 2^-4 of x, or within 2^(e - 10) where |x| is
+below 2^(e - 6). A block with a NaN or an infinity reads back as NaN throughout. 8.06 bits a value.
+K is a multiple of 8; the last block may be short.
+"""
+
+import torch
+
+from .. import _lib
+from .fused import BF16, _cdiv, _need
+from .gemv import EPI_BF16, EPI_F32, EPI_RESID, EPI_SWIGLU
+from .kv4 import _here, _no_overlap, _stream, _tensor
+
+F32 = torch.float32
+FP8_BLOCK = 128   # values that share a scale
+
+
+class Fp8Tensor:
+    """A matrix [rows, K] in 8 bits: ``codes`` uint8 [tiles, blocks, 2048] (16 rows x 128 values a
+    block) and ``scales`` uint8 [tiles, quads, 64] (16 rows x 4 blocks), as csrc/fp8_core.h lays
+    them out. ``pair``: the two halves of its rows (gate | up) lie in alternating tiles."""
+
+    __slots__ = ("codes", "scales", "rows", "K", "pair")
+
+    def __init__(self, codes, scales, rows, K, pair=False):
+        tiles, blocks = fp8_shape(rows, K, pair)
+        for t, name, shape in ((codes, "codes", (tiles, blocks, 2048)),
+                               (scales, "scales", (tiles, _cdiv(blocks, 4), 64))):
+            _need(isinstance(t, torch.Tensor) and t.dtype == torch.uint8 and t.shape == shape
+                  and t.is_contiguous(), f"{name} must be a contiguous uint8 tensor {shape}")
+        _need(codes.device == scales.device, "codes and scales must be on one device")
+        self.codes, self.scales, self.rows, self.K, self.pair = codes, scales, rows, K, bool(pair)
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def __repr__(self):
+        return (f"Fp8Tensor([{self.rows}, {self.K}]{', pair' if self.pair else ''}, "
+                f"{self.codes.device})")
+
+
+def fp8_shape(rows, K, pair=False):
+    """(tiles of 16 rows, blocks of 128 values) of a matrix [rows, K]."""
+    _need(rows >= 1 and K >= 8 and K % 8 == 0, "rows must be positive, K a positive multiple of 8")
+    _need(not pair or rows % 2 == 0, "a pair has an even number of rows")
+    tiles = 2 * _cdiv(rows // 2, 16) if pair else _cdiv(rows, 16)
+    blocks = _cdiv(K, FP8_BLOCK)
+    _need(tiles * blocks < 2 ** 31, "the matrix has 2^31 blocks or more")
+    return tiles, blocks
+
+
+def fp8_empty(rows, K, device, pair=False):
+    """An Fp8Tensor [rows, K] to be written by fp8_quantize."""
+    tiles, blocks = fp8_shape(rows, K, pair)
+    return Fp8Tensor(torch.empty(tiles, blocks, 2048, dtype=torch.uint8, device=device),
+                     torch.empty(tiles, _cdiv(blocks, 4), 64, dtype=torch.uint8, device=device),
+                     rows, K, pair)
+
+
+def _check_held(t, name, rows, K, pair, dev):
+    _need(isinstance(t, Fp8Tensor), f"{name} must be an Fp8Tensor (fp8_quantize)")
+    _need((t.rows, t.K, t.pair) == (rows, K, pair),
+          f"{name} must hold [{rows}, {K}]{' as a pair' if pair else ''}, got {t!r}")
+    _need(t.codes.is_cuda and t.codes.get_device() == dev, f"{name} must be on cuda:{dev}")
+    _need((t.codes.data_ptr() | t.scales.data_ptr()) % 16 == 0, f"{name} must be aligned to 16 bytes")
+
+
+def _check_rows(x, name, dtypes):
+    """A matrix of rows: its device and row stride."""
+    _need(isinstance(x, torch.Tensor) and x.dim() == 2, f"{name} must be [rows, K]")
+    _need(x.dtype in dtypes, f"{name} must be {' or '.join(map(str, dtypes))}, got {x.dtype}")
+    _need(x.is_cuda, f"{name} must be on the GPU")
+    rows, K = x.shape
+    _need(rows >= 1 and K >= 8 and K % 8 == 0,
+          f"{name} must have rows, and columns in a multiple of 8, got {tuple(x.shape)}")
+    stride = x.stride(0) if rows > 1 else 0
+    _need(x.stride(1) == 1 and stride % 8 == 0 and stride >= 0 and x.data_ptr() % 16 == 0,
+          f"{name}: the inner stride must be 1, the row stride a multiple of 8, the address of 16")
+    return x.get_device(), stride
+
+
+def _bytes(t):
+    """A tensor's first byte and the one behind its last (strides >= 0)."""
+    reach = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + reach * t.element_size()
+
+
+def _need_apart(a, b, what):
+    (a0, a1), (b0, b1) = _bytes(a), _bytes(b)
+    _need(a1 <= b0 or b1 <= a0, f"{what} must not overlap")
+
+
+def fp8_quantize(x, out=None, nw=None, eps=1e-6, pair=False):
+    """Quantise rows x [rows, K] (bf16 or fp32, inner stride 1, row stride a multiple of 8 or 0) into
+    ``out`` (None: a new Fp8Tensor), which is returned. ``nw`` [K] bf16: bf16 rows go through an RMSNorm with this
+    gain first, rounded as the bf16 chain is (bf16(nw * bf16(x * rstd)), statistics in fp32).
+    ``pair``: x is gate | up, [2 N, K], for an Fp8Linear with SWIGLU; ``out`` says so itself."""
+    dev, stride = _check_rows(x, "x", (BF16, F32))
+    _here(dev)
+    rows, K = x.shape
+    if nw is not None:
+        _need(x.dtype == BF16 and not pair and not (out is not None and out.pair),
+              "a norm goes with bf16 rows that are no pair")
+        _tensor(nw, "nw", BF16, (K,), dev)
+    if out is None:
+        out = fp8_empty(rows, K, x.device, pair)
+    else:
+        _check_held(out, "out", rows, K, out.pair if isinstance(out, Fp8Tensor) else pair, dev)
+        _need(out.pair or not pair, "out holds no pair")
+        _need_apart(x, out.codes, "x and out")
+        _need_apart(x, out.scales, "x and out")
+    _lib.call("ko_fp8_quantize", x.data_ptr(), x.dtype == F32, stride, rows, K, out.pair,
+              _lib.ptr(nw), eps, out.codes.data_ptr(), out.scales.data_ptr(), _stream(dev))
+    return out
+
+
+def fp8_read(t, out):
+    """The values that t holds, into out [rows, K] bf16 or fp32 (strides as x's of fp8_quantize;
+    elements must not share memory); exact in either but for values below the type's
+    least subnormal."""
+    dev, stride = _check_rows(out, "out", (BF16, F32))
+    _here(dev)
+    _need(isinstance(t, Fp8Tensor), "t must be an Fp8Tensor (fp8_quantize)")
+    _check_held(t, "t", out.shape[0], out.shape[1], t.pair, dev)
+    _no_overlap(out, "out")
+    _need_apart(out, t.codes, "t and out")
+    _need_apart(out, t.scales, "t and out")
+    _lib.call("ko_fp8_read", t.codes.data_ptr(), t.scales.data_ptr(), t.rows, t.K, t.pair,
+              out.data_ptr(), out.dtype == F32, stride, _stream(dev))
+
+
+class Fp8Linear:
+    """One projection y[M, N] = x[M, K] W[N, K]^T, x and W in 8 bits, sums in fp32, with a norm in
+    front (``norm``, gain ``nw``) and an epilogue: EPI_F32 (y fp32), EPI_BF16, EPI_RESID
+    (y = bf16(h + bf16(x W^T)); y None: h itself) or EPI_SWIGLU (W is gate | up held as a pair;
+    y = bf16(bf16(silu(g)) * u) of the bf16 products g and u).
+
+    ``x`` is [M, K] bf16 and is quantised in the call (with the norm) into a workspace of the object's,
+    or an Fp8Tensor where there is no norm. The workspace is made for ``device``, or in the first
+    call, which must not be under graph capture. Calls of one object share it: they must be
+    ordered, on one stream or by events, captured calls' replays included."""
+
+    def __init__(self, M, N, K, epi, norm, eps=1e-6, device=None):
+        _need(epi in (EPI_F32, EPI_BF16, EPI_RESID, EPI_SWIGLU), f"bad epilogue {epi}")
+        _need(M >= 1 and N >= 1, "M and N must be positive")
+        fp8_shape((2 if epi == EPI_SWIGLU else 1) * N, K, epi == EPI_SWIGLU)
+        fp8_shape(M, K)
+        self.M, self.N, self.K, self.epi, self.norm, self.eps = M, N, K, epi, bool(norm), eps
+        self._xq = None
+        if device is not None:
+            self._workspace(torch.empty(0, device=device).get_device())
+
+    def _workspace(self, dev):
+        if self._xq is None or self._xq.codes.get_device() != dev:
+            _need(not torch.cuda.is_current_stream_capturing(), "the workspace is made in the first "
+                  "call: make it before the capture, or give the object its device")
+            self._xq = fp8_empty(self.M, self.K, torch.device("cuda", dev))
+        return self._xq
+
+    def __call__(self, x, w, y=None, nw=None, h=None):
+        M, N, K, epi = self.M, self.N, self.K, self.epi
+        _need(isinstance(w, Fp8Tensor), "w must be an Fp8Tensor (fp8_quantize)")
+        _need(w.codes.is_cuda, "w must be on the GPU")
+        dev = w.codes.get_device()
+        _here(dev)
+        pair = epi == EPI_SWIGLU
+        _check_held(w, "w", 2 * N if pair else N, K, pair, dev)
+        _need((nw is not None) == self.norm, "nw goes with a norm")
+        if epi == EPI_RESID:
+            _tensor(h, "h", BF16, (M, N), dev)
+            y = h if y is None else y
+        else:
+            _need(h is None, "h goes with EPI_RESID")
+        _tensor(y, "y", F32 if epi == EPI_F32 else BF16, (M, N), dev)
+        if y is not h and epi == EPI_RESID and y.data_ptr() != h.data_ptr():
+            _need_apart(y, h, "y and h, unless they are the same,")
+        if isinstance(x, Fp8Tensor):
+            _need(not self.norm, "a norm goes with x in bf16")
+            _check_held(x, "x", M, K, False, dev)
+        else:
+            _tensor(x, "x", BF16, (M, K), dev)
+            x = fp8_quantize(x, out=self._workspace(dev), nw=nw, eps=self.eps)
+        _lib.call("ko_fp8_linear", x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(),
+                  w.scales.data_ptr(), y.data_ptr(), _lib.ptr(h), M, N, K, epi, _stream(dev))

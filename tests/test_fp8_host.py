@@ -1,0 +1,71 @@
+"""Refusals of the 8-bit matrices' ops that need no GPU: sizes, types, devices, and the C ABI's own
+checks (no kernel is launched)."""
+
+import pytest
+import torch
+
+from kernel_optim_amd import _lib
+from kernel_optim_amd.kernels import fp8 as P
+from kernel_optim_amd.kernels.gemv import EPI_ARGMAX, EPI_BF16, EPI_RESID, EPI_SWIGLU
+
+BF16 = torch.bfloat16
+
+
+def test_shapes():
+    assert P.fp8_shape(17, 136) == (2, 2)
+    assert P.fp8_shape(34, 128, pair=True) == (4, 1)
+    t = P.fp8_empty(17, 640, "cpu")
+    assert t.codes.shape == (2, 5, 2048) and t.scales.shape == (2, 2, 64)
+    assert t.nbytes == 2 * 5 * 2048 + 2 * 2 * 64
+    for bad in ((0, 8), (1, 0), (1, 12), (2 ** 31, 2 ** 12)):
+        with pytest.raises(ValueError):
+            P.fp8_shape(*bad)
+    with pytest.raises(ValueError):
+        P.fp8_shape(3, 8, pair=True)
+
+
+def test_held_tensors_are_checked():
+    t = P.fp8_empty(17, 640, "cpu")
+    for codes, scales, rows in ((t.codes[:1], t.scales, 17), (t.codes, t.scales[:, :1], 17),
+                                (t.codes.int(), t.scales, 17), (t.codes, t.scales, 33)):
+        with pytest.raises(ValueError):
+            P.Fp8Tensor(codes, scales, rows, 640)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 128, dtype=BF16)
+    t = P.fp8_empty(4, 128, "cpu")
+    for f in (lambda: P.fp8_quantize(x), lambda: P.fp8_read(t, x),
+              lambda: P.Fp8Linear(4, 4, 128, EPI_BF16, False)(x, t, y=x)):
+        with pytest.raises(ValueError):
+            f()
+
+
+@pytest.mark.parametrize("M,N,K,epi", [(0, 8, 8, EPI_BF16), (1, 0, 8, EPI_BF16),
+                                       (1, 8, 12, EPI_BF16), (1, 8, 8, EPI_ARGMAX)])
+def test_linear_refuses(M, N, K, epi):
+    with pytest.raises(ValueError):
+        P.Fp8Linear(M, N, K, epi, False)
+
+
+def test_c_abi_refuses():
+    h, p = _lib.lib(), 1 << 20   # p is never read: the checks come first
+    EINVAL, ERANGE, ENOTSUP = -22, -34, -95
+    q = lambda x=p, f32=0, stride=8, rows=1, K=8, pair=0, nw=None, codes=p, scales=p: \
+        h.ko_fp8_quantize(x, f32, stride, rows, K, pair, nw, 1e-6, codes, scales, None)
+    assert q(x=None) == q(codes=None) == q(scales=None) == EINVAL
+    assert q(x=p + 2) == q(codes=p + 8) == q(scales=p + 8) == q(nw=p + 2) == EINVAL
+    assert q(rows=0) == q(K=12) == q(K=0) == q(stride=4) == q(stride=-8) == EINVAL
+    assert q(rows=3, pair=1) == EINVAL
+    assert q(nw=p, f32=1) == q(nw=p, pair=1, rows=2) == ENOTSUP
+    assert q(rows=2 ** 31 - 1, K=2 ** 20) == ERANGE
+    r = lambda codes=p, rows=1, K=8, out=p, stride=8: \
+        h.ko_fp8_read(codes, p, rows, K, 0, out, 0, stride, None)
+    assert r(codes=None) == r(out=None) == r(out=p + 4) == r(rows=0) == r(K=4) == r(stride=1) == EINVAL
+    l = lambda xc=p, y=p, hh=p, M=1, N=8, K=8, epi=EPI_BF16: \
+        h.ko_fp8_linear(xc, p, p, p, y, hh, M, N, K, epi, None)
+    assert l(xc=None) == l(y=None) == l(M=0) == l(N=0) == l(K=12) == EINVAL
+    assert l(hh=None, epi=EPI_RESID) == l(hh=p + 2, epi=EPI_RESID) == EINVAL
+    assert l(epi=EPI_ARGMAX) == l(epi=-1) == ENOTSUP
+    assert l(N=2 ** 30) == ERANGE
+    assert l(epi=EPI_SWIGLU, M=0) == EINVAL

@@ -1,0 +1,285 @@
+"""Matrices held in 8-bit floating point on the GPU against the oracle: codes and scales bit for bit,
+values read back, and projections over the held values in 64 bits.
+
+Tolerances. A sum of K products (each exact in fp32: 8 significant bits) in fp32 in any order is
+within (K - 1) 2^-24 sum |x w| of the true one; so are fp32 results and those of up to 64 rows.
+More rows with bf16 results go through the 8-bit matrix instruction, which cuts each of 8
+neighbouring products off below 2^-13 of the binade 2^(ex + ew) of the largest, ex and ew the
+codes' exponents (-6 for codes below 2^-6): at most 8 * 2^-13 of it for the eight, so at most
+2^-10 sum 2^(ex + ew) over all K; the scales ride on both. A rounding to bf16 adds half a step,
+2^-8 of the value at most (|x| >= the least normal number; below it 2^-134)."""
+
+import pytest
+import torch
+
+from kernel_optim_amd.kernels.fp8 import Fp8Linear, Fp8Tensor, fp8_empty, fp8_quantize, fp8_read
+from kernel_optim_amd.kernels.gemv import EPI_BF16, EPI_F32, EPI_RESID, EPI_SWIGLU
+from oracle import fp8 as O
+
+pytestmark = pytest.mark.gpu
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+EPI = dict(f32=EPI_F32, bf16=EPI_BF16, resid=EPI_RESID, swiglu=EPI_SWIGLU)
+HALF = 2.0 ** -8   # bf16's half step
+
+
+def randn(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+def rows(seed, n, K):
+    """Rows of very different sizes with strong channels, a zero row and a zero block."""
+    x = randn(seed, n, K)
+    x[:, ::37] *= 30
+    x *= torch.logspace(-3, 3, n)[:, None]
+    x[n // 2] = 0
+    x[n - 1, :128] = 0
+    return x
+
+
+def same_bytes(t, x, pair=False):
+    codes, scales = O.pack(*O.quantise(x), pair)
+    assert torch.equal(t.codes.cpu(), codes)
+    assert torch.equal(t.scales.cpu(), scales)
+
+
+SHAPES = [(1, 8), (1, 128), (3, 136), (16, 512), (17, 520), (33, 2560), (100, 1048), (5, 9728)]
+
+
+@pytest.mark.parametrize("n,K", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_quantize_and_read(dev, n, K, dtype):
+    x = rows(K + n, n, K).to(dtype)
+    t = fp8_quantize(x.to(dev))
+    same_bytes(t, x)
+    out = torch.empty(n, K, dtype=dtype, device=dev)
+    fp8_read(t, out)
+    assert torch.equal(out.cpu(), O.held(x).to(F32).to(dtype))
+
+
+@pytest.mark.parametrize("n,K", [(2, 8), (32, 256), (34, 136), (1000, 520)])
+def test_pairs(dev, n, K):
+    x = rows(n, n, K).to(BF16)
+    t = fp8_quantize(x.to(dev), pair=True)
+    same_bytes(t, x, pair=True)
+    out = torch.empty(n, K, dtype=BF16, device=dev)
+    fp8_read(t, out)
+    assert torch.equal(out.cpu(), O.held(x).to(BF16))
+
+
+def test_every_scale_and_both_roundings(dev):
+    """Blocks whose maximum is every power of two, and next to 448 of it; codes at the ties."""
+    e = torch.arange(-149, 128, dtype=F64)
+    top = torch.cat((2.0 ** e, 1.75 * 2.0 ** e, (1.75 + 2.0 ** -7) * 2.0 ** e)).clamp_max(3.3e38)
+    v = O.e4m3_values() / 448
+    x = (top[:, None] * torch.cat((v, -(v[1:] + v[:-1])[:121] / 2, torch.zeros(8)))[None]).to(F32)
+    same_bytes(fp8_quantize(x.to(dev)), x)
+    same_bytes(fp8_quantize(x.to(BF16).to(dev)), x.to(BF16))
+
+
+def test_strides_and_rows_behind_the_last(dev):
+    n, K = 21, 264
+    wide = rows(3, n, 400).to(BF16).to(dev)
+    x = wide[:, 8:8 + K]
+    out = fp8_empty(n, K, dev)
+    out.codes.fill_(0xff)
+    out.scales.fill_(0xff)
+    assert fp8_quantize(x, out=out) is out
+    same_bytes(out, x.cpu())                       # padding rows and values are zeros
+    same_bytes(fp8_quantize(x[:1].expand(n, K)), x[:1].cpu().expand(n, K))
+    back = torch.full((n, 400), 7.0, device=dev)
+    fp8_read(out, back[:, 8:8 + K])
+    assert torch.equal(back[:, 8:8 + K].cpu(), O.held(x.cpu()).to(F32))
+    assert (back[:, :8] == 7).all() and (back[:, 8 + K:] == 7).all()
+
+
+def test_blocks_that_hold_no_numbers(dev):
+    x = rows(9, 40, 640).to(BF16)
+    x[3, 5], x[4, 600], x[17, 128], x[39] = float("nan"), float("inf"), -float("inf"), float("nan")
+    t = fp8_quantize(x.to(dev))
+    same_bytes(t, x)
+    for dtype in (BF16, F32):
+        out = torch.empty(40, 640, dtype=dtype, device=dev)
+        fp8_read(t, out)
+        want = O.held(x).to(dtype)
+        assert torch.equal(torch.isnan(out.cpu()), torch.isnan(want))
+        assert torch.equal(out.cpu().nan_to_num(), want.nan_to_num())
+    # a product's rows and columns with such a block are NaN, the others as without it
+    w = (0.1 * randn(10, 48, 640)).to(BF16)
+    w[7, 300] = float("nan")
+    y = torch.empty(40, 48, device=dev)
+    Fp8Linear(40, 48, 640, EPI_F32, False)(x.to(dev), fp8_quantize(w.to(dev)), y=y)
+    bad = torch.isnan(O.held(x)).any(1)[:, None] | torch.isnan(O.held(w)).any(1)[None]
+    assert torch.equal(torch.isnan(y.cpu()), bad)
+
+
+@pytest.mark.parametrize("n,K", [(1, 8), (1, 2560), (5, 136), (16, 4096), (19, 2568), (64, 9728),
+                                 (3, 16384)])
+def test_quantize_behind_a_norm(dev, n, K):
+    """The row's sum of squares in fp32 moves x * rstd by up to (K + 4) 2^-24 of itself, which may
+    move a bf16 rounding, and that a code; rows whose norm is a power of two by construction
+    (+-2^a throughout, eps 0) have no such freedom and must match bit for bit."""
+    x = torch.where(randn(n, n, K) > 0, 1.0, -1.0) * 2.0 ** (torch.arange(n) % 9 - 4)[:, None]
+    nw = (1 + 0.3 * randn(2, K)).to(BF16)
+    t = fp8_quantize(x.to(BF16).to(dev), nw=nw.to(dev), eps=0.0)
+    same_bytes(t, O.norm(x.to(BF16), nw, 0.0))
+    x = randn(n + 1, n, K).to(BF16)
+    out = torch.empty(n, K, device=dev)
+    fp8_read(fp8_quantize(x.to(dev), nw=nw.to(dev), eps=1e-6), out)
+    want = O.norm(x, nw, 1e-6)
+    # off by the norm's two bf16 roundings and a code's, each half a step, of the true value;
+    # below a code's least normal value by the block's absolute half step
+    true = x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + 1e-6) * nw.double()
+    top = torch.nn.functional.pad(want.double().abs(), (0, -K % 128)).unflatten(1, (-1, 128)).amax(-1)
+    small = (top * 2.0 ** -18 * 1.01).repeat_interleave(128, 1)[:, :K]   # 2^(e - 10), 2^e < top / 224
+    rel = (1 + HALF) ** 2 * (1 + 2.0 ** -4) * (1 + (K + 4) * 2.0 ** -24) - 1
+    assert ((out.cpu().double() - true).abs() <= rel * true.abs() + small).all()
+
+
+def check(y, epi, x, w, h=None):
+    """y against the sums in 64 bits over what (codes, scales) x and w hold, within the roundings
+    of its chain."""
+    xh, wh = O.values(*x), O.values(*w)
+    K = xh.shape[1]
+    want, size, parts = O.linear(xh, wh, epi, h)
+    if epi != "f32" and xh.shape[0] > 64:   # in units of the fp32 sums' own bound
+        cut = 2.0 ** -10 / ((K - 1) * 2.0 ** -24) * (O.binades(*x) @ O.binades(*w).t())
+        n = parts[0].shape[1] if epi == "swiglu" else 0
+        size = (size[0] + cut[:, :n], size[1] + cut[:, n:]) if n else size + cut
+    y = y.cpu().double()
+    sums = lambda s: (K - 1) * 2.0 ** -24 * s + 2.0 ** -134
+    if epi == "f32":
+        tol = sums(size)
+    elif epi == "bf16":
+        tol = sums(size) + HALF * (want.abs() + sums(size))
+    elif epi == "resid":
+        d = sums(size) + HALF * (parts.abs() + sums(size))
+        tol = d + HALF * (want.abs() + d)
+    else:
+        (g, u), (sg, su) = parts, size
+        dg = sums(sg) + HALF * (g.abs() + sums(sg))
+        du = sums(su) + HALF * (u.abs() + sums(su))
+        silu = g / (1 + torch.exp(-g))
+        ds = 1.1 * dg                       # |silu'| < 1.1
+        # fp32's exp, sum and quotient: under 2^-20 together; then bf16
+        ds = ds + (HALF + 2.0 ** -20) * (silu.abs() + ds)
+        d = ds * (u.abs() + du) + silu.abs() * du
+        tol = d + HALF * (want.abs() + d) + 2.0 ** -134
+    off = (y - want).abs()
+    assert torch.isfinite(y).all()
+    assert (off <= tol).all(), (off / tol).max()
+
+
+def projection(dev, M, N, K, epi, norm, seed=0, dtype=BF16):
+    x = randn(seed + 1, M, K)
+    x[:, ::53] *= 12
+    x[:, 0] = 200.0   # keeps every row's norm and first scale apart from the rest
+    w = (0.05 * randn(seed + 2, (2 if epi == "swiglu" else 1) * N, K)).to(BF16)
+    h = randn(seed + 3, M, N).to(BF16) if epi == "resid" else None
+    nw = (1 + 0.2 * randn(seed + 4, K)).to(BF16) if norm else None
+    return x.to(BF16), w, h, nw
+
+
+def on(dev, *ts):
+    return [None if t is None else t.to(dev) for t in ts]
+
+
+LINEAR = [(1, 16, 8), (1, 1, 128), (1, 2560, 4096), (2, 1000, 712), (3, 17, 136), (7, 130, 520),
+          (16, 256, 2560), (17, 33, 1024), (33, 999, 264), (64, 512, 1152), (65, 130, 640),
+          (100, 300, 2568), (130, 640, 896), (257, 515, 384), (300, 1024, 2560)]
+
+
+@pytest.mark.parametrize("M,N,K", LINEAR)
+@pytest.mark.parametrize("epi", list(EPI))
+def test_linear(dev, M, N, K, epi):
+    x, w, h, _ = projection(dev, M, N, K, epi, False, seed=M)
+    xd, wd, hd, _ = on(dev, x, w, h, None)
+    y = torch.full((M, N), float("nan"), device=dev, dtype=F32 if epi == "f32" else BF16)
+    op = Fp8Linear(M, N, K, EPI[epi], False)
+    held = fp8_quantize(wd, pair=epi == "swiglu")
+    op(xd, held, y=y, h=hd)
+    check(y, epi, O.quantise(x), O.quantise(w), h)
+    again = torch.full_like(y, float("nan"))
+    op(fp8_quantize(xd), held, y=again, h=hd)      # x held already: the same bits
+    assert torch.equal(again, y)
+    if epi == "resid":                             # in place
+        op(xd, held, h=hd)
+        assert torch.equal(hd, y)
+
+
+@pytest.mark.parametrize("M", [1, 5, 16, 40, 64, 130])
+@pytest.mark.parametrize("epi", ["bf16", "swiglu"])
+def test_linear_behind_a_norm(dev, M, epi):
+    """Against the product over what fp8_quantize holds of the norm, bit for bit, and that
+    against 64 bits (its own test has the norm's)."""
+    N, K = 208, 2560
+    x, w, _, nw = projection(dev, M, N, K, epi, True, seed=M)
+    xd, wd, nwd = on(dev, x, w, nw)
+    held = fp8_quantize(wd, pair=epi == "swiglu")
+    y = torch.empty(M, N, device=dev, dtype=BF16)
+    op = Fp8Linear(M, N, K, EPI[epi], True, eps=1e-6)
+    op(xd, held, y=y, nw=nwd)
+    xq = fp8_quantize(xd, nw=nwd, eps=1e-6)
+    xv = torch.empty(M, K, device=dev)
+    fp8_read(xq, xv)
+    check(y, epi, O.quantise(xv.cpu()), O.quantise(w))   # held values are held as they are
+    z = torch.empty_like(y)
+    Fp8Linear(M, N, K, EPI[epi], False)(xq, held, y=z)
+    assert torch.equal(z, y)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 48, 4096), (16, 160, 9728), (64, 96, 2560), (200, 272, 640)])
+def test_whole_numbers_are_exact(dev, M, N, K):
+    """Small whole numbers: every code is exact, no product has bits 2^-13 below another of
+    its eight, and no sum passes 2^24, so no order matters either."""
+    x = torch.randint(-8, 9, (M, K), generator=torch.Generator().manual_seed(M)).float()
+    w = torch.randint(-8, 9, (N, K), generator=torch.Generator().manual_seed(N)).float()
+    y = torch.empty(M, N, device=dev)
+    Fp8Linear(M, N, K, EPI_F32, False)(x.to(BF16).to(dev), fp8_quantize(w.to(dev)), y=y)
+    assert torch.equal(y.cpu().double(), x.double() @ w.double().t())
+
+
+def test_scales_far_apart(dev):
+    """Blocks whose scales differ by 2^100, so that products meet again near 1."""
+    M, N, K = 18, 40, 1280
+    e = (torch.arange(K) // 128 * 10 - 50).double()
+    x = (randn(1, M, K).double() * 2.0 ** e).float()
+    w = (randn(2, N, K).double() * 2.0 ** -e).float()
+    y = torch.empty(M, N, device=dev)
+    Fp8Linear(M, N, K, EPI_F32, False)(fp8_quantize(x.to(dev)), fp8_quantize(w.to(dev)), y=y)
+    check(y, "f32", O.quantise(x), O.quantise(w))
+
+
+def test_refusals(dev):
+    bf = lambda *s: torch.zeros(*s, dtype=BF16, device=dev)
+    w = fp8_quantize(bf(32, 256))
+    pair = fp8_quantize(bf(64, 256), pair=True)
+    op = Fp8Linear(4, 32, 256, EPI_BF16, False)
+    y = bf(4, 32)
+    bad = [
+        lambda: fp8_quantize(bf(4, 12)), lambda: fp8_quantize(bf(0, 8)),
+        lambda: fp8_quantize(torch.zeros(4, 8, dtype=torch.float16, device=dev)),
+        lambda: fp8_quantize(bf(4, 16)[:, 1:9]), lambda: fp8_quantize(bf(8, 4).t()),
+        lambda: fp8_quantize(bf(4, 20)[:, :8]), lambda: fp8_quantize(bf(3, 8), pair=True),
+        lambda: fp8_quantize(torch.zeros(4, 8, device=dev), nw=bf(8)),
+        lambda: fp8_quantize(bf(4, 8), nw=bf(8), pair=True),
+        lambda: fp8_quantize(bf(4, 8), nw=bf(16)), lambda: fp8_quantize(bf(4, 8), out=w),
+        lambda: fp8_quantize(bf(64, 256), out=fp8_empty(64, 256, dev), pair=True),
+        lambda: fp8_read(w, bf(32, 128)), lambda: fp8_read(w, bf(1, 256).expand(32, 256)),
+        lambda: fp8_read(w, w.codes.view(torch.int16).view(BF16).view(32, 128)),
+        lambda: op(bf(4, 256), bf(32, 256), y=y), lambda: op(bf(5, 256), w, y=y),
+        lambda: op(bf(4, 256), pair, y=y), lambda: op(bf(4, 256), w, y=bf(4, 16)),
+        lambda: op(bf(4, 256), w), lambda: op(bf(4, 256), w, y=y, nw=bf(256)),
+        lambda: op(bf(4, 256), w, y=y, h=bf(4, 32)),
+        lambda: op(bf(4, 256).float(), w, y=y),
+        lambda: Fp8Linear(4, 32, 256, EPI_RESID, False)(bf(4, 256), w, y=y),
+        lambda: Fp8Linear(4, 32, 256, EPI_BF16, True)(bf(4, 256), w, y=y),
+        lambda: Fp8Linear(4, 32, 256, EPI_BF16, True)(fp8_quantize(bf(4, 256)), w, y=y, nw=bf(256)),
+        lambda: Fp8Linear(4, 32, 256, EPI_SWIGLU, False)(bf(4, 256), w, y=y),
+    ]
+    both = bf(160)
+    bad.append(lambda: Fp8Linear(4, 32, 256, EPI_RESID, False)(
+        bf(4, 256), w, y=both[:128].view(4, 32), h=both[32:].view(4, 32)))
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"call {i} was taken")
