@@ -452,6 +452,30 @@ int ko_fp8_read(const void* codes, const void* scales, int rows, int K, int pair
 int ko_fp8_linear(const void* xc, const void* xs, const void* wc, const void* ws, void* y,
                   const void* h, int M, int N, int K, int epi, void* stream);
 
+/* ---- Sampling ---------------------------------------------------------------------
+ * In the place of torch.argmax(logits) of the reference's decode steps (engine/engine.py:299,
+ * 397): ids[b] (int64) drawn from logits [B, V] (bf16, or fp32 with f32; inner stride 1, row stride
+ * in elements; aligned to an element) with u[b] of [0, 1). temperature, top_k, top_p, min_p:
+ * [B] arrays (fp32, top_k int32), or NULL for the value beside them.
+ * In order of falling logit (ties: the lowest index first; NaN counts as -infinity, which is never
+ * drawn), p_i proportional to exp(x_i / temperature): the first top_k tokens are kept (top_k < 1:
+ * all); of these the ones with less than top_p of their mass before them (top_p >= 1 or no number:
+ * all); of these the ones with p_i >= min_p * p_max (min_p <= 0 or no number: all); the first one always. The drawn
+ * token is the first at which the running mass of the kept ones passes u times their sum.
+ * Temperature 0 (below 0, or no number) takes the first token. A row with nothing above -infinity
+ * gets -1. logprobs (optional, [B] fp32): log of the token's share of the kept mass; 0 where the
+ * first token is taken, -infinity beside -1. V <= 2^20, B <= 65535. Tokens of probability below 2^-43
+ * of the largest have none. chunks: workgroups a row is cut into (1: one launch and no
+ * scratch), at most 1024; scratch: ko_sample_scratch(B, chunks) bytes, 16-byte aligned, in any
+ * state; calls that share it must not overlap. */
+int ko_sample(const void* logits, int f32, long long stride, int B, int V, const float* u,
+              const float* temperature, float temperature1, const int* top_k, int top_k1,
+              const float* top_p, float top_p1, const float* min_p, float min_p1, long long* ids,
+              float* logprobs, void* scratch, long long scratch_bytes, int chunks, void* stream);
+
+/* Bytes of ko_sample's scratch. A size, not a status; -1 for bad arguments. */
+long long ko_sample_scratch(int B, int chunks);
+
 #ifdef __cplusplus
 }
 #endif

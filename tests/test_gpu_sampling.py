@@ -1,0 +1,242 @@
+"""Sampling on the GPU against the oracle in 64 bits.
+
+Ids must be equal. Masses are rounded to 2^-43 of the largest probability, V of them off by V 2^-43
+at most, so a drawn place or a cut that lies nearer to a border than that could differ; no test's
+numbers do. A log-probability is one rounding to fp32 (2^-24 of itself) of one whose kept mass, at
+least 1, is off by up to V 2^-43."""
+
+import math
+
+import pytest
+import torch
+
+from kernel_optim_amd.kernels.sampling import Sampler
+from oracle import sampling as O
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+INF, NAN = math.inf, math.nan
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def logits(seed, B, V, dtype, spread=2.5):
+    x = spread * torch.randn(B, V, generator=gen(seed))
+    x[torch.arange(B), torch.randint(0, V, (B,), generator=gen(seed + 1))] += 8
+    return x.to(dtype)
+
+
+def draw(dev, x, u, t=1.0, k=0, p=1.0, m=0.0, chunks=None, sampler=None):
+    B, V = x.shape
+    s = sampler or Sampler(B, V, dev)
+    if chunks is not None:
+        from kernel_optim_amd import _lib
+        s.chunks = chunks
+        n = _lib.lib().ko_sample_scratch(B, chunks)
+        s._scratch = torch.full((max(n, 16),), 0xff, dtype=torch.uint8, device=dev)
+    ids = torch.full((B,), -7, dtype=torch.int64, device=dev)
+    lp = torch.full((B,), NAN, device=dev)
+    d = lambda v: v.to(dev) if isinstance(v, torch.Tensor) else v
+    s(d(x), d(u), ids, temperature=d(t), top_k=d(k), top_p=d(p), min_p=d(m), logprobs=lp)
+    return ids.cpu(), lp.cpu().double()
+
+
+def check(dev, x, u, t=1.0, k=0, p=1.0, m=0.0, **kw):
+    ids, lp = draw(dev, x, u, t, k, p, m, **kw)
+    want, wlp = O.rows(x, u, t, k, p, m)
+    assert torch.equal(ids, want)
+    tol = 2.0 ** -24 * wlp.abs() + x.shape[1] * 2.0 ** -43
+    assert ((lp - wlp).abs() <= tol)[want >= 0].all() and (lp == wlp)[want < 0].all()
+    return ids
+
+
+SETTINGS = [(1.0, 0, 1.0, 0.0), (0.7, 50, 0.9, 0.0), (0.2, 0, 0.8, 0.0), (1.7, 0, 0.95, 0.0),
+            (1.0, 0, 1.0, 0.05), (1.3, 1000, 1.0, 0.01), (1.0, 1500, 0.9, 0.02), (0.9, 1, 1.0, 0.0),
+            (0.0, 5, 0.5, 0.5), (1.0, 3, 0.0, 0.0), (1.0, 0, 1.0, 1.0), (1.0, 20, 0.5, 0.3)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,k,p,m", SETTINGS)
+@pytest.mark.parametrize("B,V", [(3, 32003), (40, 1000), (2, 151936)])
+def test_against_the_oracle(dev, B, V, dtype, t, k, p, m):
+    x = logits(V + B, B, V, dtype)
+    check(dev, x, torch.rand(B, generator=gen(k)), t, k, p, m)
+
+
+@pytest.mark.parametrize("V", [1, 2, 3, 7, 8, 9, 63, 1025, 4096, 4097])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_small_and_odd_vocabularies(dev, V, dtype):
+    x = logits(V, 33, V, dtype, 1.0)
+    u = torch.rand(33, generator=gen(1))
+    check(dev, x, u)
+    check(dev, x, u, 0.8, min(V, 4), 0.9, 0.1)
+    check(dev, x, u, 0.8, V + 5, 0.9)
+
+
+@pytest.mark.parametrize("chunks", [1, 2, 5, 37, 300])
+@pytest.mark.parametrize("k", [0, 40])
+def test_a_row_cut_into_chunks_draws_the_same(dev, chunks, k):
+    x = logits(5, 4, 50001, BF16)
+    u = torch.rand(4, generator=gen(6))
+    check(dev, x, u, 0.9, k, 0.92, 0.001, chunks=chunks)
+
+
+@pytest.mark.parametrize("chunks", [1, 8])
+@pytest.mark.parametrize("B", [1, 100])
+def test_settings_of_each_row(dev, B, chunks):
+    x = logits(8, B, 20011, BF16)
+    pick = lambda v, d, s: torch.tensor(v, dtype=d)[torch.randint(0, len(v), (B,), generator=gen(s))]
+    t = pick([0.0, -1.0, NAN, 0.3, 0.7, 1.0, 1.5, 100.0], F32, 1)
+    k = pick([0, -3, 1, 2, 20, 1024, 1025, 20011, 2 ** 31 - 1], torch.int32, 2)
+    p = pick([1.0, 2.0, NAN, 0.0, 0.1, 0.9, 0.99], F32, 3)
+    m = pick([0.0, -1.0, NAN, 0.01, 0.2, 1.0, 7.0], F32, 4)
+    clean = torch.where(m == 7, 2.0, m.nan_to_num(0.0))   # above 1: the first token
+    u = torch.rand(B, generator=gen(9))
+    want = O.rows(x, u, t, k.long(), torch.where(torch.isnan(p), 1.0, p), clean)[0]
+    ids, _ = draw(dev, x, u, t, k, p, m, chunks=chunks)
+    # min_p above 1 keeps the first token alone, though others may tie with it
+    assert torch.equal(ids, want)
+
+
+@pytest.mark.parametrize("u", [0.0, 2.0 ** -24, 0.5, 1 - 2.0 ** -24, 1.0, 7.0, -0.5, NAN])
+def test_the_ends_of_u(dev, u):
+    x = logits(12, 2, 3001, BF16)
+    for k, p in ((0, 1.0), (30, 1.0), (0, 0.9)):
+        check(dev, x, torch.full((2,), u), 1.0, k, p)
+
+
+@pytest.mark.parametrize("chunks", [1, 6])
+@pytest.mark.parametrize("k,p,m", [(0, 1.0, 0.0), (100, 1.0, 0.0), (0, 0.5, 0.0), (5000, 0.7, 0.5),
+                                   (0, 1.0, 1.0)])
+def test_ties(dev, chunks, k, p, m):
+    """More equal logits than a bin's tokens are given room in LDS, and a few above them."""
+    x = torch.zeros(3, 24001, dtype=BF16)
+    x[1, 17] = x[1, 20000] = 2.0
+    x[2] = torch.randint(0, 4, (24001,), generator=gen(3)).to(BF16)
+    x[2, ::5] = -0.0
+    u = torch.tensor([0.3, 0.6, 0.9])
+    check(dev, x, u, 1.0, k, p, m, chunks=chunks)
+    check(dev, x.float(), u, 1.0, k, p, m, chunks=chunks)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("chunks", [1, 4])
+def test_crowded_bins(dev, dtype, chunks):
+    """Distinct logits so near to each other that thousands share a bin."""
+    x = (1 + 1e-3 * torch.randn(3, 30000, generator=gen(4))).to(dtype)
+    x[1] = -x[1]
+    x[2] = (x[2] - 1) * 1e-3                 # of both signs
+    u = torch.tensor([0.2, 0.77, 0.4])
+    for k, p, m in ((0, 1.0, 0.0), (9000, 1.0, 0.0), (0, 0.4, 0.0), (12000, 0.6, 0.999)):
+        check(dev, x, u, 1.0, k, p, m, chunks=chunks)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("chunks", [1, 3])
+def test_masked_and_infinite_logits(dev, dtype, chunks):
+    x = logits(20, 9, 5003, dtype)
+    x[0] = -INF                              # nothing left
+    x[1] = NAN
+    x[2, 1:] = -INF                          # one token
+    x[3, ::2], x[3, 1::4] = -INF, NAN
+    x[4, [7, 9, 4000]] = INF                 # only these count
+    x[5] = torch.finfo(dtype).min            # the type's lowest value: equal, and drawn
+    x[6, 100:] = torch.finfo(dtype).min
+    x[7, 3], x[7, 4] = torch.finfo(dtype).max, -torch.finfo(dtype).max
+    u = torch.rand(9, generator=gen(21))
+    for s in ((1.0, 0, 1.0, 0.0), (0.8, 20, 0.9, 0.0), (2.0, 0, 0.7, 0.1), (0.0, 0, 1.0, 0.0)):
+        check(dev, x, u, *s, chunks=chunks)
+
+
+@pytest.mark.parametrize("t", [1e-45, 1e-30, 1e-3, 50.0, 1e30, INF])
+def test_extreme_temperatures(dev, t):
+    x = logits(30, 4, 2003, F32)
+    x[1] *= 1e30
+    x[2, 100:] = -INF
+    u = torch.rand(4, generator=gen(31))
+    check(dev, x, u, t)
+    check(dev, x, u, t, 10, 0.9, 0.1)
+
+
+def test_views(dev):
+    """Rows of a wider tensor, at any alignment, and one row for all."""
+    wide = logits(40, 6, 4003, BF16).to(dev)
+    u = torch.rand(6, generator=gen(41))
+    for lo, hi in ((0, 4003), (1, 4001), (3, 1000), (5, 6)):
+        x = wide[:, lo:hi]
+        check(dev, x, u, 1.0, 10, 0.9)
+        check(dev, x, u)
+    check(dev, wide[:1, 1:].expand(6, 4002), u)
+    check(dev, wide.float()[:, 3:], u)
+
+
+def test_the_largest_vocabulary(dev):
+    x = logits(50, 1, 1 << 20, BF16)
+    check(dev, x, torch.tensor([0.6]))
+    check(dev, x, torch.tensor([0.6]), 0.8, 200, 0.95)
+
+
+def test_without_logprobs_and_twice(dev):
+    x, u = logits(60, 5, 60000, BF16).to(dev), torch.rand(5, generator=gen(1)).to(dev)
+    s = Sampler(5, 60000, dev)
+    ids = [torch.empty(5, dtype=torch.int64, device=dev) for _ in range(3)]
+    for i in ids:
+        s(x, u, i, temperature=0.9, top_p=0.9)
+    assert torch.equal(ids[0], ids[1]) and torch.equal(ids[0], ids[2])
+
+
+@pytest.mark.parametrize("k", [0, 30])
+def test_captured(dev, k):
+    """Replays with new logits, numbers and settings in place, eager calls between them."""
+    B, V = 3, 40003
+    x, u = torch.zeros(B, V, dtype=BF16, device=dev), torch.zeros(B, device=dev)
+    t = torch.ones(B, device=dev)
+    ids, lp = torch.zeros(B, dtype=torch.int64, device=dev), torch.zeros(B, device=dev)
+    s, eager = Sampler(B, V, dev), Sampler(B, V, dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s(x, u, ids, temperature=t, top_k=k, top_p=0.9, logprobs=lp)
+    for i in range(4):
+        new = logits(70 + i, B, V, BF16)
+        x.copy_(new)
+        u.copy_(torch.rand(B, generator=gen(80 + i)))
+        t.fill_(0.5 + 0.3 * i)
+        graph.replay()
+        check(dev, new, u.cpu(), t.cpu(), k, 0.9, sampler=eager)
+        want, wlp = draw(dev, new, u, t, k, 0.9, sampler=eager)
+        torch.cuda.synchronize()
+        assert torch.equal(ids.cpu(), want) and torch.equal(lp.cpu().double(), wlp)
+
+
+def test_frequencies(dev):
+    """100,000 even steps of u over one row draw every kept token as often as its share, to one."""
+    V, n = 50, 50000
+    x = logits(90, 1, V, F32).expand(n, V).to(dev)
+    u = ((torch.arange(n) + 0.5) / n).to(F32)
+    ids, _ = draw(dev, x, u.to(dev), 1.0, 0, 0.97)
+    w = O.weights(*(lambda r: (r, O.order(r), 1.0))(x[0].cpu().double().numpy()))
+    m = O.kept(w, 0, 0.97, 0.0)
+    share = torch.from_numpy(w[:m] / w[:m].sum())
+    order = torch.from_numpy(O.order(x[0].cpu().double().numpy()))
+    got = torch.bincount(ids, minlength=V)[order].double()
+    assert (got[m:] == 0).all()
+    assert ((got[:m] - n * share).abs() <= 2 + n * 2.0 ** -24).all()
+
+
+def test_refusals(dev):
+    x = torch.zeros(2, 16, dtype=BF16, device=dev)
+    u, ids = torch.zeros(2, device=dev), torch.zeros(2, dtype=torch.int64, device=dev)
+    s = Sampler(2, 16, dev)
+    i32 = torch.zeros(2, dtype=torch.int32, device=dev)
+    bad = [dict(logits=x[:1]), dict(logits=x.half()), dict(logits=x.cpu()), dict(logits=x.t().contiguous().t()),
+           dict(u=u.double()), dict(u=u[:1]), dict(u=u.cpu()), dict(ids=ids.int()),
+           dict(temperature=-0.5), dict(temperature=NAN), dict(temperature=u.double()),
+           dict(temperature="1"), dict(top_k=-1), dict(top_k=2.5), dict(top_k=ids), dict(top_k=u),
+           dict(top_p=-0.1), dict(top_p=1.5), dict(top_p=i32), dict(min_p=2.0), dict(min_p=NAN),
+           dict(logprobs=u.half()), dict(logprobs=u[:1]), dict(min_p=torch.zeros(4, device=dev)[::2])]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            s(**(dict(logits=x, u=u, ids=ids) | kw))
+            pytest.fail(f"{kw} was taken")

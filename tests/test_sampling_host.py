@@ -1,0 +1,37 @@
+"""Refusals of sampling that need no GPU, and the C ABI's own checks (no kernel is launched)."""
+
+import pytest
+
+from kernel_optim_amd import _lib
+from kernel_optim_amd.kernels import sampling as S
+
+
+@pytest.mark.parametrize("B,V,device", [(0, 8, "cuda:0"), (65536, 8, "cuda:0"), (1, 0, "cuda:0"),
+                                        (1, (1 << 20) + 1, "cuda:0"), (1, 8, "cpu")])
+def test_sampler_refuses(B, V, device):
+    with pytest.raises(ValueError):
+        S.Sampler(B, V, device)
+
+
+def test_chunks():
+    for B in (1, 2, 64, 300, 65535):
+        for V in (1, 4096, 4097, 151936, 1 << 20):
+            c = S._chunks(B, V)
+            assert 1 <= c <= 1024 and (c == 1 or B * c <= 512)
+
+
+def test_c_abi_refuses():
+    h, p = _lib.lib(), 1 << 20   # p is never read: the checks come first
+    EINVAL, ERANGE = -22, -34
+
+    def call(x=p, f32=0, stride=8, B=1, V=8, u=p, ids=p, scratch=p, n=1 << 20, chunks=2):
+        return h.ko_sample(x, f32, stride, B, V, u, None, 1.0, None, 0, None, 1.0, None, 0.0, ids,
+                           None, scratch, n, chunks, None)
+
+    assert call(x=None) == call(u=None) == call(ids=None) == call(scratch=None) == EINVAL
+    assert call(x=p + 1) == call(x=p + 2, f32=1) == call(scratch=p + 8) == EINVAL
+    assert call(B=0) == call(V=0) == call(stride=-1) == call(chunks=0) == EINVAL
+    assert call(n=h.ko_sample_scratch(1, 2) - 1) == EINVAL
+    assert call(V=(1 << 20) + 1) == call(B=65536) == call(chunks=1025) == ERANGE
+    assert h.ko_sample_scratch(0, 1) == h.ko_sample_scratch(1, 0) == h.ko_sample_scratch(1, 1025) == -1
+    assert h.ko_sample_scratch(7, 1) == 0
