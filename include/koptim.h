@@ -446,11 +446,14 @@ int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K,
 int ko_fp8_read(const void* codes, const void* scales, int rows, int K, int pair, void* out,
                 int out_f32, long long stride, void* stream);
 
-/* y[M, N] = x W^T of x [M, K] (codes xc, scales xs) and W [N, K] (wc, ws), sums in fp32. epi 0: y
+/* y[M, N] = x W^T of x [M, K] and W [N, K] (codes wc, scales ws), sums in fp32. x: bf16, contiguous, which
+ * the call quantises (behind a norm with gain nw, as ko_fp8_quantize), with xc and xs, a matrix
+ * [M, K], as scratch; or NULL, and xc and xs hold it. epi 0: y
  * fp32; 1: bf16; 2 (RESID): y = bf16(h + bf16(sum)), h [M, N] bf16, which may be y; 3 (SWIGLU): W is
  * gate | up [2 N, K] held as a pair, y = bf16(bf16(silu(bf16(gate sum))) * bf16(up sum)). */
-int ko_fp8_linear(const void* xc, const void* xs, const void* wc, const void* ws, void* y,
-                  const void* h, int M, int N, int K, int epi, void* stream);
+int ko_fp8_linear(const void* x, const void* nw, float eps, void* xc, void* xs, const void* wc,
+                  const void* ws, void* y, const void* h, int M, int N, int K, int epi,
+                  void* stream);
 
 /* ---- Sampling ---------------------------------------------------------------------
  * In the place of torch.argmax(logits) of the reference's decode steps (engine/engine.py:299,

@@ -88,8 +88,8 @@ SIGNATURES = {
     "ko_fp8_quantize": [_c_void_p, _int, _ll, _int, _int, _int, _c_void_p, _f, _c_void_p, _c_void_p,
                         _c_void_p],
     "ko_fp8_read": [_c_void_p, _c_void_p, _int, _int, _int, _c_void_p, _int, _ll, _c_void_p],
-    "ko_fp8_linear": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _int, _int,
-                      _int, _int, _c_void_p],
+    "ko_fp8_linear": [_c_void_p, _c_void_p, _f, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                      _c_void_p, _c_void_p, _int, _int, _int, _int, _c_void_p],
     "ko_sample": [_c_void_p, _int, _ll, _int, _int, _c_void_p, _c_void_p, _f, _c_void_p, _int,
                   _c_void_p, _f, _c_void_p, _f, _c_void_p, _c_void_p, _c_void_p, _ll, _int,
                   _c_void_p],

@@ -90,6 +90,40 @@ __device__ __forceinline__ uint32_t umax_xor32(uint32_t u) {
   return max((uint32_t)p[0], (uint32_t)p[1]);
 }
 
+// A block in registers: lane l holds the values 64 j + 16 (l / 16) + 0..15, j = 0, 1, of row l % 16.
+// Its codes, in the lane's bytes of the layout above; returns the row's scale byte.
+__device__ __forceinline__ uint32_t fp8_quantize_block(const float (&v)[2][16], uint4 (&c)[2]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+  top = umax_xor32(umax_xor16(top));
+  const uint32_t b = fp8_scale_byte(top);
+  const float inv = fp8_inverse(min(b, 247u));
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = b == 255 ? 0x7f7f7f7fu
+                      : fp8_pack4(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
+    c[j] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return b;
+}
+
+// The sum of the squares of the row's 128 values, in every lane of the row. A row's sum adds its
+// blocks' sums in order, whichever kernel forms it, so all find the same norm.
+__device__ __forceinline__ float fp8_square_sum(const float (&v)[2][16]) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += v[j][i] * v[j][i];
+  return sum_xor32(sum_xor16(s));
+}
+
 // 8 codes (the dwords w0, w1) times 2^(b - 127) as bf16; scale = b << 23.
 __device__ __forceinline__ bf16x8 fp8_to_bf16(uint32_t w0, uint32_t w1, float scale) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);

@@ -3,22 +3,11 @@
 // Tiled product: a workgroup stages the blocks of its x and W tiles for one step of 128 values in
 // LDS by direct loads and multiplies the step before. W is the matrix instruction's first factor, so
 // that a lane ends with 4 neighbouring columns of a row of y.
-#include "fp8_core.h"
+#include "fp8_linear.h"
 
 namespace {
 
 using namespace ko;
-
-enum { EPI_F32 = 0, EPI_BF16 = 1, EPI_RESID = 2, EPI_SWIGLU = 3 };
-
-struct LinearArgs {
-  const uint8_t *xc, *wc;     // codes
-  const uint32_t *xs, *ws;    // scales
-  void* y;
-  const uint16_t* h;          // RESID: what is added; may be y
-  int M, N, K;
-  int xt, wt;                 // tiles of x and of W
-};
 
 typedef __attribute__((address_space(1))) const void g_void;
 typedef __attribute__((address_space(3))) void l_void;
@@ -37,43 +26,6 @@ __device__ __forceinline__ i32x8 frag(const uint8_t* block, int lane) {
 template <int I>
 __device__ __forceinline__ f32x4 mfma(i32x8 a, i32x8 b, f32x4 c, uint32_t sa, uint32_t sb) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, I, (int)sa, I, (int)sb);
-}
-
-// Columns n .. n + 3 of row m; v2: the second half's sums (SWIGLU). The roundings are those of
-// the bf16 chain: the product, silu(gate) and their product, or the product and the sum with h,
-// each to bf16.
-template <int EPI>
-__device__ __forceinline__ void store4(const LinearArgs& a, int m, int n, f32x4 v, f32x4 v2) {
-  if (m >= a.M || n >= a.N) return;
-  const long long o = (long long)m * a.N + n;
-  const bool whole = (a.N & 3) == 0;   // n is a multiple of 4: so is every row's beginning
-  if constexpr (EPI == EPI_F32) {
-    float* y = static_cast<float*>(a.y) + o;
-    if (whole) *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
-    else
-      for (int i = 0; i < 4 && n + i < a.N; ++i) y[i] = v[i];
-    return;
-  }
-  uint16_t* y = static_cast<uint16_t*>(a.y) + o;
-  float r[4];
-  uint16_t hv[4] = {};
-  if constexpr (EPI == EPI_RESID) {
-    if (whole) *reinterpret_cast<uint2*>(hv) = *reinterpret_cast<const uint2*>(a.h + o);
-    else
-      for (int i = 0; i < 4 && n + i < a.N; ++i) hv[i] = a.h[o + i];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r[i] = v[i];
-    if constexpr (EPI == EPI_RESID) r[i] = bf16_to_f32(hv[i]) + round_bf16(v[i]);
-    if constexpr (EPI == EPI_SWIGLU) {
-      const float g = round_bf16(v[i]), u = round_bf16(v2[i]);
-      r[i] = round_bf16(g / (1.0f + expf(-g))) * u;
-    }
-  }
-  if (whole) *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]));
-  else
-    for (int i = 0; i < 4 && n + i < a.N; ++i) y[i] = f32_to_bf16(r[i]);
 }
 
 // acc += the 16 x 16 products of a block of W and one of x; byte I of sw and sx are their scales.
@@ -183,11 +135,17 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_kernel(LinearArgs a, int nb
     if constexpr (EPI == EPI_SWIGLU) {
 #pragma unroll
       for (int i = 0; i < TN; i += 2)
-        store4<EPI>(a, m, ((n0 + wn * TN + i) >> 1) * 16 + 4 * g, acc[i][j], acc[i + 1][j]);
+        store4<EPI>(a, m, ((n0 + wn * TN + i) >> 1) * 16 + 4 * g, acc[i][j], acc[i + 1][j],
+                    make_uint2(0, 0));
     } else {
+      uint2 hv[TN] = {};
+      if constexpr (EPI == EPI_RESID) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) hv[i] = load4(a, m, (n0 + wn * TN + i) * 16 + 4 * g);
+      }
 #pragma unroll
       for (int i = 0; i < TN; ++i)
-        store4<EPI>(a, m, (n0 + wn * TN + i) * 16 + 4 * g, acc[i][j], acc[i][j]);
+        store4<EPI>(a, m, (n0 + wn * TN + i) * 16 + 4 * g, acc[i][j], acc[i][j], hv[i]);
     }
   }
 }
@@ -207,15 +165,23 @@ int launch(const LinearArgs& a, hipStream_t s) {
 
 extern "C" {
 
-int ko_fp8_linear(const void* xc, const void* xs, const void* wc, const void* ws, void* y,
-                  const void* h, int M, int N, int K, int epi, void* stream) {
+int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K, int pair,
+                    const void* nw, float eps, void* codes, void* scales, void* stream);
+
+int ko_fp8_linear(const void* x, const void* nw, float eps, void* xc, void* xs, const void* wc,
+                  const void* ws, void* y, const void* h, int M, int N, int K, int epi,
+                  void* stream) {
   if (!xc || !xs || !wc || !ws || !y || M < 1 || N < 1 || K < 8 || (K & 7)) return KO_EINVAL;
   if (epi < EPI_F32 || epi > EPI_SWIGLU) return KO_ENOTSUP;
-  if (epi == EPI_RESID && !h) return KO_EINVAL;
-  const uintptr_t all = (uintptr_t)xc | (uintptr_t)xs | (uintptr_t)wc | (uintptr_t)ws | (uintptr_t)y;
+  if ((epi == EPI_RESID && !h) || (nw && !x)) return KO_EINVAL;
+  const uintptr_t all = (uintptr_t)xc | (uintptr_t)xs | (uintptr_t)wc | (uintptr_t)ws | (uintptr_t)y |
+                        (uintptr_t)x | (uintptr_t)nw;
   if ((all | (uintptr_t)h) & 15) return KO_EINVAL;
   if (N > 0x3fffffff) return KO_ERANGE;
   LinearArgs a;
+  a.x = static_cast<const uint16_t*>(x);
+  a.nw = static_cast<const uint16_t*>(nw);
+  a.eps = eps;
   a.xc = static_cast<const uint8_t*>(xc);
   a.wc = static_cast<const uint8_t*>(wc);
   a.xs = static_cast<const uint32_t*>(xs);
@@ -226,6 +192,12 @@ int ko_fp8_linear(const void* xc, const void* xs, const void* wc, const void* ws
   a.xt = (int)fp8_tiles(M, false);
   a.wt = (int)(epi == EPI_SWIGLU ? 2 * fp8_tiles(N, false) : fp8_tiles(N, false));
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool few = M <= 16;
+  if (x && !(few && few_rows_quantized(a))) {
+    if (const int st = ko_fp8_quantize(x, 0, K, M, K, 0, nw, eps, xc, xs, stream)) return st;
+    a.x = a.nw = nullptr;
+  }
+  if (few) return launch_few_rows(a, epi, s);
   switch (epi) {
     case EPI_F32: return launch<EPI_F32>(a, s);
     case EPI_BF16: return launch<EPI_BF16>(a, s);

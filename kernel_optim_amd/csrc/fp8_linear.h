@@ -1,0 +1,69 @@
+// What the projections' kernels share: arguments, epilogues, and the quantiser of a block in a
+// wavefront's registers.
+#pragma once
+
+#include "fp8_core.h"
+
+namespace ko {
+
+enum { EPI_F32 = 0, EPI_BF16 = 1, EPI_RESID = 2, EPI_SWIGLU = 3 };
+
+struct LinearArgs {
+  const uint8_t *xc, *wc;     // codes
+  const uint32_t *xs, *ws;    // scales
+  const uint16_t *x, *nw;     // or x in bf16, and the gain of a norm in front of it
+  float eps;
+  void* y;
+  const uint16_t* h;          // RESID: what is added; may be y
+  int M, N, K;
+  int xt, wt;                 // tiles of x and of W
+};
+
+// RESID: columns n .. n + 3 of h's row m as packed bf16, loaded ahead of the sums they are added to.
+__device__ __forceinline__ uint2 load4(const LinearArgs& a, int m, int n) {
+  uint2 v = make_uint2(0, 0);
+  if (m >= a.M || n >= a.N) return v;
+  const uint16_t* h = a.h + (long long)m * a.N + n;
+  if ((a.N & 3) == 0) return *reinterpret_cast<const uint2*>(h);
+  v.x = h[0] | (n + 1 < a.N ? (uint32_t)h[1] << 16 : 0u);
+  if (n + 2 < a.N) v.y = h[2] | (n + 3 < a.N ? (uint32_t)h[3] << 16 : 0u);
+  return v;
+}
+
+// Columns n .. n + 3 of row m; v2: the second half's sums (SWIGLU); hv: load4 (RESID). The roundings
+// are those of the bf16 chain: the product, silu(gate) and their product, or the product and the
+// sum with h, each to bf16.
+template <int EPI>
+__device__ __forceinline__ void store4(const LinearArgs& a, int m, int n, f32x4 v, f32x4 v2, uint2 hv) {
+  if (m >= a.M || n >= a.N) return;
+  const long long o = (long long)m * a.N + n;
+  const bool whole = (a.N & 3) == 0;   // n is a multiple of 4: so is every row's beginning
+  if constexpr (EPI == EPI_F32) {
+    float* y = static_cast<float*>(a.y) + o;
+    if (whole) *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+      for (int i = 0; i < 4 && n + i < a.N; ++i) y[i] = v[i];
+    return;
+  }
+  uint16_t* y = static_cast<uint16_t*>(a.y) + o;
+  float r[4];
+  const float h[4] = {bf16lo(hv.x), bf16hi(hv.x), bf16lo(hv.y), bf16hi(hv.y)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = v[i];
+    if constexpr (EPI == EPI_RESID) r[i] = h[i] + round_bf16(v[i]);
+    if constexpr (EPI == EPI_SWIGLU) {
+      const float g = round_bf16(v[i]), u = round_bf16(v2[i]);
+      r[i] = round_bf16(g / (1.0f + expf(-g))) * u;
+    }
+  }
+  if (whole) *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]));
+  else
+    for (int i = 0; i < 4 && n + i < a.N; ++i) y[i] = f32_to_bf16(r[i]);
+}
+
+// fp8_few.hip: up to 16 rows of x (codes, or bf16 with or without a norm).
+bool few_rows_quantized(const LinearArgs& a);   // whether it quantises this x itself
+int launch_few_rows(const LinearArgs& a, int epi, hipStream_t s);
+
+}  // namespace ko

@@ -36,25 +36,12 @@ __device__ __forceinline__ void load16(const void* x, long long at, int k, int K
   }
 }
 
-// One block's codes from the lane's 2 x 16 values; returns the row's scale byte.
+// One block's codes into the matrix; returns the row's scale byte.
 __device__ __forceinline__ uint32_t store_block(const float (&v)[2][16], uint8_t* block, int lane) {
-  uint32_t top = 0;
+  uint4 c[2];
+  const uint32_t b = fp8_quantize_block(v, c);
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
-  top = umax_xor32(umax_xor16(top));
-  const uint32_t b = fp8_scale_byte(top);
-  const float inv = fp8_inverse(min(b, 247u));
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = b == 255 ? 0x7f7f7f7fu
-                      : fp8_pack4(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
-    *reinterpret_cast<uint4*>(block + 1024 * j + 16 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+  for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4*>(block + 1024 * j + 16 * lane) = c[j];
   return b;
 }
 
@@ -87,37 +74,31 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ 
   if (g == 0) scales[(t * Q + q) * 16 + r] = sc;
 }
 
-constexpr int NORM_WAVES = 16;
+constexpr int NORM_WAVES = 16, NORM_BLOCKS = 1024;   // K up to 131,072
 
 // RMSNorm in front (bf16 rows): a workgroup takes a tile, sums the squares of its 16 rows in
-// fp32, and its wavefronts quantise bf16(nw * bf16(x * rstd)) quad by quad. The rows are read
+// fp32, and its wavefronts quantise bf16(nw * bf16(x * rstd)) block by block. The rows are read
 // twice, the second time from the caches (16 rows of 2560 values: 80 KB).
 __global__ __launch_bounds__(64 * NORM_WAVES) void quantize_norm_kernel(
     const uint16_t* __restrict__ x, long long stride, int rows, int K,
     const uint16_t* __restrict__ nw, float eps, uint8_t* __restrict__ codes,
     uint32_t* __restrict__ scales) {
-  __shared__ float s_sq[NORM_WAVES][16];
+  extern __shared__ float s_sq[];   // [blocks][16]
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   const int Q = fp8_quads(K), KB = fp8_blocks(K);
   const long long t = blockIdx.x;
   const int row = fp8_row(t, r, rows, false);
   const long long at = (long long)max(row, 0) * stride;
-  float sq = 0.f;
   for (int kb = wv; kb < KB; kb += NORM_WAVES) {
     float v[2][16];
 #pragma unroll
     for (int j = 0; j < 2; ++j) load16<false>(x, at, kb * 128 + 64 * j + 16 * g, K, row >= 0, v[j]);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sq += v[j][i] * v[j][i];
+    const float sq = fp8_square_sum(v);
+    if (g == 0) s_sq[kb * 16 + r] = sq;
   }
-  sq = sum_xor32(sum_xor16(sq));
-  if (g == 0) s_sq[wv][r] = sq;
   __syncthreads();
   float tot = 0.f;
-#pragma unroll
-  for (int i = 0; i < NORM_WAVES; ++i) tot += s_sq[i][r];
+  for (int kb = 0; kb < KB; ++kb) tot += s_sq[kb * 16 + r];
   const float rstd = row >= 0 ? rsqrtf(tot / (float)K + eps) : 0.f;   // eps may be 0
   uint8_t* sc = reinterpret_cast<uint8_t*>(scales);
   for (int kb = wv; kb < 4 * Q; kb += NORM_WAVES) {
@@ -206,13 +187,14 @@ int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K,
   if (const int st = check(rows, K, pair, stride)) return st;
   if (!al16(x) || !al16(codes) || !al16(scales) || (nw && !al16(nw))) return KO_EINVAL;
   if (nw && (x_f32 || pair)) return KO_ENOTSUP;
+  if (nw && fp8_blocks(K) > NORM_BLOCKS) return KO_ERANGE;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const long long tiles = fp8_tiles(rows, pair);
   uint8_t* c = static_cast<uint8_t*>(codes);
   uint32_t* sc = static_cast<uint32_t*>(scales);
   if (nw) {
-    hipLaunchKernelGGL(quantize_norm_kernel, dim3((unsigned)tiles), dim3(64 * NORM_WAVES), 0, s,
-                       static_cast<const uint16_t*>(x), stride, rows, K,
+    hipLaunchKernelGGL(quantize_norm_kernel, dim3((unsigned)tiles), dim3(64 * NORM_WAVES),
+                       64 * fp8_blocks(K), s, static_cast<const uint16_t*>(x), stride, rows, K,
                        static_cast<const uint16_t*>(nw), eps, c, sc);
     return KO_LAUNCH_STATUS();
   }

@@ -106,10 +106,15 @@ def test_blocks_that_hold_no_numbers(dev):
     # a product's rows and columns with such a block are NaN, the others as without it
     w = (0.1 * randn(10, 48, 640)).to(BF16)
     w[7, 300] = float("nan")
-    y = torch.empty(40, 48, device=dev)
-    Fp8Linear(40, 48, 640, EPI_F32, False)(x.to(dev), fp8_quantize(w.to(dev)), y=y)
     bad = torch.isnan(O.held(x)).any(1)[:, None] | torch.isnan(O.held(w)).any(1)[None]
-    assert torch.equal(torch.isnan(y.cpu()), bad)
+    for lo, hi in ((0, 40), (3, 19), (0, 1)):
+        y = torch.empty(hi - lo, 48, device=dev)
+        Fp8Linear(hi - lo, 48, 640, EPI_F32, False)(x[lo:hi].to(dev), fp8_quantize(w.to(dev)), y=y)
+        assert torch.equal(torch.isnan(y.cpu()), bad[lo:hi])
+    many = torch.cat((x, x, x))                    # the 8-bit matrix instruction
+    y = torch.empty(120, 48, device=dev, dtype=BF16)
+    Fp8Linear(120, 48, 640, EPI_BF16, False)(many.to(dev), fp8_quantize(w.to(dev)), y=y)
+    assert torch.equal(torch.isnan(y.cpu()), torch.cat((bad, bad, bad)))
 
 
 @pytest.mark.parametrize("n,K", [(1, 8), (1, 2560), (5, 136), (16, 4096), (19, 2568), (64, 9728),
@@ -183,7 +188,8 @@ def on(dev, *ts):
     return [None if t is None else t.to(dev) for t in ts]
 
 
-LINEAR = [(1, 16, 8), (1, 1, 128), (1, 2560, 4096), (2, 1000, 712), (3, 17, 136), (7, 130, 520),
+LINEAR = [(1, 16, 8), (1, 5000, 256), (16, 8203, 640), (4, 64, 3000), (9, 48, 9728), (16, 40, 12296),
+          (1, 1, 128), (1, 2560, 4096), (2, 1000, 712), (3, 17, 136), (7, 130, 520),
           (16, 256, 2560), (17, 33, 1024), (33, 999, 264), (64, 512, 1152), (65, 130, 640),
           (100, 300, 2568), (130, 640, 896), (257, 515, 384), (300, 1024, 2560)]
 
@@ -206,12 +212,13 @@ def test_linear(dev, M, N, K, epi):
         assert torch.equal(hd, y)
 
 
-@pytest.mark.parametrize("M", [1, 5, 16, 40, 64, 130])
+@pytest.mark.parametrize("M,K", [(1, 2560), (5, 2560), (16, 2560), (40, 2560), (64, 2560),
+                                 (130, 2560), (3, 128), (16, 264), (2, 2568), (16, 4096)])
 @pytest.mark.parametrize("epi", ["bf16", "swiglu"])
-def test_linear_behind_a_norm(dev, M, epi):
+def test_linear_behind_a_norm(dev, M, K, epi):
     """Against the product over what fp8_quantize holds of the norm, bit for bit, and that
     against 64 bits (its own test has the norm's)."""
-    N, K = 208, 2560
+    N = 208
     x, w, _, nw = projection(dev, M, N, K, epi, True, seed=M)
     xd, wd, nwd = on(dev, x, w, nw)
     held = fp8_quantize(wd, pair=epi == "swiglu")
