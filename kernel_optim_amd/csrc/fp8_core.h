@@ -30,8 +30,9 @@
 // scales of 4 blocks and the instruction's op_sel picks one. Rows past the end and values past
 // K are zeros; so is the padding of scales.
 //
-// A pair (gate | up, [2 n, K]) has its tiles alternate: 2 t is rows 16 t.. of the first half,
-// 2 t + 1 of the second, each half padded to whole tiles.
+// A pair (gate | up, [2 n, K]) has 8 rows of either half in a tile: rows 0..7 of tile t are 8 t.. of
+// the first half, rows 8..15 of the second, each half padded to whole eights. A lane and the one 32
+// places on then end with the sums of a gate column and of its up column.
 #pragma once
 
 #include "ko_common.h"
@@ -47,7 +48,7 @@ constexpr int FP8_BLOCK = 2048;   // bytes of a block of codes: 16 rows, 128 val
 __host__ __device__ __forceinline__ int fp8_blocks(int K) { return (K + 127) >> 7; }
 __host__ __device__ __forceinline__ int fp8_quads(int K) { return (K + 511) >> 9; }
 __host__ __device__ __forceinline__ long long fp8_tiles(int rows, bool pair) {
-  return pair ? 2ll * ((rows / 2 + 15) / 16) : (rows + 15ll) / 16;
+  return pair ? (rows / 2 + 7ll) / 8 : (rows + 15ll) / 16;
 }
 
 // The row of [rows, K] that row r of tile t holds, or -1.
@@ -57,8 +58,8 @@ __device__ __forceinline__ int fp8_row(long long t, int r, int rows, bool pair) 
     return row < rows ? (int)row : -1;
   }
   const int n = rows >> 1;
-  const long long row = (t >> 1) * 16 + r;
-  return row < n ? (int)((t & 1) * n + row) : -1;
+  const long long row = t * 8 + (r & 7);
+  return row < n ? (int)((r >> 3) * n + row) : -1;
 }
 
 // The scale's byte for a block whose largest |x| has these bits (NaN and infinity sort above
@@ -113,15 +114,49 @@ __device__ __forceinline__ uint32_t fp8_quantize_block(const float (&v)[2][16], 
   return b;
 }
 
-// The sum of the squares of the row's 128 values, in every lane of the row. A row's sum adds its
-// blocks' sums in order, whichever kernel forms it, so all find the same norm.
-__device__ __forceinline__ float fp8_square_sum(const float (&v)[2][16]) {
+// The sum of the squares of 8 values, in order.
+__device__ __forceinline__ float fp8_squares(const float* v) {
   float s = 0.f;
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int i = 0; i < 8; ++i) s += v[i] * v[i];
+  return s;
+}
+// The sum of the squares of a block's row of 128, its eights' sums c = 0..15 added as a tree: c and
+// c + 8, then 4, 2 and 1 apart. A row's sum adds its blocks' in order. Every kernel forms both so,
+// whatever its lanes hold, and all find the same norm. Here the block is in registers as above.
+__device__ __forceinline__ float fp8_square_sum(const float (&v)[2][16]) {
+  float s[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += v[j][i] * v[j][i];
-  return sum_xor32(sum_xor16(s));
+  for (int p = 0; p < 2; ++p)
+    s[p] = sum_xor16(sum_xor32(fp8_squares(v[0] + 8 * p) + fp8_squares(v[1] + 8 * p)));
+  return s[0] + s[1];
+}
+
+// 8 values of a block's row in each of 16 neighbouring lanes (a DPP row): their codes; returns the
+// block's scale byte. q: packed bf16.
+__device__ __forceinline__ uint32_t fp8_quantize8(const uint4& q, uint2& c) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t top = 0;   // of 15-bit magnitudes, which compare as the floats do
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+  int m = (int)top;
+  m = max(m, dpp_i<0x128>(m));
+  m = max(m, dpp_i<0x124>(m));
+  m = max(m, dpp_i<0x122>(m));
+  m = max(m, dpp_i<0x121>(m));
+  const uint32_t b = fp8_scale_byte((uint32_t)m << 16);
+  const float inv = fp8_inverse(min(b, 247u));
+  c.x = b == 255 ? 0x7f7f7f7fu
+                 : fp8_pack4(bf16lo(w[0]), bf16hi(w[0]), bf16lo(w[1]), bf16hi(w[1]), inv);
+  c.y = b == 255 ? 0x7f7f7f7fu
+                 : fp8_pack4(bf16lo(w[2]), bf16hi(w[2]), bf16lo(w[3]), bf16hi(w[3]), inv);
+  return b;
+}
+
+// bf16(gain * bf16(x * rstd)) of packed pairs, as the bf16 chain rounds.
+__device__ __forceinline__ uint32_t fp8_norm2(uint32_t x, uint32_t w, float rstd) {
+  const uint32_t t = pack_bf16x2(bf16lo(x) * rstd, bf16hi(x) * rstd);
+  return pack_bf16x2(bf16lo(w) * bf16lo(t), bf16hi(w) * bf16hi(t));
 }
 
 // 8 codes (the dwords w0, w1) times 2^(b - 127) as bf16; scale = b << 23.

@@ -66,7 +66,7 @@ template <int EPI, bool WIDE, int WN, int WM, int TN, int TM>
 __global__ __launch_bounds__(64 * WN * WM) void gemm_kernel(LinearArgs a, int nblocks) {
   constexpr int W = WN * WM, NT = WN * TN, MT = WM * TM, CH = 2 * (NT + MT) / W;
   static_assert(CH * W == 2 * (NT + MT), "every wavefront loads as much");
-  static_assert(EPI != EPI_SWIGLU || TN % 2 == 0, "gate and up tiles of a wavefront in pairs");
+  static_assert(EPI != EPI_SWIGLU || TN % 2 == 0, "a wavefront's tiles in twos");
   __shared__ __attribute__((aligned(16))) uint8_t s_buf[2][(NT + MT) * FP8_BLOCK];
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int wn = wv % WN, wm = wv / WN;
@@ -133,10 +133,19 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_kernel(LinearArgs a, int nb
   for (int j = 0; j < TM; ++j) {
     const int m = (m0 + wm * TM + j) * 16 + r;
     if constexpr (EPI == EPI_SWIGLU) {
+      // two tiles' gate sums in one register, their up sums in the other
 #pragma unroll
-      for (int i = 0; i < TN; i += 2)
-        store4<EPI>(a, m, ((n0 + wn * TN + i) >> 1) * 16 + 4 * g, acc[i][j], acc[i + 1][j],
-                    make_uint2(0, 0));
+      for (int i = 0; i < TN; i += 2) {
+        f32x4 gate, up;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][e]),
+                                                          __float_as_uint(acc[i + 1][j][e]), false, false);
+          gate[e] = __uint_as_float(p[0]);
+          up[e] = __uint_as_float(p[1]);
+        }
+        store4<EPI>(a, m, (n0 + wn * TN + i + (g >> 1)) * 8 + 4 * (g & 1), gate, up, make_uint2(0, 0));
+      }
     } else {
       uint2 hv[TN] = {};
       if constexpr (EPI == EPI_RESID) {
@@ -190,9 +199,9 @@ int ko_fp8_linear(const void* x, const void* nw, float eps, void* xc, void* xs, 
   a.h = static_cast<const uint16_t*>(h);
   a.M = M, a.N = N, a.K = K;
   a.xt = (int)fp8_tiles(M, false);
-  a.wt = (int)(epi == EPI_SWIGLU ? 2 * fp8_tiles(N, false) : fp8_tiles(N, false));
+  a.wt = (int)(epi == EPI_SWIGLU ? fp8_tiles(2 * N, true) : fp8_tiles(N, false));
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool few = M <= 16;
+  const bool few = few_rows_served(a);
   if (x && !(few && few_rows_quantized(a))) {
     if (const int st = ko_fp8_quantize(x, 0, K, M, K, 0, nw, eps, xc, xs, stream)) return st;
     a.x = a.nw = nullptr;

@@ -63,7 +63,8 @@ __device__ __forceinline__ void store4(const LinearArgs& a, int m, int n, f32x4 
 }
 
 // fp8_few.hip: up to 16 rows of x (codes, or bf16 with or without a norm).
-bool few_rows_quantized(const LinearArgs& a);   // whether it quantises this x itself
+bool few_rows_served(const LinearArgs& a);
+bool few_rows_quantized(const LinearArgs& a);   // whether it takes this x in bf16
 int launch_few_rows(const LinearArgs& a, int epi, hipStream_t s);
 
 }  // namespace ko

@@ -118,6 +118,67 @@ __global__ __launch_bounds__(64 * NORM_WAVES) void quantize_norm_kernel(
   }
 }
 
+// Few bf16 rows: a workgroup for each row of a tile (padding rows among them), 8 values a thread, so
+// that a decode step's rows are spread over the GPU. It stores 8 bytes at a time, which many rows
+// would feel.
+constexpr int FEW = 256;       // rows
+constexpr int ROW_LOADS = 8;   // K up to 8 * 1024 * ROW_LOADS
+
+template <bool NORM>
+__global__ __launch_bounds__(1024) void quantize_row_kernel(const uint16_t* __restrict__ x,
+                                                            long long stride, int rows, int K,
+                                                            int pair,
+                                                            const uint16_t* __restrict__ nw,
+                                                            float eps, uint8_t* __restrict__ codes,
+                                                            uint8_t* __restrict__ scales) {
+  extern __shared__ float s_sq[];   // NORM: [blocks]
+  const int KB = fp8_blocks(K), Q = fp8_quads(K), T = blockDim.x, all = 16 * KB;
+  const long long t = blockIdx.x >> 4;
+  const int r = blockIdx.x & 15, row = fp8_row(t, r, rows, pair);
+  const uint16_t* src = x + (long long)max(row, 0) * stride;
+  uint4 q[ROW_LOADS], w[NORM ? ROW_LOADS : 1];
+#pragma unroll
+  for (int i = 0; i < ROW_LOADS; ++i) {
+    const int e = i * T + (int)threadIdx.x;
+    if (e >= all) break;
+    const bool in = row >= 0 && 8 * e < K;
+    q[i] = in ? ldg16(src + 8 * e) : make_uint4(0, 0, 0, 0);
+    if constexpr (NORM) w[i] = in ? ldg16(nw + 8 * e) : make_uint4(0, 0, 0, 0);
+  }
+  float rstd = 0.f;
+  if constexpr (NORM) {
+#pragma unroll
+    for (int i = 0; i < ROW_LOADS; ++i) {
+      const int e = i * T + (int)threadIdx.x;
+      if (e >= all) break;
+      const float v[8] = {bf16lo(q[i].x), bf16hi(q[i].x), bf16lo(q[i].y), bf16hi(q[i].y),
+                          bf16lo(q[i].z), bf16hi(q[i].z), bf16lo(q[i].w), bf16hi(q[i].w)};
+      const float sq = row_sum16(fp8_squares(v));
+      if ((e & 15) == 0) s_sq[e >> 4] = sq;
+    }
+    __syncthreads();
+    float tot = 0.f;
+    for (int kb = 0; kb < KB; ++kb) tot += s_sq[kb];
+    rstd = row >= 0 ? rsqrtf(tot / (float)K + eps) : 0.f;   // eps may be 0
+  }
+#pragma unroll
+  for (int i = 0; i < ROW_LOADS; ++i) {
+    const int e = i * T + (int)threadIdx.x;
+    if (e >= all) break;
+    if constexpr (NORM)
+      q[i] = make_uint4(fp8_norm2(q[i].x, w[i].x, rstd), fp8_norm2(q[i].y, w[i].y, rstd),
+                        fp8_norm2(q[i].z, w[i].z, rstd), fp8_norm2(q[i].w, w[i].w, rstd));
+    uint2 c;
+    const uint32_t b = fp8_quantize8(q[i], c);
+    const int kb = e >> 4;
+    *reinterpret_cast<uint2*>(codes + (t * KB + kb) * FP8_BLOCK + ((e >> 1) & 7) * 256 + r * 16 +
+                              8 * (e & 1)) = c;
+    if ((e & 15) == 0) scales[((t * Q + (kb >> 2)) * 16 + r) * 4 + (kb & 3)] = (uint8_t)b;
+  }
+  if ((int)threadIdx.x < 4 * Q - KB)   // the last quad's padding
+    scales[((t * Q + Q - 1) * 16 + r) * 4 + 3 - (int)threadIdx.x] = 0;
+}
+
 // The values back: a wavefront for each block, rows written in pieces of 16 values.
 template <bool F32OUT>
 __global__ __launch_bounds__(256) void read_kernel(const uint8_t* __restrict__ codes,
@@ -192,6 +253,21 @@ int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K,
   const long long tiles = fp8_tiles(rows, pair);
   uint8_t* c = static_cast<uint8_t*>(codes);
   uint32_t* sc = static_cast<uint32_t*>(scales);
+  const int all = 16 * fp8_blocks(K);
+  if (!x_f32 && rows <= FEW && all <= 1024 * ROW_LOADS) {
+    const int per = (all + ROW_LOADS - 1) / ROW_LOADS;
+    const int threads = all <= 1024 ? (all + 63) / 64 * 64 : per <= 640 ? 640 : 1024;
+    const dim3 grid((unsigned)(16 * tiles));
+    if (nw)
+      hipLaunchKernelGGL(quantize_row_kernel<true>, grid, dim3(threads), 4 * fp8_blocks(K), s,
+                         static_cast<const uint16_t*>(x), stride, rows, K, pair,
+                         static_cast<const uint16_t*>(nw), eps, c, static_cast<uint8_t*>(scales));
+    else
+      hipLaunchKernelGGL(quantize_row_kernel<false>, grid, dim3(threads), 0, s,
+                         static_cast<const uint16_t*>(x), stride, rows, K, pair, nullptr, 0.f, c,
+                         static_cast<uint8_t*>(scales));
+    return KO_LAUNCH_STATUS();
+  }
   if (nw) {
     hipLaunchKernelGGL(quantize_norm_kernel, dim3((unsigned)tiles), dim3(64 * NORM_WAVES),
                        64 * fp8_blocks(K), s, static_cast<const uint16_t*>(x), stride, rows, K,

@@ -30,7 +30,7 @@ FP8_BLOCK = 128   # values that share a scale
 class Fp8Tensor:
     """A matrix [rows, K] in 8 bits: ``codes`` uint8 [tiles, blocks, 2048] (16 rows x 128 values a
     block) and ``scales`` uint8 [tiles, quads, 64] (16 rows x 4 blocks), as csrc/fp8_core.h lays
-    them out. ``pair``: the two halves of its rows (gate | up) lie in alternating tiles."""
+    them out. ``pair``: a tile has 8 rows of each half of the rows (gate | up)."""
 
     __slots__ = ("codes", "scales", "rows", "K", "pair")
 
@@ -56,7 +56,7 @@ def fp8_shape(rows, K, pair=False):
     """(tiles of 16 rows, blocks of 128 values) of a matrix [rows, K]."""
     _need(rows >= 1 and K >= 8 and K % 8 == 0, "rows must be positive, K a positive multiple of 8")
     _need(not pair or rows % 2 == 0, "a pair has an even number of rows")
-    tiles = 2 * _cdiv(rows // 2, 16) if pair else _cdiv(rows, 16)
+    tiles = _cdiv(rows // 2, 8) if pair else _cdiv(rows, 16)
     blocks = _cdiv(K, FP8_BLOCK)
     _need(tiles * blocks < 2 ** 31, "the matrix has 2^31 blocks or more")
     return tiles, blocks

@@ -70,15 +70,15 @@ def pack(codes, scales, pair=False):
     halves = 2 if pair else 1
     n = codes.shape[0] // halves
     blocks = scales.shape[1]
-    T = -(-n // 16)
-    out = torch.zeros(T * halves, blocks, 2048, dtype=torch.uint8)
-    sc = torch.zeros(T * halves, -(-blocks // 4), 64, dtype=torch.uint8)
+    T = -(-n // (16 // halves))
+    out = torch.zeros(T, blocks, 2048, dtype=torch.uint8)
+    sc = torch.zeros(T, -(-blocks // 4), 64, dtype=torch.uint8)
     k = torch.arange(blocks * 128)
     kb, j, g, i = k // 128, k % 128 // 64, k % 64 // 16, k % 16
     b = torch.arange(blocks)
     for row in range(codes.shape[0]):
         h, m = divmod(row, n)
-        t, r = m // 16 * halves + h, m % 16
+        t, r = (m // 8, 8 * h + m % 8) if pair else (m // 16, m % 16)
         out[t, kb, 1024 * j + 16 * (16 * g + r) + i] = codes[row]
         sc[t, b // 4, 4 * r + b % 4] = scales[row]
     return out, sc
