@@ -1,7 +1,7 @@
 // y = x W^T with W in 8 bits for up to 16 rows of x: one weight pass at memory speed.
 //
 // The 16 rows are one tile of the matrix instruction. A workgroup's wavefronts share K: each streams
-// its few blocks of one tile of W after another, two tiles' loads in flight at any time; a tile's
+// its few blocks of one tile of W after another, two or three tiles' loads in flight at any time; a tile's
 // partial sums meet in LDS, and one wavefront in turn adds and stores them. The codes go through bf16 to the matrix instruction (sums
 // in fp32 throughout): 16 conversions and 4 instructions of 16 cycles a block of 2 KB, a quarter of
 // the time in which it comes from memory.
@@ -35,11 +35,11 @@ __device__ __forceinline__ void widen(const uint4 (&c)[2], uint32_t b, bf16x8 (&
   }
 }
 
-// IN: 0 codes, 1 bf16, 2 bf16 behind a norm. BPW blocks a wavefront, at most WMAX wavefronts.
-template <int EPI, int IN, int BPW, int WMAX>
+// IN: 0 codes, 1 bf16, 2 bf16 behind a norm. BPW blocks a wavefront, at most WMAX wavefronts; SETS
+// tiles in flight.
+template <int EPI, int IN, int BPW, int WMAX, int SETS>
 __global__ __launch_bounds__(64 * WMAX) void few_kernel(LinearArgs a) {
   constexpr bool HOLD = BPW <= 2;                 // x as bf16 in registers for the whole launch
-  constexpr int SETS = BPW <= 3 ? 2 : 1;          // tiles in flight
   __shared__ f32x4 s_part[2][WMAX][64];
   __shared__ float s_sq[IN == 2 ? WMAX * BPW * OWN : 1], s_rstd[OWN];
   __shared__ uint4 s_gain[IN == 2 ? WMAX * BPW * 16 : 1];
@@ -54,8 +54,9 @@ __global__ __launch_bounds__(64 * WMAX) void few_kernel(LinearArgs a) {
   // this workgroup's steps: its tiles of W
   const int steps = (a.wt - 1 - (int)blockIdx.x) / GRID + 1;
   const uint8_t* wl = a.wc + 16 * lane;
-  auto load = [&](int st, Weights<BPW>& w) {
-    if (st >= steps) return;
+  Weights<BPW> ws[SETS];
+  auto load = [&](int st, int set) {
+    Weights<BPW>& w = ws[set];
     const long long tile = (int)blockIdx.x + st * GRID;
     const uint8_t* c = wl + (tile * KB + kb0) * FP8_BLOCK;
     const uint32_t* sc = a.ws + tile * Q * 16 + r;
@@ -69,7 +70,10 @@ __global__ __launch_bounds__(64 * WMAX) void few_kernel(LinearArgs a) {
       else w.s[i] = w.s[0];
     }
   };
-  Weights<BPW> wa, wb;
+  auto load_first = [&]() {   // a workgroup with fewer steps: its last one again
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) load(min(i, steps - 1), i);
+  };
 
   // x's codes as the lane multiplies them: rows past M are zeros. Codes in memory that are not held
   // are loaded two blocks ahead.
@@ -105,8 +109,7 @@ __global__ __launch_bounds__(64 * WMAX) void few_kernel(LinearArgs a) {
 #pragma unroll
     for (int i = 0; i < AHEAD && i < BPW; ++i) load_x(i);
     __builtin_amdgcn_sched_barrier(0);   // x ahead of the weights
-    load(0, wa);
-    if constexpr (SETS == 2) load(1, wb);
+    load_first();
   } else {
     // an eighth e of x: 8 values of row e / (16 KB); 16 neighbouring lanes have a block's row
     const int per = KB * 16, all = M * per;
@@ -123,8 +126,7 @@ __global__ __launch_bounds__(64 * WMAX) void few_kernel(LinearArgs a) {
     if constexpr (IN == 2)   // per <= 16 * BPW * W <= T (BPW <= 4)
       if (8 * (int)threadIdx.x < a.K) gain = ldg16(a.nw + 8 * threadIdx.x);
     __builtin_amdgcn_sched_barrier(0);   // x ahead of the weights
-    load(0, wa);
-    if constexpr (SETS == 2) load(1, wb);
+    load_first();
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (IN == 2) {
       if ((int)threadIdx.x < per) s_gain[threadIdx.x] = gain;
@@ -170,12 +172,12 @@ __global__ __launch_bounds__(64 * WMAX) void few_kernel(LinearArgs a) {
     for (int i = 0; i < BPW; ++i) operand(i, x[i]);
   }
 
-  auto step = [&](int st, Weights<BPW>& w) {
+  auto step = [&](int st, int set, auto load_next) {
+    const Weights<BPW>& w = ws[set];
     const bool mine = wv == st % W;   // this wavefront adds the tile's sums
     const int tile = (int)blockIdx.x + st * GRID;
     uint2 hv = make_uint2(0, 0);
-    if constexpr (EPI == EPI_RESID)
-      if (mine) hv = load4(a, r, tile * 16 + 4 * g);
+    if constexpr (EPI == EPI_RESID) hv = load4(a, r, tile * 16 + 4 * g);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < BPW; ++i) {
@@ -195,11 +197,10 @@ __global__ __launch_bounds__(64 * WMAX) void few_kernel(LinearArgs a) {
       load_x(0);
       load_x(1);
     }
-    load(st + SETS, w);
+    load_next();
     __syncthreads();   // of the next step but one: every wavefront is past this step's sums
     if (mine) {
-      f32x4 sum = s_part[st & 1][0][lane];
-      for (int i = 1; i < W; ++i) sum += s_part[st & 1][i][lane];
+      const f32x4 sum = add_parts(s_part[st & 1], 1, W, lane);
       if constexpr (EPI == EPI_SWIGLU) {
         f32x4 up;   // 32 lanes on
 #pragma unroll
@@ -213,24 +214,25 @@ __global__ __launch_bounds__(64 * WMAX) void few_kernel(LinearArgs a) {
       }
     }
   };
-  for (int st = 0; st < steps; st += SETS) {
-    step(st, wa);
-    if constexpr (SETS == 2)
-      if (st + 1 < steps) step(st + 1, wb);
-  }
+  pipeline<SETS>(steps, load, step);
 }
 
 template <int EPI, int IN>
 int launch(const LinearArgs& a, hipStream_t s) {
   const int KB = fp8_blocks(a.K);
   const dim3 grid(a.wt < GRID ? a.wt : GRID);
-#define KO_FEW(B, WM) \
-  hipLaunchKernelGGL((few_kernel<EPI, IN, B, WM>), grid, dim3(64 * ((KB + B - 1) / B)), 0, s, a)
-  if (KB <= 20) KO_FEW(2, 10);
-  else if (KB <= 32) KO_FEW(2, 16);
-  else if constexpr (IN < 2) {
-    if (KB <= 48) KO_FEW(3, 16);
-    else KO_FEW(5, 16);
+#define KO_FEW(B, WM, S) \
+  hipLaunchKernelGGL((few_kernel<EPI, IN, B, WM, S>), grid, dim3(64 * ((KB + B - 1) / B)), 0, s, a)
+  const bool one = a.wt <= GRID;   // a step for every workgroup
+  if (KB <= 20) {
+    if (one) KO_FEW(2, 10, 1);
+    else KO_FEW(2, 10, 2);
+  } else if (KB <= 32) {
+    if (one) KO_FEW(2, 16, 1);
+    else KO_FEW(2, 16, 2);
+  } else if constexpr (IN < 2) {
+    if (KB <= 48) KO_FEW(3, 16, 1);
+    else KO_FEW(5, 16, 1);
   }
 #undef KO_FEW
   return KO_LAUNCH_STATUS();

@@ -163,10 +163,8 @@ template <int EPI>
 int launch(const LinearArgs& a, hipStream_t s) {
   const int nb = (a.wt + 7) / 8, mb = (a.xt + 7) / 8;
   if ((long long)nb * mb > 0x7fffffffll) return KO_ERANGE;
-  if (EPI == EPI_F32 || a.M <= 64)
-    hipLaunchKernelGGL((gemm_kernel<EPI, true, 2, 2, 4, 4>), dim3(nb * mb), dim3(256), 0, s, a, nb);
-  else if constexpr (EPI != EPI_F32)
-    hipLaunchKernelGGL((gemm_kernel<EPI, false, 2, 2, 4, 4>), dim3(nb * mb), dim3(256), 0, s, a, nb);
+  hipLaunchKernelGGL((gemm_kernel<EPI, EPI == EPI_F32, 2, 2, 4, 4>), dim3(nb * mb), dim3(256), 0, s,
+                     a, nb);
   return KO_LAUNCH_STATUS();
 }
 
@@ -207,6 +205,7 @@ int ko_fp8_linear(const void* x, const void* nw, float eps, void* xc, void* xs, 
     a.x = a.nw = nullptr;
   }
   if (few) return launch_few_rows(a, epi, s);
+  if (mid_rows_served(a, epi)) return launch_mid_rows(a, epi, s);
   switch (epi) {
     case EPI_F32: return launch<EPI_F32>(a, s);
     case EPI_BF16: return launch<EPI_BF16>(a, s);

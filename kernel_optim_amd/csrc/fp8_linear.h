@@ -20,14 +20,53 @@ struct LinearArgs {
 };
 
 // RESID: columns n .. n + 3 of h's row m as packed bf16, loaded ahead of the sums they are added to.
+// Rows and columns past the end read an element that is there (unused): no lane skips the load, so
+// what is waited for behind it stays exact.
 __device__ __forceinline__ uint2 load4(const LinearArgs& a, int m, int n) {
-  uint2 v = make_uint2(0, 0);
-  if (m >= a.M || n >= a.N) return v;
-  const uint16_t* h = a.h + (long long)m * a.N + n;
-  if ((a.N & 3) == 0) return *reinterpret_cast<const uint2*>(h);
-  v.x = h[0] | (n + 1 < a.N ? (uint32_t)h[1] << 16 : 0u);
-  if (n + 2 < a.N) v.y = h[2] | (n + 3 < a.N ? (uint32_t)h[3] << 16 : 0u);
-  return v;
+  const uint16_t* h = a.h + (long long)min(m, a.M - 1) * a.N;
+  if ((a.N & 3) == 0) return *reinterpret_cast<const uint2*>(h + min(n, a.N - 4));
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = h[min(n + i, a.N - 1)];
+  return make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+}
+
+// The sum of W wavefronts' partial sums, part[i * stride][lane], in order, 4 reads at a time.
+__device__ __forceinline__ f32x4 add_parts(const f32x4 (*part)[64], int stride, int W, int lane) {
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < W; i += 4) {
+    f32x4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = part[min(i + j, W - 1) * stride][lane];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < W) sum += v[j];
+  }
+  return sum;
+}
+
+// Steps st = 0 .. steps - 1 with SETS steps' loads in flight: load(st, set) loads, step(st, set)
+// computes and then calls its third argument, which loads the step SETS ahead into the set. In all
+// groups of SETS steps but the last two no load is under a condition: behind one, a wait for
+// an earlier load would have to wait for all.
+template <int SETS, class Load, class Step>
+__device__ __forceinline__ void pipeline(int steps, Load load, Step step) {
+  int st = 0;
+  for (; steps - st >= 2 * SETS; st += SETS) {
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) step(st + i, i, [&]() { load(st + i + SETS, i); });
+  }
+  if (steps - st > SETS) {
+#pragma unroll
+    for (int i = 0; i < SETS; ++i)
+      step(st + i, i, [&]() {
+        if (st + i + SETS < steps) load(st + i + SETS, i);
+      });
+    st += SETS;
+  }
+#pragma unroll
+  for (int i = 0; i < SETS; ++i)
+    if (st + i < steps) step(st + i, i, []() {});
 }
 
 // Columns n .. n + 3 of row m; v2: the second half's sums (SWIGLU); hv: load4 (RESID). The roundings
@@ -66,5 +105,9 @@ __device__ __forceinline__ void store4(const LinearArgs& a, int m, int n, f32x4 
 bool few_rows_served(const LinearArgs& a);
 bool few_rows_quantized(const LinearArgs& a);   // whether it takes this x in bf16
 int launch_few_rows(const LinearArgs& a, int epi, hipStream_t s);
+
+// fp8_mid.hip: up to 64 rows of x in codes.
+bool mid_rows_served(const LinearArgs& a, int epi);
+int launch_mid_rows(const LinearArgs& a, int epi, hipStream_t s);
 
 }  // namespace ko
