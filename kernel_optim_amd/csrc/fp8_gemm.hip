@@ -23,77 +23,84 @@ __device__ __forceinline__ i32x8 frag(const uint8_t* block, int lane) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-template <int I>
-__device__ __forceinline__ f32x4 mfma(i32x8 a, i32x8 b, f32x4 c, uint32_t sa, uint32_t sb) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, I, (int)sa, I, (int)sb);
+__device__ __forceinline__ void widen(i32x8 c, uint32_t b, bf16x8 (&out)[4]) {
+  const float s = __uint_as_float((b & 255u) << 23);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = fp8_to_bf16((uint32_t)c[2 * i], (uint32_t)c[2 * i + 1], s);
 }
 
-// acc += the 16 x 16 products of a block of W and one of x; byte I of sw and sx are their scales.
+// acc += the 16 x 16 products of a block of W and TM of x; byte I of the dwords are their scales.
 // WIDE: through bf16 (fp8_core.h).
-template <int I, bool WIDE>
-struct Frag;
-template <int I>
-struct Frag<I, false> {
-  i32x8 v;
-  uint32_t s;
-  __device__ __forceinline__ void load(const uint8_t* block, int lane, uint32_t scales) {
-    v = frag(block, lane);
-    s = scales;
-  }
-};
-template <int I>
-struct Frag<I, true> {
-  bf16x8 v[4];
-  __device__ __forceinline__ void load(const uint8_t* block, int lane, uint32_t scales) {
-    const i32x8 c = frag(block, lane);
-    const float sc = __uint_as_float(((scales >> (8 * I)) & 255u) << 23);
+template <int I, bool WIDE, int TM>
+__device__ __forceinline__ void multiply(i32x8 w, uint32_t sw, const i32x8 (&x)[TM],
+                                         const uint32_t (&sx)[TM], f32x4 (&acc)[TM]) {
+  if constexpr (!WIDE) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = fp8_to_bf16((uint32_t)c[2 * i], (uint32_t)c[2 * i + 1], sc);
-  }
-};
-template <int I>
-__device__ __forceinline__ f32x4 multiply(const Frag<I, false>& w, const Frag<I, false>& x, f32x4 c) {
-  return mfma<I>(w.v, x.v, c, w.s, x.s);
-}
-template <int I>
-__device__ __forceinline__ f32x4 multiply(const Frag<I, true>& w, const Frag<I, true>& x, f32x4 c) {
+    for (int j = 0; j < TM; ++j)
+      acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x[j], acc[j], 0, 0, I, (int)sw, I,
+                                                                (int)sx[j]);
+  } else {
+    bf16x8 f[4], v[4];
+    widen(w, sw >> (8 * I), f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], x.v[i], c, 0, 0, 0);
-  return c;
+    for (int j = 0; j < TM; ++j) {
+      widen(x[j], sx[j] >> (8 * I), v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[e], v[e], acc[j], 0, 0, 0);
+    }
+  }
 }
 
-template <int EPI, bool WIDE, int WN, int WM, int TN, int TM>
+// Waits until all but the N youngest loads of this wavefront (and its LDS reads) are done, then for
+// the workgroup.
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// WN x WM wavefronts of TN x TM tiles each; STAGES buffers of a step's blocks. With two, a step's loads
+// have the products of the step before to arrive in, and the compiler may mix their issue with those;
+// with more (small tiles, whose steps are shorter than a load) the waits are counted.
+template <int EPI, bool WIDE, int WN, int WM, int TN, int TM, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM) void gemm_kernel(LinearArgs a, int nblocks) {
   constexpr int W = WN * WM, NT = WN * TN, MT = WM * TM, CH = 2 * (NT + MT) / W;
   static_assert(CH * W == 2 * (NT + MT), "every wavefront loads as much");
   static_assert(EPI != EPI_SWIGLU || TN % 2 == 0, "a wavefront's tiles in twos");
-  __shared__ __attribute__((aligned(16))) uint8_t s_buf[2][(NT + MT) * FP8_BLOCK];
+  __shared__ __attribute__((aligned(16))) uint8_t s_buf[STAGES][(NT + MT) * FP8_BLOCK];
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int wn = wv % WN, wm = wv / WN;
   const int KB = fp8_blocks(a.K), Q = fp8_quads(a.K);
   const int nb = blockIdx.x % nblocks, mb = blockIdx.x / nblocks;
   const int n0 = nb * NT, m0 = mb * MT;   // this workgroup's first tiles
 
-  // tiles past the end: the last one, their results unused
+  // Addresses are uniform but for the lane's place in a block. Tiles past the end: the last one,
+  // their results unused.
   const uint8_t* src[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int c = wv * CH + i, t = c >> 1;
     const long long tile = t < NT ? min(n0 + t, a.wt - 1) : min(m0 + t - NT, a.xt - 1);
-    src[i] = (t < NT ? a.wc : a.xc) + tile * KB * FP8_BLOCK + (c & 1) * 1024 + 16 * lane;
+    src[i] = (t < NT ? a.wc : a.xc) + tile * KB * FP8_BLOCK + (c & 1) * 1024;
   }
-  auto stage = [&](int kb, int buf) {
+  auto stage = [&](int kb, int buf) {   // past the end: the last step again, unused
+    const int at = min(kb, KB - 1) * FP8_BLOCK;
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
-      load_lds(src[i] + (long long)kb * FP8_BLOCK, s_buf[buf] + (wv * CH + i) * 1024);
+    for (int i = 0; i < CH; ++i) load_lds(src[i] + at + 16 * lane, s_buf[buf] + (wv * CH + i) * 1024);
   };
-  const uint32_t *ws[TN], *xs[TM];
+  uint32_t sw[TN], sx[TM], next_w[TN], next_x[TM];   // a quad's scales, and the next one's
+  auto load_scales = [&](int q) {
+    q = min(q, Q - 1);   // past the end: unused
 #pragma unroll
-  for (int i = 0; i < TN; ++i)
-    ws[i] = a.ws + (long long)min(n0 + wn * TN + i, a.wt - 1) * Q * 16 + r;
+    for (int i = 0; i < TN; ++i)
+      next_w[i] = (a.ws + ((long long)min(n0 + wn * TN + i, a.wt - 1) * Q + q) * 16)[r];
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-    xs[i] = a.xs + (long long)min(m0 + wm * TM + i, a.xt - 1) * Q * 16 + r;
+    for (int i = 0; i < TM; ++i)
+      next_x[i] = (a.xs + ((long long)min(m0 + wm * TM + i, a.xt - 1) * Q + q) * 16)[r];
+  };
 
   f32x4 acc[TN][TM];
 #pragma unroll
@@ -101,27 +108,38 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_kernel(LinearArgs a, int nb
 #pragma unroll
     for (int j = 0; j < TM; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
 
-  stage(0, 0);
+  if constexpr (STAGES > 2) load_scales(0);
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) stage(i, i);
+  int buf = 0;   // of the step
   for (int q = 0; q < Q; ++q) {
-    uint32_t sw[TN], sx[TM];
+    if constexpr (STAGES == 2) load_scales(q);
 #pragma unroll
-    for (int i = 0; i < TN; ++i) sw[i] = ws[i][q * 16];
+    for (int i = 0; i < TN; ++i) sw[i] = next_w[i];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) sx[i] = xs[i][q * 16];
+    for (int i = 0; i < TM; ++i) sx[i] = next_x[i];
 #define KO_STEP(I)                                                                       \
   if (4 * q + I < KB) {                                                                  \
     const int kb = 4 * q + I;                                                            \
-    __syncthreads(); /* this step's blocks are there, the other buffer is read out */    \
-    if (kb + 1 < KB) stage(kb + 1, (I + 1) & 1);                                         \
-    const uint8_t* sb = s_buf[I & 1];                                                    \
-    Frag<I, WIDE> fw[TN], fx[TM];                                                        \
+    /* this step's blocks are there, and the last step's buffer is read out */           \
+    if constexpr (STAGES == 2) {                                                         \
+      __syncthreads();                                                                   \
+      if (kb + 1 < KB) stage(kb + 1, (I + 1) & 1);                                       \
+    } else {                                                                             \
+      wait_barrier<CH * (STAGES - 2)>();                                                 \
+      stage(kb + STAGES - 1, buf == 0 ? STAGES - 1 : buf - 1);                           \
+      if constexpr (I == 0) load_scales(q + 1);                                          \
+      __builtin_amdgcn_sched_barrier(0);                                                 \
+    }                                                                                    \
+    const uint8_t* sb = s_buf[STAGES == 2 ? I & 1 : buf];                                \
+    i32x8 w[TN], x[TM];                                                                  \
     _Pragma("unroll") for (int j = 0; j < TM; ++j)                                       \
-        fx[j].load(sb + (NT + wm * TM + j) * FP8_BLOCK, lane, sx[j]);                    \
+        x[j] = frag(sb + (NT + wm * TM + j) * FP8_BLOCK, lane);                          \
     _Pragma("unroll") for (int i = 0; i < TN; ++i)                                       \
-        fw[i].load(sb + (wn * TN + i) * FP8_BLOCK, lane, sw[i]);                         \
+        w[i] = frag(sb + (wn * TN + i) * FP8_BLOCK, lane);                               \
     _Pragma("unroll") for (int i = 0; i < TN; ++i)                                       \
-        _Pragma("unroll") for (int j = 0; j < TM; ++j)                                   \
-            acc[i][j] = multiply(fw[i], fx[j], acc[i][j]);                               \
+        multiply<I, WIDE, TM>(w[i], sw[i], x, sx, acc[i]);                               \
+    buf = buf == STAGES - 1 ? 0 : buf + 1;                                               \
   }
     KO_STEP(0)
     KO_STEP(1)
@@ -159,13 +177,39 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_kernel(LinearArgs a, int nb
   }
 }
 
+template <int EPI, bool WIDE, int WN, int WM, int TN, int TM, int STAGES>
+int launch_tiled(const LinearArgs& a, hipStream_t s) {
+  constexpr int NT = WN * TN, MT = WM * TM;
+  const int nb = (a.wt + NT - 1) / NT, mb = (a.xt + MT - 1) / MT;
+  if ((long long)nb * mb > 0x7fffffffll) return KO_ERANGE;
+  hipLaunchKernelGGL((gemm_kernel<EPI, WIDE, WN, WM, TN, TM, STAGES>), dim3(nb * mb),
+                     dim3(64 * WN * WM), 0, s, a, nb);
+  return KO_LAUNCH_STATUS();
+}
+
+// Workgroups of tiles of 16 t x 16 t columns and rows.
+long long groups(const LinearArgs& a, int t) {
+  return ((a.wt + t - 1ll) / t) * ((a.xt + t - 1ll) / t);
+}
+
+// The tile by what its rounds of workgroups take, in us of K = 2560 (a round of 256, 512 and 768
+// workgroups: one, two and three a CU):
+//   256 x 256: 40 a round                        (8192 x 6144: 120 us against 135, 128 x 128)
+//   128 x 128: 18 up to 256 workgroups, then 22.5 a round       (2048 x 19456: 114 against 123)
+//   64 x 64:   10.4 up to 256, 11.7 up to 512, then 15.5 a round    (128 x 6144: 10.5 against 18)
 template <int EPI>
 int launch(const LinearArgs& a, hipStream_t s) {
-  const int nb = (a.wt + 7) / 8, mb = (a.xt + 7) / 8;
-  if ((long long)nb * mb > 0x7fffffffll) return KO_ERANGE;
-  hipLaunchKernelGGL((gemm_kernel<EPI, EPI == EPI_F32, 2, 2, 4, 4>), dim3(nb * mb), dim3(256), 0, s,
-                     a, nb);
-  return KO_LAUNCH_STATUS();
+  if constexpr (EPI == EPI_F32) {
+    return launch_tiled<EPI, true, 2, 2, 4, 4, 2>(a, s);
+  } else {
+    const long long n16 = groups(a, 16), n8 = groups(a, 8), n4 = groups(a, 4);
+    const double t16 = 40.0 * ((n16 + 255) / 256);
+    const double t8 = n8 <= 256 ? 18.0 : 22.5 * ((n8 + 511) / 512);
+    const double t4 = n4 <= 256 ? 10.4 : n4 <= 512 ? 11.7 : 15.5 * ((n4 + 767) / 768);
+    if (t4 < t8 && t4 < t16) return launch_tiled<EPI, false, 2, 2, 2, 2, 3>(a, s);
+    if (t8 <= t16) return launch_tiled<EPI, false, 2, 2, 4, 4, 2>(a, s);
+    return launch_tiled<EPI, false, 4, 2, 4, 8, 2>(a, s);
+  }
 }
 
 }  // namespace

@@ -3,8 +3,9 @@
 // As for fewer rows a workgroup's 8 wavefronts share K and stream tiles of W, but every block of W
 // now meets 2 or 4 blocks of x: a wavefront holds the codes of its blocks of x in registers for the
 // whole launch (K = 2560, 64 rows: 96 of its 256), where loads of x between those of W would make
-// each wait for the weights ahead of it, and widens them as it multiplies. Longer rows do not fit:
-// they take x with W, block by block, several blocks ahead.
+// each wait for the weights ahead of it. Longer rows do not fit: they take x with W, block by
+// block, several blocks ahead. 2 tiles go through bf16 (fp8_core.h); 4 would spill the registers so
+// (64 rows of gate/up 36 us) and go to the matrix instruction as codes (19 us).
 #include "fp8_linear.h"
 
 namespace {

@@ -192,7 +192,8 @@ LINEAR = [(1, 16, 8), (1, 5000, 256), (16, 8203, 640), (4, 64, 3000), (9, 48, 97
           (1, 1, 128), (1, 2560, 4096), (2, 1000, 712), (3, 17, 136), (7, 130, 520),
           (16, 256, 2560), (17, 33, 1024), (33, 999, 264), (64, 512, 1152), (65, 130, 640),
           (20, 5000, 264), (32, 72, 9728), (50, 33, 12296), (61, 4200, 3080), (40, 4112, 2560),
-          (100, 300, 2568), (130, 640, 896), (257, 515, 384), (300, 1024, 2560)]
+          (100, 300, 2568), (130, 640, 896), (257, 515, 384), (300, 1024, 2560),
+          (1030, 4100, 712), (4133, 4800, 392)]
 
 
 @pytest.mark.parametrize("M,N,K", LINEAR)
