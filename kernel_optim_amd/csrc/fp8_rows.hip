@@ -8,33 +8,57 @@ namespace {
 
 using namespace ko;
 
-// The 16 values [k, k + 16) of a row as fp32; values from K on are zero. K is a multiple of 8
-// and rows are 16-byte aligned.
+// A lane's 2 x 16 values of a block's row (k: the first), packed as they come; values from K on are
+// zero. K is a multiple of 8 and rows are 16-byte aligned. No load is under a condition (what lies
+// past the end reads the row's beginning), so that many are on their way at once.
 template <bool F32IN>
-__device__ __forceinline__ void load16(const void* x, long long at, int k, int K, bool ok,
-                                       float (&v)[16]) {
+struct Raw {
+  static constexpr int L = F32IN ? 2 : 1;   // loads of 8 values
+  uint4 q[2][2][L];
+  __device__ __forceinline__ void load(const void* x, long long at, int k, int K) {
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    const bool in = ok && k + 8 * p < K;
-    if constexpr (F32IN) {
-      const float* s = static_cast<const float*>(x) + at + k + 8 * p;
-      const uint4 a = in ? ldg16(s) : make_uint4(0, 0, 0, 0);
-      const uint4 b = in ? ldg16(s + 4) : make_uint4(0, 0, 0, 0);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[8 * p + i] = __uint_as_float(w[i]);
-    } else {
-      const uint4 a = in ? ldg16(static_cast<const uint16_t*>(x) + at + k + 8 * p)
-                         : make_uint4(0, 0, 0, 0);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+      for (int p = 0; p < 2; ++p) {
+        const int e = k + 64 * j + 8 * p;
+        const long long o = at + (e < K ? e : 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[8 * p + 2 * i] = bf16lo(w[i]);
-        v[8 * p + 2 * i + 1] = bf16hi(w[i]);
+        for (int l = 0; l < L; ++l)
+          q[j][p][l] = F32IN ? ldg16(static_cast<const float*>(x) + o + 4 * l)
+                             : ldg16(static_cast<const uint16_t*>(x) + o);
       }
-    }
   }
-}
+  __device__ __forceinline__ void clear(int k, int K, bool ok) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        if (!ok || k + 64 * j + 8 * p >= K) {
+#pragma unroll
+          for (int l = 0; l < L; ++l) q[j][p][l] = make_uint4(0, 0, 0, 0);
+        }
+  }
+  __device__ __forceinline__ void unpack(float (&v)[2][16]) const {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+          const uint4 t = q[j][p][l];
+          const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (F32IN) {
+              v[j][8 * p + 4 * l + i] = __uint_as_float(w[i]);
+            } else {
+              v[j][8 * p + 2 * i] = bf16lo(w[i]);
+              v[j][8 * p + 2 * i + 1] = bf16hi(w[i]);
+            }
+          }
+        }
+  }
+};
 
 // One block's codes into the matrix; returns the row's scale byte.
 __device__ __forceinline__ uint32_t store_block(const float (&v)[2][16], uint8_t* block, int lane) {
@@ -61,60 +85,98 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ 
   const int row = fp8_row(t, r, rows, pair);
   const long long at = (long long)max(row, 0) * stride;
   uint32_t sc = 0;
+  Raw<F32IN> raw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) raw[i].load(x, at, (4 * q + i) * 128 + 16 * g, K);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int kb = 4 * q + i;
     if (kb < KB) {
       float v[2][16];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) load16<F32IN>(x, at, kb * 128 + 64 * j + 16 * g, K, row >= 0, v[j]);
+      raw[i].clear(kb * 128 + 16 * g, K, row >= 0);
+      raw[i].unpack(v);
       sc |= store_block(v, codes + (t * KB + kb) * FP8_BLOCK, lane) << (8 * i);
     }
   }
   if (g == 0) scales[(t * Q + q) * 16 + r] = sc;
 }
 
-constexpr int NORM_WAVES = 16, NORM_BLOCKS = 1024;   // K up to 131,072
+constexpr int NORM_BLOCKS = 1024;   // K up to 131,072
 
 // RMSNorm in front (bf16 rows): a workgroup takes a tile, sums the squares of its 16 rows in
-// fp32, and its wavefronts quantise bf16(nw * bf16(x * rstd)) block by block. The rows are read
-// twice, the second time from the caches (16 rows of 2560 values: 80 KB).
-__global__ __launch_bounds__(64 * NORM_WAVES) void quantize_norm_kernel(
+// fp32, and its wavefronts quantise bf16(nw * bf16(x * rstd)). R blocks a wavefront stay in
+// registers between the two; R = 0 (long rows) reads them again.
+template <int R>
+__global__ __launch_bounds__(1024) void quantize_norm_kernel(
     const uint16_t* __restrict__ x, long long stride, int rows, int K,
     const uint16_t* __restrict__ nw, float eps, uint8_t* __restrict__ codes,
     uint32_t* __restrict__ scales) {
   extern __shared__ float s_sq[];   // [blocks][16]
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, W = blockDim.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
   const int Q = fp8_quads(K), KB = fp8_blocks(K);
   const long long t = blockIdx.x;
   const int row = fp8_row(t, r, rows, false);
   const long long at = (long long)max(row, 0) * stride;
-  for (int kb = wv; kb < KB; kb += NORM_WAVES) {
+  Raw<false> raw[R ? R : 1];
+  auto fetch = [&](int i, int kb) {
+    raw[i].load(x, at, min(kb, KB - 1) * 128 + 16 * g, K);
+  };
+  auto squares = [&](int i, int kb) {
+    if (kb >= KB) return;
     float v[2][16];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) load16<false>(x, at, kb * 128 + 64 * j + 16 * g, K, row >= 0, v[j]);
+    raw[i].clear(kb * 128 + 16 * g, K, row >= 0);
+    raw[i].unpack(v);
     const float sq = fp8_square_sum(v);
     if (g == 0) s_sq[kb * 16 + r] = sq;
+  };
+  if constexpr (R) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) fetch(i, wv + i * W);
+#pragma unroll
+    for (int i = 0; i < R; ++i) squares(i, wv + i * W);
+  } else {
+    for (int kb = wv; kb < KB; kb += W) fetch(0, kb), squares(0, kb);
   }
   __syncthreads();
   float tot = 0.f;
   for (int kb = 0; kb < KB; ++kb) tot += s_sq[kb * 16 + r];
   const float rstd = row >= 0 ? rsqrtf(tot / (float)K + eps) : 0.f;   // eps may be 0
   uint8_t* sc = reinterpret_cast<uint8_t*>(scales);
-  for (int kb = wv; kb < 4 * Q; kb += NORM_WAVES) {
+  auto quantize = [&](int i, int kb) {
     uint32_t b = 0;
     if (kb < KB) {
-      float v[2][16], w[16];
+      float v[2][16];
+      Raw<false> gain;
+      gain.load(nw, 0, kb * 128 + 16 * g, K);
+      gain.clear(kb * 128 + 16 * g, K, row >= 0);   // padding rows stay zeros, with no sign
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        load16<false>(x, at, kb * 128 + 64 * j + 16 * g, K, row >= 0, v[j]);
-        load16<false>(nw, 0, kb * 128 + 64 * j + 16 * g, K, row >= 0, w);
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[j][i] = round_bf16(w[i] * round_bf16(v[j][i] * rstd));
-      }
+        for (int p = 0; p < 2; ++p) {
+          uint4& q = raw[i].q[j][p][0];
+          const uint4 w = gain.q[j][p][0];
+          q = make_uint4(fp8_norm2(q.x, w.x, rstd), fp8_norm2(q.y, w.y, rstd),
+                         fp8_norm2(q.z, w.z, rstd), fp8_norm2(q.w, w.w, rstd));
+        }
+      raw[i].unpack(v);
       b = store_block(v, codes + (t * KB + kb) * FP8_BLOCK, lane);
     }
-    if (g == 0) sc[((t * Q + (kb >> 2)) * 16 + r) * 4 + (kb & 3)] = (uint8_t)b;
+    if (g == 0 && kb < 4 * Q) sc[((t * Q + (kb >> 2)) * 16 + r) * 4 + (kb & 3)] = (uint8_t)b;
+  };
+  if constexpr (R) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) quantize(i, wv + i * W);
+    if (wv == 0)   // the last quad's padding
+      for (int kb = R * W; kb < 4 * Q; ++kb) quantize(0, kb);
+  } else {
+    for (int kb = wv; kb < 4 * Q; kb += W) {
+      if (kb < KB) {
+        fetch(0, kb);
+        raw[0].clear(kb * 128 + 16 * g, K, row >= 0);
+      }
+      quantize(0, kb);
+    }
   }
 }
 
@@ -269,9 +331,15 @@ int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K,
     return KO_LAUNCH_STATUS();
   }
   if (nw) {
-    hipLaunchKernelGGL(quantize_norm_kernel, dim3((unsigned)tiles), dim3(64 * NORM_WAVES),
-                       64 * fp8_blocks(K), s, static_cast<const uint16_t*>(x), stride, rows, K,
-                       static_cast<const uint16_t*>(nw), eps, c, sc);
+    const int KB = fp8_blocks(K);
+    const uint16_t *xb = static_cast<const uint16_t*>(x), *wb = static_cast<const uint16_t*>(nw);
+#define KO_NORM(R, WAVES)                                                                      \
+  hipLaunchKernelGGL(quantize_norm_kernel<R>, dim3((unsigned)tiles), dim3(64 * (WAVES)), 64 * KB, s, \
+                     xb, stride, rows, K, wb, eps, c, sc)
+    if (KB <= 32) KO_NORM(2, (KB + 1) / 2);
+    else if (KB <= 64) KO_NORM(4, (KB + 3) / 4);
+    else KO_NORM(0, 16);
+#undef KO_NORM
     return KO_LAUNCH_STATUS();
   }
   const long long units = tiles * fp8_quads(K);

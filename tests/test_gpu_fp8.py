@@ -42,7 +42,7 @@ def same_bytes(t, x, pair=False):
     assert torch.equal(t.scales.cpu(), scales)
 
 
-SHAPES = [(1, 8), (1, 128), (3, 136), (16, 512), (17, 520), (33, 2560), (100, 1048), (5, 9728)]
+SHAPES = [(300, 8), (321, 264), (270, 2176), (257, 4096), (259, 9736), (1, 8), (1, 128), (3, 136), (16, 512), (17, 520), (33, 2560), (100, 1048), (5, 9728)]
 
 
 @pytest.mark.parametrize("n,K", SHAPES)
@@ -56,7 +56,7 @@ def test_quantize_and_read(dev, n, K, dtype):
     assert torch.equal(out.cpu(), O.held(x).to(F32).to(dtype))
 
 
-@pytest.mark.parametrize("n,K", [(2, 8), (32, 256), (34, 136), (1000, 520)])
+@pytest.mark.parametrize("n,K", [(2, 8), (32, 256), (34, 136), (1000, 520), (602, 2200)])
 def test_pairs(dev, n, K):
     x = rows(n, n, K).to(BF16)
     t = fp8_quantize(x.to(dev), pair=True)
@@ -118,7 +118,8 @@ def test_blocks_that_hold_no_numbers(dev):
 
 
 @pytest.mark.parametrize("n,K", [(1, 8), (1, 2560), (5, 136), (16, 4096), (19, 2568), (64, 9728),
-                                 (3, 16384)])
+                                 (3, 16384), (300, 8), (257, 2560), (261, 4096), (259, 712),
+                                 (300, 8192), (257, 8704)])
 def test_quantize_behind_a_norm(dev, n, K):
     """The row's sum of squares in fp32 moves x * rstd by up to (K + 4) 2^-24 of itself, which may
     move a bf16 rounding, and that a code; rows whose norm is a power of two by construction
