@@ -7,13 +7,16 @@
 // bits: sums of up to 2^20 of them are exact in 64 bits in any order, so atomics and splits of a row do
 // not show in the result. A token of probability below 2^-43 of the largest has mass 0.
 //
+// Three launches, the first two of which cut a row into chunks, as does the third:
 // - maxima: the largest logit of each chunk of a row and its first index (greedy rows end here).
-// - histogram: tokens by z = (max - x) log2(e) / T in 2048 bins over 44 octaves, counts and masses
-//   (a row with a small top-k takes counts only: no exp for its whole vocabulary), first in LDS, then
-//   added to the row's in memory. The last workgroup of a row finishes it: a running sum over the
-//   bins gives the bin of a place, the bin's tokens are gathered from the row (in the caches by
-//   now), sorted in LDS, and the place lies where their running sum says. A bin of more tokens
-//   than LDS is given (equal logits, say) is narrowed down digit by digit of (logit, index) instead.
+// - bins: tokens by z = (max - x) log2(e) / T in 2048 bins over 44 octaves, masses (a row with a small
+//   top-k counts only: no exp for its whole vocabulary) in LDS, then added to the row's in memory. A
+//   row's last workgroup forms running sums over the bins, which give the bins in which the cuts and
+//   the drawn token can lie: a cut moves the places behind it by no more than its bin's mass.
+// - draw: the tokens of these bins, of all chunks, meet in one list; a row's last workgroup sorts it by
+//   (falling logit, index) and finds the exact places in its running masses. Where the list is too
+//   long for LDS (thousands of equal logits, say) it narrows every place down over the whole row, 8 bits
+//   of (logit, index) at a time.
 // A row that is one chunk does all of it in one workgroup and one launch.
 #include "ko_common.h"
 
@@ -23,13 +26,24 @@ using namespace ko;
 
 typedef unsigned long long u64;
 
-constexpr int NT = 1024, NW = NT / 64;
+constexpr int NT = 512, NW = NT / 64;
 constexpr int BINS = 2048, CAP = 2048;
 constexpr int SHIFT = 42;             // a mass of 1 is 2^42: 2^20 tokens sum below 2^63
 constexpr float ZMAX = SHIFT + 2;     // octaves: masses from here on are 0
 constexpr float PER_OCTAVE = BINS / ZMAX;
 constexpr int K_COUNTED = 1024;       // top-k up to here: counts alone find the kept tokens
+constexpr int SPANS = 3;
 constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
+
+// What a row's places need of its bins, as picked from the running sums.
+struct Picked {
+  u64 before[SPANS];          // the mass, and the count, before each span of bins
+  u64 all, minp;              // the mass of all tokens, and of those that min_p keeps (not of counted rows)
+  uint32_t count[SPANS];
+  float hi[SPANS], lo[SPANS];    // the spans' logits, falling; lo > hi: no span
+  uint32_t total;             // tokens in the bins
+  uint32_t slow;              // counted rows whose k-th token's bin reaches past the list
+};
 
 struct Rows {
   const void* x;
@@ -41,9 +55,12 @@ struct Rows {
   int top_k1;
   long long* ids;
   float* logp;
-  u64* best;      // [B][chunks]: ordered logit << 32 | ~index
-  u64* mass;      // [B][BINS + 1]: the last is min-p's
-  uint32_t* count;   // [B][BINS + 1]: the last is the arrival counter
+  // scratch, [B] each
+  u64* best;         // [chunks]: ordered logit << 32 | ~index
+  u64* mass;         // [BINS + 1]: the last is min-p's
+  u64* list;         // [CAP]
+  Picked* picked;
+  uint32_t* count;   // [BINS + 4]: the last are two arrival counters and the list's length
 };
 
 // Larger floats have larger patterns; -0 is 0. NaN does not come here.
@@ -88,7 +105,8 @@ struct Row {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // f(index, logit) for the elements of the vectors [v0, v1), U loads of a thread at a time.
+  // f(index, logit) for the elements of the vectors [v0, v1), U loads of a thread at a time; elements
+  // outside the row are NaN.
   template <int U, class F>
   __device__ __forceinline__ void each(int v0, int v1, F f) const {
     for (int v = v0 + threadIdx.x; v < v1; v += U * NT) {
@@ -141,7 +159,7 @@ struct Scale {
     invd = LOG2E / (double)t;
     inv = fminf((float)(2 * invd), 3.0e38f);
   }
-  // -1: a token of mass 0 (a logit of -infinity or NaN among them).
+  // Never falls as x falls; -1: a token of mass 0 (a logit of -infinity or NaN among them).
   __device__ __forceinline__ int bin(float x) const {
     if (top == __builtin_huge_valf()) return x == top ? 0 : -1;
     const float z = fmaf(x, -0.5f, 0.5f * top) * inv;   // falls with x, roundings and all
@@ -150,24 +168,47 @@ struct Scale {
   __device__ __forceinline__ double octaves(float x) const {
     return x == top ? 0.0 : ((double)top - (double)x) * invd;
   }
-  __device__ __forceinline__ u64 mass(float x, double* w) const {
-    *w = exp2(-octaves(x));
-    return (u64)(*w * (double)(1ull << SHIFT) + 0.5);
+  // 2^SHIFT exp((x - top) / T) within 2^-46 of itself: 2^-z = 2^-n exp(-(z - n) ln 2), |z - n| <= 1/2, by
+  // the exponential's series (the first term left out, 0.347^12 / 12!, is 2^-47).
+  __device__ __forceinline__ double scaled(float x) const {
+    const double z = fmin(octaves(x), 2.0 * ZMAX), n = __builtin_rint(z), y = (n - z) * LN2;
+    double p = 1.0 / 39916800;
+    p = fma(p, y, 1.0 / 3628800);
+    p = fma(p, y, 1.0 / 362880);
+    p = fma(p, y, 1.0 / 40320);
+    p = fma(p, y, 1.0 / 5040);
+    p = fma(p, y, 1.0 / 720);
+    p = fma(p, y, 1.0 / 120);
+    p = fma(p, y, 1.0 / 24);
+    p = fma(p, y, 1.0 / 6);
+    p = fma(p, y, 0.5);
+    p = fma(p, y, 1.0);
+    p = fma(p, y, 1.0);
+    return __builtin_ldexp(p, SHIFT - (int)n);
   }
+  // The nearest whole number of one below 2^52: the last bits of its sum with 2^52.
+  static __device__ __forceinline__ u64 whole(double v) {
+    return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ u64 mass(float x) const { return whole(scaled(x)); }
 };
 
 struct Shared {
   uint32_t count[BINS];   // of each bin, then running
   u64 mass[BINS];
-  u64 key[CAP], cum[CAP];
   u64 part[NW];
   u64 minp;
-  u64 found, found_mass;
+  int at;
+};
+struct List {
+  u64 key[CAP], cum[CAP];
+  u64 part[NW];
+  u64 base[SPANS];
+  int first[SPANS];
+  u64 found, found_mass, minp;
   uint32_t n;
   int at;
-  u64 best;
 };
-
 __device__ __forceinline__ u64 shfl_up(u64 v, int d) {
   return ((u64)(uint32_t)__shfl_up((int)(v >> 32), d) << 32) | (uint32_t)__shfl_up((int)(uint32_t)v, d);
 }
@@ -206,34 +247,33 @@ __device__ u64 block_max(u64 v, u64* part) {
 
 template <bool F32>
 __device__ u64 best_of(const Row<F32>& row, int v0, int v1, u64* part) {
-  u64 best = 0;   // nothing: no logit is a number above -infinity
-  row.template each<4>(v0, v1, [&](int i, float x) {
-    if (x > -__builtin_huge_valf()) {
-      const u64 c = (u64)ordered(x) << 32 | (uint32_t)~i;
-      best = c > best ? c : best;
-    }
+  float best = -__builtin_huge_valf();
+  int at = -1;   // nothing: no logit is a number above -infinity
+  row.template each<4>(v0, v1, [&](int i, float x) {   // a thread's indexes rise
+    if (x > best) best = x, at = i;
   });
-  return block_max(best, part);
+  return block_max(at < 0 ? 0 : (u64)ordered(best) << 32 | (uint32_t)~at, part);
 }
 
 // Counts and masses of the vectors' tokens by bin, into s.
 template <bool F32>
-__device__ void histogram(const Row<F32>& row, int v0, int v1, const Scale& sc, bool masses, float mp,
-                          Shared& s) {
+__device__ void histogram(const Row<F32>& row, int v0, int v1, const Scale& sc, bool counts,
+                          bool masses, float mp, Shared& s) {
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += NT) s.count[i] = 0, s.mass[i] = 0;
   if (threadIdx.x == 0) s.minp = 0;
   __syncthreads();
   u64 kept = 0;
-  row.template each<4>(v0, v1, [&](int, float x) {
+  const double least = (double)mp * (double)(1ull << SHIFT);
+  row.template each<2>(v0, v1, [&](int, float x) {
     const int b = sc.bin(x);
     if (b < 0) return;
-    atomicAdd(&s.count[b], 1u);
+    if (counts) atomicAdd(&s.count[b], 1u);
     if (masses) {
-      double w;
-      const u64 m = sc.mass(x, &w);
+      const double w = sc.scaled(x);
+      const u64 m = Scale::whole(w);
       atomicAdd(&s.mass[b], m);
-      if (w >= (double)mp) kept += m;
+      if (w >= least) kept += m;
     }
   });
   if (masses && mp > 0.f) atomicAdd(&s.minp, kept);
@@ -242,64 +282,22 @@ __device__ void histogram(const Row<F32>& row, int v0, int v1, const Scale& sc, 
 
 // Bins to running sums.
 __device__ void accumulate(Shared& s) {
-  const int t = threadIdx.x;
-  const uint32_t c0 = s.count[2 * t], c1 = s.count[2 * t + 1];
-  const u64 m0 = s.mass[2 * t], m1 = s.mass[2 * t + 1];
-  const u64 c = running(c0 + c1, s.part), m = running(m0 + m1, s.part);
-  s.count[2 * t] = (uint32_t)c - c1, s.count[2 * t + 1] = (uint32_t)c;
-  s.mass[2 * t] = m - m1, s.mass[2 * t + 1] = m;
-  __syncthreads();
-}
-
-// The tokens of bins [b0, b1] into s.key, sorted by (falling logit, index); s.cum: their running
-// mass. At most CAP.
-template <bool F32>
-__device__ void gather(const Row<F32>& row, const Scale& sc, int b0, int b1, Shared& s) {
-  __syncthreads();
-  if (threadIdx.x == 0) s.n = 0;
-  __syncthreads();
-  row.template each<4>(0, row.vectors, [&](int i, float x) {
-    const int b = sc.bin(x);
-    if (b >= b0 && b <= b1) {
-      const uint32_t at = atomicAdd(&s.n, 1u);
-      if (at < CAP) s.key[at] = (u64)~ordered(x) << 32 | (uint32_t)i;
-    }
-  });
-  __syncthreads();
-  const int n = min((int)s.n, CAP);
-  int m = 64;
-  while (m < n) m <<= 1;
-  for (int i = n + threadIdx.x; i < m; i += NT) s.key[i] = ~0ull;
-  __syncthreads();
-  for (int size = 2; size <= m; size <<= 1)
-    for (int d = size >> 1; d > 0; d >>= 1) {
-      if ((int)threadIdx.x < m / 2) {
-        const int i = ((int)threadIdx.x / d) * 2 * d + (int)threadIdx.x % d;
-        const u64 a = s.key[i], b = s.key[i + d];
-        if ((a > b) == ((i & size) == 0)) s.key[i] = b, s.key[i + d] = a;
-      }
-      __syncthreads();
-    }
-  u64 w[2];
-  double unused;
+  constexpr int EACH = BINS / NT;
+  const int t = threadIdx.x * EACH;
+  u64 c = 0, m = 0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = 2 * threadIdx.x + j;
-    w[j] = i < n ? sc.mass(unordered(~(uint32_t)(s.key[i] >> 32)), &unused) : 0;
+  for (int i = 0; i < EACH; ++i) c += s.count[t + i], m += s.mass[t + i];
+  u64 rc = running(c, s.part) - c, rm = running(m, s.part) - m;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    rc += s.count[t + i], rm += s.mass[t + i];
+    s.count[t + i] = (uint32_t)rc, s.mass[t + i] = rm;
   }
-  const u64 c = running(w[0] + w[1], s.part);
-  s.cum[2 * threadIdx.x] = c - w[1], s.cum[2 * threadIdx.x + 1] = c;
   __syncthreads();
 }
 
-struct Place {
-  u64 key, mass;   // the token, and the mass up to and with it
-};
-
-// The first token of the order at which the count or the mass reaches target >= 1 (the caller sees
-// to it that one does).
-template <bool F32>
-__device__ Place find(const Row<F32>& row, const Scale& sc, bool by_count, u64 target, Shared& s) {
+// The first bin at which the running count or mass reaches target (one does).
+__device__ int bin_of(bool by_count, u64 target, Shared& s) {
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += NT) {
     const u64 here = by_count ? s.count[i] : s.mass[i];
@@ -307,22 +305,206 @@ __device__ Place find(const Row<F32>& row, const Scale& sc, bool by_count, u64 t
     if (here >= target && before < target) s.at = i;
   }
   __syncthreads();
-  const int b = s.at;
-  const uint32_t c0 = b ? s.count[b - 1] : 0;
-  const u64 m0 = b ? s.mass[b - 1] : 0;
-  const int n = (int)(s.count[b] - c0);
-  if (n <= CAP) {
-    gather(row, sc, b, b, s);
-    for (int i = threadIdx.x; i < n; i += NT) {
-      const u64 here = by_count ? c0 + i + 1 : m0 + s.cum[i];
-      const u64 before = by_count ? c0 + i : m0 + (i ? s.cum[i - 1] : 0);
-      if (here >= target && before < target) s.found = s.key[i], s.found_mass = m0 + s.cum[i];
+  return s.at;
+}
+
+// u's place in a kept mass, and top-p's in one: 1 and more, at most the mass. Neither falls as the
+// mass rises.
+__device__ __forceinline__ u64 draw(float u, u64 kept) {
+  const double t = (double)u * (double)kept;
+  const u64 target = t > 0.0 ? (u64)fmin(t, (double)kept) + 1 : 1;   // u that is no number: 0
+  return target < kept ? target : kept;
+}
+__device__ __forceinline__ u64 nucleus(float p, u64 mass) {
+  const double t = ceil((double)p * (double)mass);
+  const u64 target = t > 1.0 ? (u64)t : 1;
+  return target < mass ? target : mass;
+}
+__device__ __forceinline__ u64 least_kept(u64 minp) {   // nothing reaches a min_p above 1: the first token
+  return minp ? minp : 1ull << SHIFT;
+}
+
+// The bounds of the logits of bins [b0, b1]: of all numbers in order the first and the last, by
+// halving; by one thread each.
+__device__ float span_end(const Scale& sc, int b0, int b1, bool low) {
+  uint32_t lo = ordered(-__builtin_huge_valf()), hi = ordered(sc.top);   // bin(lo) < 0 <= bin(hi)
+  // low: the least logit of a bin up to b1; else the largest of a bin from b0 on (or lo's, none)
+  if (!low && b0 == 0) return sc.top;
+  const int limit = low ? b1 : b0 - 1;   // the least logit of a bin up to limit
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    const int b = sc.bin(unordered(mid));
+    if (b >= 0 && b <= limit) hi = mid;
+    else lo = mid;
+  }
+  return unordered(low ? hi : hi - 1);
+}
+
+// Which bins a row's places can lie in, from running sums in s (counts only if counted).
+__device__ void pick(const Settings& st, const Scale& sc, Shared& s, Picked* out) {
+  const uint32_t total = s.count[BINS - 1];
+  // spans of bins [f, l] for the places of top-k, top-p and the draw, in falling order of bins; l < f: none
+  int kf = 1, kl = 0, pf = 1, pl = 0, uf = 1, ul = 0;
+  uint32_t slow = 0;
+  if (st.counted()) {
+    kf = 0, kl = bin_of(true, min((uint32_t)st.k, total), s);
+    slow = s.count[kl] > CAP;
+  } else {
+    u64 lo = s.mass[BINS - 1], hi = lo;   // what the kept mass lies between
+    auto within = [&](int f, int l) {
+      hi = s.mass[l];
+      lo = (f ? s.mass[f - 1] : 0) + 1;
+      lo = lo < hi ? lo : hi;
+    };
+    if (st.k && (uint32_t)st.k < total) {
+      kf = kl = bin_of(true, (u64)st.k, s);
+      within(kf, kl);
+    }
+    if (st.p < 1.f) {
+      pf = bin_of(false, nucleus(st.p, lo), s), pl = bin_of(false, nucleus(st.p, hi), s);
+      within(pf, pl);
+    }
+    if (st.mp > 0.f) {
+      const u64 m = least_kept(s.minp);
+      lo = lo < m ? lo : m, hi = hi < m ? hi : m;
+    }
+    uf = bin_of(false, draw(st.u, lo), s), ul = bin_of(false, draw(st.u, hi), s);
+    // spans that meet become one: a token is gathered once
+    if (pf <= pl && ul >= pf) pf = min(pf, uf), uf = 1, ul = 0;
+    if (kf <= kl && pf <= pl && pl >= kf) kf = min(kf, pf), pf = 1, pl = 0;
+    if (kf <= kl && uf <= ul && ul >= kf) kf = min(kf, uf), uf = 1, ul = 0;
+  }
+  const int t = threadIdx.x;
+  if (t < SPANS) {
+    const int f = t == 0 ? kf : t == 1 ? pf : uf, l = t == 0 ? kl : t == 1 ? pl : ul;
+    out->hi[t] = f <= l ? span_end(sc, f, l, false) : 0.f;
+    out->lo[t] = f <= l ? span_end(sc, f, l, true) : 1.f;
+    out->before[t] = f <= l && f ? s.mass[f - 1] : 0;
+    out->count[t] = f <= l && f ? s.count[f - 1] : 0;
+  }
+  if (t == 0) out->all = s.mass[BINS - 1], out->minp = s.minp, out->total = total, out->slow = slow;
+}
+
+// The row's tokens of the spans among the vectors, into the list of this workgroup.
+template <bool F32>
+__device__ void gather(const Row<F32>& row, int v0, int v1, const Picked& p, List& l) {
+  __syncthreads();
+  if (threadIdx.x == 0) l.n = 0;
+  __syncthreads();
+  const float h0 = p.hi[0], h1 = p.hi[1], h2 = p.hi[2], l0 = p.lo[0], l1 = p.lo[1], l2 = p.lo[2];
+  row.template each<4>(v0, v1, [&](int i, float x) {
+    if ((x >= l0 && x <= h0) || (x >= l1 && x <= h1) || (x >= l2 && x <= h2)) {
+      const uint32_t at = atomicAdd(&l.n, 1u);
+      if (at < CAP) l.key[at] = (u64)~ordered(x) << 32 | (uint32_t)i;
+    }
+  });
+  __syncthreads();
+}
+
+// l.key[0 .. n) in rising order: by falling logit, then index.
+__device__ void sort(List& l, int n) {
+  int m = 64;
+  while (m < n) m <<= 1;
+  for (int i = n + threadIdx.x; i < m; i += NT) l.key[i] = ~0ull;
+  __syncthreads();
+  for (int size = 2; size <= m; size <<= 1)
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      for (int t = threadIdx.x; t < m / 2; t += NT) {
+        const int i = 2 * t - (t & (d - 1));   // t / d * 2 d + t % d
+        const u64 a = l.key[i], b = l.key[i + d];
+        if ((a > b) == ((i & size) == 0)) l.key[i] = b, l.key[i + d] = a;
+      }
+      __syncthreads();
+    }
+}
+
+__device__ __forceinline__ float logit_of(u64 key) { return unordered(~(uint32_t)(key >> 32)); }
+
+__device__ void result(const Rows& r, long long b, const Scale& sc, u64 key, u64 kept) {
+  if (threadIdx.x) return;
+  r.ids[b] = (uint32_t)key;
+  if (r.logp) {
+    const double octaves = sc.octaves(logit_of(key));
+    r.logp[b] = (float)(-octaves * LN2 - log((double)kept) + SHIFT * LN2);
+  }
+}
+
+// The row's token from the sorted list of all the spans' tokens.
+__device__ void finish(const Rows& r, long long b, const Settings& st, const Scale& sc,
+                       const Picked& p, List& l, int n) {
+  sort(l, n);
+  constexpr int EACH = CAP / NT;
+  const int t = threadIdx.x * EACH;
+  u64 w[EACH], sum = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    w[i] = t + i < n ? sc.mass(logit_of(l.key[t + i])) : 0;
+    sum += w[i];
+  }
+  u64 run = running(sum, l.part) - sum;
+  // where each span begins: what its tokens' masses and places lack of the row's
+  auto span_of = [&](u64 key) {
+    const float x = logit_of(key);
+    return x >= p.lo[0] && x <= p.hi[0] ? 0 : x >= p.lo[1] && x <= p.hi[1] ? 1 : 2;
+  };
+  if (threadIdx.x == 0) l.minp = 0;
+  __syncthreads();
+  u64 kept_minp = 0;
+  const double least = (double)st.mp * (double)(1ull << SHIFT);
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (t + i >= n) break;
+    const int j = span_of(l.key[t + i]);
+    if (t + i == 0 || span_of(l.key[t + i - 1]) != j) l.base[j] = p.before[j] - run, l.first[j] = t + i;
+    run += w[i];
+    l.cum[t + i] = run;
+    if (sc.scaled(logit_of(l.key[t + i])) >= least) kept_minp += w[i];
+  }
+  if (st.counted() && st.mp > 0.f) atomicAdd(&l.minp, kept_minp);
+  __syncthreads();
+  auto place = [&](bool by_count, u64 target) {   // l.found, l.found_mass: the token that reaches it
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (t + i >= n) break;
+      const int j = span_of(l.key[t + i]);
+      const u64 mass = l.cum[t + i] + l.base[j], here = by_count ? p.count[j] + (t + i - l.first[j]) + 1 : mass;
+      if (here >= target && here - (by_count ? 1 : w[i]) < target)
+        l.found = l.key[t + i], l.found_mass = mass;
     }
     __syncthreads();
-    return {s.found, s.found_mass};
+  };
+  u64 kept;
+  if (st.k && ((uint32_t)st.k < p.total || st.counted())) {
+    place(true, min((uint32_t)st.k, p.total));
+    kept = l.found_mass;
+  } else {
+    kept = p.all;
   }
-  // 8 bits of the key at a time, over the row; s.cum and s.key hold the digit's masses and counts
-  u64 prefix = 0, known = 0, count = c0, mass = m0;
+  if (st.p < 1.f) {
+    place(false, nucleus(st.p, kept));
+    kept = l.found_mass;
+  }
+  if (st.mp > 0.f) {
+    const u64 m = least_kept(st.counted() ? l.minp : p.minp);
+    kept = m < kept ? m : kept;
+  }
+  place(false, draw(st.u, kept));
+  result(r, b, sc, l.found, kept);
+}
+
+struct Place {
+  u64 key, mass;   // the token, and the mass up to and with it
+};
+
+// The first token of the order at which the count or the mass reaches target, over the whole row: its
+// bin from the running sums in s, then 8 bits of its key at a time (counts and masses of the digits
+// in l).
+template <bool F32>
+__device__ Place narrow(const Row<F32>& row, const Scale& sc, bool by_count, u64 target, Shared& s,
+                        List& l) {
+  const int b = bin_of(by_count, target, s);
+  u64 prefix = 0, known = 0, count = b ? s.count[b - 1] : 0, mass = b ? s.mass[b - 1] : 0;
   for (int shift = 56; shift >= 0; shift -= 8) {
     if (!F32 && (shift == 32 || shift == 40)) {
       // a bf16 logit's lower half is zeros: in the key ones, of a negative logit zeros
@@ -331,116 +513,52 @@ __device__ Place find(const Row<F32>& row, const Scale& sc, bool by_count, u64 t
       continue;
     }
     __syncthreads();
-    if (threadIdx.x < 256) s.cum[threadIdx.x] = s.key[threadIdx.x] = 0;
+    if (threadIdx.x < 256) l.cum[threadIdx.x] = l.key[threadIdx.x] = 0;
     __syncthreads();
-    row.template each<4>(0, row.vectors, [&](int i, float x) {
+    row.template each<2>(0, row.vectors, [&](int i, float x) {
       if (sc.bin(x) != b) return;
       const u64 key = (u64)~ordered(x) << 32 | (uint32_t)i;
       if ((key & known) != prefix) return;
-      double w;
       const int digit = (int)(key >> shift) & 255;
-      atomicAdd(&s.key[digit], 1ull);
-      atomicAdd(&s.cum[digit], sc.mass(x, &w));
+      atomicAdd(&l.key[digit], 1ull);
+      atomicAdd(&l.cum[digit], sc.mass(x));
     });
     __syncthreads();
-    const u64 c = threadIdx.x < 256 ? s.key[threadIdx.x] : 0, m = threadIdx.x < 256 ? s.cum[threadIdx.x] : 0;
-    const u64 rc = count + running(c, s.part), rm = mass + running(m, s.part);
+    const bool in = threadIdx.x < 256;
+    const u64 c = in ? l.key[threadIdx.x] : 0, m = in ? l.cum[threadIdx.x] : 0;
+    const u64 rc = count + running(c, l.part), rm = mass + running(m, l.part);
     const u64 here = by_count ? rc : rm, before = by_count ? rc - c : rm - m;
-    if (threadIdx.x < 256 && here >= target && before < target) {
-      s.at = threadIdx.x;
-      s.found = rc - c, s.found_mass = rm - m;
-    }
+    if (in && here >= target && before < target) l.at = threadIdx.x, l.found = rc - c, l.found_mass = rm - m;
     __syncthreads();
-    const u64 digit = (u64)s.at;
-    prefix |= digit << shift, known |= 0xffull << shift;
-    count = s.found, mass = s.found_mass;
+    prefix |= (u64)l.at << shift, known |= 0xffull << shift;
+    count = l.found, mass = l.found_mass;
   }
-  double w;
-  const u64 own = sc.mass(unordered(~(uint32_t)(prefix >> 32)), &w);
-  return {prefix, mass + own};
+  return {prefix, mass + sc.mass(logit_of(prefix))};
 }
 
-// u's place in a kept mass.
-__device__ __forceinline__ u64 draw(float u, u64 kept) {
-  const double t = (double)u * (double)kept;
-  const u64 target = t > 0.0 ? (u64)fmin(t, (double)kept) + 1 : 1;   // u that is no number: 0
-  return target < kept ? target : kept;
-}
-
-__device__ __forceinline__ u64 nucleus(float p, u64 mass) {
-  const double t = ceil((double)p * (double)mass);
-  const u64 target = t > 1.0 ? (u64)t : 1;
-  return target < mass ? target : mass;
-}
-
-__device__ void result(const Rows& r, long long b, const Scale& sc, u64 key, u64 kept) {
-  if (threadIdx.x) return;
-  r.ids[b] = (uint32_t)key;
-  if (r.logp) {
-    const float x = unordered(~(uint32_t)(key >> 32));
-    r.logp[b] = (float)(-sc.octaves(x) * LN2 - log((double)kept) + SHIFT * LN2);
-  }
-}
-
-// The row's token from its bins (counts and, unless counted, masses) in s.
+// The row's token without a list, from running sums in s.
 template <bool F32>
-__device__ void finish(const Rows& r, long long b, const Row<F32>& row, const Settings& st,
-                       const Scale& sc, Shared& s) {
-  accumulate(s);
-  const uint32_t total = s.count[BINS - 1];
-  if (st.counted()) {
-    const uint32_t k = min((uint32_t)st.k, total);
-    for (int i = threadIdx.x; i < BINS; i += NT)
-      if (s.count[i] >= k && (i ? s.count[i - 1] : 0) < k) s.at = i;
-    __syncthreads();
-    const int last = s.at;
-    if (s.count[last] <= CAP) {
-      // every token down to the k-th's bin, in order: all places are in s.cum
-      gather(row, sc, 0, last, s);
-      u64 kept = s.cum[k - 1];
-      if (st.p < 1.f) {
-        const u64 target = nucleus(st.p, kept);
-        for (int i = threadIdx.x; i < (int)k; i += NT)
-          if (s.cum[i] >= target && (i ? s.cum[i - 1] : 0) < target) s.found_mass = s.cum[i];
-        __syncthreads();
-        kept = s.found_mass;
-      }
-      if (st.mp > 0.f) {
-        double w = 1.0, w1 = 0.0;
-        for (int i = threadIdx.x; i < (int)k; i += NT) {
-          sc.mass(unordered(~(uint32_t)(s.key[i] >> 32)), &w);
-          if (i + 1 < (int)k) sc.mass(unordered(~(uint32_t)(s.key[i + 1] >> 32)), &w1);
-          else w1 = -1.0;
-          if ((w >= (double)st.mp || i == 0) && !(w1 >= (double)st.mp)) s.minp = s.cum[i];
-        }
-        __syncthreads();
-        kept = s.minp < kept ? s.minp : kept;
-      }
-      const u64 target = draw(st.u, kept);
-      for (int i = threadIdx.x; i < (int)k; i += NT)
-        if (s.cum[i] >= target && (i ? s.cum[i - 1] : 0) < target) s.found = s.key[i];
-      __syncthreads();
-      result(r, b, sc, s.found, kept);
-      return;
-    }
-    histogram(row, 0, row.vectors, sc, true, st.mp, s);
+__device__ void finish_slowly(const Rows& r, long long b, const Row<F32>& row, const Settings& st,
+                              const Scale& sc, Shared& s, List& l) {
+  if (st.counted()) {   // its masses, too
+    histogram(row, 0, row.vectors, sc, true, true, st.mp, s);
     accumulate(s);
   }
   u64 kept = s.mass[BINS - 1];
-  if (st.k && (uint32_t)st.k < total) kept = find(row, sc, true, (u64)st.k, s).mass;
-  if (st.p < 1.f) kept = find(row, sc, false, nucleus(st.p, kept), s).mass;
+  if (st.k && (uint32_t)st.k < s.count[BINS - 1]) kept = narrow(row, sc, true, (u64)st.k, s, l).mass;
+  if (st.p < 1.f) kept = narrow(row, sc, false, nucleus(st.p, kept), s, l).mass;
   if (st.mp > 0.f) {
-    const u64 least = s.minp ? s.minp : 1ull << SHIFT;   // nothing reaches min_p > 1: the first token
-    kept = least < kept ? least : kept;
+    const u64 m = least_kept(s.minp);
+    kept = m < kept ? m : kept;
   }
-  const Place at = find(row, sc, false, draw(st.u, kept), s);
+  const Place at = narrow(row, sc, false, draw(st.u, kept), s, l);
   result(r, b, sc, at.key, kept);
 }
 
 // What needs no more than the row's best; true if that was all.
-__device__ bool decided(const Rows& r, long long b, const Settings& st, u64 best) {
+__device__ bool decided(const Rows& r, long long b, const Settings& st, u64 best, bool write) {
   if (best && !st.first()) return false;
-  if (threadIdx.x == 0) {
+  if (write && threadIdx.x == 0) {
     r.ids[b] = best ? (long long)(uint32_t)~(uint32_t)best : -1;
     if (r.logp) r.logp[b] = best ? 0.f : -__builtin_huge_valf();
   }
@@ -450,37 +568,55 @@ __device__ bool decided(const Rows& r, long long b, const Settings& st, u64 best
 template <bool F32>
 __global__ __launch_bounds__(NT) void sample_kernel(Rows r) {
   __shared__ Shared s;
+  __shared__ List l;
+  __shared__ Picked p;
   const long long b = blockIdx.x;
   const Row<F32> row(r, b);
   const Settings st(r, b);
   const u64 best = best_of(row, 0, row.vectors, s.part);
-  if (decided(r, b, st, best)) return;
+  if (decided(r, b, st, best, true)) return;
   const Scale sc(unordered((uint32_t)(best >> 32)), st.t);
-  histogram(row, 0, row.vectors, sc, !st.counted(), st.mp, s);
-  finish(r, b, row, st, sc, s);
+  histogram(row, 0, row.vectors, sc, st.k > 0, !st.counted(), st.mp, s);
+  accumulate(s);
+  pick(st, sc, s, &p);
+  __syncthreads();
+  if (!p.slow) {
+    gather(row, 0, row.vectors, p, l);
+    if (l.n <= CAP) {
+      finish(r, b, st, sc, p, l, (int)l.n);
+      return;
+    }
+  }
+  finish_slowly(r, b, row, st, sc, s, l);
 }
+
+// The chunk of vectors that workgroup c of a row takes.
+template <bool F32>
+struct Chunk {
+  int v0, v1;
+  __device__ Chunk(const Rows& r, const Row<F32>& row) {
+    const int per = (row.vectors + r.chunks - 1) / r.chunks, c = blockIdx.x;
+    v0 = min(c * per, row.vectors), v1 = min((c + 1) * per, row.vectors);
+  }
+};
 
 template <bool F32>
 __global__ __launch_bounds__(NT) void maxima_kernel(Rows r) {
   __shared__ u64 part[NW];
   const long long b = blockIdx.y;
-  const int c = blockIdx.x;
   const Row<F32> row(r, b);
-  const int per = (row.vectors + r.chunks - 1) / r.chunks;
-  // the row's bins, to be added to by the next launch
-  for (int i = c * NT + threadIdx.x; i <= BINS; i += r.chunks * NT)
-    r.mass[b * (BINS + 1) + i] = 0, r.count[b * (BINS + 1) + i] = 0;
-  const u64 best = best_of(row, min(c * per, row.vectors), min((c + 1) * per, row.vectors), part);
-  if (threadIdx.x == 0) r.best[b * r.chunks + c] = best;
+  const Chunk<F32> c(r, row);
+  // the row's bins and counters, for the launches that follow
+  for (int i = blockIdx.x * NT + threadIdx.x; i < BINS + 4; i += r.chunks * NT) {
+    r.count[b * (BINS + 4) + i] = 0;
+    if (i <= BINS) r.mass[b * (BINS + 1) + i] = 0;
+  }
+  const u64 best = best_of(row, c.v0, c.v1, part);
+  if (threadIdx.x == 0) r.best[b * r.chunks + blockIdx.x] = best;
 }
 
-template <bool F32>
-__global__ __launch_bounds__(NT) void bins_kernel(Rows r) {
-  __shared__ Shared s;
-  const long long b = blockIdx.y;
-  const int c = blockIdx.x;
-  const Row<F32> row(r, b);
-  const Settings st(r, b);
+// The best of the row's chunks.
+__device__ u64 best_of_chunks(const Rows& r, long long b) {
   u64 best = 0;
   for (int i = threadIdx.x & 63; i < r.chunks; i += 64) {
     const u64 o = r.best[b * r.chunks + i];
@@ -491,36 +627,99 @@ __global__ __launch_bounds__(NT) void bins_kernel(Rows r) {
     const u64 o = shfl_xor(best, d);
     best = o > best ? o : best;
   }
-  if (!best || st.first()) {
-    if (c == 0) decided(r, b, st, best);
-    return;
-  }
-  const Scale sc(unordered((uint32_t)(best >> 32)), st.t);
-  const int per = (row.vectors + r.chunks - 1) / r.chunks;
-  const bool masses = !st.counted();
-  histogram(row, min(c * per, row.vectors), min((c + 1) * per, row.vectors), sc, masses, st.mp, s);
-  u64* mass = r.mass + b * (BINS + 1);
-  uint32_t* count = r.count + b * (BINS + 1);
-  for (int i = threadIdx.x; i < BINS; i += NT) {
-    if (!s.count[i]) continue;
-    __hip_atomic_fetch_add(count + i, s.count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (masses) __hip_atomic_fetch_add(mass + i, s.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  if (threadIdx.x == 0 && s.minp)
-    __hip_atomic_fetch_add(mass + BINS, s.minp, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __builtin_amdgcn_s_waitcnt(0);   // this thread's additions are performed
+  return best;
+}
+
+// Counts this workgroup in (everything it stored before is performed); true in the row's last.
+__device__ bool last_of(uint32_t* counter, int chunks, int* at) {
+  __builtin_amdgcn_s_waitcnt(0);   // this thread's stores and atomics
   __syncthreads();
   if (threadIdx.x == 0)
-    s.at = (int)__hip_atomic_fetch_add(count + BINS, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *at = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  if (s.at != r.chunks - 1) return;
+  return *at == chunks - 1;
+}
+
+// The row's sums of all chunks, into s.
+__device__ void load_bins(const Rows& r, long long b, bool counts, bool masses, Shared& s) {
+  const u64* mass = r.mass + b * (BINS + 1);
+  const uint32_t* count = r.count + b * (BINS + 4);
+  __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += NT) {
-    s.count[i] = __hip_atomic_load(count + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s.count[i] = counts ? __hip_atomic_load(count + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
     s.mass[i] = masses ? __hip_atomic_load(mass + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
   }
   if (threadIdx.x == 0) s.minp = __hip_atomic_load(mass + BINS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  finish(r, b, row, st, sc, s);
+}
+
+template <bool F32>
+__global__ __launch_bounds__(NT) void bins_kernel(Rows r) {
+  __shared__ Shared s;
+  const long long b = blockIdx.y;
+  const Row<F32> row(r, b);
+  const Settings st(r, b);
+  const u64 best = best_of_chunks(r, b);
+  if (decided(r, b, st, best, blockIdx.x == 0)) return;
+  const Scale sc(unordered((uint32_t)(best >> 32)), st.t);
+  const Chunk<F32> c(r, row);
+  const bool counts = st.k > 0, masses = !st.counted();
+  histogram(row, c.v0, c.v1, sc, counts, masses, st.mp, s);
+  u64* mass = r.mass + b * (BINS + 1);
+  uint32_t* count = r.count + b * (BINS + 4);
+  for (int i = threadIdx.x; i < BINS; i += NT) {
+    if (counts && s.count[i])
+      __hip_atomic_fetch_add(count + i, s.count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (masses && s.mass[i])
+      __hip_atomic_fetch_add(mass + i, s.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (threadIdx.x == 0 && s.minp)
+    __hip_atomic_fetch_add(mass + BINS, s.minp, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_of(count + BINS, r.chunks, &s.at)) return;
+  load_bins(r, b, counts, masses, s);
+  accumulate(s);
+  pick(st, sc, s, r.picked + b);
+}
+
+template <bool F32>
+__global__ __launch_bounds__(NT) void draw_kernel(Rows r) {
+  __shared__ Shared s;
+  __shared__ List l;
+  __shared__ Picked p;
+  const long long b = blockIdx.y;
+  const Row<F32> row(r, b);
+  const Settings st(r, b);
+  const u64 best = best_of_chunks(r, b);
+  if (decided(r, b, st, best, false)) return;
+  const Scale sc(unordered((uint32_t)(best >> 32)), st.t);
+  if (threadIdx.x == 0) p = r.picked[b];
+  __syncthreads();
+  uint32_t* count = r.count + b * (BINS + 4);
+  u64* list = r.list + b * CAP;
+  if (!p.slow) {
+    const Chunk<F32> c(r, row);
+    gather(row, c.v0, c.v1, p, l);
+    if (l.n) {
+      if (threadIdx.x == 0)
+        l.at = (int)__hip_atomic_fetch_add(count + BINS + 2, l.n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      for (int i = threadIdx.x; i < (int)l.n && l.at + i < CAP; i += NT)
+        __hip_atomic_store(list + l.at + i, l.key[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (!last_of(count + BINS + 1, r.chunks, &s.at)) return;
+  const uint32_t n = __hip_atomic_load(count + BINS + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (p.slow || n > CAP) {
+    if (!st.counted()) {
+      load_bins(r, b, st.k > 0, true, s);
+      accumulate(s);
+    }
+    finish_slowly(r, b, row, st, sc, s, l);
+    return;
+  }
+  for (int i = threadIdx.x; i < (int)n; i += NT)
+    l.key[i] = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  finish(r, b, st, sc, p, l, (int)n);   // the list of all chunks, in whatever order: sorted first
 }
 
 }  // namespace
@@ -530,7 +729,7 @@ extern "C" {
 long long ko_sample_scratch(int B, int chunks) {
   if (B < 1 || chunks < 1 || chunks > 1024) return -1;
   if (chunks == 1) return 0;
-  return (long long)B * (8 * chunks + 12 * (BINS + 1));
+  return (long long)B * (8 * (chunks + BINS + 1 + CAP) + sizeof(Picked) + 4 * (BINS + 4));
 }
 
 int ko_sample(const void* logits, int f32, long long stride, int B, int V, const float* u,
@@ -550,7 +749,9 @@ int ko_sample(const void* logits, int f32, long long stride, int B, int V, const
   r.ids = ids, r.logp = logprobs;
   r.best = static_cast<u64*>(scratch);
   r.mass = r.best + (long long)B * chunks;
-  r.count = reinterpret_cast<uint32_t*>(r.mass + (long long)B * (BINS + 1));
+  r.list = r.mass + (long long)B * (BINS + 1);
+  r.picked = reinterpret_cast<Picked*>(r.list + (long long)B * CAP);
+  r.count = reinterpret_cast<uint32_t*>(r.picked + B);
   const hipStream_t s = static_cast<hipStream_t>(stream);
 #define KO_SAMPLE(F)                                                                    \
   if (chunks == 1) {                                                                    \
@@ -558,6 +759,7 @@ int ko_sample(const void* logits, int f32, long long stride, int B, int V, const
   } else {                                                                              \
     hipLaunchKernelGGL(maxima_kernel<F>, dim3(chunks, B), dim3(NT), 0, s, r);           \
     hipLaunchKernelGGL(bins_kernel<F>, dim3(chunks, B), dim3(NT), 0, s, r);             \
+    hipLaunchKernelGGL(draw_kernel<F>, dim3(chunks, B), dim3(NT), 0, s, r);             \
   }
   if (f32) {
     KO_SAMPLE(true)
