@@ -13,10 +13,9 @@
 //   top-k counts only: no exp for its whole vocabulary) in LDS, then added to the row's in memory. A
 //   row's last workgroup forms running sums over the bins, which give the bins in which the cuts and
 //   the drawn token can lie: a cut moves the places behind it by no more than its bin's mass.
-// - draw: the tokens of these bins, of all chunks, meet in one list; a row's last workgroup sorts it by
-//   (falling logit, index) and finds the exact places in its running masses. Where the list is too
-//   long for LDS (thousands of equal logits, say) it narrows every place down over the whole row, 8 bits
-//   of (logit, index) at a time.
+// - draw: the tokens of these bins, of all chunks, meet in one list, in which a row's last workgroup
+//   narrows the exact places down, 8 bits of (logit, index) at a time. Where the list is too long for
+//   LDS (thousands of equal logits, say) it does the same over the whole row.
 // A row that is one chunk does all of it in one workgroup and one launch.
 #include "ko_common.h"
 
@@ -37,9 +36,10 @@ constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
 
 // What a row's places need of its bins, as picked from the running sums.
 struct Picked {
-  u64 before[SPANS];          // the mass, and the count, before each span of bins
+  u64 best;                   // the row's, as in maxima
+  u64 before[SPANS], upto[SPANS];   // the mass before each span of bins, and with it
   u64 all, minp;              // the mass of all tokens, and of those that min_p keeps (not of counted rows)
-  uint32_t count[SPANS];
+  uint32_t count[SPANS];      // the count before each
   float hi[SPANS], lo[SPANS];    // the spans' logits, falling; lo > hi: no span
   uint32_t total;             // tokens in the bins
   uint32_t slow;              // counted rows whose k-th token's bin reaches past the list
@@ -58,9 +58,10 @@ struct Rows {
   // scratch, [B] each
   u64* best;         // [chunks]: ordered logit << 32 | ~index
   u64* mass;         // [BINS + 1]: the last is min-p's
-  u64* list;         // [CAP]
+  u64* list;         // [chunks][CAP]
   Picked* picked;
-  uint32_t* count;   // [BINS + 4]: the last are two arrival counters and the list's length
+  uint32_t* count;   // [BINS + 4]: the last are two arrival counters
+  uint32_t* found;   // [chunks]: the tokens that a chunk found for the list
 };
 
 // Larger floats have larger patterns; -0 is 0. NaN does not come here.
@@ -198,36 +199,55 @@ struct Shared {
   u64 mass[BINS];
   u64 part[NW];
   u64 minp;
-  int at;
+  int at[2];
+  u64 digit_count[256], digit_mass[256], found, found_mass;   // narrow's
 };
 struct List {
-  u64 key[CAP], cum[CAP];
+  u64 key[CAP], w[CAP];   // tokens by (falling logit, index), in any order, and their masses
+  u64 digit_mass[256];
+  uint32_t digit_count[256];
   u64 part[NW];
-  u64 base[SPANS];
-  int first[SPANS];
-  u64 found, found_mass, minp;
-  uint32_t n;
+  u64 found, found_mass;
+  uint32_t found_count, found_n, n;
   int at;
 };
-__device__ __forceinline__ u64 shfl_up(u64 v, int d) {
-  return ((u64)(uint32_t)__shfl_up((int)(v >> 32), d) << 32) | (uint32_t)__shfl_up((int)(uint32_t)v, d);
-}
+// Used one after the other.
+union Both {
+  Shared s;
+  List l;
+  __device__ Both() {}
+};
 __device__ __forceinline__ u64 shfl_xor(u64 v, int d) {
   return ((u64)(uint32_t)__shfl_xor((int)(v >> 32), d) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, d);
+}
+// v of the lane n places below in the 16-lane row, 0 where there is none (CTRL: 0x110 + n).
+template <int CTRL>
+__device__ __forceinline__ u64 row_below(u64 v) {
+  return ((u64)(uint32_t)dpp_i<CTRL>((int)(v >> 32)) << 32) | (uint32_t)dpp_i<CTRL>((int)(uint32_t)v);
+}
+__device__ __forceinline__ u64 readlane64(u64 v, int l) {
+  return ((u64)(uint32_t)readlane((int)(v >> 32), l) << 32) | (uint32_t)readlane((int)(uint32_t)v, l);
+}
+// The sum of v over the wavefront's lanes up to and with this one (all lanes active).
+__device__ __forceinline__ u64 wave_running(u64 v) {
+  v += row_below<0x111>(v);
+  v += row_below<0x112>(v);
+  v += row_below<0x114>(v);
+  v += row_below<0x118>(v);
+  const u64 t0 = readlane64(v, 15), t1 = readlane64(v, 31), t2 = readlane64(v, 47);
+  const int row = lane_id() >> 4;
+  return v + (row >= 1 ? t0 : 0) + (row >= 2 ? t1 : 0) + (row >= 3 ? t2 : 0);
 }
 
 // The sum of v over the threads up to and with this one.
 __device__ u64 running(u64 v, u64* part) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 o = shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+  v = wave_running(v);
   __syncthreads();
   if (lane == 63) part[wv] = v;
   __syncthreads();
-  for (int i = 0; i < wv; ++i) v += part[i];
+#pragma unroll
+  for (int i = 0; i < NW - 1; ++i) v += i < wv ? part[i] : 0;
   return v;
 }
 
@@ -296,16 +316,20 @@ __device__ void accumulate(Shared& s) {
   __syncthreads();
 }
 
-// The first bin at which the running count or mass reaches target (one does).
-__device__ int bin_of(bool by_count, u64 target, Shared& s) {
+// The first bins at which the running count or mass reaches either target (some bin does).
+__device__ int2 bins_of(bool by_count, u64 target0, u64 target1, Shared& s) {
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += NT) {
     const u64 here = by_count ? s.count[i] : s.mass[i];
     const u64 before = i ? (by_count ? s.count[i - 1] : s.mass[i - 1]) : 0;
-    if (here >= target && before < target) s.at = i;
+    if (here >= target0 && before < target0) s.at[0] = i;
+    if (here >= target1 && before < target1) s.at[1] = i;
   }
   __syncthreads();
-  return s.at;
+  return make_int2(s.at[0], s.at[1]);
+}
+__device__ int bin_of(bool by_count, u64 target, Shared& s) {
+  return bins_of(by_count, target, target, s).x;
 }
 
 // u's place in a kept mass, and top-p's in one: 1 and more, at most the mass. Neither falls as the
@@ -324,18 +348,22 @@ __device__ __forceinline__ u64 least_kept(u64 minp) {   // nothing reaches a min
   return minp ? minp : 1ull << SHIFT;
 }
 
-// The bounds of the logits of bins [b0, b1]: of all numbers in order the first and the last, by
-// halving; by one thread each.
+// The least (low) or the largest logit of bins [b0, b1]: of all numbers in order, by cutting what is
+// left in 65 with a wavefront's 64 lanes.
 __device__ float span_end(const Scale& sc, int b0, int b1, bool low) {
-  uint32_t lo = ordered(-__builtin_huge_valf()), hi = ordered(sc.top);   // bin(lo) < 0 <= bin(hi)
-  // low: the least logit of a bin up to b1; else the largest of a bin from b0 on (or lo's, none)
   if (!low && b0 == 0) return sc.top;
-  const int limit = low ? b1 : b0 - 1;   // the least logit of a bin up to limit
+  // the largest is next to the least of the bins before
+  const int limit = low ? b1 : b0 - 1;
+  uint32_t lo = ordered(-__builtin_huge_valf()), hi = ordered(sc.top);   // bin(lo) < 0 <= bin(hi) <= limit
   while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
+    const uint32_t step = max((hi - lo) / 65, 1u);
+    const uint32_t mid = min(lo + step * (uint32_t)(lane_id() + 1), hi - 1);
     const int b = sc.bin(unordered(mid));
-    if (b >= 0 && b <= limit) hi = mid;
-    else lo = mid;
+    const u64 in = __ballot(b >= 0 && b <= limit);   // from some lane on
+    const int first = in ? __builtin_ctzll(in) : 64;
+    const uint32_t below = first ? (uint32_t)readlane((int)mid, first - 1) : lo;
+    hi = first < 64 ? (uint32_t)readlane((int)mid, first) : hi;
+    lo = below;
   }
   return unordered(low ? hi : hi - 1);
 }
@@ -361,28 +389,38 @@ __device__ void pick(const Settings& st, const Scale& sc, Shared& s, Picked* out
       within(kf, kl);
     }
     if (st.p < 1.f) {
-      pf = bin_of(false, nucleus(st.p, lo), s), pl = bin_of(false, nucleus(st.p, hi), s);
+      const int2 p = bins_of(false, nucleus(st.p, lo), nucleus(st.p, hi), s);
+      pf = p.x, pl = p.y;
       within(pf, pl);
     }
     if (st.mp > 0.f) {
       const u64 m = least_kept(s.minp);
       lo = lo < m ? lo : m, hi = hi < m ? hi : m;
     }
-    uf = bin_of(false, draw(st.u, lo), s), ul = bin_of(false, draw(st.u, hi), s);
+    const int2 u = bins_of(false, draw(st.u, lo), draw(st.u, hi), s);
+    uf = u.x, ul = u.y;
     // spans that meet become one: a token is gathered once
     if (pf <= pl && ul >= pf) pf = min(pf, uf), uf = 1, ul = 0;
     if (kf <= kl && pf <= pl && pl >= kf) kf = min(kf, pf), pf = 1, pl = 0;
     if (kf <= kl && uf <= ul && ul >= kf) kf = min(kf, uf), uf = 1, ul = 0;
   }
-  const int t = threadIdx.x;
-  if (t < SPANS) {
-    const int f = t == 0 ? kf : t == 1 ? pf : uf, l = t == 0 ? kl : t == 1 ? pl : ul;
-    out->hi[t] = f <= l ? span_end(sc, f, l, false) : 0.f;
-    out->lo[t] = f <= l ? span_end(sc, f, l, true) : 1.f;
-    out->before[t] = f <= l && f ? s.mass[f - 1] : 0;
-    out->count[t] = f <= l && f ? s.count[f - 1] : 0;
+  const int wv = uniform(threadIdx.x >> 6), j = wv >> 1;   // a wavefront for each end of a span
+  if (j < SPANS) {
+    const int f = j == 0 ? kf : j == 1 ? pf : uf, l = j == 0 ? kl : j == 1 ? pl : ul;
+    const bool low = wv & 1;
+    const float end = f <= l ? span_end(sc, f, l, low) : low ? 1.f : 0.f;
+    if ((threadIdx.x & 63) == 0) {
+      if (low) {
+        out->lo[j] = end;
+      } else {
+        out->hi[j] = end;
+        out->before[j] = f <= l && f ? s.mass[f - 1] : 0;
+        out->upto[j] = f <= l ? s.mass[l] : 0;
+        out->count[j] = f <= l && f ? s.count[f - 1] : 0;
+      }
+    }
   }
-  if (t == 0) out->all = s.mass[BINS - 1], out->minp = s.minp, out->total = total, out->slow = slow;
+  if (threadIdx.x == 0) out->all = s.mass[BINS - 1], out->minp = s.minp, out->total = total, out->slow = slow;
 }
 
 // The row's tokens of the spans among the vectors, into the list of this workgroup.
@@ -401,23 +439,6 @@ __device__ void gather(const Row<F32>& row, int v0, int v1, const Picked& p, Lis
   __syncthreads();
 }
 
-// l.key[0 .. n) in rising order: by falling logit, then index.
-__device__ void sort(List& l, int n) {
-  int m = 64;
-  while (m < n) m <<= 1;
-  for (int i = n + threadIdx.x; i < m; i += NT) l.key[i] = ~0ull;
-  __syncthreads();
-  for (int size = 2; size <= m; size <<= 1)
-    for (int d = size >> 1; d > 0; d >>= 1) {
-      for (int t = threadIdx.x; t < m / 2; t += NT) {
-        const int i = 2 * t - (t & (d - 1));   // t / d * 2 d + t % d
-        const u64 a = l.key[i], b = l.key[i + d];
-        if ((a > b) == ((i & size) == 0)) l.key[i] = b, l.key[i + d] = a;
-      }
-      __syncthreads();
-    }
-}
-
 __device__ __forceinline__ float logit_of(u64 key) { return unordered(~(uint32_t)(key >> 32)); }
 
 __device__ void result(const Rows& r, long long b, const Scale& sc, u64 key, u64 kept) {
@@ -429,64 +450,108 @@ __device__ void result(const Rows& r, long long b, const Scale& sc, u64 key, u64
   }
 }
 
-// The row's token from the sorted list of all the spans' tokens.
+// The row's token from the list of all the spans' tokens: a place lies in one span, and there 8 bits of
+// the key at a time narrow it down, until one token is left. The keys are the lists' without the
+// bits that are always the same, and a place begins below those that its span's keys share: atomics on
+// one digit that all tokens have would come one after the other.
+template <bool F32>
 __device__ void finish(const Rows& r, long long b, const Settings& st, const Scale& sc,
                        const Picked& p, List& l, int n) {
-  sort(l, n);
-  constexpr int EACH = CAP / NT;
-  const int t = threadIdx.x * EACH;
-  u64 w[EACH], sum = 0;
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    w[i] = t + i < n ? sc.mass(logit_of(l.key[t + i])) : 0;
-    sum += w[i];
-  }
-  u64 run = running(sum, l.part) - sum;
-  // where each span begins: what its tokens' masses and places lack of the row's
-  auto span_of = [&](u64 key) {
-    const float x = logit_of(key);
-    return x >= p.lo[0] && x <= p.hi[0] ? 0 : x >= p.lo[1] && x <= p.hi[1] ? 1 : 2;
+  const int ibits = 32 - __builtin_clz((uint32_t)r.V);   // of an index
+  auto narrow_key = [&](uint32_t logit_key, uint32_t index) {   // logit_key: ~ordered
+    return (u64)(F32 ? logit_key : logit_key >> 16) << ibits | index;
   };
-  if (threadIdx.x == 0) l.minp = 0;
-  __syncthreads();
-  u64 kept_minp = 0;
+  constexpr int EACH = CAP / NT;
+  u64 key[EACH], nkey[EACH], w[EACH], kept_minp = 0;
+  int span[EACH];
   const double least = (double)st.mp * (double)(1ull << SHIFT);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    if (t + i >= n) break;
-    const int j = span_of(l.key[t + i]);
-    if (t + i == 0 || span_of(l.key[t + i - 1]) != j) l.base[j] = p.before[j] - run, l.first[j] = t + i;
-    run += w[i];
-    l.cum[t + i] = run;
-    if (sc.scaled(logit_of(l.key[t + i])) >= least) kept_minp += w[i];
+    const int at = threadIdx.x + i * NT;
+    key[i] = at < n ? l.key[at] : ~0ull;
+    nkey[i] = narrow_key((uint32_t)(key[i] >> 32), (uint32_t)key[i]);
+    const float x = logit_of(key[i]);
+    span[i] = at >= n ? -1 : x >= p.lo[0] && x <= p.hi[0] ? 0 : x >= p.lo[1] && x <= p.hi[1] ? 1 : 2;
+    const double m = at < n ? sc.scaled(x) : 0.0;
+    w[i] = Scale::whole(m);
+    if (m >= least) kept_minp += w[i];
   }
-  if (st.counted() && st.mp > 0.f) atomicAdd(&l.minp, kept_minp);
-  __syncthreads();
-  auto place = [&](bool by_count, u64 target) {   // l.found, l.found_mass: the token that reaches it
+  u64 minp = p.minp;
+  if (st.counted() && st.mp > 0.f) {   // the list has all that min_p may keep
+    const u64 sum = running(kept_minp, l.part);
+    if (threadIdx.x == NT - 1) l.found_mass = sum;
     __syncthreads();
+    minp = l.found_mass;
+    __syncthreads();
+  }
+  // the token at which the count or the mass reaches target: l.found, l.found_mass
+  auto place = [&](bool by_count, u64 target) {
+    // its span: the lists of rows that are counted have one
+    int j = 0;
+    if (!st.counted())
+      j = by_count ? 0   // top-k's own span, or the one that it met
+          : target > p.before[2] && target <= p.upto[2] ? 2
+          : target > p.before[1] && target <= p.upto[1] ? 1 : 0;
+    const u64 first = narrow_key(~ordered(p.hi[j]), 0);
+    const u64 last = narrow_key(~ordered(p.lo[j]), (1u << ibits) - 1);
+    int left = first == last ? 0 : 64 - __builtin_clzll(first ^ last);   // bits not known
+    u64 prefix = first >> left, mass = p.before[j];
+    uint32_t count = p.count[j];
+    while (left > 0) {
+      const int shift = max(left - 8, 0);
+      __syncthreads();
+      if (threadIdx.x < 256) l.digit_mass[threadIdx.x] = 0, l.digit_count[threadIdx.x] = 0;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      if (t + i >= n) break;
-      const int j = span_of(l.key[t + i]);
-      const u64 mass = l.cum[t + i] + l.base[j], here = by_count ? p.count[j] + (t + i - l.first[j]) + 1 : mass;
-      if (here >= target && here - (by_count ? 1 : w[i]) < target)
-        l.found = l.key[t + i], l.found_mass = mass;
+      for (int i = 0; i < EACH; ++i)
+        if (span[i] == j && nkey[i] >> left == prefix) {
+          const int digit = (int)(nkey[i] >> shift) & ((1 << (left - shift)) - 1);
+          atomicAdd(&l.digit_count[digit], 1u);
+          atomicAdd(&l.digit_mass[digit], w[i]);
+        }
+      __syncthreads();
+      if (threadIdx.x < 64) {   // 4 digits a lane
+        u64 m[4], sm = 0;
+        uint32_t c[4], sn = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          m[i] = l.digit_mass[4 * threadIdx.x + i], c[i] = l.digit_count[4 * threadIdx.x + i];
+          sm += m[i], sn += c[i];
+        }
+        u64 rm = mass + wave_running(sm) - sm;
+        uint32_t rc = count + (uint32_t)wave_incl_scan((int)sn) - sn;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const u64 before = by_count ? rc : rm, here = before + (by_count ? c[i] : m[i]);
+          if (here >= target && before < target)
+            l.at = 4 * threadIdx.x + i, l.found_mass = rm, l.found_count = rc, l.found_n = c[i];
+          rm += m[i], rc += c[i];
+        }
+      }
+      __syncthreads();
+      prefix = prefix << (left - shift) | (u64)l.at;
+      left = shift;
+      mass = l.found_mass, count = l.found_count;
+      if (l.found_n == 1) break;
     }
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (span[i] == j && nkey[i] >> left == prefix) l.found = key[i], l.found_mass = mass + w[i];
+    __syncthreads();
   };
-  u64 kept;
+  u64 kept = p.all;
   if (st.k && ((uint32_t)st.k < p.total || st.counted())) {
     place(true, min((uint32_t)st.k, p.total));
     kept = l.found_mass;
-  } else {
-    kept = p.all;
   }
   if (st.p < 1.f) {
     place(false, nucleus(st.p, kept));
     kept = l.found_mass;
   }
   if (st.mp > 0.f) {
-    const u64 m = least_kept(st.counted() ? l.minp : p.minp);
+    const u64 m = least_kept(minp);
     kept = m < kept ? m : kept;
   }
   place(false, draw(st.u, kept));
@@ -498,11 +563,9 @@ struct Place {
 };
 
 // The first token of the order at which the count or the mass reaches target, over the whole row: its
-// bin from the running sums in s, then 8 bits of its key at a time (counts and masses of the digits
-// in l).
+// bin from the running sums in s, then 8 bits of its key at a time.
 template <bool F32>
-__device__ Place narrow(const Row<F32>& row, const Scale& sc, bool by_count, u64 target, Shared& s,
-                        List& l) {
+__device__ Place narrow(const Row<F32>& row, const Scale& sc, bool by_count, u64 target, Shared& s) {
   const int b = bin_of(by_count, target, s);
   u64 prefix = 0, known = 0, count = b ? s.count[b - 1] : 0, mass = b ? s.mass[b - 1] : 0;
   for (int shift = 56; shift >= 0; shift -= 8) {
@@ -512,46 +575,45 @@ __device__ Place narrow(const Row<F32>& row, const Scale& sc, bool by_count, u64
       known |= 0xffull << shift;
       continue;
     }
+    const bool in = threadIdx.x < 256;
     __syncthreads();
-    if (threadIdx.x < 256) l.cum[threadIdx.x] = l.key[threadIdx.x] = 0;
+    if (in) s.digit_count[threadIdx.x] = s.digit_mass[threadIdx.x] = 0;
     __syncthreads();
     row.template each<2>(0, row.vectors, [&](int i, float x) {
       if (sc.bin(x) != b) return;
       const u64 key = (u64)~ordered(x) << 32 | (uint32_t)i;
       if ((key & known) != prefix) return;
       const int digit = (int)(key >> shift) & 255;
-      atomicAdd(&l.key[digit], 1ull);
-      atomicAdd(&l.cum[digit], sc.mass(x));
+      atomicAdd(&s.digit_count[digit], 1ull);
+      atomicAdd(&s.digit_mass[digit], sc.mass(x));
     });
     __syncthreads();
-    const bool in = threadIdx.x < 256;
-    const u64 c = in ? l.key[threadIdx.x] : 0, m = in ? l.cum[threadIdx.x] : 0;
-    const u64 rc = count + running(c, l.part), rm = mass + running(m, l.part);
+    const u64 c = in ? s.digit_count[threadIdx.x] : 0, m = in ? s.digit_mass[threadIdx.x] : 0;
+    const u64 rc = count + running(c, s.part), rm = mass + running(m, s.part);
     const u64 here = by_count ? rc : rm, before = by_count ? rc - c : rm - m;
-    if (in && here >= target && before < target) l.at = threadIdx.x, l.found = rc - c, l.found_mass = rm - m;
+    if (in && here >= target && before < target)
+      s.at[0] = threadIdx.x, s.found = rc - c, s.found_mass = rm - m;
     __syncthreads();
-    prefix |= (u64)l.at << shift, known |= 0xffull << shift;
-    count = l.found, mass = l.found_mass;
+    prefix |= (u64)s.at[0] << shift, known |= 0xffull << shift;
+    count = s.found, mass = s.found_mass;
   }
   return {prefix, mass + sc.mass(logit_of(prefix))};
 }
 
-// The row's token without a list, from running sums in s.
+// The row's token without a list, by one workgroup.
 template <bool F32>
 __device__ void finish_slowly(const Rows& r, long long b, const Row<F32>& row, const Settings& st,
-                              const Scale& sc, Shared& s, List& l) {
-  if (st.counted()) {   // its masses, too
-    histogram(row, 0, row.vectors, sc, true, true, st.mp, s);
-    accumulate(s);
-  }
+                              const Scale& sc, Shared& s) {
+  histogram(row, 0, row.vectors, sc, true, true, st.mp, s);
+  accumulate(s);
   u64 kept = s.mass[BINS - 1];
-  if (st.k && (uint32_t)st.k < s.count[BINS - 1]) kept = narrow(row, sc, true, (u64)st.k, s, l).mass;
-  if (st.p < 1.f) kept = narrow(row, sc, false, nucleus(st.p, kept), s, l).mass;
+  if (st.k && (uint32_t)st.k < s.count[BINS - 1]) kept = narrow(row, sc, true, (u64)st.k, s).mass;
+  if (st.p < 1.f) kept = narrow(row, sc, false, nucleus(st.p, kept), s).mass;
   if (st.mp > 0.f) {
     const u64 m = least_kept(s.minp);
     kept = m < kept ? m : kept;
   }
-  const Place at = narrow(row, sc, false, draw(st.u, kept), s, l);
+  const Place at = narrow(row, sc, false, draw(st.u, kept), s);
   result(r, b, sc, at.key, kept);
 }
 
@@ -567,9 +629,10 @@ __device__ bool decided(const Rows& r, long long b, const Settings& st, u64 best
 
 template <bool F32>
 __global__ __launch_bounds__(NT) void sample_kernel(Rows r) {
-  __shared__ Shared s;
-  __shared__ List l;
+  __shared__ Both both;
   __shared__ Picked p;
+  Shared& s = both.s;
+  List& l = both.l;
   const long long b = blockIdx.x;
   const Row<F32> row(r, b);
   const Settings st(r, b);
@@ -582,12 +645,13 @@ __global__ __launch_bounds__(NT) void sample_kernel(Rows r) {
   __syncthreads();
   if (!p.slow) {
     gather(row, 0, row.vectors, p, l);
-    if (l.n <= CAP) {
-      finish(r, b, st, sc, p, l, (int)l.n);
+    const int n = (int)l.n;
+    if (n <= CAP) {
+      finish<F32>(r, b, st, sc, p, l, n);
       return;
     }
   }
-  finish_slowly(r, b, row, st, sc, s, l);
+  finish_slowly(r, b, row, st, sc, s);
 }
 
 // The chunk of vectors that workgroup c of a row takes.
@@ -660,6 +724,7 @@ __global__ __launch_bounds__(NT) void bins_kernel(Rows r) {
   const Row<F32> row(r, b);
   const Settings st(r, b);
   const u64 best = best_of_chunks(r, b);
+  if (blockIdx.x == 0 && threadIdx.x == 0) r.picked[b].best = best;
   if (decided(r, b, st, best, blockIdx.x == 0)) return;
   const Scale sc(unordered((uint32_t)(best >> 32)), st.t);
   const Chunk<F32> c(r, row);
@@ -675,7 +740,7 @@ __global__ __launch_bounds__(NT) void bins_kernel(Rows r) {
   }
   if (threadIdx.x == 0 && s.minp)
     __hip_atomic_fetch_add(mass + BINS, s.minp, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (!last_of(count + BINS, r.chunks, &s.at)) return;
+  if (!last_of(count + BINS, r.chunks, s.at)) return;
   load_bins(r, b, counts, masses, s);
   accumulate(s);
   pick(st, sc, s, r.picked + b);
@@ -683,43 +748,52 @@ __global__ __launch_bounds__(NT) void bins_kernel(Rows r) {
 
 template <bool F32>
 __global__ __launch_bounds__(NT) void draw_kernel(Rows r) {
-  __shared__ Shared s;
-  __shared__ List l;
+  __shared__ Both both;
   __shared__ Picked p;
+  __shared__ int s_arrived;
+  Shared& s = both.s;
+  List& l = both.l;
   const long long b = blockIdx.y;
   const Row<F32> row(r, b);
   const Settings st(r, b);
-  const u64 best = best_of_chunks(r, b);
-  if (decided(r, b, st, best, false)) return;
-  const Scale sc(unordered((uint32_t)(best >> 32)), st.t);
-  if (threadIdx.x == 0) p = r.picked[b];
+  if (threadIdx.x < sizeof(Picked) / 4)
+    reinterpret_cast<uint32_t*>(&p)[threadIdx.x] = reinterpret_cast<const uint32_t*>(r.picked + b)[threadIdx.x];
   __syncthreads();
-  uint32_t* count = r.count + b * (BINS + 4);
-  u64* list = r.list + b * CAP;
+  if (decided(r, b, st, p.best, false)) return;
+  const Scale sc(unordered((uint32_t)(p.best >> 32)), st.t);
+  uint32_t* found = r.found + b * r.chunks;
+  u64* list = r.list + b * r.chunks * CAP;
   if (!p.slow) {
     const Chunk<F32> c(r, row);
     gather(row, c.v0, c.v1, p, l);
-    if (l.n) {
-      if (threadIdx.x == 0)
-        l.at = (int)__hip_atomic_fetch_add(count + BINS + 2, l.n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __syncthreads();
-      for (int i = threadIdx.x; i < (int)l.n && l.at + i < CAP; i += NT)
-        __hip_atomic_store(list + l.at + i, l.key[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    u64* mine = list + (long long)blockIdx.x * CAP;
+    for (int i = threadIdx.x; i < min((int)l.n, CAP); i += NT)
+      __hip_atomic_store(mine + i, l.key[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0)
+      __hip_atomic_store(found + blockIdx.x, l.n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  if (!last_of(count + BINS + 1, r.chunks, &s.at)) return;
-  const uint32_t n = __hip_atomic_load(count + BINS + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (p.slow || n > CAP) {
-    if (!st.counted()) {
-      load_bins(r, b, st.k > 0, true, s);
-      accumulate(s);
+  if (!last_of(r.count + b * (BINS + 4) + BINS + 1, r.chunks, &s_arrived)) return;
+  // the chunks' tokens, one chunk behind the other
+  int n = 0;
+  if (!p.slow)
+    for (int c = 0; c < r.chunks && n <= CAP; c += 64) {
+      const int at = c + (int)(threadIdx.x & 63);
+      const int m = at < r.chunks ? (int)__hip_atomic_load(found + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+      const int end = n + wave_incl_scan(min(m, CAP + 1)), first = end - min(m, CAP + 1);
+      // a wavefront for each chunk in turn
+      for (int i = uniform(threadIdx.x >> 6); i < 64 && c + i < r.chunks; i += NW) {
+        const int f = readlane(first, i), e = readlane(end, i);
+        for (int j = f + (int)(threadIdx.x & 63); j < min(e, CAP); j += 64)
+          l.key[j] = __hip_atomic_load(list + (long long)(c + i) * CAP + (j - f), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+      }
+      n = readlane(end, 63);
     }
-    finish_slowly(r, b, row, st, sc, s, l);
+  if (p.slow || n > CAP) {
+    finish_slowly(r, b, row, st, sc, s);
     return;
   }
-  for (int i = threadIdx.x; i < (int)n; i += NT)
-    l.key[i] = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  finish(r, b, st, sc, p, l, (int)n);   // the list of all chunks, in whatever order: sorted first
+  finish<F32>(r, b, st, sc, p, l, n);
 }
 
 }  // namespace
@@ -729,7 +803,8 @@ extern "C" {
 long long ko_sample_scratch(int B, int chunks) {
   if (B < 1 || chunks < 1 || chunks > 1024) return -1;
   if (chunks == 1) return 0;
-  return (long long)B * (8 * (chunks + BINS + 1 + CAP) + sizeof(Picked) + 4 * (BINS + 4));
+  return (long long)B * (8ll * (chunks + BINS + 1) + 8ll * CAP * chunks + sizeof(Picked) +
+                         4ll * (BINS + 4 + chunks));
 }
 
 int ko_sample(const void* logits, int f32, long long stride, int B, int V, const float* u,
@@ -750,8 +825,9 @@ int ko_sample(const void* logits, int f32, long long stride, int B, int V, const
   r.best = static_cast<u64*>(scratch);
   r.mass = r.best + (long long)B * chunks;
   r.list = r.mass + (long long)B * (BINS + 1);
-  r.picked = reinterpret_cast<Picked*>(r.list + (long long)B * CAP);
+  r.picked = reinterpret_cast<Picked*>(r.list + (long long)B * chunks * CAP);
   r.count = reinterpret_cast<uint32_t*>(r.picked + B);
+  r.found = r.count + (long long)B * (BINS + 4);
   const hipStream_t s = static_cast<hipStream_t>(stream);
 #define KO_SAMPLE(F)                                                                    \
   if (chunks == 1) {                                                                    \

@@ -12,7 +12,7 @@ import torch
 
 from .. import _lib
 from .fused import BF16, _cdiv, _need
-from .kv4 import _here, _stream
+from .kv4 import _current_device, _here, _stream
 
 F32 = torch.float32
 MAX_VOCAB = 1 << 20
@@ -60,23 +60,55 @@ class Sampler:
         receives the log of the token's share of the kept mass (0 where the first token is
         taken, -infinity beside the id -1)."""
         B, V, dev = self.B, self.V, self._dev
-        _here(dev)
-        _need(isinstance(logits, torch.Tensor) and logits.dtype in (BF16, F32)
-              and tuple(logits.shape) == (B, V), f"logits must be [{B}, {V}] in bf16 or fp32")
-        _need(logits.is_cuda and logits.get_device() == dev, f"logits must be on cuda:{dev}")
-        _need(logits.stride(1) == 1 or V == 1, "logits: the inner stride must be 1")
-        _vector(u, "u", F32, B, dev)
-        _vector(ids, "ids", torch.int64, B, dev)
-        if logprobs is not None:
-            _vector(logprobs, "logprobs", F32, B, dev)
-        t = _setting(temperature, "temperature", F32, B, dev, lambda v: v >= 0)
-        k = _setting(top_k, "top_k", torch.int32, B, dev, lambda v: v >= 0 and int(v) == v)
-        p = _setting(top_p, "top_p", F32, B, dev, lambda v: 0 <= v <= 1)
-        m = _setting(min_p, "min_p", F32, B, dev, lambda v: 0 <= v <= 1)
-        _lib.call("ko_sample", logits.data_ptr(), logits.dtype == F32,
-                  logits.stride(0) if B > 1 else 0, B, V, u.data_ptr(), *t, k[0],
-                  min(int(k[1]), V), *p, *m, ids.data_ptr(), _lib.ptr(logprobs),
+        usual = self._usual(logits, u, ids, logprobs)
+        if usual is None:
+            _here(dev)
+            _need(isinstance(logits, torch.Tensor) and logits.dtype in (BF16, F32)
+                  and tuple(logits.shape) == (B, V), f"logits must be [{B}, {V}] in bf16 or fp32")
+            _need(logits.is_cuda and logits.get_device() == dev, f"logits must be on cuda:{dev}")
+            _need(logits.stride(1) == 1 or V == 1, "logits: the inner stride must be 1")
+            _vector(u, "u", F32, B, dev)
+            _vector(ids, "ids", torch.int64, B, dev)
+            if logprobs is not None:
+                _vector(logprobs, "logprobs", F32, B, dev)
+            usual = (logits.data_ptr(), u.data_ptr(), ids.data_ptr(), _lib.ptr(logprobs))
+        t = _setting(temperature, "temperature", F32, B, dev, _at_least_0)
+        k = _setting(top_k, "top_k", torch.int32, B, dev, _whole)
+        p = _setting(top_p, "top_p", F32, B, dev, _share)
+        m = _setting(min_p, "min_p", F32, B, dev, _share)
+        _lib.call("ko_sample", usual[0], logits.dtype is F32, logits.stride(0) if B > 1 else 0, B, V,
+                  usual[1], *t, k[0], min(int(k[1]), V), *p, *m, usual[2], usual[3],
                   self._scratch.data_ptr(), self._scratch.numel(), self.chunks, _stream(dev))
+
+    def _usual(self, logits, u, ids, logprobs):
+        """The addresses of a call that needs no closer look, else None."""
+        try:
+            B, dev = self.B, self._dev
+            if (logits.shape == (B, self.V) and logits.dtype in (BF16, F32) and logits.is_contiguous()
+                    and u.dtype is F32 and ids.dtype is torch.int64 and u.shape == ids.shape == (B,)
+                    and u.is_contiguous() and ids.is_contiguous()
+                    and dev == logits.get_device() == u.get_device() == ids.get_device()
+                    == _current_device()):
+                if logprobs is None:
+                    return logits.data_ptr(), u.data_ptr(), ids.data_ptr(), None
+                if (logprobs.dtype is F32 and logprobs.shape == (B,) and logprobs.is_contiguous()
+                        and logprobs.get_device() == dev):
+                    return logits.data_ptr(), u.data_ptr(), ids.data_ptr(), logprobs.data_ptr()
+        except (AttributeError, TypeError, RuntimeError):
+            pass   # no tensors: the tests above say which
+        return None
+
+
+def _at_least_0(v):
+    return v >= 0
+
+
+def _whole(v):
+    return v >= 0 and int(v) == v
+
+
+def _share(v):
+    return 0 <= v <= 1
 
 
 def _vector(t, name, dtype, B, dev):
@@ -88,7 +120,9 @@ def _vector(t, name, dtype, B, dev):
 def _setting(v, name, dtype, B, dev, valid):
     """(address, value) of a setting, one of them unused."""
     if isinstance(v, torch.Tensor):
-        _vector(v, name, dtype, B, dev)
+        if not (v.dtype is dtype and v.shape == (B,) and v.is_contiguous() and v.get_device() == dev):
+            _vector(v, name, dtype, B, dev)   # says what is wrong
         return v.data_ptr(), 0
-    _need(isinstance(v, (int, float)) and valid(v), f"{name} is out of range: {v!r}")
+    if not (isinstance(v, (int, float)) and valid(v)):
+        raise ValueError(f"{name} is out of range: {v!r}")
     return None, v
