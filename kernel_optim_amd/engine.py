@@ -40,21 +40,32 @@ value with the scales of the default groups of 32, ENGINE_KV_GROUP or kv_group):
 the same memory and a decode step that reads as much less of them. The prompt attends to
 its own K and V in bf16, layer by layer, before they are quantised; decode and verify
 steps attend to what the cache holds.
+
+With ENGINE_WEIGHT_FORMAT=fp8 (or weight_format="fp8") the projections and the LM head are held in 8-bit
+floating point, quantised at load (kernels.fp8; 8.06 bits a value), and their inputs quantised in
+every step: the prompt, decode and verify steps all run on these. The embedding and the norms stay
+bf16.
+
+``generate(..., sampling=Sampling(...))`` draws its tokens instead of taking the largest logit
+(kernels.sampling), by random numbers from a seed; it does not speculate.
 """
 
 import os
 import sys
 import time
 import weakref
+from dataclasses import dataclass
 
 import torch
 
 from .kernels.fused import DecodeAttention, add_rms_norm, qk_norm_rope, rope_rows, silu_mul
+from .kernels.fp8 import Fp8Linear
 from .kernels.kv4 import Kv4Attention, kv4_append, kv4_block_bytes, kv4_cache, kv4_write
 from .kernels.gemv import (EPI_ARGMAX, EPI_BF16, EPI_RESID, EPI_SWIGLU, ROWS_MAX, Gemv, argmax_rows,
                            embed_ss, tile_weights, uses_tiled)
-from .model import Qwen3Config, load_checkpoint, random_weights
-from .prefill import prefill
+from .kernels.sampling import Sampler
+from .model import Qwen3Config, fp8_weights, load_checkpoint, random_weights
+from .prefill import prefill, prefill_fp8
 
 DEVICE = "cuda:0"
 LOG = os.environ.get("ENGINE_LOG", "0") == "1"
@@ -95,8 +106,40 @@ MIN_ADVANCE = (float(os.environ["ENGINE_MIN_ADVANCE"]) if "ENGINE_MIN_ADVANCE" i
 # the KV cache: "bf16", or "kv4" (4 bits, in groups of KV_GROUP values)
 KV_CACHE = os.environ.get("ENGINE_KV_CACHE", "bf16")
 KV_GROUP = int(os.environ.get("ENGINE_KV_GROUP", "32"))
+# the projections and the LM head: "bf16", or "fp8" (8 bits, a scale for each 128 values of a row)
+WEIGHT_FORMAT = os.environ.get("ENGINE_WEIGHT_FORMAT", "bf16")
 PIN_RESULTS = 64 << 20   # bytes of verify results in pinned memory that callers may hold
 FUSED_VERIFY_ROWS = 16   # verify rows the fused GEMVs take in one weight pass
+
+
+@dataclass(frozen=True)
+class Sampling:
+    """How generate() draws tokens (kernels.sampling.Sampler): numbers for all sequences, or a list with
+    one for each. ``seed``: of the random numbers, one a sequence and step."""
+
+    temperature: object = 1.0
+    top_k: object = 0
+    top_p: object = 1.0
+    min_p: object = 0.0
+    seed: int = 0
+
+    def columns(self, B):
+        """The settings as tensors [B] on the CPU, checked: temperature, top_k, top_p, min_p."""
+        out = []
+        for name, dtype, valid in (("temperature", torch.float32, lambda v: v >= 0),
+                                   ("top_k", torch.int32, lambda v: v >= 0 and int(v) == v),
+                                   ("top_p", torch.float32, lambda v: 0 <= v <= 1),
+                                   ("min_p", torch.float32, lambda v: 0 <= v <= 1)):
+            v = getattr(self, name)
+            v = list(v) if isinstance(v, (list, tuple)) else [v] * B
+            if len(v) != B:
+                raise ValueError(f"{name} has {len(v)} values for {B} sequences")
+            if not all(isinstance(x, (int, float)) and valid(x) for x in v):
+                raise ValueError(f"{name} is out of range: {v}")
+            if name == "top_k":
+                v = [min(int(x), 2 ** 31 - 1) for x in v]
+            out.append(torch.tensor(v, dtype=dtype))
+        return out
 
 
 def draft_len(B):
@@ -338,7 +381,7 @@ class HostCopies:
 
 class Engine:
     def __init__(self, model_path: str, keep_logits: bool = False, spec=None,
-                 decode_graph=None, kv_cache=None, kv_group=None) -> None:
+                 decode_graph=None, kv_cache=None, kv_group=None, weight_format=None) -> None:
         self._t0 = time.monotonic()
         if model_path.startswith("random"):
             seed = int(model_path.split(":", 1)[1]) if ":" in model_path else 0
@@ -358,21 +401,21 @@ class Engine:
             raise FileNotFoundError(
                 f"{model_path}: no *.safetensors weights (pass 'random[:seed]' or set "
                 "ENGINE_RANDOM_INIT=1 for random weights over its config.json)")
-        self._init(cfg, w, keep_logits, spec, decode_graph, kv_cache, kv_group)
+        self._init(cfg, w, keep_logits, spec, decode_graph, kv_cache, kv_group, weight_format)
 
     @classmethod
     def from_weights(cls, cfg, weights, keep_logits=False, spec=None, decode_graph=None,
-                     kv_cache=None, kv_group=None):
+                     kv_cache=None, kv_group=None, weight_format=None):
         """Engine over weights already in the decode layout (moved to the GPU)."""
         from .model import weights_to
         self = cls.__new__(cls)
         self._t0 = time.monotonic()
         self._init(cfg, weights_to(weights, DEVICE), keep_logits, spec, decode_graph, kv_cache,
-                   kv_group)
+                   kv_group, weight_format)
         return self
 
     def _init(self, cfg, w, keep_logits, spec=None, decode_graph=None, kv_cache=None,
-              kv_group=None):
+              kv_group=None, weight_format=None):
         """spec: prompt-lookup speculation on (True) or off (False); None takes
         ENGINE_SPEC (off unless set to 1). decode_graph: "auto" (the fused-GEMV
         decode graph up to 32 sequences, or 64 where auto_graph says so, the
@@ -380,8 +423,11 @@ class Engine:
         and keep the faster), "fused" or "hipblaslt"; None takes
         ENGINE_DECODE_GRAPH (auto unless set). kv_cache: "bf16" or "kv4" (K and V in 4
         bits); None takes ENGINE_KV_CACHE (bf16 unless set). kv_group: the 4-bit cache's values
-        that share a scale, 32, 64 or 128; None takes ENGINE_KV_GROUP (32 unless set)."""
+        that share a scale, 32, 64 or 128; None takes ENGINE_KV_GROUP (32 unless set).
+        weight_format: "bf16" or "fp8" (8 bits; its one decode graph leaves decode_graph nothing to
+        choose); None takes ENGINE_WEIGHT_FORMAT (bf16 unless set)."""
         self.spec = SPEC if spec is None else bool(spec)
+        self.sampled = False   # whether the captured step draws its tokens
         self.min_advance = MIN_ADVANCE   # None: the measured break-even
         kind = DECODE_GRAPH if decode_graph is None else decode_graph
         if kind not in ("auto", "timed", "fused", "hipblaslt"):
@@ -396,7 +442,13 @@ class Engine:
             kv4_block_bytes(cfg.head_dim, self.kv_group)   # refuses a group it does not serve
         if cfg.head_dim != 128 or cfg.nq != 4 * cfg.nkv:
             raise ValueError("the decode kernels serve head_dim 128 with 4 query heads per KV head")
-        self.cfg, self.w = cfg, w
+        fmt = WEIGHT_FORMAT if weight_format is None else weight_format
+        if fmt not in ("bf16", "fp8"):
+            raise ValueError(f"weight_format must be bf16 or fp8, not {fmt!r}")
+        if fmt == "fp8" and decode_graph not in (None, "auto"):
+            raise ValueError("weight_format fp8 has one decode graph: leave decode_graph at auto")
+        self.weight_format = fmt
+        self.cfg, self.w = cfg, fp8_weights(w) if fmt == "fp8" else w
         self.keep_logits = keep_logits
         self._cos = self._sin = None
         self._shape = None
@@ -413,16 +465,17 @@ class Engine:
         if self._cos is None or self._cos.shape[0] < n:
             self._cos, self._sin = _rope_tables(n, self.cfg.head_dim, self.cfg.theta, DEVICE)
 
-    def _setup(self, B, S, N):
-        key = (B, S, N)
+    def _setup(self, B, S, N, sampled=False):
+        key = (B, S, N, sampled)
         if self._shape == key:
             return
         self._shape = None
         self.g1 = self.gk = None
+        self.sampled = sampled
         self.k_cache = self.v_cache = self.kv4 = None
         torch.cuda.empty_cache()
         cfg = self.cfg
-        self.K = draft_len(B) if self.spec and N > 2 else 0
+        self.K = draft_len(B) if self.spec and N > 2 and not sampled else 0
         # with speculation a sequence can run ahead of the slowest by N + K tokens
         need = S + 2 * N + 2 * self.K + 2 if self.K else S + N + 1
         cap = -(-need // 16) * 16
@@ -445,8 +498,14 @@ class Engine:
         self.attn_out = torch.zeros_like(self.q1)
         self.act = torch.zeros(B, cfg.inter, dtype=bf, device=dev)
         self.rope = torch.zeros(B, 2, cfg.head_dim, dtype=bf, device=dev)
-        self.logits = (torch.zeros(B, cfg.vocab, dtype=bf, device=dev) if self.keep_logits
-                       else None)
+        self.logits = (torch.zeros(B, cfg.vocab, dtype=bf, device=dev)
+                       if self.keep_logits or sampled or self.weight_format == "fp8" else None)
+        if sampled:
+            self.sampler = Sampler(B, cfg.vocab, dev)
+            # the settings, and a step's random numbers, where the captured step reads them
+            self.settings = [torch.zeros(B, dtype=t, device=dev)
+                             for t in (torch.float32, torch.int32, torch.float32, torch.float32)]
+            self.u = torch.zeros(B, dtype=torch.float32, device=dev)
         # ids of step j land in row j: the prefill's by a copy, the decode steps'
         # straight from the LM head's tail (ring_ctr: the next row it writes)
         self.pin_ids = torch.empty(N + 1, B, dtype=torch.int64, pin_memory=True)
@@ -466,7 +525,9 @@ class Engine:
                    down=[l["down"] for l in L], lm=[self.w["lm_head"]])
         deadline = time.monotonic() + TUNE_BUDGET_S
         kind = self.decode_graph
-        if kind == "auto":
+        if self.weight_format == "fp8":
+            kind = "fp8"
+        elif kind == "auto":
             kind = auto_graph(cfg, B)
         elif kind == "timed" and B > FUSED_MAX_TIMED:
             kind = "hipblaslt"
@@ -476,6 +537,9 @@ class Engine:
             g_fused = self._setup_fused(raw, deadline)
         if kind in ("timed", "hipblaslt"):
             g_mm = self._setup_mm()
+        if kind == "fp8":
+            self.g8 = self._fp8_projections(B)
+            g_mm = self._capture(self._step1_fp8)
         if kind == "timed":
             # keep whichever decode graph is faster here, measured during setup
             t_f = min(self._time_graph(g_fused) for _ in range(2))
@@ -507,6 +571,16 @@ class Engine:
                           else torch.zeros(B, cfg.vocab, dtype=bf, device=dev))
         return self._capture(self._step1_mm)
 
+    def _fp8_projections(self, M):
+        """A step's projections of M rows on 8-bit weights."""
+        cfg = self.cfg
+        H, e = cfg.hidden, cfg.eps
+        return dict(qkv=Fp8Linear(M, cfg.nqkv, H, EPI_BF16, True, e, DEVICE),
+                    o=Fp8Linear(M, H, cfg.nq * cfg.head_dim, EPI_RESID, False, device=DEVICE),
+                    gu=Fp8Linear(M, cfg.inter, H, EPI_SWIGLU, True, e, DEVICE),
+                    down=Fp8Linear(M, H, cfg.inter, EPI_RESID, False, device=DEVICE),
+                    lm=Fp8Linear(M, cfg.vocab, H, EPI_BF16, True, e, DEVICE))
+
     def _setup_verify(self, raw, deadline):
         """Buffers, GEMVs and the captured graph of the verify step, and the
         break-even tokens per verify step (engine.py:209-223)."""
@@ -537,15 +611,18 @@ class Engine:
             # T-token tiles and the merge as its own launch: one wavefront per row,
             # where the fused combine would merge a pair's T x 4 rows in one wavefront
             self.attnk = DecodeAttention(B, T, self.cap, cfg.nq, cfg.nkv, cfg.head_dim, dev)
-        self.verify_fused = M <= FUSED_VERIFY_ROWS
-        if self.verify_fused:   # one weight pass per projection on the fused GEMVs
+        fp8 = self.weight_format == "fp8"
+        self.verify_fused = M <= FUSED_VERIFY_ROWS or fp8
+        if fp8:
+            self.gvk, self.gwk = self._fp8_projections(M), raw
+        elif self.verify_fused:   # one weight pass per projection on the fused GEMVs
             self.gvk, self.gwk = build_decode_gemvs(cfg, M, raw, deadline, self._tiled,
                                                     tune=TUNE, log="verify ")
         else:                   # hipBLASLt GEMMs between the fused ops
             self.nT = torch.zeros(M, H, dtype=bf, device=dev)
             self.guT = torch.zeros(M, 2 * cfg.inter, dtype=bf, device=dev)
         self.logitsT = (torch.zeros(M, cfg.vocab, dtype=bf, device=dev)
-                        if self.keep_logits or not self.verify_fused else None)
+                        if self.keep_logits or not self.verify_fused or fp8 else None)
         self.gk = self._capture(self._stepk)
         t1 = min(self._time_graph(self.g1) for _ in range(2))
         tk = min(self._time_graph(self.gk) for _ in range(2))
@@ -596,7 +673,9 @@ class Engine:
         return ((self.k_cache[i], self.v_cache[i]) if self.kv4 is None else (self.kv4[i], None))
 
     def _fuse_o(self):
-        return FUSE_OPROJ and self.kv4 is None and self.attn.oproj_fusable()
+        # a sampled step's ids do not pass the ring that reports a wait that gave up
+        return (FUSE_OPROJ and self.kv4 is None and not self.sampled and self.weight_format == "bf16"
+                and self.attn.oproj_fusable())
 
     def _check_sync(self):
         if self.kv4 is None:
@@ -616,6 +695,12 @@ class Engine:
                          *self._caches(i), self._cos, self._sin, self.pos,
                          self.rope, cfg.eps, fuse_o,
                          next_norm=L[i + 1]["w_in"] if i + 1 < len(L) else None, normed=i > 0)
+        if self.sampled:
+            g["lm"](h, W["lm"][0], y=self.logits, nw=self.w["final_norm"], ids=self.ids)
+            self._choose(self.logits)
+            self._advance()
+            rope_rows(self.pos, self._cos, self._sin, self.rope)   # the next step's
+            return
         # LM head + greedy ids + pos += 1 + the next step's embedding rows and RoPE
         # rows + the ids into the pinned host ring, in one call
         g["lm"](h, W["lm"][0], y=self.logits, nw=self.w["final_norm"], ids=self.ids,
@@ -646,9 +731,38 @@ class Engine:
             h.add_(torch.mm(self.act, lw["down"].t()))
         add_rms_norm(h, None, self.w["final_norm"], self.nrm, eps)
         torch.mm(self.nrm, self.w["lm_head"].t(), out=self.logits_mm)
-        argmax_rows(self.logits_mm, self.ids)
+        self._choose(self.logits_mm)
+        self._advance()
+
+    def _step1_fp8(self):
+        """One decode token per sequence on 8-bit weights: 5 projections a layer and step as in
+        _step1, which quantise their inputs themselves."""
+        cfg, w, g, h = self.cfg, self.w, self.g8, self.h   # h holds embed[ids]
+        rope_rows(self.pos, self._cos, self._sin, self.rope)
+        for i, lw in enumerate(w["layers"]):
+            g["qkv"](h, lw["qkv"], y=self.qkv, nw=lw["w_in"])
+            caches = (self.kv4[i],) if self.kv4 is not None else self._caches(i)
+            self.attn.decode_qkv(self.qkv, lw["q_norm"], lw["k_norm"], self._cos, self._sin,
+                                 self.pos, *caches, self.attn_out, cfg.eps, rope=self.rope)
+            g["o"](self.attn_out, lw["o"], h=h)
+            g["gu"](h, lw["gu"], y=self.act, nw=lw["w_post"])
+            g["down"](self.act, lw["down"], h=h)
+        g["lm"](h, w["lm_head"], y=self.logits, nw=w["final_norm"])
+        self._choose(self.logits)
+        self._advance()
+
+    def _choose(self, logits):
+        """The step's ids from its logits: drawn, or the greedy ones."""
+        if self.sampled:
+            t, k, p, m = self.settings
+            self.sampler(logits, self.u, self.ids, temperature=t, top_k=k, top_p=p, min_p=m)
+        else:
+            argmax_rows(logits, self.ids)
+
+    def _advance(self):
+        """The next step's positions and input rows."""
         self.pos.add_(1)
-        embed_ss(self.ids, self.w["embed"], h, None)
+        embed_ss(self.ids, self.w["embed"], self.h, None)
 
     def _stepk(self):
         """Verify step (engine.py:403-416): vin[b] = [last accepted token, K drafts]
@@ -687,7 +801,10 @@ class Engine:
                 torch.mm(self.nT, lw["gu"].t(), out=self.guT)
                 silu_mul(self.guT, self.actT)
                 h.add_(torch.mm(self.actT, lw["down"].t()))
-        if fused:
+        if self.weight_format == "fp8":
+            g["lm"](h, W["lm"][0], y=self.logitsT, nw=self.w["final_norm"])
+            argmax_rows(self.logitsT, self.vout.view(-1))
+        elif fused:
             g["lm"](h, W["lm"][0], y=self.logitsT, nw=self.w["final_norm"], ids=self.vout.view(-1))
         else:
             add_rms_norm(h, None, self.w["final_norm"], self.nT, eps)
@@ -725,8 +842,12 @@ class Engine:
             kc, vc = (torch.empty(1, B, self.cfg.nkv, S, self.cfg.head_dim, dtype=torch.bfloat16,
                                   device=prompt.device) for _ in range(2))
             sink = lambda i, k, v: kv4_write(k, v, self.kv4[i])
-        ids, logits = prefill(self.cfg, self.w, prompt, kc, vc, self._cos, self._sin, sink)
-        self.ids.copy_(ids)
+        run = prefill_fp8 if self.weight_format == "fp8" else prefill
+        ids, logits = run(self.cfg, self.w, prompt, kc, vc, self._cos, self._sin, sink)
+        if self.sampled:
+            self._choose(logits)
+        else:
+            self.ids.copy_(ids)
         self._set_pos(prompt.shape[1])
         embed_ss(self.ids, self.w["embed"], self.h, None)   # the first decode step's input
         if self.logits is not None:
@@ -773,15 +894,22 @@ class Engine:
 
     # --------------------------------------------------------------- generate
     @torch.inference_mode()
-    def generate(self, input_ids: list, max_new_tokens: int):
+    def generate(self, input_ids: list, max_new_tokens: int, sampling=None):
         N = max_new_tokens
         if N <= 0:
             return
         B, S = len(input_ids), len(input_ids[0])
+        columns = sampling.columns(B) if sampling is not None else None
         # nothing from an earlier call may still write the ring or the caches
         torch.cuda.synchronize()
-        self._setup(B, S, N)
+        self._setup(B, S, N, sampled=sampling is not None)
         stream = torch.cuda.current_stream()
+        numbers = None
+        if sampling is not None:
+            for t, v in zip(self.settings, columns):
+                t.copy_(v)
+            numbers = torch.rand(N, B, generator=torch.Generator().manual_seed(sampling.seed)).to(DEVICE)
+            self.u.copy_(numbers[0])
         try:
             prompt = torch.tensor(input_ids, dtype=torch.int64).pin_memory().to(
                 DEVICE, non_blocking=True)
@@ -796,13 +924,19 @@ class Engine:
             # the host waits for row j to fill (rows start at -1) instead of
             # recording an event per step; the hipBLASLt step's ids are copied
             # after each replay and waited for with an event.
-            ring = self.step_kind == "fused"
+            ring = self.step_kind == "fused" and not self.sampled
             if ring:
                 self._ring_np[1:] = -1
                 self.ring_ctr.fill_(1)
+
+            def replay(j):
+                if numbers is not None:
+                    self.u.copy_(numbers[j])   # behind the step that reads the last ones
+                self.g1.replay()
+
             # Keep one replay in flight: queue step j before waiting for step j-1.
             if N > 1:
-                self.g1.replay()
+                replay(1)
                 if not ring:
                     ids_h[1].copy_(self.ids, non_blocking=True)
                     ev[1].record(stream)
@@ -810,7 +944,7 @@ class Engine:
             yield ids_h[0].tolist()
             for j in range(1, N):
                 if j + 1 < N:
-                    self.g1.replay()
+                    replay(j + 1)
                     if not ring:
                         ids_h[j + 1].copy_(self.ids, non_blocking=True)
                         ev[j + 1].record(stream)

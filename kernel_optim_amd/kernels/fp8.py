@@ -5,7 +5,8 @@ caller's, every call launches on the current stream of the current device and ne
 (so calls can be captured), and a bad argument raises ValueError before anything is launched.
 
 - ``fp8_quantize``: rows [rows, K] in bf16 or fp32, behind an RMSNorm if asked, to 8 bits (a
-  weight once at load, a projection's input in every call); ``fp8_read`` gives the values back;
+  weight once at load, a projection's input in every call); ``fp8_read`` gives the values back,
+  ``fp8_slice`` a part of the rows;
 - ``Fp8Linear``: ``Gemv`` (engine/kernels/gemv.py:109-150) with both factors in 8 bits, for any
   number of rows: y = x W^T with a norm in front and the F32, BF16, RESID or SWIGLU epilogue.
 
@@ -68,6 +69,16 @@ def fp8_empty(rows, K, device, pair=False):
     return Fp8Tensor(torch.empty(tiles, blocks, 2048, dtype=torch.uint8, device=device),
                      torch.empty(tiles, _cdiv(blocks, 4), 64, dtype=torch.uint8, device=device),
                      rows, K, pair)
+
+
+def fp8_slice(t, begin, end):
+    """Rows begin .. end - 1 of t, which share its memory: begin a multiple of 16, end too unless it is
+    the last row. Not of a pair."""
+    _need(isinstance(t, Fp8Tensor) and not t.pair, "t must be an Fp8Tensor that is no pair")
+    _need(0 <= begin < end <= t.rows and begin % 16 == 0 and (end % 16 == 0 or end == t.rows),
+          f"rows {begin} to {end} of {t.rows} are not whole tiles")
+    at = slice(begin // 16, _cdiv(end, 16))
+    return Fp8Tensor(t.codes[at], t.scales[at], end - begin, t.K)
 
 
 def _check_held(t, name, rows, K, pair, dev):

@@ -103,6 +103,16 @@ def weights_to(w, device):
     return out
 
 
+def fp8_weights(w):
+    """Weights on the GPU with every projection and the LM head in 8 bits (kernels.fp8): a new dict; the
+    embedding, which is gathered from, and the norm gains are w's own."""
+    from .kernels.fp8 import fp8_quantize
+    layers = [{k: fp8_quantize(v, pair=k == "gu") if k in ("qkv", "o", "gu", "down") else v
+               for k, v in l.items()} for l in w["layers"]]
+    return dict(embed=w["embed"], final_norm=w["final_norm"], lm_head=fp8_quantize(w["lm_head"]),
+                layers=layers)
+
+
 def load_checkpoint(path, device="cpu"):
     """(config, weights) from a local HF Qwen3 directory: config.json and
     *.safetensors shards. Builds the concatenated qkv / gate-up layout."""

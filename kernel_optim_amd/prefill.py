@@ -27,7 +27,9 @@ import torch.autograd.forward_ad as forward_ad
 import torch.nn.functional as F
 from torch.utils._device import DeviceContext
 
+from .kernels.fp8 import Fp8Linear, fp8_empty, fp8_quantize, fp8_slice
 from .kernels.fused import prefill_norm, prefill_qkv, silu_mul2
+from .kernels.gemv import EPI_BF16, EPI_RESID, EPI_SWIGLU
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -258,4 +260,42 @@ def prefill(cfg, w, prompt, k_cache, v_cache, cos, sin, sink=None):
         x = x + delta
     xl = rmsnorm(x[:, -1:], w["final_norm"], cfg.eps)
     logits = F.linear(xl, w["lm_head"])[:, -1]
+    return torch.argmax(logits, dim=-1), logits
+
+
+@torch.no_grad()
+def prefill_fp8(cfg, w, prompt, k_cache, v_cache, cos, sin, sink=None):
+    """prefill with the projections and the LM head in 8 bits (model.fp8_weights): the norms, the
+    residual adds and SwiGLU are the projections' own, q, k and v take the row kernel of the
+    bf16 prefill, attention is the same. Arguments and results as prefill's."""
+    B, S = prompt.shape
+    H, nq, nkv, d, eps, dev = cfg.hidden, cfg.nq, cfg.nkv, cfg.head_dim, cfg.eps, prompt.device
+    M, wide, narrow = B * S, nq * d, nkv * d
+    exact_gqa = gqa_exact(dev)
+    x = F.embedding(prompt, w["embed"]).view(M, H)
+    new = lambda n: torch.empty(M, n, dtype=BF16, device=dev)
+    held, act = fp8_empty(M, H, dev), new(cfg.inter)
+    qkv = [Fp8Linear(M, n, H, EPI_BF16, False, device=dev) for n in (wide, narrow, narrow)]
+    o = Fp8Linear(M, H, wide, EPI_RESID, False, device=dev)
+    gu = Fp8Linear(M, cfg.inter, H, EPI_SWIGLU, True, eps, device=dev)
+    down = Fp8Linear(M, H, cfg.inter, EPI_RESID, False, device=dev)
+    ends = (0, wide, wide + narrow, wide + 2 * narrow)
+    for i, lw in enumerate(w["layers"]):
+        kc, vc = (k_cache[i], v_cache[i]) if sink is None else (k_cache[0], v_cache[0])
+        fp8_quantize(x, out=held, nw=lw["w_in"], eps=eps)
+        q, k, v = new(wide), new(narrow), new(narrow)
+        for op, y, a, b in zip(qkv, (q, k, v), ends, ends[1:]):
+            op(held, fp8_slice(lw["qkv"], a, b), y=y)
+        prefill_qkv(q, k, v, lw["q_norm"], lw["k_norm"], cos, sin, kc, vc, eps)
+        a = causal_attention(q.view(B, S, nq, d).transpose(1, 2), kc[:, :, :S], vc[:, :, :S],
+                             d ** -0.5, exact_gqa)
+        o(a.transpose(1, 2).reshape(M, wide), lw["o"], h=x)
+        gu(x, lw["gu"], y=act, nw=lw["w_post"])
+        down(act, lw["down"], h=x)
+        if sink is not None:
+            sink(i, kc[:, :, :S], vc[:, :, :S])
+    last = x.view(B, S, H)[:, -1].contiguous()
+    logits = torch.empty(B, cfg.vocab, dtype=BF16, device=dev)
+    Fp8Linear(B, cfg.vocab, H, EPI_BF16, True, eps, device=dev)(last, w["lm_head"], y=logits,
+                                                               nw=w["final_norm"])
     return torch.argmax(logits, dim=-1), logits

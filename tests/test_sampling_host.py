@@ -35,3 +35,14 @@ def test_c_abi_refuses():
     assert call(V=(1 << 20) + 1) == call(B=65536) == call(chunks=1025) == ERANGE
     assert h.ko_sample_scratch(0, 1) == h.ko_sample_scratch(1, 0) == h.ko_sample_scratch(1, 1025) == -1
     assert h.ko_sample_scratch(7, 1) == 0
+
+
+def test_engine_settings():
+    from kernel_optim_amd.engine import Sampling
+    t, k, p, m = Sampling(temperature=[0.5, 1], top_k=2 ** 40, top_p=0.25).columns(2)
+    assert t.tolist() == [0.5, 1.0] and k.tolist() == [2 ** 31 - 1] * 2
+    assert p.tolist() == [0.25, 0.25] and m.tolist() == [0.0, 0.0]
+    for bad in (Sampling(temperature=-1), Sampling(top_k=1.5), Sampling(top_p=2), Sampling(min_p="0"),
+                Sampling(temperature=[1.0]), Sampling(min_p=float("nan"))):
+        with pytest.raises(ValueError):
+            bad.columns(2)
