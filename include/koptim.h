@@ -449,10 +449,15 @@ int ko_fp8_read(const void* codes, const void* scales, int rows, int K, int pair
  * the call quantises (behind a norm with gain nw, as ko_fp8_quantize), with xc and xs, a matrix
  * [M, K], as scratch; or NULL, and xc and xs hold it. epi 0: y
  * fp32; 1: bf16; 2 (RESID): y = bf16(h + bf16(sum)), h [M, N] bf16, which may be y; 3 (SWIGLU): W is
- * gate | up [2 N, K] held as a pair, y = bf16(bf16(silu(bf16(gate sum))) * bf16(up sum)). */
+ * gate | up [2 N, K] held as a pair, y = bf16(bf16(silu(bf16(gate sum))) * bf16(up sum)). scratch: of
+ * ko_fp8_linear_scratch bytes, 16-byte aligned, zeroed before the first call and left fit for the next;
+ * calls that share it, or xc and xs, must not overlap. */
 int ko_fp8_linear(const void* x, const void* nw, float eps, void* xc, void* xs, const void* wc,
-                  const void* ws, void* y, const void* h, int M, int N, int K, int epi,
-                  void* stream);
+                  const void* ws, void* y, const void* h, void* scratch, long long scratch_bytes,
+                  int M, int N, int K, int epi, void* stream);
+
+/* Bytes of ko_fp8_linear's scratch, 0 among them. A size, not a status; -1 for bad arguments. */
+long long ko_fp8_linear_scratch(int M, int N, int K, int epi);
 
 /* ---- Sampling ---------------------------------------------------------------------
  * In the place of torch.argmax(logits) of the reference's decode steps (engine/engine.py:299,

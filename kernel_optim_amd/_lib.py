@@ -89,7 +89,8 @@ SIGNATURES = {
                         _c_void_p],
     "ko_fp8_read": [_c_void_p, _c_void_p, _int, _int, _int, _c_void_p, _int, _ll, _c_void_p],
     "ko_fp8_linear": [_c_void_p, _c_void_p, _f, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
-                      _c_void_p, _c_void_p, _int, _int, _int, _int, _c_void_p],
+                      _c_void_p, _c_void_p, _c_void_p, _ll, _int, _int, _int, _int, _c_void_p],
+    "ko_fp8_linear_scratch": [_int, _int, _int, _int],
     "ko_sample": [_c_void_p, _int, _ll, _int, _int, _c_void_p, _c_void_p, _f, _c_void_p, _int,
                   _c_void_p, _f, _c_void_p, _f, _c_void_p, _c_void_p, _c_void_p, _ll, _int,
                   _c_void_p],
@@ -98,7 +99,8 @@ SIGNATURES = {
 
 # Entry points whose return value is a size, not a status.
 RESTYPES = {"ko_gemv_argmax_scratch": _ll, "ko_decode_attn_qkv_oproj_sync_ints": _ll,
-            "ko_kv4_attn_scratch": _ll, "ko_sample_scratch": _ll}
+            "ko_kv4_attn_scratch": _ll, "ko_sample_scratch": _ll,
+            "ko_fp8_linear_scratch": _ll}
 
 _ERRORS = {-22: "invalid argument", -34: "size out of range", -95: "unsupported shape"}
 

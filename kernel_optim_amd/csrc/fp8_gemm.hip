@@ -147,6 +147,8 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_kernel(LinearArgs a, int nb
     KO_STEP(3)
 #undef KO_STEP
   }
+  // no load into LDS outlives the workgroup: past the end there are some that nothing waited for
+  if constexpr (STAGES > 2) __builtin_amdgcn_s_waitcnt(15 << 8 | 7 << 4);
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
     const int m = (m0 + wm * TM + j) * 16 + r;
@@ -214,22 +216,39 @@ int launch(const LinearArgs& a, hipStream_t s) {
 
 }  // namespace
 
+static void set_sizes(LinearArgs& a, int M, int N, int K, int epi) {
+  a.M = M, a.N = N, a.K = K;
+  a.xt = (int)fp8_tiles(M, false);
+  a.wt = (int)(epi == EPI_SWIGLU ? fp8_tiles(2 * N, true) : fp8_tiles(N, false));
+}
+
 extern "C" {
+
+long long ko_fp8_linear_scratch(int M, int N, int K, int epi) {
+  if (M < 1 || N < 1 || N > 0x3fffffff || K < 8 || (K & 7) || epi < EPI_F32 || epi > EPI_SWIGLU) return -1;
+  LinearArgs a;
+  set_sizes(a, M, N, K, epi);
+  return !few_rows_served(a) && mid_rows_served(a, epi) ? mid_rows_scratch(a) : 0;
+}
 
 int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K, int pair,
                     const void* nw, float eps, void* codes, void* scales, void* stream);
 
 int ko_fp8_linear(const void* x, const void* nw, float eps, void* xc, void* xs, const void* wc,
-                  const void* ws, void* y, const void* h, int M, int N, int K, int epi,
-                  void* stream) {
+                  const void* ws, void* y, const void* h, void* scratch, long long scratch_bytes,
+                  int M, int N, int K, int epi, void* stream) {
   if (!xc || !xs || !wc || !ws || !y || M < 1 || N < 1 || K < 8 || (K & 7)) return KO_EINVAL;
   if (epi < EPI_F32 || epi > EPI_SWIGLU) return KO_ENOTSUP;
   if ((epi == EPI_RESID && !h) || (nw && !x)) return KO_EINVAL;
   const uintptr_t all = (uintptr_t)xc | (uintptr_t)xs | (uintptr_t)wc | (uintptr_t)ws | (uintptr_t)y |
                         (uintptr_t)x | (uintptr_t)nw;
-  if ((all | (uintptr_t)h) & 15) return KO_EINVAL;
+  if ((all | (uintptr_t)h | (uintptr_t)scratch) & 15) return KO_EINVAL;
   if (N > 0x3fffffff) return KO_ERANGE;
+  const long long need = ko_fp8_linear_scratch(M, N, K, epi);
+  if (need && (!scratch || scratch_bytes < need)) return KO_EINVAL;
   LinearArgs a;
+  a.counters = static_cast<int*>(scratch);
+  a.part = static_cast<float*>(scratch) + 1024;
   a.x = static_cast<const uint16_t*>(x);
   a.nw = static_cast<const uint16_t*>(nw);
   a.eps = eps;
@@ -239,9 +258,7 @@ int ko_fp8_linear(const void* x, const void* nw, float eps, void* xc, void* xs, 
   a.ws = static_cast<const uint32_t*>(ws);
   a.y = y;
   a.h = static_cast<const uint16_t*>(h);
-  a.M = M, a.N = N, a.K = K;
-  a.xt = (int)fp8_tiles(M, false);
-  a.wt = (int)(epi == EPI_SWIGLU ? fp8_tiles(2 * N, true) : fp8_tiles(N, false));
+  set_sizes(a, M, N, K, epi);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool few = few_rows_served(a);
   if (x && !(few && few_rows_quantized(a))) {

@@ -17,6 +17,8 @@ struct LinearArgs {
   const uint16_t* h;          // RESID: what is added; may be y
   int M, N, K;
   int xt, wt;                 // tiles of x and of W
+  float* part;                // scratch: partial sums,
+  int* counters;              // and counters, zero before every call and behind it
 };
 
 // RESID: columns n .. n + 3 of h's row m as packed bf16, loaded ahead of the sums they are added to.
@@ -108,6 +110,7 @@ int launch_few_rows(const LinearArgs& a, int epi, hipStream_t s);
 
 // fp8_mid.hip: up to 64 rows of x in codes.
 bool mid_rows_served(const LinearArgs& a, int epi);
+long long mid_rows_scratch(const LinearArgs& a);   // bytes
 int launch_mid_rows(const LinearArgs& a, int epi, hipStream_t s);
 
 }  // namespace ko

@@ -3,8 +3,7 @@
 // As for fewer rows a workgroup's 8 wavefronts share K and stream tiles of W, but every block of W
 // now meets 2 or 4 blocks of x: a wavefront holds the codes of its blocks of x in registers for the
 // whole launch (K = 2560, 64 rows: 96 of its 256), where loads of x between those of W would make
-// each wait for the weights ahead of it. Longer rows do not fit: they take x with W, block by
-// block, several blocks ahead. 2 tiles go through bf16 (fp8_core.h); 4 would spill the registers so
+// each wait for the weights ahead of it. Longer rows do not fit: they are split. 2 tiles go through bf16 (fp8_core.h); 4 would spill the registers so
 // (64 rows of gate/up 36 us) and go to the matrix instruction as codes (19 us).
 #include "fp8_linear.h"
 
@@ -66,12 +65,11 @@ __device__ __forceinline__ void multiply(const Block& w, const Block (&x)[MT], f
   }
 }
 
-// The sums of W wavefronts for tile t of x and a tile of W, stored.
+// The sums of tile t of x and a tile of W, stored.
 template <int EPI>
-__device__ __forceinline__ void finish(const LinearArgs& a, const f32x4 (*part)[64], int stride, int W,
-                                       int tile, int t, int lane, uint2 hv) {
+__device__ __forceinline__ void finish(const LinearArgs& a, f32x4 sum, int tile, int t, int lane,
+                                       uint2 hv) {
   const int r = lane & 15, g = lane >> 4, m = 16 * t + r;
-  const f32x4 sum = add_parts(part, stride, W, lane);
   if constexpr (EPI == EPI_SWIGLU) {
     f32x4 up;   // 32 lanes on
 #pragma unroll
@@ -130,47 +128,96 @@ __global__ __launch_bounds__(64 * WMAX) void mid_kernel(LinearArgs a) {
     load_next();
     __syncthreads();   // of the next step but one: every wavefront is past this step's sums
     for (int t = mine; t < MT; t += W)
-      finish<EPI>(a, &s_part[st & 1][0][t], MT, W, tile, t, lane,
+      finish<EPI>(a, add_parts(&s_part[st & 1][0][t], MT, W, lane), tile, t, lane,
                   EPI == EPI_RESID && t != mine ? load4(a, 16 * t + r, tile * 16 + 4 * g) : hv);
   };
   pipeline<SETS>(steps, load, step);
 }
 
-// Any K: a workgroup takes one tile of W, its wavefronts a run of blocks each, D of them ahead.
+// Longer rows: a workgroup takes two tiles of W and one of S runs of K's blocks, its wavefronts a part
+// of the run each, D blocks of x and W ahead. One workgroup a CU then reads as little as it can: a CU
+// takes in some 45 bytes a ns, from whichever cache, and 80 workgroups that read all of K (of 9728
+// values by 64 rows, 160 with one tile each: 20 us) leave most of them idle. The S partial sums of
+// a pair of tiles meet in memory, where the last of its workgroups adds them in order.
 template <int EPI, int MT>
-__global__ __launch_bounds__(64 * WMAX) void mid_deep_kernel(LinearArgs a) {
-  constexpr int W = WMAX, D = 4;
-  __shared__ f32x4 s_part[W][MT][64];
+__global__ __launch_bounds__(64 * WMAX) void split_kernel(LinearArgs a, int S) {
+  constexpr int W = WMAX, NT = 2, D = MT == 4 ? 2 : 4, PARTS = MT * NT;
+  __shared__ f32x4 s_part[W][PARTS][64];
+  __shared__ int s_arrived;
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int KB = fp8_blocks(a.K), Q = fp8_quads(a.K);
-  const int begin = KB * wv / W, end = KB * (wv + 1) / W, tile = blockIdx.x;
-  Block x[D][MT], w[D];
+  const int pair = blockIdx.x / S, run = blockIdx.x - pair * S;
+  const int r0 = KB * run / S, r1 = KB * (run + 1) / S;
+  const int begin = r0 + (r1 - r0) * wv / W, end = r0 + (r1 - r0) * (wv + 1) / W;
+  const int tile0 = pair * NT;
+  Block x[D][MT], w[D][NT];
   auto load = [&](int kb, int i) {
     if (kb >= end) return;
-    w[i].load_w(a, tile, kb, KB, Q, lane);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) w[i][t].load_w(a, min(tile0 + t, a.wt - 1), kb, KB, Q, lane);
 #pragma unroll
     for (int t = 0; t < MT; ++t) x[i][t].load_x(a, min(t, a.xt - 1), kb, KB, Q, lane);
   };
 #pragma unroll
   for (int i = 0; i < D; ++i) load(begin + i, i);
+  // wavefront wv < PARTS ends with the sums of tile wv / MT of W and wv % MT of x
+  const int tile = tile0 + wv / MT, xt = wv % MT;
   uint2 hv = make_uint2(0, 0);
-  if constexpr (EPI == EPI_RESID)
-    if (wv < MT) hv = load4(a, 16 * wv + r, tile * 16 + 4 * g);
-  f32x4 acc[MT];
+  if constexpr (EPI == EPI_RESID) hv = load4(a, 16 * xt + r, tile * 16 + 4 * g);
+  f32x4 acc[NT][MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = {0.f, 0.f, 0.f, 0.f};
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[n][t] = {0.f, 0.f, 0.f, 0.f};
   for (int k0 = begin; k0 < end; k0 += D) {
 #pragma unroll
     for (int i = 0; i < D; ++i) {
       if (k0 + i >= end) break;
-      multiply<MT>(w[i], x[i], acc);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) multiply<MT>(w[i][n], x[i], acc[n]);
       load(k0 + i + D, i);
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) s_part[wv][t][lane] = acc[t];
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) s_part[wv][n * MT + t][lane] = acc[n][t];
   __syncthreads();
-  if (wv < MT) finish<EPI>(a, &s_part[0][wv], MT, W, tile, wv, lane, hv);
+  const bool adds = wv < PARTS;   // uniform per wavefront
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (adds) sum = add_parts(&s_part[0][wv], PARTS, W, lane);
+  if (S > 1) {
+    typedef unsigned long long u64;
+    u64* slots = reinterpret_cast<u64*>(a.part) + (long long)pair * S * PARTS * 128;
+    if (adds) {
+      u64* mine = slots + ((long long)run * PARTS + wv) * 128 + 2 * lane;
+      const u64* v = reinterpret_cast<const u64*>(&sum);
+      __hip_atomic_store(mine, v[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(mine + 1, v[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __builtin_amdgcn_s_waitcnt(0);   // this thread's slot stores are performed
+    __syncthreads();
+    if (threadIdx.x == 0)
+      s_arrived = __hip_atomic_fetch_add(a.counters + pair, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (s_arrived != S - 1) return;
+    if (threadIdx.x == 0)   // for the next call
+      __hip_atomic_store(a.counters + pair, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (adds) {
+      sum = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < S; ++i) {
+        const uint4 v = ldg16_coherent(slots + ((long long)i * PARTS + wv) * 128 + 2 * lane);
+        sum += (f32x4){__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+      }
+    }
+  }
+  if (adds && tile < a.wt) finish<EPI>(a, sum, tile, xt, lane, hv);
+}
+
+int split_pairs(const LinearArgs& a) { return (a.wt + 1) / 2; }
+int split_runs(const LinearArgs& a) {
+  const int s = 256 / split_pairs(a), most = fp8_blocks(a.K) / WMAX;   // a block for every wavefront
+  return s < 1 ? 1 : s < most ? s : most;
 }
 
 template <int EPI, int MT>
@@ -187,7 +234,10 @@ int launch(const LinearArgs& a, hipStream_t s) {
   } else if (KB <= 32) {
     if (one || MT == 4) KO_MID(4, 1);   // 64 rows: a second set would spill
     else KO_MID(4, MT == 4 ? 1 : 2);
-  } else hipLaunchKernelGGL((mid_deep_kernel<EPI, MT>), dim3(a.wt), dim3(64 * WMAX), 0, s, a);
+  } else {
+    const int S = split_runs(a);
+    hipLaunchKernelGGL((split_kernel<EPI, MT>), dim3(split_pairs(a) * S), dim3(64 * WMAX), 0, s, a, S);
+  }
 #undef KO_MID
   return KO_LAUNCH_STATUS();
 }
@@ -195,6 +245,12 @@ int launch(const LinearArgs& a, hipStream_t s) {
 }  // namespace
 
 namespace ko {
+
+long long mid_rows_scratch(const LinearArgs& a) {
+  const int S = split_runs(a);
+  // the counters first: their place does not depend on the number of rows
+  return fp8_blocks(a.K) <= 32 || S == 1 ? 0 : 4096 + (long long)split_pairs(a) * S * 8192;
+}
 
 bool mid_rows_served(const LinearArgs& a, int epi) { return a.xt <= (epi == EPI_F32 ? 2 : 4); }
 

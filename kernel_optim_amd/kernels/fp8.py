@@ -131,8 +131,9 @@ def fp8_quantize(x, out=None, nw=None, eps=1e-6, pair=False):
     else:
         _check_held(out, "out", rows, K, out.pair if isinstance(out, Fp8Tensor) else pair, dev)
         _need(out.pair or not pair, "out holds no pair")
-        _need_apart(x, out.codes, "x and out")
-        _need_apart(x, out.scales, "x and out")
+        for t in (x,) if nw is None else (x, nw):
+            _need_apart(t, out.codes, "out and what it is made of")
+            _need_apart(t, out.scales, "out and what it is made of")
     _lib.call("ko_fp8_quantize", x.data_ptr(), x.dtype == F32, stride, rows, K, out.pair,
               _lib.ptr(nw), eps, out.codes.data_ptr(), out.scales.data_ptr(), _stream(dev))
     return out
@@ -162,7 +163,8 @@ class Fp8Linear:
     ``x`` is [M, K] bf16 and is quantised in the call (with the norm) into a workspace of the object's,
     or an Fp8Tensor where there is no norm. The workspace is made for ``device``, or in the first
     call, which must not be under graph capture. Calls of one object share it: they must be
-    ordered, on one stream or by events, captured calls' replays included."""
+    ordered, on one stream or by events, captured calls' replays included. y (and h where it is y) must
+    not overlap x, nw or w."""
 
     def __init__(self, M, N, K, epi, norm, eps=1e-6, device=None):
         _need(epi in (EPI_F32, EPI_BF16, EPI_RESID, EPI_SWIGLU), f"bad epilogue {epi}")
@@ -170,7 +172,14 @@ class Fp8Linear:
         fp8_shape((2 if epi == EPI_SWIGLU else 1) * N, K, epi == EPI_SWIGLU)
         fp8_shape(M, K)
         self.M, self.N, self.K, self.epi, self.norm, self.eps = M, N, K, epi, bool(norm), eps
-        self._xq = None
+        self._xq = self._scratch = None
+        wide = (2 if epi == EPI_SWIGLU else 1) * N
+        tiles, blocks = fp8_shape(wide, K, epi == EPI_SWIGLU)
+        # what _usual compares with: shapes, W's rows, and bytes of x, y, h, nw and W
+        self._x, self._y, self._nw = torch.Size((M, K)), torch.Size((M, N)), torch.Size((K,))
+        self._rows, self._dtype = wide, F32 if epi == EPI_F32 else BF16
+        self._bytes = (2 * M * K, M * N * (4 if epi == EPI_F32 else 2), 2 * M * N, 2 * K,
+                       tiles * blocks * 2048, tiles * _cdiv(blocks, 4) * 64)
         if device is not None:
             self._workspace(torch.empty(0, device=device).get_device())
 
@@ -178,30 +187,32 @@ class Fp8Linear:
         if self._xq is None or self._xq.codes.get_device() != dev:
             _need(not torch.cuda.is_current_stream_capturing(), "the workspace is made in the first "
                   "call: make it before the capture, or give the object its device")
-            self._xq = fp8_empty(self.M, self.K, torch.device("cuda", dev))
+            at = torch.device("cuda", dev)
+            n = _lib.lib().ko_fp8_linear_scratch(self.M, self.N, self.K, self.epi)
+            # the counters among it start at zero, and every call leaves them there
+            self._scratch = torch.zeros(max(n, 16), dtype=torch.uint8, device=at)
+            self._xq = fp8_empty(self.M, self.K, at)
         return self._xq
 
     def _usual(self, x, w, y, nw, h):
         """The C arguments of a call that needs no closer look, else None: tests that name each
         fault take longer than a short call on the GPU."""
         try:
-            q, rows = self._xq, x.shape
-            dev, pair = q.codes.get_device(), self.epi == EPI_SWIGLU
-            if self.epi == EPI_RESID:
+            q = self._xq
+            dev, epi = q.codes.get_device(), self.epi
+            nx, ny, nh, nn, nc, ns = self._bytes
+            hp = np = 0
+            if epi == EPI_RESID:
                 hp = h.data_ptr()
                 if y is None:
                     y = h
-                if not (h.dtype is BF16 and h.shape == (self.M, self.N) and h.is_contiguous()
-                        and h.get_device() == dev
-                        and (y is h or abs(y.data_ptr() - hp) >= 2 * h.numel())):
+                if not (h.dtype is BF16 and h.shape == self._y and h.is_contiguous()
+                        and h.get_device() == dev and (y is h or abs(y.data_ptr() - hp) >= nh)):
                     return None
-            else:
-                hp = 0
-                if h is not None:
-                    return None
-            np = 0
+            elif h is not None:
+                return None
             if self.norm:
-                if not (nw.dtype is BF16 and nw.shape == (self.K,) and nw.is_contiguous()
+                if not (nw.dtype is BF16 and nw.shape == self._nw and nw.is_contiguous()
                         and nw.get_device() == dev):
                     return None
                 np = nw.data_ptr()
@@ -209,15 +220,20 @@ class Fp8Linear:
                 return None
             wc, ws, xp, yp = w.codes, w.scales, x.data_ptr(), y.data_ptr()
             cp, sp = wc.data_ptr(), ws.data_ptr()
-            if (type(w) is Fp8Tensor and w.rows == (2 * self.N if pair else self.N)
-                    and w.K == self.K and w.pair is pair and rows == (self.M, self.K)
-                    and y.shape == (self.M, self.N) and x.dtype is BF16
-                    and y.dtype is (F32 if self.epi == EPI_F32 else BF16) and x.is_contiguous()
+            # y apart from what other workgroups still read
+            if (-ny < yp - xp < nx or -ny < yp - cp < nc or -ny < yp - sp < ns
+                    or np and -ny < yp - np < nn):
+                return None
+            if (type(w) is Fp8Tensor and w.rows == self._rows and w.K == self.K
+                    and w.pair is (epi == EPI_SWIGLU) and x.shape == self._x and y.shape == self._y
+                    and x.dtype is BF16 and y.dtype is self._dtype and x.is_contiguous()
                     and y.is_contiguous() and dev == wc.get_device() == x.get_device()
                     == y.get_device() == _current_device()
                     and not (xp | yp | cp | sp | np | hp) & 15):
+                t = self._scratch
                 return (xp, np or None, self.eps, q.codes.data_ptr(), q.scales.data_ptr(), cp, sp, yp,
-                        hp or None, self.M, self.N, self.K, self.epi, _stream(dev))
+                        hp or None, t.data_ptr(), t.numel(), self.M, self.N, self.K, epi,
+                        _stream(dev))
         except (AttributeError, TypeError, RuntimeError):
             pass   # no tensors: the tests below say which
         return None
@@ -246,12 +262,17 @@ class Fp8Linear:
         if isinstance(x, Fp8Tensor):
             _need(not self.norm, "a norm goes with x in bf16")
             _check_held(x, "x", M, K, False, dev)
+            self._workspace(dev)
             q, x = x, None
         else:
             _tensor(x, "x", BF16, (M, K), dev)
             if self.norm:
                 _tensor(nw, "nw", BF16, (K,), dev)
             q = self._workspace(dev)
+        for t in (x, nw, w.codes, w.scales, q.codes, q.scales):   # other workgroups still read these
+            if t is not None:
+                _need_apart(y, t, "y and what the call reads (but h)")
         _lib.call("ko_fp8_linear", _lib.ptr(x), _lib.ptr(nw), self.eps, q.codes.data_ptr(),
                   q.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), y.data_ptr(),
-                  _lib.ptr(h), M, N, K, epi, _stream(dev))
+                  _lib.ptr(h), self._scratch.data_ptr(), self._scratch.numel(), M, N, K, epi,
+                  _stream(dev))

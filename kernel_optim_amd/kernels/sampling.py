@@ -58,7 +58,7 @@ class Sampler:
         as the call runs: a temperature that is not above 0 is 0, a top_k below 1 is 0, a top_p that
         is not below 1 is 1, a min_p that is not above 0 is 0. logprobs [B] fp32 (optional)
         receives the log of the token's share of the kept mass (0 where the first token is
-        taken, -infinity beside the id -1)."""
+        taken, -infinity beside the id -1). ids and logprobs must not overlap the other tensors."""
         B, V, dev = self.B, self.V, self._dev
         usual = self._usual(logits, u, ids, logprobs)
         if usual is None:
@@ -76,6 +76,16 @@ class Sampler:
         k = _setting(top_k, "top_k", torch.int32, B, dev, _whole)
         p = _setting(top_p, "top_p", F32, B, dev, _share)
         m = _setting(min_p, "min_p", F32, B, dev, _share)
+        # outputs apart from what a row's other workgroups still read
+        ins = [(usual[0], logits.element_size() * ((B - 1) * logits.stride(0) + V)), (usual[1], 4 * B)]
+        ins += [(a, 4 * B) for a, _ in (t, k, p, m) if a]
+        outs = [(usual[2], 8 * B)] + ([(usual[3], 4 * B)] if usual[3] else [])
+        for a, n in outs:
+            for c, size in ins + [o for o in outs if o[0] != a]:
+                if a < c + size and c < a + n:
+                    raise ValueError("ids and logprobs must not overlap what the call reads, or each other")
+        if len(outs) == 2 and outs[0][0] == outs[1][0]:
+            raise ValueError("ids and logprobs must not overlap")
         _lib.call("ko_sample", usual[0], logits.dtype is F32, logits.stride(0) if B > 1 else 0, B, V,
                   usual[1], *t, k[0], min(int(k[1]), V), *p, *m, usual[2], usual[3],
                   self._scratch.data_ptr(), self._scratch.numel(), self.chunks, _stream(dev))

@@ -62,11 +62,18 @@ def test_c_abi_refuses():
     r = lambda codes=p, rows=1, K=8, out=p, stride=8: \
         h.ko_fp8_read(codes, p, rows, K, 0, out, 0, stride, None)
     assert r(codes=None) == r(out=None) == r(out=p + 4) == r(rows=0) == r(K=4) == r(stride=1) == EINVAL
-    l = lambda x=None, nw=None, xc=p, y=p, hh=p, M=1, N=8, K=8, epi=EPI_BF16: \
-        h.ko_fp8_linear(x, nw, 0.0, xc, p, p, p, y, hh, M, N, K, epi, None)
+    l = lambda t=p, n=1 << 40, x=None, nw=None, xc=p, y=p, hh=p, M=1, N=8, K=8, epi=EPI_BF16: \
+        h.ko_fp8_linear(x, nw, 0.0, xc, p, p, p, y, hh, t, n, M, N, K, epi, None)
     assert l(x=p + 2) == l(nw=p) == l(x=p, nw=p + 2) == EINVAL
     assert l(xc=None) == l(y=None) == l(M=0) == l(N=0) == l(K=12) == EINVAL
     assert l(hh=None, epi=EPI_RESID) == l(hh=p + 2, epi=EPI_RESID) == EINVAL
     assert l(epi=EPI_ARGMAX) == l(epi=-1) == ENOTSUP
     assert l(N=2 ** 30) == ERANGE
     assert l(epi=EPI_SWIGLU, M=0) == EINVAL
+    assert l(t=p + 4) == EINVAL
+    need = h.ko_fp8_linear_scratch(64, 2560, 9728, EPI_RESID)
+    assert need > 0 and l(M=64, N=2560, K=9728, epi=EPI_RESID, n=need - 1) == EINVAL
+    assert l(M=64, N=2560, K=9728, epi=EPI_RESID, t=None) == EINVAL
+    assert h.ko_fp8_linear_scratch(1, 2560, 9728, EPI_RESID) == 0
+    for bad in ((0, 8, 8, 0), (1, 0, 8, 0), (1, 8, 12, 0), (1, 8, 8, 4), (1, 2 ** 30, 8, 0)):
+        assert h.ko_fp8_linear_scratch(*bad) == -1

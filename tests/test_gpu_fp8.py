@@ -192,7 +192,7 @@ def on(dev, *ts):
 LINEAR = [(1, 16, 8), (1, 5000, 256), (16, 8203, 640), (4, 64, 3000), (9, 48, 9728), (16, 40, 12296),
           (1, 1, 128), (1, 2560, 4096), (2, 1000, 712), (3, 17, 136), (7, 130, 520),
           (16, 256, 2560), (17, 33, 1024), (33, 999, 264), (64, 512, 1152), (65, 130, 640),
-          (20, 5000, 264), (32, 72, 9728), (50, 33, 12296), (61, 4200, 3080), (40, 4112, 2560),
+          (20, 5000, 264), (32, 72, 9728), (64, 2560, 9728), (24, 1304, 4616), (50, 33, 12296), (61, 4200, 3080), (40, 4112, 2560),
           (100, 300, 2568), (130, 640, 896), (257, 515, 384), (300, 1024, 2560),
           (1030, 4100, 712), (4133, 4800, 392)]
 
@@ -289,7 +289,68 @@ def test_refusals(dev):
     both = bf(160)
     bad.append(lambda: Fp8Linear(4, 32, 256, EPI_RESID, False)(
         bf(4, 256), w, y=both[:128].view(4, 32), h=both[32:].view(4, 32)))
+    square, ws = bf(32, 256), fp8_quantize(bf(256, 256))
+    sq = Fp8Linear(32, 256, 256, EPI_BF16, False)
+    bad += [lambda: sq(square, ws, y=square),                 # y over x, over a norm's gain, over w
+            lambda: Fp8Linear(32, 256, 256, EPI_RESID, False)(square, ws, h=square),
+            lambda: Fp8Linear(1, 256, 256, EPI_BF16, True)(bf(1, 256), ws, y=square[:1], nw=square[0]),
+            lambda: sq(square, ws, y=ws.codes.view(-1)[:16384].view(BF16).view(32, 256))]
     for i, f in enumerate(bad):
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"call {i} was taken")
+
+
+@pytest.mark.parametrize("M,N,K,epi,norm", [(1, 208, 2560, "swiglu", True), (4, 160, 9728, "resid", False),
+                                            (16, 640, 4096, "bf16", False), (33, 320, 2560, "bf16", True),
+                                            (64, 256, 9728, "bf16", False), (150, 512, 1152, "swiglu", True),
+                                            (70, 300, 712, "f32", False)])
+def test_captured_and_on_another_stream(dev, M, N, K, epi, norm):
+    """Replays with new rows in place, each against an eager call of another object between them, and
+    the same on a side stream."""
+    x, w, h, nw = projection(dev, M, N, K, epi, norm, seed=M)
+    xd, wd, hd, nwd = on(dev, x, w, h, nw)
+    held = fp8_quantize(wd, pair=epi == "swiglu")
+    dtype = F32 if epi == "f32" else BF16
+    y, z = (torch.zeros(M, N, device=dev, dtype=dtype) for _ in range(2))
+    kw = dict(nw=nwd, h=hd)
+    lazy, eager = (Fp8Linear(M, N, K, EPI[epi], norm) for _ in range(2))
+    op = Fp8Linear(M, N, K, EPI[epi], norm, device=dev)
+    op(xd, held, y=y, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        op(xd, held, y=y, **kw)
+        with pytest.raises(ValueError):   # its workspace would belong to the graph
+            lazy(xd, held, y=y, **kw)
+    for i in range(4):
+        xd.copy_(projection(dev, M, N, K, epi, norm, seed=100 + i)[0])
+        y.fill_(7)
+        graph.replay()
+        eager(xd, held, y=z, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(y, z)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        xd.mul_(2)
+        eager(xd, held, y=y, **kw)
+        y.add_(1)
+    torch.cuda.current_stream().wait_stream(side)
+    eager(xd, held, y=z, **kw)
+    assert torch.equal(y, z + 1)
+
+
+def test_slices_share_memory(dev):
+    from kernel_optim_amd.kernels.fp8 import fp8_slice
+    x = rows(5, 75, 264).to(BF16)
+    t = fp8_quantize(x.to(dev))
+    for a, b in ((0, 16), (16, 64), (64, 75), (0, 75)):
+        part = fp8_slice(t, a, b)
+        out = torch.empty(b - a, 264, dtype=BF16, device=dev)
+        fp8_read(part, out)
+        assert torch.equal(out.cpu(), O.held(x[a:b]).to(BF16))
+        assert part.codes.data_ptr() == t.codes.data_ptr() + a // 16 * 3 * 2048
+    for a, b in ((0, 17), (8, 16), (16, 16), (64, 80), (-16, 16)):
+        with pytest.raises(ValueError):
+            fp8_slice(t, a, b)

@@ -80,6 +80,16 @@ def test_two_layers_at_full_width(dev, monkeypatch):
     check(monkeypatch, cfg, w, prompt, toks, logits, 80)
 
 
+@pytest.mark.parametrize("S", [1, 2, 9])
+def test_short_prompts(dev, monkeypatch, S):
+    cfg, n = SMALL, 4
+    w = perturbed_weights(cfg, seed=5)
+    prompt = prompts(cfg, 2, S)
+    toks, logits = Engine.from_weights(cfg, w, keep_logits=True, weight_format="fp8").trace(
+        prompt.tolist(), n)
+    check(monkeypatch, cfg, w, prompt, toks, logits, 16)
+
+
 def test_weights_are_held_in_8_bits(dev):
     cfg = SMALL
     w = weights_to(perturbed_weights(cfg, seed=5), dev)

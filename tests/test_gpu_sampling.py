@@ -236,6 +236,9 @@ def test_refusals(dev):
            dict(temperature="1"), dict(top_k=-1), dict(top_k=2.5), dict(top_k=ids), dict(top_k=u),
            dict(top_p=-0.1), dict(top_p=1.5), dict(top_p=i32), dict(min_p=2.0), dict(min_p=NAN),
            dict(logprobs=u.half()), dict(logprobs=u[:1]), dict(min_p=torch.zeros(4, device=dev)[::2])]
+    t4 = torch.ones(2, device=dev)
+    bad += [dict(logprobs=u), dict(temperature=t4, logprobs=t4),
+            dict(logprobs=ids.view(torch.float32)[:2]), dict(u=ids.view(torch.float32)[1:3])]
     for kw in bad:
         with pytest.raises(ValueError):
             s(**(dict(logits=x, u=u, ids=ids) | kw))
