@@ -23,8 +23,8 @@
 //   where its codes' own rounding is 2^-4. A typical sum is 2^-14 off.
 // - the codes times their scale as bf16 (exact: 4 significant bits) on
 //   v_mfma_f32_16x16x32_bf16, half the rate, whose sums are fp32 throughout.
-// Few rows wait for memory, not for the matrix cores, and an fp32 result shows its sums' last bits:
-// these take the second; many rows with bf16 results, whose step is 2^-8, the first.
+// Up to 32 rows wait for memory, not for the matrix cores, and an fp32 result shows its sums' last
+// bits: these take the second; more rows with bf16 results, whose step is 2^-8, the first.
 //
 // Scales: [tile][quad of blocks][16 rows][4 blocks] bytes, so a lane's dword holds its row's
 // scales of 4 blocks and the instruction's op_sel picks one. Rows past the end and values past

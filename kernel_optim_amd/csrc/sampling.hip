@@ -17,6 +17,11 @@
 //   narrows the exact places down, 8 bits of (logit, index) at a time. Where the list is too long for
 //   LDS (thousands of equal logits, say) it does the same over the whole row.
 // A row that is one chunk does all of it in one workgroup and one launch.
+//
+// 64 rows of 151,936 bf16 logits, mixed settings: maxima 6.3 us (3.1 TB/s), bins 30.6 (an exponential
+// of 64 bits and an LDS atomic a token bound it, not the 19 MB), draw 20.6 (the places' passes, one
+// after the other). One row, top-k 50: 2.6, 10.1 and 10.7, in chunks of 4096: latency of the trips to
+// memory on which the next step depends.
 #include "ko_common.h"
 
 namespace {

@@ -47,7 +47,8 @@ every step: the prompt, decode and verify steps all run on these. The embedding 
 bf16.
 
 ``generate(..., sampling=Sampling(...))`` draws its tokens instead of taking the largest logit
-(kernels.sampling), by random numbers from a seed; it does not speculate.
+(kernels.sampling), by random numbers from a seed; it does not speculate. A change between the two
+captures the decode step anew.
 """
 
 import os
