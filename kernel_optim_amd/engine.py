@@ -64,7 +64,7 @@ from .kernels.fp8 import Fp8Linear
 from .kernels.kv4 import Kv4Attention, kv4_append, kv4_block_bytes, kv4_cache, kv4_write
 from .kernels.gemv import (EPI_ARGMAX, EPI_BF16, EPI_RESID, EPI_SWIGLU, ROWS_MAX, Gemv, argmax_rows,
                            embed_ss, tile_weights, uses_tiled)
-from .kernels.sampling import Sampler
+from .kernels.sampling import Sampler, _whole
 from .model import Qwen3Config, fp8_weights, load_checkpoint, random_weights
 from .prefill import prefill, prefill_fp8
 
@@ -128,7 +128,7 @@ class Sampling:
         """The settings as tensors [B] on the CPU, checked: temperature, top_k, top_p, min_p."""
         out = []
         for name, dtype, valid in (("temperature", torch.float32, lambda v: v >= 0),
-                                   ("top_k", torch.int32, lambda v: v >= 0 and int(v) == v),
+                                   ("top_k", torch.int32, _whole),
                                    ("top_p", torch.float32, lambda v: 0 <= v <= 1),
                                    ("min_p", torch.float32, lambda v: 0 <= v <= 1)):
             v = getattr(self, name)

@@ -114,7 +114,7 @@ def _at_least_0(v):
 
 
 def _whole(v):
-    return v >= 0 and int(v) == v
+    return v >= 0 and (isinstance(v, int) or v.is_integer())
 
 
 def _share(v):

@@ -243,3 +243,23 @@ def test_refusals(dev):
         with pytest.raises(ValueError):
             s(**(dict(logits=x, u=u, ids=ids) | kw))
             pytest.fail(f"{kw} was taken")
+
+
+def test_two_samplers_at_once(dev):
+    """Each on a stream of its own, neither waiting for the other."""
+    B, V = 4, 60001
+    x = [logits(95 + i, B, V, BF16).to(dev) for i in range(2)]
+    u = [torch.rand(8, B, generator=gen(97 + i)).to(dev) for i in range(2)]
+    one, two = Sampler(B, V, dev), [Sampler(B, V, dev) for _ in range(2)]
+    want = [torch.stack([draw(dev, x[i], u[i][j], 0.8, 40, 0.9, sampler=one)[0] for j in range(8)])
+            for i in range(2)]
+    got = [torch.zeros(8, B, dtype=torch.int64, device=dev) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for j in range(8):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                two[i](x[i], u[i][j], got[i][j], temperature=0.8, top_k=40, top_p=0.9)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(got[i].cpu(), want[i])

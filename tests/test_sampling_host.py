@@ -46,3 +46,12 @@ def test_engine_settings():
                 Sampling(temperature=[1.0]), Sampling(min_p=float("nan"))):
         with pytest.raises(ValueError):
             bad.columns(2)
+
+
+@pytest.mark.parametrize("k", [float("inf"), float("nan"), 2.5, -1])
+def test_top_k_is_a_whole_number(k):
+    from kernel_optim_amd.engine import Sampling
+    with pytest.raises(ValueError):
+        Sampling(top_k=k).columns(1)
+    with pytest.raises(ValueError):
+        S._setting(k, "top_k", None, 1, 0, S._whole)
