@@ -202,12 +202,19 @@ long long groups(const LinearArgs& a, int t) {
 //   256 x 256: 40 a round                        (8192 x 6144: 120 us against 135, 128 x 128)
 //   128 x 128: 18 up to 256 workgroups, then 22.5 a round       (2048 x 19456: 114 against 123)
 //   64 x 64:   10.4 up to 256, 11.7 up to 512, then 15.5 a round    (128 x 6144: 10.5 against 18)
+// and through bf16, where rounds follow one another with less of a gap:
+//   128 x 128: 26 up to 256 workgroups, 40 up to 409, then 40 for each 512    (1024 x 19456: 102 against 133)
+//   64 x 64:   12.5, 17.7 and 24 up to 256, 512 and 712, then 20.5 for each 768   (128 x 6144: 13 against 25)
 template <int EPI>
 int launch(const LinearArgs& a, hipStream_t s) {
+  const long long n8 = groups(a, 8), n4 = groups(a, 4);
   if constexpr (EPI == EPI_F32) {
+    const double t8 = n8 <= 256 ? 26.0 : fmax(40.0, 8.0 + 40.0 / 512 * n8);
+    const double t4 = n4 <= 256 ? 12.5 : n4 <= 512 ? 17.7 : fmax(24.0, 5.0 + 20.5 / 768 * n4);
+    if (t4 < t8) return launch_tiled<EPI, true, 2, 2, 2, 2, 3>(a, s);
     return launch_tiled<EPI, true, 2, 2, 4, 4, 2>(a, s);
   } else {
-    const long long n16 = groups(a, 16), n8 = groups(a, 8), n4 = groups(a, 4);
+    const long long n16 = groups(a, 16);
     const double t16 = 40.0 * ((n16 + 255) / 256);
     const double t8 = n8 <= 256 ? 18.0 : 22.5 * ((n8 + 511) / 512);
     const double t4 = n4 <= 256 ? 10.4 : n4 <= 512 ? 11.7 : 15.5 * ((n4 + 767) / 768);
