@@ -122,7 +122,7 @@ __device__ __forceinline__ float fp8_squares(const float* v) {
   return s;
 }
 // The sum of the squares of a block's row of 128, its eights' sums c = 0..15 added as a tree: c and
-// c + 8, then 4, 2 and 1 apart. A row's sum adds its blocks' in order. Every kernel forms both so,
+// c + 8, then 4, 2 and 1 apart. A row's sum adds its blocks' in order, in 64 bits. Every kernel forms both so,
 // whatever its lanes hold, and all find the same norm. Here the block is in registers as above.
 __device__ __forceinline__ float fp8_square_sum(const float (&v)[2][16]) {
   float s[2];
@@ -151,6 +151,16 @@ __device__ __forceinline__ uint32_t fp8_quantize8(const uint4& q, uint2& c) {
   c.y = b == 255 ? 0x7f7f7f7fu
                  : fp8_pack4(bf16lo(w[2]), bf16hi(w[2]), bf16lo(w[3]), bf16hi(w[3]), inv);
   return b;
+}
+
+// 1 / sqrt(sum / K + eps), to fp32's nearest but for one in millions: the instruction's, which is up to
+// an ulp off, with one of Newton's steps in 64 bits. Every bit of it that is wrong moves that much more of a
+// row's values over a bf16 border, and some of their codes with them; a row has one.
+__device__ __forceinline__ float fp8_rstd(double sum, int K, float eps) {
+  const double v = sum / K + (double)eps;
+  const float y = rsqrtf((float)v);
+  if (!(v > 1e-37 && v < 1e37)) return y;   // no row's but one of zeros or of huge values
+  return (float)(y * (1.5 - 0.5 * v * y * y));
 }
 
 // bf16(gain * bf16(x * rstd)) of packed pairs, as the bf16 chain rounds.

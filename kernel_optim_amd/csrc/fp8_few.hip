@@ -145,9 +145,9 @@ __global__ __launch_bounds__(64 * WMAX) void few_kernel(LinearArgs a) {
       }
       __syncthreads();
       if ((int)threadIdx.x < M) {
-        float tot = 0.f;
+        double tot = 0.0;
         for (int kb = 0; kb < KB; ++kb) tot += s_sq[threadIdx.x * KB + kb];
-        s_rstd[threadIdx.x] = rsqrtf(tot / (float)a.K + a.eps);
+        s_rstd[threadIdx.x] = fp8_rstd(tot, a.K, a.eps);
       }
       __syncthreads();
     }

@@ -142,9 +142,9 @@ __global__ __launch_bounds__(1024) void quantize_norm_kernel(
     for (int kb = wv; kb < KB; kb += W) fetch(0, kb), squares(0, kb);
   }
   __syncthreads();
-  float tot = 0.f;
+  double tot = 0.0;
   for (int kb = 0; kb < KB; ++kb) tot += s_sq[kb * 16 + r];
-  const float rstd = row >= 0 ? rsqrtf(tot / (float)K + eps) : 0.f;   // eps may be 0
+  const float rstd = row >= 0 ? fp8_rstd(tot, K, eps) : 0.f;   // eps may be 0
   uint8_t* sc = reinterpret_cast<uint8_t*>(scales);
   auto quantize = [&](int i, int kb) {
     uint32_t b = 0;
@@ -223,9 +223,9 @@ __global__ __launch_bounds__(1024) void quantize_row_kernel(const uint16_t* __re
       if ((e & 15) == 0) s_sq[e >> 4] = sq;
     }
     __syncthreads();
-    float tot = 0.f;
+    double tot = 0.0;
     for (int kb = 0; kb < KB; ++kb) tot += s_sq[kb];
-    rstd = row >= 0 ? rsqrtf(tot / (float)K + eps) : 0.f;   // eps may be 0
+    rstd = row >= 0 ? fp8_rstd(tot, K, eps) : 0.f;   // eps may be 0
   }
 #pragma unroll
   for (int i = 0; i < ROW_LOADS; ++i) {
