@@ -433,8 +433,8 @@ long long ko_kv4_attn_scratch(int rows, int d, int group, int grid);
  * and block of 128 values: codes uint8 [tiles][ceil(K / 128)][2048], scales uint8
  * [tiles][ceil(K / 512)][64] (kernel_optim_amd/csrc/fp8_core.h has the layout), tiles =
  * ceil(rows / 16), or of a pair (gate | up: even rows, 8 of either half in a tile) ceil(rows / 16) too. The scale is the least 2^e >= 2^-127 with max |x| <= 448 * 2^e, a code x / 2^e
- * rounded to nearest (ties to even); a block with a NaN or an infinity holds NaN. All pointers
- * 16-byte aligned.
+ * rounded to nearest (ties to even; 240 for 256 at 2^120, so that finite values stay finite); a block
+ * with a NaN or an infinity holds NaN. All pointers 16-byte aligned.
  *
  * ko_fp8_quantize: x [rows, K] bf16 (x_f32 0) or fp32, row stride in elements (a multiple of 8, or 0),
  * into codes and scales, which must not overlap x. nw (optional, [K] bf16; bf16 rows, no pair): the

@@ -3,8 +3,9 @@
 // A matrix [rows, K] is held as OCP e4m3 codes with one scale 2^(b - 127), b a byte, for each
 // (row, 128 values of K): value = code * scale. b is the least with max |x| <= 448 * scale, so
 // the largest value's code lies in (224, 448] and a code is within 2^-4 of its value (relative;
-// below 2^-6 of the scale within 2^-10 of it). A power of two costs nothing against a scale of
-// more bits: codes are floating point themselves, dividing by it is exact, and the instructions
+// below 2^-6 of the scale within 2^-10 of it). It is the nearest code but for one: at the largest
+// scale, 2^120, a code of 256 would stand for 2^128, past the largest fp32 and bf16, so values
+// from 248 * 2^120 on get 240. A power of two costs nothing against a scale of more bits: codes are floating point themselves, dividing by it is exact, and the instructions
 // that take codes apply it, so sums stay in the accumulators.
 // A block with a NaN or an infinity holds NaN codes and b = 255: it reads back as NaN.
 //
@@ -63,7 +64,7 @@ __device__ __forceinline__ int fp8_row(long long t, int r, int rows, bool pair) 
 }
 
 // The scale's byte for a block whose largest |x| has these bits (NaN and infinity sort above
-// every number): 448 = 1.75 * 2^8.
+// every number): 448 = 1.75 * 2^8. At most 247, or 255.
 __device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax_bits) {
   const int e = (int)(amax_bits >> 23), b = e - 8 + ((amax_bits & 0x7fffffu) > 0x600000u);
   return e == 255 ? 255u : (uint32_t)max(b, 0);
@@ -80,6 +81,12 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true);
   return (uint32_t)w;
+}
+
+// Four codes of a block whose scale byte is 247 or more: NaN (255), or with 240 for 256, the largest
+// that such a block can have.
+__device__ __forceinline__ uint32_t fp8_top4(uint32_t w, uint32_t b) {
+  return b == 255 ? 0x7f7f7f7fu : w - ((w & w >> 1 & w >> 2 & w >> 3 & 0x08080808u) >> 3);
 }
 
 __device__ __forceinline__ uint32_t umax_xor16(uint32_t u) {
@@ -106,9 +113,10 @@ __device__ __forceinline__ uint32_t fp8_quantize_block(const float (&v)[2][16], 
   for (int j = 0; j < 2; ++j) {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = b == 255 ? 0x7f7f7f7fu
-                      : fp8_pack4(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
+    for (int i = 0; i < 4; ++i) {
+      w[i] = fp8_pack4(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
+      if (b >= 247) w[i] = fp8_top4(w[i], b);
+    }
     c[j] = make_uint4(w[0], w[1], w[2], w[3]);
   }
   return b;
@@ -146,10 +154,9 @@ __device__ __forceinline__ uint32_t fp8_quantize8(const uint4& q, uint2& c) {
   m = max(m, dpp_i<0x121>(m));
   const uint32_t b = fp8_scale_byte((uint32_t)m << 16);
   const float inv = fp8_inverse(min(b, 247u));
-  c.x = b == 255 ? 0x7f7f7f7fu
-                 : fp8_pack4(bf16lo(w[0]), bf16hi(w[0]), bf16lo(w[1]), bf16hi(w[1]), inv);
-  c.y = b == 255 ? 0x7f7f7f7fu
-                 : fp8_pack4(bf16lo(w[2]), bf16hi(w[2]), bf16lo(w[3]), bf16hi(w[3]), inv);
+  c.x = fp8_pack4(bf16lo(w[0]), bf16hi(w[0]), bf16lo(w[1]), bf16hi(w[1]), inv);
+  c.y = fp8_pack4(bf16lo(w[2]), bf16hi(w[2]), bf16lo(w[3]), bf16hi(w[3]), inv);
+  if (b >= 247) c.x = fp8_top4(c.x, b), c.y = fp8_top4(c.y, b);
   return b;
 }
 

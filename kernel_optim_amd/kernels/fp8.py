@@ -12,9 +12,10 @@ caller's, every call launches on the current stream of the current device and ne
 
 A value is held as an OCP e4m3 code times its block's scale, a power of two: a block is 128
 neighbouring values of a row, and the scale the least 2^e >= 2^-127 with max |x| <= 448 * 2^e. A code
-is x / 2^e rounded to nearest (ties to even): within 2^-4 of x, or within 2^(e - 10) where |x| is
-below 2^(e - 6). A block with a NaN or an infinity reads back as NaN throughout. 8.06 bits a value.
-K is a multiple of 8; the last block may be short.
+is x / 2^e rounded to nearest (ties to even; at e = 120 256 becomes 240, as 2^128 is no number of
+either type): within 2^-4 of x, or within 2^(e - 10) where |x| is below 2^(e - 6). A block with a
+NaN or an infinity reads back as NaN throughout. 8.06 bits a value. K is a multiple of 8; the last
+block may be short.
 """
 
 import torch

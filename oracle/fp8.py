@@ -2,7 +2,8 @@
 in 64 bits, the block layout by index, and the projections over the held values.
 
 kernel_optim_amd/kernels/fp8.py states the rule: a block of 128 values of a row has the least power
-of two s >= 2^-127 with max |x| <= 448 s, and holds x / s rounded to e4m3."""
+of two s >= 2^-127 with max |x| <= 448 s, and holds x / s rounded to e4m3, but 240 where that
+gives 256 and s is 2^120 (256 s is past fp32's largest)."""
 
 import torch
 
@@ -31,6 +32,7 @@ def quantise(x):
     c = torch.searchsorted(mid, v.abs())             # ties: the lower code,
     tie = (c < 126) & (v.abs() == mid[c.clamp_max(125)])
     c = torch.where(tie & (c % 2 == 1), c + 1, c)    # unless the upper one is even
+    c = torch.where((b[..., None] == 247) & (c == 0x78), 0x77, c)   # 256 -> 240
     c = torch.where(torch.signbit(v), c + 128, c)
     c = torch.where(bad[..., None], 0x7f, c)
     return c.to(torch.uint8).flatten(1), torch.where(bad, 255, b).to(torch.uint8)

@@ -59,3 +59,16 @@ def test_layout_holds_every_value_once(rows, K, pair):
     c, s = O.pack(codes, scales, pair)
     assert torch.equal(c[c > 0].sort().values, codes.flatten().sort().values)
     assert torch.equal(s[s > 0].sort().values, scales.flatten().sort().values)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_finite_values_stay_finite(dtype):
+    """Up to the type's largest, within 2^-4: no code stands for 2^128."""
+    top = torch.finfo(dtype).max
+    x = torch.tensor([top, -top, 248 * 2.0 ** 120, 247 * 2.0 ** 120, -255 * 2.0 ** 120, 1.0]).to(dtype)
+    v = O.held(torch.cat((x, torch.zeros(2, dtype=dtype)))[None])[0, :6]
+    assert torch.isfinite(v.to(dtype)).all()
+    assert ((v - x.double()).abs() <= 2.0 ** -4 * x.double().abs())[:5].all() and v[5] == 0
+    assert v[0] == 240 * 2.0 ** 120 == -v[1] == v[2] == v[3] == -v[4]
+    below = torch.tensor([[224 * 2.0 ** 120, 2.0 ** 119, 256 * 2.0 ** 119]])
+    assert (O.held(torch.nn.functional.pad(below, (0, 5)))[0, :3] == below.double()).all()
