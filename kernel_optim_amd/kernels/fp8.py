@@ -177,7 +177,8 @@ class Fp8Linear:
 
     ``x`` is [M, K] bf16 and is quantised in the call (with the norm) into a workspace of the object's,
     or an Fp8Tensor where there is no norm. The workspace is made for ``device``, or in the first
-    call, which must not be under graph capture. Calls of one object share it: they must be
+    call, which must not be under graph capture; the object stays on that device, and has to outlive
+    the graphs that captured its calls. Calls of one object share it: they must be
     ordered, on one stream or by events, captured calls' replays included. y (and h where it is y) must
     not overlap x, nw or w."""
 
@@ -196,10 +197,16 @@ class Fp8Linear:
         self._bytes = (2 * M * K, M * N * (4 if epi == EPI_F32 else 2), 2 * M * N, 2 * K,
                        tiles * blocks * 2048, tiles * _cdiv(blocks, 4) * 64)
         if device is not None:
-            self._workspace(torch.empty(0, device=device).get_device())
+            device = torch.device(device)
+            _need(device.type == "cuda", "device must be a GPU")
+            self._workspace(torch.cuda.current_device() if device.index is None else device.index)
 
     def _workspace(self, dev):
-        if self._xq is None or self._xq.codes.get_device() != dev:
+        if self._xq is not None:
+            # a new one would free what captured calls use
+            at = self._xq.codes.get_device()
+            _need(at == dev, f"the object's workspace is on cuda:{at}: make another object for cuda:{dev}")
+        else:
             _need(not torch.cuda.is_current_stream_capturing(), "the workspace is made in the first "
                   "call: make it before the capture, or give the object its device")
             at = torch.device("cuda", dev)

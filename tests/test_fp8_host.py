@@ -77,3 +77,17 @@ def test_c_abi_refuses():
     assert h.ko_fp8_linear_scratch(1, 2560, 9728, EPI_RESID) == 0
     for bad in ((0, 8, 8, 0), (1, 0, 8, 0), (1, 8, 12, 0), (1, 8, 8, 4), (1, 2 ** 30, 8, 0)):
         assert h.ko_fp8_linear_scratch(*bad) == -1
+
+
+def test_linear_keeps_to_one_device():
+    """Another device's call would free the workspace that captured calls use."""
+    from types import SimpleNamespace
+    op = P.Fp8Linear(4, 32, 256, EPI_BF16, False)
+    made = SimpleNamespace(codes=SimpleNamespace(get_device=lambda: 0))
+    op._xq = made
+    assert op._workspace(0) is made
+    with pytest.raises(ValueError):
+        op._workspace(1)
+    assert op._xq is made
+    with pytest.raises(ValueError):
+        P.Fp8Linear(4, 32, 256, EPI_BF16, False, device="cpu")
