@@ -73,6 +73,7 @@ class Gemv:
         self.cfg = self.candidates()[0]
         self._part = None
         self._rows = self._xn = None
+        self._kept = {}    # name of a buffer -> all that it was
         self._tiles = {}   # id(row-major weight) -> (weakref to it, its tiled copy)
         self.us = float("nan")
         self.tune_log = []
@@ -121,9 +122,21 @@ class Gemv:
     def xn_buffer(self, device):
         """The normalised input of a layout-5 norm projection, which the residual
         projection before it fills (``nxt``): one weight pass of 64 rows."""
-        if self._xn is None or self._xn.device != device:
-            self._xn = torch.zeros(ROWS_MAX * self.K, dtype=BF16, device=device)
-        return self._xn
+        return self._buffer("_xn", ROWS_MAX * self.K, BF16, device)
+
+    def _buffer(self, name, n, dtype, device):
+        """The object's buffer of that name, n elements or more and zeros at first. One that a larger
+        one or another device's replaces stays: captured calls may use it."""
+        t = getattr(self, name)
+        if t is None or t.device != device or t.numel() < n:
+            device = torch.empty(0, device=device).device
+            kept = self._kept.setdefault(name, [])
+            t = next((k for k in kept if k.device == device and k.numel() >= n), None)
+            if t is None:
+                t = torch.zeros(n, dtype=dtype, device=device)
+                kept.append(t)
+            setattr(self, name, t)
+        return t
 
     def candidates(self):
         """Launch configurations, the default first. The default is always a
@@ -161,12 +174,7 @@ class Gemv:
         launch leaves them there); layout 5 has one of its own, as it leaves sums
         where those counters are."""
         n = _lib.lib().ko_gemv_argmax_scratch(self.N, *cfg)
-        name = "_rows" if cfg[0] == 5 else "_part"
-        t = getattr(self, name)
-        if t is None or t.device != device or t.numel() < n:
-            t = torch.zeros(max(n, 2), dtype=torch.float32, device=device)
-            setattr(self, name, t)
-        return t
+        return self._buffer("_rows" if cfg[0] == 5 else "_part", max(n, 2), torch.float32, device)
 
     def _weight_for(self, w, cfg):
         """The weight tensor this configuration reads: ``w`` itself, or for a tiled

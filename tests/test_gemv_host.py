@@ -75,3 +75,23 @@ def test_engine_refuses_a_directory_without_weights(tmp_path, monkeypatch):
     monkeypatch.delenv("ENGINE_RANDOM_INIT", raising=False)
     with pytest.raises(FileNotFoundError, match="safetensors"):
         Engine(str(tmp_path))
+
+
+def test_buffers_that_were_replaced_stay():
+    """A graph may have captured calls on the scratch that a larger configuration replaces, or on
+    another device's: none of them is freed, and none is made twice."""
+    import gc
+    import weakref
+    cpu, meta = torch.device("cpu"), torch.device("meta")
+    g = Gemv(16, H, 9728, EPI_RESID, False)
+    a = weakref.ref(g._scratch(cpu, (4, 10, 0)))
+    b = weakref.ref(g._scratch(cpu, (4, 10, 4)))
+    assert b().numel() > a().numel() and b() is not a()
+    g._scratch(meta, (4, 10, 4))
+    gc.collect()
+    assert a() is not None and b() is not None
+    assert g._scratch(cpu, (4, 10, 4)) is b()
+    assert g._scratch(cpu, (4, 10, 0)) is b()      # the largest serves them all
+    x = weakref.ref(g.xn_buffer(cpu))
+    g.xn_buffer(meta)
+    assert g.xn_buffer(cpu) is x() and g.xn_buffer("cpu") is x()
