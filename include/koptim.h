@@ -343,7 +343,7 @@ long long ko_gemv_argmax_scratch(int N, int layout, int rows, int waves);
 
 /* Replaces torch.argmax(logits, dim=-1, out=vout) of the speculative verify
  * step (engine/engine.py:413-415): ids[m] = argmax_n x[m, n] over bf16 logits
- * [M, N] with row stride ld elements (ld % 8 == 0, x 16-byte aligned), lowest
+ * [M, N] with row stride ld elements (any of at least N, x aligned to an element), lowest
  * index on ties. One workgroup per row; no memset, so it can be captured in a
  * graph. */
 int ko_argmax_rows(const void* x, long long ld, int M, int N, long long* ids, void* stream);

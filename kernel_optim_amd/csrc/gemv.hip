@@ -210,8 +210,8 @@ __global__ __launch_bounds__(FT) void argmax_finalize_kernel(
 // Greedy id of each row of bf16 logits [M, N] (row stride ld elements): one
 // 1024-thread workgroup per row, lowest index on ties (torch.argmax over the
 // verify step's logits, engine.py:413-415). Every thread reads 8 columns per
-// 16-byte load, AL loads in flight before it compares; a scalar tail covers N
-// not a multiple of 8.
+// 16-byte load, AL loads in flight before it compares; the columns in front of a
+// row's first 16-byte border and behind its last go one by one.
 constexpr int AL = 8;
 __global__ __launch_bounds__(FT) void argmax_rows_kernel(const uint16_t* __restrict__ x,
                                                          long long ld, int N,
@@ -219,20 +219,22 @@ __global__ __launch_bounds__(FT) void argmax_rows_kernel(const uint16_t* __restr
   __shared__ float2 s_best[FT / 64];
   const int m = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = t >> 6;
   const uint16_t* row = x + (long long)m * ld;
-  const int nc = N >> 3;  // whole 8-column chunks
+  const int head = min(N, (int)(-(reinterpret_cast<uintptr_t>(row) >> 1) & 7));
+  const int nc = (N - head) >> 3;  // whole 8-column chunks
   float bv = -INFINITY;
   int bi = 0x7fffffff;
+  if (t < head) better(bf16lo(row[t]), t, bv, bi);
   for (int c0 = t; c0 < nc; c0 += AL * FT) {
     uint4 u[AL];
 #pragma unroll
     for (int j = 0; j < AL; ++j) {
       const int c = c0 + j * FT;
-      u[j] = c < nc ? ldg16(row + 8 * c) : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u,
+      u[j] = c < nc ? ldg16(row + head + 8 * c) : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u,
                                                       0xff80ff80u);  // -inf
     }
 #pragma unroll
     for (int j = 0; j < AL; ++j) {
-      const int base = 8 * (c0 + j * FT);
+      const int base = head + 8 * (c0 + j * FT);
       const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(FT) void argmax_rows_kernel(const uint16_t* __restr
       }
     }
   }
-  for (int c = 8 * nc + t; c < N; c += FT) better(bf16lo(row[c]), c, bv, bi);
+  for (int c = head + 8 * nc + t; c < N; c += FT) better(bf16lo(row[c]), c, bv, bi);
 #define KO_ROW_STEP(CTRL)                                                                   \
   {                                                                                         \
     const float ov = dpp_f<CTRL>(bv);                                                       \
@@ -454,7 +456,7 @@ int ko_gemv_tile(const void* w, void* wt, int rows, int K, void* stream) {
 }
 
 int ko_argmax_rows(const void* x, long long ld, int M, int N, long long* ids, void* stream) {
-  if (!x || !ids || M < 1 || N < 1 || ld < N || (ld & 7) || !al16(x)) return KO_EINVAL;
+  if (!x || !ids || M < 1 || N < 1 || ld < N || (reinterpret_cast<uintptr_t>(x) & 1)) return KO_EINVAL;
   hipLaunchKernelGGL(argmax_rows_kernel, dim3(M), dim3(FT), 0, static_cast<hipStream_t>(stream),
                      static_cast<const uint16_t*>(x), ld, N, ids);
   return KO_LAUNCH_STATUS();
