@@ -42,7 +42,6 @@ namespace ko {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int FP8_BLOCK = 2048;   // bytes of a block of codes: 16 rows, 128 values
 

@@ -106,9 +106,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ 
 
 constexpr int NORM_BLOCKS = 1024;   // K up to 131,072
 
-// RMSNorm in front (bf16 rows): a workgroup takes a tile, sums the squares of its 16 rows in
-// fp32, and its wavefronts quantise bf16(nw * bf16(x * rstd)). R blocks a wavefront stay in
-// registers between the two; R = 0 (long rows) reads them again.
+// RMSNorm in front (bf16 rows): a workgroup takes a tile, sums the squares of its 16 rows (a block's
+// in fp32, blocks in 64 bits), and its wavefronts quantise bf16(nw * bf16(x * rstd)). R blocks a
+// wavefront stay in registers between the two; R = 0 (long rows) reads them again.
 template <int R>
 __global__ __launch_bounds__(1024) void quantize_norm_kernel(
     const uint16_t* __restrict__ x, long long stride, int rows, int K,

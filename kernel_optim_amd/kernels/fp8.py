@@ -126,8 +126,9 @@ def _need_apart(a, b, what):
 
 def fp8_quantize(x, out=None, nw=None, eps=1e-6, pair=False):
     """Quantise rows x [rows, K] (bf16 or fp32, inner stride 1, row stride a multiple of 8 or 0) into
-    ``out`` (None: a new Fp8Tensor), which is returned. ``nw`` [K] bf16: bf16 rows go through an RMSNorm with this
-    gain first, rounded as the bf16 chain is (bf16(nw * bf16(x * rstd)), statistics in fp32).
+    ``out`` (None: a new Fp8Tensor), which is returned. ``nw`` [K] bf16: bf16 rows go through an
+    RMSNorm with this gain first, rounded as the bf16 chain is (bf16(nw * bf16(x * rstd)), a block's
+    squares summed in fp32, the blocks in 64 bits).
     ``pair``: x is gate | up, [2 N, K], for an Fp8Linear with SWIGLU; ``out`` says so itself."""
     dev, stride = _check_rows(x, "x", (BF16, F32))
     _here(dev)
