@@ -429,7 +429,7 @@ long long ko_kv4_attn_scratch(int rows, int d, int group, int grid);
 
 /* ---- Matrices held in 8-bit floating point --------------------------------------
  * No counterpart in the reference, whose weights are bf16.
- * A matrix [rows, K], K % 8 == 0, is held as e4m3 codes and one power-of-two scale for each row
+ * A matrix [rows, K], K % 8 == 0, K <= 2^27, is held as e4m3 codes and one power-of-two scale for each row
  * and block of 128 values: codes uint8 [tiles][ceil(K / 128)][2048], scales uint8
  * [tiles][ceil(K / 512)][64] (kernel_optim_amd/csrc/fp8_core.h has the layout), tiles =
  * ceil(rows / 16), or of a pair (gate | up: even rows, 8 of either half in a tile) ceil(rows / 16) too. The scale is the least 2^e >= 2^-127 with max |x| <= 448 * 2^e, a code x / 2^e

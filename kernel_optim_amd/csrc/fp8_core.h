@@ -44,6 +44,10 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int FP8_BLOCK = 2048;   // bytes of a block of codes: 16 rows, 128 values
+constexpr int FP8_K_MAX = 1 << 27;   // so that a byte's place in a tile stays below 2^31
+
+// Whether one launch takes as many workgroups: a grid has fewer than 2^32 threads.
+inline bool fp8_launchable(long long groups, int threads) { return groups * threads < 1ll << 32; }
 
 __host__ __device__ __forceinline__ int fp8_blocks(int K) { return (K + 127) >> 7; }
 __host__ __device__ __forceinline__ int fp8_quads(int K) { return (K + 511) >> 9; }

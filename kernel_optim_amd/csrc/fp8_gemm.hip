@@ -186,7 +186,7 @@ template <int EPI, bool WIDE, int WN, int WM, int TN, int TM, int STAGES>
 int launch_tiled(const LinearArgs& a, hipStream_t s) {
   constexpr int NT = WN * TN, MT = WM * TM;
   const int nb = (a.wt + NT - 1) / NT, mb = (a.xt + MT - 1) / MT;
-  if ((long long)nb * mb > 0x7fffffffll) return KO_ERANGE;
+  if (!fp8_launchable((long long)nb * mb, 64 * WN * WM)) return KO_ERANGE;
   hipLaunchKernelGGL((gemm_kernel<EPI, WIDE, WN, WM, TN, TM, STAGES>), dim3(nb * mb),
                      dim3(64 * WN * WM), 0, s, a, nb);
   return KO_LAUNCH_STATUS();
@@ -235,7 +235,7 @@ static void set_sizes(LinearArgs& a, int M, int N, int K, int epi) {
 extern "C" {
 
 long long ko_fp8_linear_scratch(int M, int N, int K, int epi) {
-  if (M < 1 || N < 1 || N > 0x3fffffff || K < 8 || (K & 7) || epi < EPI_F32 || epi > EPI_SWIGLU) return -1;
+  if (M < 1 || N < 1 || N > 0x3fffffff || K < 8 || K > FP8_K_MAX || (K & 7) || epi < EPI_F32 || epi > EPI_SWIGLU) return -1;
   LinearArgs a;
   set_sizes(a, M, N, K, epi);
   return !few_rows_served(a) && mid_rows_served(a, epi) ? mid_rows_scratch(a) : 0;
@@ -253,7 +253,7 @@ int ko_fp8_linear(const void* x, const void* nw, float eps, void* xc, void* xs, 
   const uintptr_t all = (uintptr_t)xc | (uintptr_t)xs | (uintptr_t)wc | (uintptr_t)ws | (uintptr_t)y |
                         (uintptr_t)x | (uintptr_t)nw;
   if ((all | (uintptr_t)h | (uintptr_t)scratch) & 15) return KO_EINVAL;
-  if (N > 0x3fffffff) return KO_ERANGE;
+  if (N > 0x3fffffff || K > FP8_K_MAX) return KO_ERANGE;
   const long long need = ko_fp8_linear_scratch(M, N, K, epi);
   if (need && (!scratch || scratch_bytes < need)) return KO_EINVAL;
   LinearArgs a;

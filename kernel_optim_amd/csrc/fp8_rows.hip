@@ -298,7 +298,7 @@ __global__ __launch_bounds__(256) void read_kernel(const uint8_t* __restrict__ c
 int check(int rows, int K, int pair, long long stride) {
   if (rows < 1 || K < 8 || (K & 7) || stride < 0 || (stride & 7) || (pair && (rows & 1)))
     return KO_EINVAL;
-  if (fp8_tiles(rows, pair) * fp8_blocks(K) > 0x7fffffffll) return KO_ERANGE;
+  if (K > FP8_K_MAX || fp8_tiles(rows, pair) * fp8_blocks(K) > 0x7fffffffll) return KO_ERANGE;
   return KO_OK;
 }
 
@@ -337,6 +337,7 @@ int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K,
   if (nw) {
     const int KB = fp8_blocks(K);
     const uint16_t *xb = static_cast<const uint16_t*>(x), *wb = static_cast<const uint16_t*>(nw);
+    if (!fp8_launchable(tiles, 64 * (KB <= 32 ? (KB + 1) / 2 : 16))) return KO_ERANGE;
 #define KO_NORM(R, WAVES)                                                                      \
   hipLaunchKernelGGL(quantize_norm_kernel<R>, dim3((unsigned)tiles), dim3(64 * (WAVES)), 64 * KB, s, \
                      xb, stride, rows, K, wb, eps, c, sc)
@@ -347,6 +348,7 @@ int ko_fp8_quantize(const void* x, int x_f32, long long stride, int rows, int K,
     return KO_LAUNCH_STATUS();
   }
   const long long units = tiles * fp8_quads(K);
+  if (!fp8_launchable((units + 3) / 4, 256)) return KO_ERANGE;
   const dim3 grid((unsigned)((units + 3) / 4));
   if (x_f32)
     hipLaunchKernelGGL(quantize_kernel<true>, grid, dim3(256), 0, s, x, stride, rows, K, pair, c,
@@ -363,6 +365,7 @@ int ko_fp8_read(const void* codes, const void* scales, int rows, int K, int pair
   if (const int st = check(rows, K, pair, stride)) return st;
   if (!al16(codes) || !al16(scales) || !al16(out)) return KO_EINVAL;
   const long long units = fp8_tiles(rows, pair) * fp8_blocks(K);
+  if (!fp8_launchable((units + 3) / 4, 256)) return KO_ERANGE;
   const dim3 grid((unsigned)((units + 3) / 4));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (out_f32)

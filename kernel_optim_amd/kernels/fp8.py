@@ -2,7 +2,8 @@
 
 The ops stand beside ``kernels.gemv``'s for bf16 weights and follow their manner: tensors are the
 caller's, every call launches on the current stream of the current device and never synchronises
-(so calls can be captured), and a bad argument raises ValueError before anything is launched.
+(so calls can be captured), and a bad argument raises ValueError before anything is launched
+(RuntimeError where a call is too large for one launch: 2^26 blocks to read, 2^26 runs of 4 to write).
 
 - ``fp8_quantize``: rows [rows, K] in bf16 or fp32, behind an RMSNorm if asked, to 8 bits (a
   weight once at load, a projection's input in every call); ``fp8_read`` gives the values back,
@@ -14,8 +15,8 @@ A value is held as an OCP e4m3 code times its block's scale, a power of two: a b
 neighbouring values of a row, and the scale the least 2^e >= 2^-127 with max |x| <= 448 * 2^e. A code
 is x / 2^e rounded to nearest (ties to even; at e = 120 256 becomes 240, as 2^128 is no number of
 either type): within 2^-4 of x, or within 2^(e - 10) where |x| is below 2^(e - 6). A block with a
-NaN or an infinity reads back as NaN throughout. 8.06 bits a value. K is a multiple of 8; the last
-block may be short.
+NaN or an infinity reads back as NaN throughout. 8.06 bits a value. K is a multiple of 8, up to 2^27;
+the last block may be short.
 """
 
 import torch
@@ -61,6 +62,7 @@ def fp8_shape(rows, K, pair=False):
     tiles = _cdiv(rows // 2, 8) if pair else _cdiv(rows, 16)
     blocks = _cdiv(K, FP8_BLOCK)
     _need(tiles * blocks < 2 ** 31, "the matrix has 2^31 blocks or more")
+    _need(rows < 2 ** 31 and K <= 2 ** 27, f"2^31 rows or more, or more than 2^27 columns: [{rows}, {K}]")
     return tiles, blocks
 
 

@@ -91,3 +91,26 @@ def test_linear_keeps_to_one_device():
     assert op._xq is made
     with pytest.raises(ValueError):
         P.Fp8Linear(4, 32, 256, EPI_BF16, False, device="cpu")
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Rows and columns that a C int, or a byte's place in a tile as one, does not hold."""
+    assert P.fp8_shape(1, 2 ** 27) == (1, 2 ** 20)
+    for bad in ((1, 2 ** 27 + 8), (1, 2 ** 31 - 8), (1, 2 ** 32 + 8), (2 ** 31, 8), (2 ** 32 + 5, 8)):
+        with pytest.raises(ValueError):
+            P.fp8_shape(*bad)
+    for M, N, K in ((1, 8, 2 ** 32 + 8), (2 ** 32 + 1, 8, 8), (1, 2 ** 32 + 8, 8), (1, 8, 2 ** 27 + 8)):
+        with pytest.raises(ValueError):
+            P.Fp8Linear(M, N, K, EPI_BF16, False)
+    h, p, ERANGE = _lib.lib(), 1 << 20, -34   # p is never read: the checks come first
+    K = 2 ** 27 + 8
+    assert h.ko_fp8_quantize(p, 0, K, 1, K, 0, None, 1e-6, p, p, None) == ERANGE
+    assert h.ko_fp8_read(p, p, 1, K, 0, p, 0, K, None) == ERANGE
+    assert h.ko_fp8_linear(None, None, 0.0, p, p, p, p, p, None, p, 1 << 40, 1, 8, K, EPI_BF16,
+                           None) == ERANGE
+    assert h.ko_fp8_linear_scratch(1, 8, K, EPI_BF16) == -1
+    # more threads than a grid has
+    assert h.ko_fp8_quantize(p, 0, 8, 2 ** 30, 8, 0, None, 1e-6, p, p, None) == ERANGE
+    assert h.ko_fp8_quantize(p, 1, 8, 2 ** 30, 8, 0, None, 1e-6, p, p, None) == ERANGE
+    assert h.ko_fp8_quantize(p, 0, 8, 2 ** 30, 8, 0, p, 1e-6, p, p, None) == ERANGE
+    assert h.ko_fp8_read(p, p, 2 ** 30, 8, 0, p, 0, 8, None) == ERANGE
