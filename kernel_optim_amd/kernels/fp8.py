@@ -28,6 +28,7 @@ from .kv4 import _current_device, _here, _no_overlap, _stream, _tensor
 
 F32 = torch.float32
 FP8_BLOCK = 128   # values that share a scale
+NORM_K = 2 ** 17   # the longest rows that a norm in front takes
 
 
 class Fp8Tensor:
@@ -128,7 +129,7 @@ def _need_apart(a, b, what):
 
 def fp8_quantize(x, out=None, nw=None, eps=1e-6, pair=False):
     """Quantise rows x [rows, K] (bf16 or fp32, inner stride 1, row stride a multiple of 8 or 0) into
-    ``out`` (None: a new Fp8Tensor), which is returned. ``nw`` [K] bf16: bf16 rows go through an
+    ``out`` (None: a new Fp8Tensor), which is returned. ``nw`` [K] bf16, K <= 2^17: bf16 rows go through an
     RMSNorm with this gain first, rounded as the bf16 chain is (bf16(nw * bf16(x * rstd)), a block's
     squares summed in fp32, the blocks in 64 bits).
     ``pair``: x is gate | up, [2 N, K], for an Fp8Linear with SWIGLU; ``out`` says so itself."""
@@ -138,6 +139,7 @@ def fp8_quantize(x, out=None, nw=None, eps=1e-6, pair=False):
     if nw is not None:
         _need(x.dtype == BF16 and not pair and not (out is not None and out.pair),
               "a norm goes with bf16 rows that are no pair")
+        _need(K <= NORM_K, f"a norm goes with rows of up to {NORM_K} values, got {K}")
         _tensor(nw, "nw", BF16, (K,), dev)
     if out is None:
         out = fp8_empty(rows, K, x.device, pair)
@@ -170,7 +172,7 @@ def fp8_read(t, out):
 
 class Fp8Linear:
     """One projection y[M, N] = x[M, K] W[N, K]^T, x and W in 8 bits, sums in fp32, with a norm in
-    front (``norm``, gain ``nw``) and an epilogue: EPI_F32 (y fp32), EPI_BF16, EPI_RESID
+    front (``norm``, gain ``nw``, K <= 2^17) and an epilogue: EPI_F32 (y fp32), EPI_BF16, EPI_RESID
     (y = bf16(h + bf16(x W^T)); y None: h itself) or EPI_SWIGLU (W is gate | up held as a pair;
     y = bf16(bf16(silu(g)) * u) of the bf16 products g and u).
 
@@ -190,6 +192,7 @@ class Fp8Linear:
         _need(M >= 1 and N >= 1, "M and N must be positive")
         fp8_shape((2 if epi == EPI_SWIGLU else 1) * N, K, epi == EPI_SWIGLU)
         fp8_shape(M, K)
+        _need(not norm or K <= NORM_K, f"a norm goes with rows of up to {NORM_K} values, got {K}")
         self.M, self.N, self.K, self.epi, self.norm, self.eps = M, N, K, epi, bool(norm), eps
         self._xq = self._scratch = None
         wide = (2 if epi == EPI_SWIGLU else 1) * N

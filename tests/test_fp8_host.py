@@ -114,3 +114,11 @@ def test_sizes_past_32_bits_are_refused():
     assert h.ko_fp8_quantize(p, 1, 8, 2 ** 30, 8, 0, None, 1e-6, p, p, None) == ERANGE
     assert h.ko_fp8_quantize(p, 0, 8, 2 ** 30, 8, 0, p, 1e-6, p, p, None) == ERANGE
     assert h.ko_fp8_read(p, p, 2 ** 30, 8, 0, p, 0, 8, None) == ERANGE
+
+
+def test_a_norm_of_longer_rows_is_refused():
+    """As every bad argument by ValueError, when the object is made."""
+    P.Fp8Linear(2, 8, 2 ** 17, EPI_BF16, True)
+    P.Fp8Linear(2, 8, 2 ** 17 + 8, EPI_BF16, False)
+    with pytest.raises(ValueError):
+        P.Fp8Linear(2, 8, 2 ** 17 + 8, EPI_BF16, True)

@@ -79,3 +79,13 @@ def test_rows_in_a_projection(dev, M, K, size, eps):
     fp8_read(t, want)
     assert torch.equal(y, want)
     compare(t, O.norm(x, nw, eps))
+
+
+@pytest.mark.parametrize("n", [1, 33])
+def test_the_longest_rows(dev, n):
+    """2^17 values; longer ones are refused."""
+    x, nw = inputs(n, 2 ** 17, 1e-3, n)
+    compare(fp8_quantize(x.to(dev), nw=nw.to(dev), eps=1e-6), O.norm(x, nw, 1e-6))
+    x, nw = (torch.zeros(*s, dtype=BF16, device=dev) for s in ((n, 2 ** 17 + 8), (2 ** 17 + 8,)))
+    with pytest.raises(ValueError):
+        fp8_quantize(x, nw=nw)
