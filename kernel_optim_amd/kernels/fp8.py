@@ -137,7 +137,7 @@ def fp8_quantize(x, out=None, nw=None, eps=1e-6, pair=False):
     _here(dev)
     rows, K = x.shape
     if nw is not None:
-        _need(x.dtype == BF16 and not pair and not (out is not None and out.pair),
+        _need(x.dtype == BF16 and not pair and not (isinstance(out, Fp8Tensor) and out.pair),
               "a norm goes with bf16 rows that are no pair")
         _need(K <= NORM_K, f"a norm goes with rows of up to {NORM_K} values, got {K}")
         _tensor(nw, "nw", BF16, (K,), dev)
