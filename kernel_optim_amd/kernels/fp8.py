@@ -181,20 +181,23 @@ class Fp8Linear:
     bf16 result (step 2^-8) does not show.
 
     ``x`` is [M, K] bf16 and is quantised in the call (with the norm) into a workspace of the object's,
-    or an Fp8Tensor where there is no norm. The workspace is made for ``device``, or in the first
+    or an Fp8Tensor where there is no norm; with ``held`` always the latter, and the workspace, M K bytes
+    otherwise, is small. The workspace is made for ``device``, or in the first
     call, which must not be under graph capture; the object stays on that device, and has to outlive
     the graphs that captured its calls. Calls of one object share it: they must be
     ordered, on one stream or by events, captured calls' replays included. y (and h where it is y) must
     not overlap x, nw or w."""
 
-    def __init__(self, M, N, K, epi, norm, eps=1e-6, device=None):
+    def __init__(self, M, N, K, epi, norm, eps=1e-6, device=None, held=False):
         _need(epi in (EPI_F32, EPI_BF16, EPI_RESID, EPI_SWIGLU), f"bad epilogue {epi}")
         _need(M >= 1 and N >= 1, "M and N must be positive")
         fp8_shape((2 if epi == EPI_SWIGLU else 1) * N, K, epi == EPI_SWIGLU)
         fp8_shape(M, K)
         _need(not norm or K <= NORM_K, f"a norm goes with rows of up to {NORM_K} values, got {K}")
+        _need(not (norm and held), "a norm goes with x in bf16")
         self.M, self.N, self.K, self.epi, self.norm, self.eps = M, N, K, epi, bool(norm), eps
-        self._xq = self._scratch = None
+        self.held = bool(held)
+        self._dev = self._xq = self._scratch = None
         wide = (2 if epi == EPI_SWIGLU else 1) * N
         tiles, blocks = fp8_shape(wide, K, epi == EPI_SWIGLU)
         # what _usual compares with: shapes, W's rows, and bytes of x, y, h, nw and W
@@ -208,18 +211,18 @@ class Fp8Linear:
             self._workspace(torch.cuda.current_device() if device.index is None else device.index)
 
     def _workspace(self, dev):
-        if self._xq is not None:
-            # a new one would free what captured calls use
-            at = self._xq.codes.get_device()
-            _need(at == dev, f"the object's workspace is on cuda:{at}: make another object for cuda:{dev}")
-        else:
+        if self._dev is None:
             _need(not torch.cuda.is_current_stream_capturing(), "the workspace is made in the first "
                   "call: make it before the capture, or give the object its device")
             at = torch.device("cuda", dev)
             n = _lib.lib().ko_fp8_linear_scratch(self.M, self.N, self.K, self.epi)
             # the counters among it start at zero, and every call leaves them there
             self._scratch = torch.zeros(max(n, 16), dtype=torch.uint8, device=at)
-            self._xq = fp8_empty(self.M, self.K, at)
+            self._xq = None if self.held else fp8_empty(self.M, self.K, at)
+            self._dev = dev
+        # a new one would free what captured calls use
+        _need(self._dev == dev, f"the object's workspace is on cuda:{self._dev}: make another object "
+              f"for cuda:{dev}")
         return self._xq
 
     def _usual(self, x, w, y, nw, h):
@@ -293,6 +296,7 @@ class Fp8Linear:
             self._workspace(dev)
             q, x = x, None
         else:
+            _need(not self.held, "x must be an Fp8Tensor, as the object was made with held")
             _tensor(x, "x", BF16, (M, K), dev)
             if self.norm:
                 _tensor(nw, "nw", BF16, (K,), dev)

@@ -275,7 +275,7 @@ def prefill_fp8(cfg, w, prompt, k_cache, v_cache, cos, sin, sink=None):
     x = F.embedding(prompt, w["embed"]).view(M, H)
     new = lambda n: torch.empty(M, n, dtype=BF16, device=dev)
     held, act = fp8_empty(M, H, dev), new(cfg.inter)
-    qkv = [Fp8Linear(M, n, H, EPI_BF16, False, device=dev) for n in (wide, narrow, narrow)]
+    qkv = [Fp8Linear(M, n, H, EPI_BF16, False, device=dev, held=True) for n in (wide, narrow, narrow)]
     o = Fp8Linear(M, H, wide, EPI_RESID, False, device=dev)
     gu = Fp8Linear(M, cfg.inter, H, EPI_SWIGLU, True, eps, device=dev)
     down = Fp8Linear(M, H, cfg.inter, EPI_RESID, False, device=dev)

@@ -81,10 +81,9 @@ def test_c_abi_refuses():
 
 def test_linear_keeps_to_one_device():
     """Another device's call would free the workspace that captured calls use."""
-    from types import SimpleNamespace
     op = P.Fp8Linear(4, 32, 256, EPI_BF16, False)
-    made = SimpleNamespace(codes=SimpleNamespace(get_device=lambda: 0))
-    op._xq = made
+    op._dev, op._xq = 0, object()
+    made = op._xq
     assert op._workspace(0) is made
     with pytest.raises(ValueError):
         op._workspace(1)
@@ -122,3 +121,8 @@ def test_a_norm_of_longer_rows_is_refused():
     P.Fp8Linear(2, 8, 2 ** 17 + 8, EPI_BF16, False)
     with pytest.raises(ValueError):
         P.Fp8Linear(2, 8, 2 ** 17 + 8, EPI_BF16, True)
+
+
+def test_held_goes_without_a_norm():
+    with pytest.raises(ValueError):
+        P.Fp8Linear(4, 32, 256, EPI_BF16, True, held=True)
