@@ -25,7 +25,8 @@
 // - the codes times their scale as bf16 (exact: 4 significant bits) on
 //   v_mfma_f32_16x16x32_bf16, half the rate, whose sums are fp32 throughout.
 // Up to 32 rows wait for memory, not for the matrix cores, and an fp32 result shows its sums' last
-// bits: these take the second; more rows with bf16 results, whose step is 2^-8, the first.
+// bits: these take the second; more rows with bf16 results, whose step is 2^-8, the first. So a row's
+// bf16 result may be another in its last bit among 33 rows than among 32.
 //
 // Scales: [tile][quad of blocks][16 rows][4 blocks] bytes, so a lane's dword holds its row's
 // scales of 4 blocks and the instruction's op_sel picks one. Rows past the end and values past

@@ -136,12 +136,13 @@ __global__ __launch_bounds__(64 * WMAX) void mid_kernel(LinearArgs a) {
 }
 
 // Longer rows: a workgroup takes two tiles of W and one of S runs of K's blocks, its wavefronts a part
-// of the run each, D blocks of x and W ahead. One workgroup a CU then reads as little as it can: a CU
-// takes in some 45 bytes a ns, from whichever cache, and 80 workgroups that read all of K (of 9728
-// values by 64 rows, 160 with one tile each: 20 us) leave most of them idle. The S partial sums of
+// of the run each, D blocks of x and W ahead. With all of K, 80 workgroups (2560 columns) would read
+// 622 KB of x each and leave most CUs idle (160 with one tile each: 20 us for 9728 values by 64 rows);
+// a CU takes in what others read too at 70 (256 KB) to 120 bytes a ns (4 MB), from L2, and its
+// share of what nobody else reads at 25 with all 256 at it. The S partial sums of
 // a pair of tiles meet in memory, where the last of its workgroups adds them in order. 9728 values by
-// 64 rows, 2560 columns: 13.4 us, some 305 KB a workgroup (7 us at that rate), the rest latency and
-// the meeting.
+// 64 rows, 2560 columns: 13.4 us, in which a workgroup reads 208 KB of x and 104 KB of W, about 3 and 4 us
+// at those rates; the rest is latency and the meeting (wavefronts wait in 65 % of their cycles).
 template <int EPI, int MT>
 __global__ __launch_bounds__(64 * WMAX) void split_kernel(LinearArgs a, int S) {
   constexpr int W = WMAX, NT = 2, D = MT == 4 ? 2 : 4, PARTS = MT * NT;

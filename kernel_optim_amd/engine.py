@@ -47,8 +47,8 @@ every step: the prompt, decode and verify steps all run on these. The embedding 
 bf16.
 
 ``generate(..., sampling=Sampling(...))`` draws its tokens instead of taking the largest logit
-(kernels.sampling), by random numbers from a seed; it does not speculate. A change between the two
-captures the decode step anew.
+(kernels.sampling), by random numbers from a seed; it does not speculate. A sequence whose logits are
+all NaN or -infinity gets the id -1. A change between the two captures the decode step anew.
 """
 
 import os
@@ -856,7 +856,9 @@ class Engine:
 
     @torch.inference_mode()
     def step(self):
-        """Replay one decode step (for callers that drive decoding themselves)."""
+        """Replay one decode step (for callers that drive decoding themselves). Behind a generate()
+        that drew its tokens, the step draws too, with the numbers [B] in ``u``, which the caller
+        renews."""
         self.g1.replay()
 
     @torch.inference_mode()
