@@ -36,7 +36,7 @@ class Sampler:
     probability, below which a token is never drawn. NaN counts as -infinity; a row with nothing above -infinity gets the id -1.
 
     The object holds the scratch of its calls: they must be ordered, on one stream or by events,
-    captured calls' replays included."""
+    captured calls' replays included, and it has to outlive the graphs that captured them."""
 
     def __init__(self, B, V, device):
         _need(1 <= B <= MAX_ROWS, f"B must be 1 to {MAX_ROWS}")
