@@ -5,8 +5,9 @@
 // the largest value's code lies in (224, 448] and a code is within 2^-4 of its value (relative;
 // below 2^-6 of the scale within 2^-10 of it). It is the nearest code but for one: at the largest
 // scale, 2^120, a code of 256 would stand for 2^128, past the largest fp32 and bf16, so values
-// from 248 * 2^120 on get 240. A power of two costs nothing against a scale of more bits: codes are floating point themselves, dividing by it is exact, and the instructions
-// that take codes apply it, so sums stay in the accumulators.
+// from 248 * 2^120 on get 240. A power of two costs nothing against a scale of more bits: codes are
+// floating point themselves, dividing by it is exact, and the instructions that take codes apply
+// it, so sums stay in the accumulators.
 // A block with a NaN or an infinity holds NaN codes and b = 255: it reads back as NaN.
 //
 // Codes lie in the order in which v_mfma_scale_f32_16x16x128_f8f6f4 takes them: a tile of 16 rows

@@ -237,7 +237,8 @@ static void set_sizes(LinearArgs& a, int M, int N, int K, int epi) {
 extern "C" {
 
 long long ko_fp8_linear_scratch(int M, int N, int K, int epi) {
-  if (M < 1 || N < 1 || N > 0x3fffffff || K < 8 || K > FP8_K_MAX || (K & 7) || epi < EPI_F32 || epi > EPI_SWIGLU) return -1;
+  if (M < 1 || N < 1 || N > 0x3fffffff || K < 8 || K > FP8_K_MAX || (K & 7)) return -1;
+  if (epi < EPI_F32 || epi > EPI_SWIGLU) return -1;
   LinearArgs a;
   set_sizes(a, M, N, K, epi);
   return !few_rows_served(a) && mid_rows_served(a, epi) ? mid_rows_scratch(a) : 0;

@@ -15,17 +15,18 @@
 //   the drawn token can lie: a cut moves the places behind it by no more than its bin's mass.
 // - draw: the tokens of these bins, of all chunks, meet in one list, in which a row's last workgroup
 //   narrows the exact places down, 8 bits of (logit, index) at a time. Where the list is too long for
-//   LDS, more than 2048 tokens, it does the same over the whole row, alone: thousands of equal logits, or
-//   flat distributions. A bin is 0.015 T wide, so normal logits of deviation s over 151,936 tokens come
-//   to it from T = 2.3 s on, earlier with several filters. One row then takes 0.40 to 0.47 ms, with
-//   top-p 0.65 to 0.84, with top-k past 1024 besides 0.80 to 1.03 (64 rows: 0.62 to 0.77, 1.0 to 1.3, 1.1
-//   to 1.5), where it takes 0.026 (0.057) else.
+//   LDS, more than 2048 tokens, it does the same over the whole row, alone: thousands of equal
+//   logits, or flat distributions. A bin is 0.015 T wide, so normal logits of deviation s over 151,936
+//   tokens come to it from T = 2.3 s on, earlier with several filters. One row then takes 0.40 to
+//   0.47 ms, with top-p 0.65 to 0.84, with top-k past 1024 besides 0.80 to 1.03 (64 rows: 0.62 to
+//   0.77, 1.0 to 1.3, 1.1 to 1.5), where it takes 0.026 (0.057) else.
 // A row that is one chunk does all of it in one workgroup and one launch.
 //
 // 64 rows of 151,936 bf16 logits, mixed settings: maxima 6.3 us (3.1 TB/s), bins 30.6 (an exponential
 // of 64 bits and an LDS atomic a token, half of whose LDS cycles are conflicts, not the 19 MB; the
-// wavefronts wait in 56 % of their cycles), draw 20.6 (the places' passes, one after the other). One row, top-k 50: 2.6, 10.1 and 10.7, in chunks of 4096: latency of the trips to
-// memory on which the next step depends.
+// wavefronts wait in 56 % of their cycles), draw 20.6 (the places' passes, one after the other). One
+// row, top-k 50: 2.6, 10.1 and 10.7, in chunks of 4096: latency of the trips to memory on which the next
+// step depends.
 #include "ko_common.h"
 
 namespace {

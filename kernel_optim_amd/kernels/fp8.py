@@ -182,11 +182,11 @@ class Fp8Linear:
 
     ``x`` is [M, K] bf16 and is quantised in the call (with the norm) into a workspace of the object's,
     or an Fp8Tensor where there is no norm; with ``held`` always the latter, and the workspace, M K bytes
-    otherwise, is small. The workspace is made for ``device``, or in the first
-    call, which must not be under graph capture; the object stays on that device, and has to outlive
-    the graphs that captured its calls. Calls of one object share it: they must be
-    ordered, on one stream or by events, captured calls' replays included. y (and h where it is y) must
-    not overlap x, nw or w."""
+    otherwise, is small. The workspace is made for ``device``, or in the first call, which must not be
+    under graph capture, on the stream that is current then. The object stays on that device, and has
+    to outlive the graphs that captured its calls. Calls of one object share the workspace: they
+    must be ordered behind its making and each other, on one stream or by events, captured calls'
+    replays included. y (and h where it is y) must not overlap x, nw or w."""
 
     def __init__(self, M, N, K, epi, norm, eps=1e-6, device=None, held=False):
         _need(epi in (EPI_F32, EPI_BF16, EPI_RESID, EPI_SWIGLU), f"bad epilogue {epi}")
